@@ -357,6 +357,130 @@ SPARK_API int spark_ipc_close(void* ptr, int64_t offset);
 SPARK_API int spark_silu_mul_rows(const void* gate, const void* up, int64_t ld_in, void* out, int64_t ld_out,
                                   int dtype, int64_t rows, int64_t cols, void* stream);
 
+/* ---------------------------------------------------------------- tree decoding
+ * The operators between the projections of a decode step that carries a small
+ * tree of drafted tokens per sequence (spark_linear_batch runs the projections
+ * of up to 16 tokens for nearly the price of one): rotary positions, attention
+ * over a paged K/V cache and the tree, verification of the tree against the
+ * target's distribution, and the append of accepted tokens to the cache.  No
+ * counterpart in the reference, whose generate loop leaves these to its model
+ * library (04_scripts/inference_v3.py:108-123).
+ *
+ * A tree is a parent array [batch, nodes]: parent -1 hangs the node on the last
+ * context token, parent j < i on node j, any other value marks the node (and
+ * what hangs on it) unused.  Strides are in elements; the innermost dimension
+ * (head_dim, vocab) has unit stride.  *err is an error word that
+ * spark_workspace_check reads: 8 a position outside the table, 9 a page, length
+ * or index outside the cache, 10 a bounded wait that expired, 11 a token id
+ * outside the vocabulary. */
+
+/* Rotary positions of q and of k (k may be NULL) in one launch, out of place or
+ * in place (y == x with equal strides).  For pair i of a head at position p,
+ * c = table[p, i], s = table[p, rot_dim / 2 + i]:
+ *     (a, b) -> (a c - b s, b c + a s),   inverse: s -> -s (the backward pass);
+ * the pair is (x[i], x[rot_dim / 2 + i]), interleaved: (x[2 i], x[2 i + 1]).
+ * Values rot_dim..head_dim - 1 are copied.  x [batch, tokens, heads, head_dim]
+ * of dtype with strides xs (batch, token, head), y with ys; positions
+ * [batch, tokens] contiguous, 4- or 8-byte integers; table fp32 [table_rows,
+ * rot_dim] (cosines, then sines; any scaling for long contexts is in it).  A
+ * position outside the table gives a zero row and error 8 in *err. */
+typedef struct {
+    const void* x;
+    void* y;
+    int64_t heads;
+    int64_t xs[3], ys[3];
+} SparkRopeHeads;
+SPARK_API int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int dtype, int64_t batch, int64_t tokens,
+                         int head_dim, int rot_dim, int interleaved, int inverse, const void* positions,
+                         int position_bytes, const float* table, int64_t table_rows, int* err, void* stream);
+
+/* A paged K/V cache: token n of sequence b lies in page page_table[b, n /
+ * page_size], row n % page_size.  k and v: element (page, row, head, 0) with
+ * strides (page, row, head) k_stride / v_stride; lens [batch]: tokens in it. */
+typedef struct {
+    void *k, *v;
+    int64_t k_stride[3], v_stride[3];
+    int64_t pages, page_size, kv_heads, head_dim;
+    const int* page_table;
+    int64_t page_table_stride, max_pages;
+    const int* lens;
+    int64_t dtype;
+} SparkPagedCache;
+
+/* Appends new tokens to the cache: for j < n_b, K/V row index[b, j] (index NULL:
+ * row j) of k / v [batch, tokens, kv_heads, head_dim] (strides batch, token, head)
+ * goes to position lens[b] + j.  n_b = counts[b] (counts NULL: all `width`
+ * columns of index, or all tokens).  new_lens [batch] = lens + n_b; it may not be
+ * lens itself.  What does not fit the sequence's pages is left out, a bad page
+ * number or index skips its token; both set error 9 in *err. */
+SPARK_API int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens, const void* k,
+                              const int64_t* k_stride, const void* v, const int64_t* v_stride, const int* index,
+                              int64_t width, const int* counts, int* new_lens, int* err, void* stream);
+
+/* Attention of a tree of drafted tokens: node t of sequence b sees the lens[b]
+ * tokens of the cache, itself and its ancestors.  q and out [batch, nodes,
+ * q_heads, head_dim], k and v (the nodes' own, not in the cache) [batch, nodes,
+ * kv_heads, head_dim], all of the cache's dtype (bf16 or f16); query head h reads
+ * kv head h / (q_heads / kv_heads).
+ *     out = softmax(scale q k^T) v, lse = log sum exp (fp32 [batch, nodes,
+ *     q_heads] contiguous, or NULL)
+ * with fp32 scores, sums and accumulation.  An unused node gets a zero row and
+ * lse -inf.  nodes <= 64; head_dim a multiple of 8, at most 256.  One node per
+ * sequence is plain decode attention. */
+#define SPARK_MAX_TREE_NODES 64
+typedef struct {
+    SparkPagedCache cache;
+    int64_t batch, nodes, q_heads;
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_stride[3], kn_stride[3], vn_stride[3], out_stride[3];
+    const int* parents;
+    int64_t parents_stride; /* 0: one tree for all sequences */
+    float* lse;
+    double scale;
+} SparkTreeAttention;
+SPARK_API size_t spark_tree_attention_workspace_size(const SparkTreeAttention* a);
+SPARK_API int spark_tree_attention(const SparkTreeAttention* a, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* Verification of a drafted tree by rejection sampling.  Node 0 is the last token
+ * already accepted; the target's logits at a node give the distribution of its
+ * children, r = softmax(logits[cur] / temperature[b]).  The children c of cur are
+ * tried in index order: token x = tokens[c], drafted with probability q(x) =
+ * draft[cur, x],
+ *     accepted when uniforms[c] q(x) < r(x); then cur = c, r anew;
+ *     rejected: r <- max(r - q, 0) / sum max(r - q, 0) (r stays where nothing
+ *     is left of it).
+ * draft NULL: the children are deterministic, q is the one-hot of x.  After the
+ * last rejection, or at a leaf, next = argmax_v r(v) / noise[b, v], with
+ * exponential variates noise a sample of r; the lowest index wins a tie.
+ * Temperature 0: x is accepted when it is the argmax of the logits (the lowest
+ * index of a tie), next is that argmax.  Outputs: path [batch, nodes] = accepted
+ * nodes from node 0 on, then -1; accepted [batch] their number; next [batch].
+ * A row of logits without a distribution (a NaN, +inf, or no value above -inf)
+ * ends the sequence with next = -1.  A token id outside the vocabulary is never
+ * accepted and sets error 11 in *err. */
+typedef struct {
+    int64_t batch, nodes, vocab;
+    const void* logits;
+    int64_t logits_dtype, logits_stride[2];
+    const void* draft;
+    int64_t draft_dtype, draft_stride[2];
+    const int64_t* tokens;
+    int64_t tokens_stride;
+    const int* parents;
+    int64_t parents_stride;
+    const float* uniforms;
+    int64_t uniforms_stride;
+    const float* noise;
+    int64_t noise_stride;
+    const float* temperature; /* NULL: 1 */
+    int* path;
+    int* accepted;
+    int64_t* next;
+} SparkTreeVerify;
+SPARK_API int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

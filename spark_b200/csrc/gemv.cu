@@ -1745,7 +1745,11 @@ int spark_workspace_check(void* workspace, void* stream) {
     if (flag != 0) {
         cudaMemsetAsync(workspace, 0, sizeof(int), s);
         return set_error(SPARK_ERR_DEVICE, "a kernel reported error %d (%s)", flag,
-                         flag == 7 ? "embedding id out of range" : "bounded wait expired");
+                         flag == 7    ? "embedding id out of range"
+                         : flag == 8  ? "position outside the rotary table"
+                         : flag == 9  ? "page, length or index outside the cache"
+                         : flag == 11 ? "token id outside the vocabulary"
+                                      : "bounded wait expired");
     }
     return SPARK_OK;
 }

@@ -1,0 +1,105 @@
+// kv_cache.cu -- append of new tokens to a paged K/V cache.
+//
+// Position n of sequence b is row n % page_size of page page_table[b, n /
+// page_size].  The kernel moves rows of kv_heads x head_dim values; its bound
+// is HBM (each value is read and written once).
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace spark {
+namespace kv {
+
+struct Params {
+    SparkPagedCache c;
+    const void *k, *v;
+    int64_t ks[3], vs[3];
+    int64_t batch, tokens, width;
+    const int *index, *counts;
+    int *new_lens, *err;
+    int elem;   // bytes of a value
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Params p) {
+    const int64_t b = blockIdx.y;
+    const int64_t len = p.c.lens[b];
+    const int64_t room = p.c.max_pages * p.c.page_size - len;
+    int64_t n = p.counts ? p.counts[b] : p.width;
+    bool bad = n < 0 || n > p.width || len < 0 || n > room;
+    if (len < 0) n = 0;
+    n = n < 0 ? 0 : n;
+    n = n > p.width ? p.width : n;
+    n = n > room ? (room < 0 ? 0 : room) : n;
+    const int row = (int)(p.c.kv_heads * p.c.head_dim);
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.new_lens[b] = (int)(len + n);
+    for (int64_t j = blockIdx.x; j < n; j += gridDim.x) {
+        const int64_t src = p.index ? p.index[b * p.width + j] : j, at = len + j;
+        const int64_t page = p.c.page_table[b * p.c.page_table_stride + at / p.c.page_size];
+        if (src < 0 || src >= p.tokens || page < 0 || page >= p.c.pages) {
+            bad = true;
+            continue;
+        }
+        const int64_t r = at % p.c.page_size;
+        for (int i = threadIdx.x; i < row; i += blockDim.x) {
+            const int64_t h = i / p.c.head_dim, d = i % p.c.head_dim;
+            reinterpret_cast<T*>(p.c.k)[page * p.c.k_stride[0] + r * p.c.k_stride[1] + h * p.c.k_stride[2] + d] =
+                reinterpret_cast<const T*>(p.k)[b * p.ks[0] + src * p.ks[1] + h * p.ks[2] + d];
+            reinterpret_cast<T*>(p.c.v)[page * p.c.v_stride[0] + r * p.c.v_stride[1] + h * p.c.v_stride[2] + d] =
+                reinterpret_cast<const T*>(p.v)[b * p.vs[0] + src * p.vs[1] + h * p.vs[2] + d];
+        }
+    }
+    if (bad && threadIdx.x == 0) report_device_error(p.err, 9);
+}
+
+}  // namespace kv
+
+// The checks that every call on a paged cache makes.
+int check_cache(const SparkPagedCache* c, const char* who) {
+    SPARK_REQUIRE(c, SPARK_ERR_INVALID, "%s: null pointer", who);
+    SPARK_REQUIRE(c->pages >= 1 && c->pages < (1ll << 31) && c->page_size >= 1 && c->page_size < (1 << 24) &&
+                      c->kv_heads >= 1 && c->kv_heads < (1 << 16) && c->head_dim >= 1 && c->head_dim < (1 << 16) &&
+                      c->max_pages >= 0 && c->page_table_stride >= 0,
+                  SPARK_ERR_INVALID, "%s: bad cache size", who);
+    SPARK_REQUIRE(c->max_pages * c->page_size < (1ll << 31), SPARK_ERR_INVALID,
+                  "%s: a sequence's pages hold 2^31 tokens or more", who);
+    SPARK_REQUIRE(c->dtype >= 0 && c->dtype <= 2, SPARK_ERR_INVALID, "%s: bad dtype %d", who, (int)c->dtype);
+    return SPARK_OK;
+}
+
+}  // namespace spark
+
+extern "C" {
+
+int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens, const void* k, const int64_t* k_stride,
+                    const void* v, const int64_t* v_stride, const int* index, int64_t width, const int* counts,
+                    int* new_lens, int* err, void* stream) {
+    using namespace spark;
+    using namespace spark::kv;
+    const int rc = check_cache(cache, "spark_kv_append");
+    if (rc) return rc;
+    SPARK_REQUIRE(batch >= 0 && batch < 65536 && tokens >= 0 && width >= 0, SPARK_ERR_INVALID,
+                  "spark_kv_append: bad size (at most 65535 sequences)");
+    SPARK_REQUIRE(index || width == tokens, SPARK_ERR_INVALID, "spark_kv_append: without an index, width is tokens");
+    if (batch == 0) return SPARK_OK;
+    SPARK_REQUIRE(new_lens && new_lens != cache->lens, SPARK_ERR_INVALID,
+                  "spark_kv_append: new_lens is null or lens itself");
+    SPARK_REQUIRE(cache->k && cache->v && cache->lens && (cache->page_table || cache->max_pages == 0), SPARK_ERR_INVALID,
+                  "spark_kv_append: null pointer in the cache");
+    SPARK_REQUIRE((k && v && k_stride && v_stride) || width == 0, SPARK_ERR_INVALID, "spark_kv_append: null pointer");
+    Params p{};
+    p.c = *cache;
+    p.k = k, p.v = v;
+    for (int i = 0; i < 3 && k_stride && v_stride; ++i) p.ks[i] = k_stride[i], p.vs[i] = v_stride[i];
+    p.batch = batch, p.tokens = tokens, p.width = width, p.index = index, p.counts = counts;
+    p.new_lens = new_lens, p.err = err;
+    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(width, 1), 2048), (unsigned)batch);
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (cache->dtype == SPARK_DTYPE_F32)
+        k_kv_append<float><<<grid, 256, 0, s>>>(p);
+    else
+        k_kv_append<uint16_t><<<grid, 256, 0, s>>>(p);
+    return check_launch("spark_kv_append");
+}
+
+}  // extern "C"

@@ -482,7 +482,7 @@ def linear_batch_allreduce(batch: list[BatchOp], op: int, world: int, rank: int,
 
 def check_device_errors(device=None) -> None:
     """Raise if a kernel left an error in a workspace (synchronises)."""
-    for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()):
+    for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()):
         if device is not None and dev != device:
             continue
         call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
@@ -504,3 +504,240 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     out = torch.empty_like(g)
     call("spark_silu_mul", _p(g), _p(u), _p(out), _dt(g), g.numel(), _stream(g))
     return out
+
+
+# ------------------------------------------------------------------ tree decoding
+_tree_ws: dict[tuple[int, int], torch.Tensor] = {}
+_pack_heads = _lib.packer(_lib.SparkRopeHeads)
+_pack_cache = _lib.packer(_lib.SparkPagedCache)
+_pack_attention = _lib.packer(_lib.SparkTreeAttention)
+_pack_verify = _lib.packer(_lib.SparkTreeVerify)
+
+
+def _tree_workspace(device: torch.device, stream: int, nbytes: int = 256) -> torch.Tensor:
+    """Scratch of the tree-decoding calls, one per (device, stream): an error word,
+    then partial results that need no clearing."""
+    key = (device.index, stream)
+    with _ws_lock:
+        buf = _tree_ws.get(key)
+        if buf is None or buf.numel() < nbytes:
+            buf = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+            _tree_ws[key] = buf
+    return buf
+
+
+def _on_gpu(what: str, device: torch.device, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise RuntimeError(f"spark_b200.{what}: {name} must be on {device}, it is on {t.device}")
+
+
+def _unit(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
+         interleaved: bool = False, inverse: bool = False, out=None):
+    """Rotary positions of q [..., tokens, heads, head_dim] and k (the same with its
+    own heads, or None) in one launch (spark_rope): (q', k').  positions: [...,
+    tokens] int32 or int64; table: rotary.rope_table's fp32 [rows, rot_dim], whose
+    width says how much of the head turns.  Pairs are (i, i + rot_dim / 2), or
+    (2 i, 2 i + 1) when interleaved.  inverse turns back (the backward pass).  Up to
+    one leading (batch) dimension; strided views are read in place.  out: (q', k')
+    tensors to write to, q and k themselves among them.  A position outside the
+    table gives a zero row and an error that check_device_errors() raises."""
+    if not q.is_cuda:
+        raise RuntimeError("spark_b200.rope: q must be a CUDA tensor")
+    dev = q.device
+    _on_gpu("rope", dev, k=k, positions=positions, table=table)
+    if q.dim() not in (3, 4) or (k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1])):
+        raise ValueError(f"rope: q and k must be [(batch,) tokens, heads, head_dim] of the same tokens, got "
+                         f"{list(q.shape)} and {None if k is None else list(k.shape)}")
+    if k is not None and k.dtype != q.dtype:
+        raise TypeError(f"rope: q is {q.dtype}, k is {k.dtype}")
+    if positions.shape != q.shape[:-2]:
+        raise ValueError(f"rope: positions are {list(positions.shape)}, the tokens {list(q.shape[:-2])}")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rope: positions must be int32 or int64, got {positions.dtype}")
+    if table.dim() != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise TypeError("rope: table must be a contiguous float32 [rows, rot_dim]")
+    dt = _dt(q)
+    batch, tokens = (1, q.shape[0]) if q.dim() == 3 else q.shape[:2]
+    parts, outs = [], []
+    for i, x in enumerate((q, k)):
+        if x is None:
+            parts.append(None)
+            outs.append(None)
+            continue
+        x = _unit(x)
+        y = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out[i]
+        if y.shape != x.shape or y.dtype != x.dtype or y.device != dev or y.stride(-1) != 1:
+            raise ValueError("rope: out must have the shapes, type and device of q and k, with unit stride along the head")
+        xs, ys = x.stride(), y.stride()
+        if len(xs) == 3:
+            xs, ys = (0, *xs), (0, *ys)
+        parts.append(_pack_heads(x.data_ptr(), y.data_ptr(), x.shape[-2], *xs[:3], *ys[:3]))
+        outs.append(y)
+    pos = positions.contiguous()
+    s = torch.cuda.current_stream(dev).cuda_stream
+    ws = _tree_workspace(dev, s)
+    call("spark_rope", parts[0], parts[1], dt, batch, tokens, q.shape[-1], table.shape[1], int(interleaved),
+         int(inverse), pos.data_ptr(), pos.element_size(), table.data_ptr(), table.shape[0], ws.data_ptr(), s)
+    return outs[0], outs[1]
+
+
+def _cache_args(what: str, k_cache, v_cache, page_table, lens, dtype) -> tuple:
+    """The values of a SparkPagedCache after its checks."""
+    dev = k_cache.device
+    if not k_cache.is_cuda:
+        raise RuntimeError(f"spark_b200.{what}: the cache must be on a CUDA device")
+    _on_gpu(what, dev, v_cache=v_cache, page_table=page_table, context_lens=lens)
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError(f"{what}: k_cache and v_cache must be [pages, page_size, kv_heads, head_dim] with unit stride "
+                         "along the head")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise TypeError(f"{what}: the cache is {k_cache.dtype} and {v_cache.dtype}, the tokens are {dtype}")
+    if (page_table.dtype != torch.int32 or lens.dtype != torch.int32 or page_table.dim() != 2
+            or page_table.stride(1) != 1 or not lens.is_contiguous() or lens.shape != page_table.shape[:1]):
+        raise TypeError(f"{what}: page_table must be int32 [batch, max_pages], context_lens a contiguous int32 [batch]")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    pages, page_size, heads, dim = k_cache.shape
+    return (k_cache.data_ptr(), v_cache.data_ptr(), *ks[:3], *vs[:3], pages, page_size, heads, dim,
+            page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
+            lens.data_ptr(), _DT[dtype])
+
+
+def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+              page_table: torch.Tensor, context_lens: torch.Tensor, index: torch.Tensor | None = None,
+              counts: torch.Tensor | None = None) -> torch.Tensor:
+    """Writes K/V rows of new tokens [batch, tokens, kv_heads, head_dim] into the paged
+    cache [pages, page_size, kv_heads, head_dim] behind each sequence's context_lens
+    tokens (spark_kv_append) and returns the new lengths (int32 [batch], a new tensor).
+    index (int32 [batch, n]): which tokens, in order, e.g. tree_verify's path; counts
+    (int32 [batch]): how many of them.  Without both, all tokens go in.  What does not
+    fit a sequence's pages is left out and reported by check_device_errors()."""
+    if k_new.dim() != 4 or k_new.shape != v_new.shape or k_new.shape[2:] != k_cache.shape[2:]:
+        raise ValueError(f"kv_append: k_new and v_new must be [batch, tokens, {', '.join(map(str, k_cache.shape[2:]))}], "
+                         f"got {list(k_new.shape)} and {list(v_new.shape)}")
+    if k_new.dtype not in _DT or v_new.dtype != k_new.dtype:
+        raise TypeError(f"kv_append: float32, bfloat16 or float16 tokens, got {k_new.dtype} and {v_new.dtype}")
+    cache = _cache_args("kv_append", k_cache, v_cache, page_table, context_lens, k_new.dtype)
+    dev = k_cache.device
+    _on_gpu("kv_append", dev, k_new=k_new, v_new=v_new, index=index, counts=counts)
+    batch, tokens = k_new.shape[:2]
+    if context_lens.shape[0] != batch:
+        raise ValueError(f"kv_append: {batch} sequences of tokens, {context_lens.shape[0]} in the page table")
+    width = tokens
+    if index is not None:
+        if index.dtype != torch.int32 or index.dim() != 2 or index.shape[0] != batch:
+            raise TypeError("kv_append: index must be int32 [batch, n]")
+        index, width = index.contiguous(), index.shape[1]
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (batch,) or not counts.is_contiguous()):
+        raise TypeError("kv_append: counts must be a contiguous int32 [batch]")
+    k, v = _unit(k_new), _unit(v_new)
+    new_lens = torch.empty(batch, dtype=torch.int32, device=dev)
+    strides = (ctypes.c_int64 * 6)(*k.stride()[:3], *v.stride()[:3])
+    s = torch.cuda.current_stream(dev).cuda_stream
+    ws = _tree_workspace(dev, s)
+    at = ctypes.addressof(strides)
+    call("spark_kv_append", _pack_cache(*cache), batch, tokens, k.data_ptr(), at, v.data_ptr(), at + 24,
+         index.data_ptr() if index is not None else None, width, counts.data_ptr() if counts is not None else None,
+         new_lens.data_ptr(), ws.data_ptr(), s)
+    return new_lens
+
+
+def tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, page_table: torch.Tensor, context_lens: torch.Tensor,
+                   parents: torch.Tensor, scale: float | None = None, out: torch.Tensor | None = None,
+                   return_lse: bool = False):
+    """Attention of up to 64 drafted tokens per sequence (a tree) over the paged cache
+    and over the tree itself (spark_tree_attention).  q [batch, nodes, q_heads,
+    head_dim], k_tree / v_tree [batch, nodes, kv_heads, head_dim] (not in the cache),
+    the cache [pages, page_size, kv_heads, head_dim], page_table int32 [batch,
+    max_pages], context_lens int32 [batch], parents int32 [batch, nodes] or [nodes]:
+    -1 hangs a node on the context, j < i node i on node j, -2 marks it unused (a zero
+    row).  Each node sees the context, itself and its ancestors.  scale defaults to
+    head_dim ** -0.5.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
+    also the natural log of the softmax sums, fp32 [batch, nodes, q_heads]."""
+    if not q.is_cuda:
+        raise RuntimeError("spark_b200.tree_attention: q must be a CUDA tensor")
+    if q.dim() != 4 or k_tree.dim() != 4 or k_tree.shape != v_tree.shape or k_tree.shape[:2] != q.shape[:2]:
+        raise ValueError(f"tree_attention: q must be [batch, nodes, q_heads, head_dim], k_tree and v_tree the same with "
+                         f"kv_heads, got {list(q.shape)}, {list(k_tree.shape)}, {list(v_tree.shape)}")
+    if k_tree.shape[2:] != k_cache.shape[2:] or q.shape[3] != k_tree.shape[3]:
+        raise ValueError("tree_attention: q, k_tree, v_tree and the cache differ in heads or head_dim")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_tree.dtype != q.dtype or v_tree.dtype != q.dtype:
+        raise TypeError(f"tree_attention: bfloat16 or float16 throughout, got {q.dtype}, {k_tree.dtype}, {v_tree.dtype}")
+    cache = _cache_args("tree_attention", k_cache, v_cache, page_table, context_lens, q.dtype)
+    dev = q.device
+    _on_gpu("tree_attention", dev, k_cache=k_cache, k_tree=k_tree, v_tree=v_tree, parents=parents)
+    batch, nodes, heads, dim = q.shape
+    if context_lens.shape[0] != batch:
+        raise ValueError(f"tree_attention: {batch} sequences of queries, {context_lens.shape[0]} in the page table")
+    if parents.dtype != torch.int32 or parents.shape not in ((nodes,), (batch, nodes)):
+        raise TypeError(f"tree_attention: parents must be int32 [{nodes}] or [{batch}, {nodes}]")
+    parents = _unit(parents)
+    q, k, v = _unit(q), _unit(k_tree), _unit(v_tree)
+    y = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
+    if y.shape != q.shape or y.dtype != q.dtype or y.device != dev or y.stride(3) != 1:
+        raise ValueError("tree_attention: out must have q's shape, type and device, with unit stride along the head")
+    lse = torch.empty(batch, nodes, heads, dtype=torch.float32, device=dev) if return_lse else None
+    a = _pack_attention(*cache, batch, nodes, heads, q.data_ptr(), k.data_ptr(), v.data_ptr(), y.data_ptr(),
+                        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *y.stride()[:3], parents.data_ptr(),
+                        parents.stride(0) if parents.dim() == 2 else 0, lse.data_ptr() if return_lse else 0,
+                        dim ** -0.5 if scale is None else scale)
+    s = torch.cuda.current_stream(dev).cuda_stream
+    ws = _tree_workspace(dev, s, int(_lib.lib().spark_tree_attention_workspace_size(a)))
+    call("spark_tree_attention", a, ws.data_ptr(), ws.numel(), s)
+    return (y, lse) if return_lse else y
+
+
+def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, uniforms: torch.Tensor,
+                noise: torch.Tensor, draft_probs: torch.Tensor | None = None,
+                temperature: torch.Tensor | float = 1.0):
+    """Verification of a drafted tree by rejection sampling (spark_tree_verify).
+    logits [batch, nodes, vocab]: the target's at every node; tokens int64 and parents
+    int32 [batch, nodes] (parents also [nodes]); node 0 is the last token already
+    accepted.  uniforms fp32 [batch, nodes] in [0, 1), noise fp32 [batch, vocab]
+    exponential variates.  draft_probs [batch, nodes, vocab]: the distribution that
+    each node's children were sampled from (independently); None for deterministic
+    children.  temperature: a number or fp32 [batch]; 0 takes the argmax.  Returns
+    path int32 [batch, nodes] (accepted nodes from node 0, then -1), accepted int32
+    [batch] (how many) and next int64 [batch], the token after them (-1 where the
+    logits give no distribution)."""
+    if not logits.is_cuda:
+        raise RuntimeError("spark_b200.tree_verify: logits must be a CUDA tensor")
+    dev = logits.device
+    _on_gpu("tree_verify", dev, tokens=tokens, parents=parents, uniforms=uniforms, noise=noise, draft_probs=draft_probs)
+    if logits.dim() != 3:
+        raise ValueError(f"tree_verify: logits must be [batch, nodes, vocab], got {list(logits.shape)}")
+    batch, nodes, vocab = logits.shape
+    if draft_probs is not None and draft_probs.shape != logits.shape:
+        raise ValueError(f"tree_verify: draft_probs are {list(draft_probs.shape)}, logits {list(logits.shape)}")
+    if tokens.shape != (batch, nodes) or uniforms.shape != (batch, nodes) or noise.shape != (batch, vocab):
+        raise ValueError(f"tree_verify: tokens and uniforms must be [{batch}, {nodes}], noise [{batch}, {vocab}]")
+    if tokens.dtype != torch.int64 or uniforms.dtype != torch.float32 or noise.dtype != torch.float32:
+        raise TypeError("tree_verify: tokens must be int64, uniforms and noise float32")
+    if parents.dtype != torch.int32 or parents.shape not in ((nodes,), (batch, nodes)):
+        raise TypeError(f"tree_verify: parents must be int32 [{nodes}] or [{batch}, {nodes}]")
+    if not isinstance(temperature, torch.Tensor):
+        temperature = None if temperature == 1.0 else torch.full((batch,), float(temperature), device=dev)
+    elif temperature.dtype != torch.float32 or temperature.shape != (batch,) or temperature.device != dev:
+        raise TypeError(f"tree_verify: temperature must be a number or float32 [{batch}] on {dev}")
+    x, d = _unit(logits), _unit(draft_probs) if draft_probs is not None else None
+    tokens, parents, uniforms, noise = _unit(tokens), _unit(parents), _unit(uniforms), _unit(noise)
+    if temperature is not None:
+        temperature = temperature.contiguous()
+    path = torch.empty(batch, nodes, dtype=torch.int32, device=dev)
+    accepted = torch.empty(batch, dtype=torch.int32, device=dev)
+    last = torch.empty(batch, dtype=torch.int64, device=dev)
+    a = _pack_verify(batch, nodes, vocab, x.data_ptr(), _dt(x), *x.stride()[:2], d.data_ptr() if d is not None else 0,
+                     _dt(d) if d is not None else 0, *(d.stride()[:2] if d is not None else (0, 0)),
+                     tokens.data_ptr(), tokens.stride(0), parents.data_ptr(),
+                     parents.stride(0) if parents.dim() == 2 else 0, uniforms.data_ptr(), uniforms.stride(0),
+                     noise.data_ptr(), noise.stride(0), temperature.data_ptr() if temperature is not None else 0,
+                     path.data_ptr(), accepted.data_ptr(), last.data_ptr())
+    s = torch.cuda.current_stream(dev).cuda_stream
+    ws = _tree_workspace(dev, s)
+    call("spark_tree_verify", a, ws.data_ptr(), s)
+    return path, accepted, last
