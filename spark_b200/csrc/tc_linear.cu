@@ -800,6 +800,18 @@ int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64
     return SPARK_OK;
 }
 
+int encode_4d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t* dims,
+              const uint64_t* stride_bytes, const uint32_t* box, CUtensorMapSwizzle sw) {
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+    const cuuint64_t st[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+    const cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = g_encode(map, dt, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(SPARK_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return SPARK_OK;
+}
+
 int sm_count_cached(int dev) {
     static int cnt[64] = {};
     if (dev < 0 || dev >= 64) return 148;

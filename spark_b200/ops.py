@@ -536,6 +536,13 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _tma(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it where the kernels' 16-byte loads do not fit its address or strides."""
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 and s >= 0 for s, n in zip(t.stride()[:-1], t.shape) if n > 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
          interleaved: bool = False, inverse: bool = False, out=None):
     """Rotary positions of q [..., tokens, heads, head_dim] and k (the same with its
@@ -657,7 +664,8 @@ def tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, 
     max_pages], context_lens int32 [batch], parents int32 [batch, nodes] or [nodes]:
     -1 hangs a node on the context, j < i node i on node j, -2 marks it unused (a zero
     row).  Each node sees the context, itself and its ancestors.  scale defaults to
-    head_dim ** -0.5.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
+    head_dim ** -0.5, it must be positive.  page_size and head_dim (up to 256) must be
+    multiples of 8.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
     also the natural log of the softmax sums, fp32 [batch, nodes, q_heads]."""
     if not q.is_cuda:
         raise RuntimeError("spark_b200.tree_attention: q must be a CUDA tensor")
@@ -677,7 +685,7 @@ def tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, 
     if parents.dtype != torch.int32 or parents.shape not in ((nodes,), (batch, nodes)):
         raise TypeError(f"tree_attention: parents must be int32 [{nodes}] or [{batch}, {nodes}]")
     parents = _unit(parents)
-    q, k, v = _unit(q), _unit(k_tree), _unit(v_tree)
+    q, k, v = _tma(q), _tma(k_tree), _tma(v_tree)
     y = torch.empty(q.shape, dtype=q.dtype, device=dev) if out is None else out
     if y.shape != q.shape or y.dtype != q.dtype or y.device != dev or y.stride(3) != 1:
         raise ValueError("tree_attention: out must have q's shape, type and device, with unit stride along the head")
