@@ -14,24 +14,31 @@
 // as those below 1 -- since a rescale is a round trip of O through registers.
 //
 // Work: an item is (sequence, kv head, tile of rows), its tiles are the context
-// in steps of kTok tokens and last the tree.  All tiles of all items form one
+// in steps of 128 tokens (64 for heads above 128 wide) and last the tree.  All tiles of all items form one
 // sequence cut into equal contiguous ranges, one per CTA (one CTA per SM), so
 // that ragged batches and single long sequences fill the GPU alike without the
 // host knowing the lengths.  Where a range cuts an item, the parts leave O, m
-// and l in the workspace and a second kernel adds them in order: the result
-// does not depend on timing.
+// and l in the workspace; once all parts of an item are there (the launch is
+// cooperative, all CTAs run at the same time and end their ranges at about the
+// same time) its CTAs add them, each a share of the values, in the CTAs' order:
+// the result does not depend on timing.
 //
-// Roles (320 threads):
-//   warps 0-3, 4-7  softmax: two groups, a thread owns one row (TMEM lane).  Up
-//                   to 128 rows: both groups have the same rows and take tiles in
-//                   turn, each with its own m, l and O, added at the end of the
-//                   item.  Above: group g has rows 128 g.. of the item's 256 and
-//                   takes every tile.  Heads above 128 wide leave room for one O
-//                   only: group 0 works alone on tiles of 64 tokens.
-//                   A group writes its weights over the scores they came from (the
+// Roles (384 threads):
+//   warps 0-3, 4-7  softmax: two groups (streams), a thread owns one row (TMEM
+//                   lane).  Up to 128 rows (whole nodes): both groups have the same
+//                   rows and take tiles in turn, each with its own m, l and O, added
+//                   at the end of the item.  Above: group g has its own rows, the
+//                   item's g-th 128, and takes every tile.  Heads above 128 wide leave room for
+//                   one O only: group 0 works alone, on two score buffers in turn.
+//                   The group writes its weights over the scores they came from (the
 //                   A operand of the second product is read from TMEM).
-//   warp 8          loads K and V tiles by TMA, page by page, into a ring of slots.
-//   warp 9          allocates TMEM and issues the MMAs.
+//   warps 8, 9      load K and V tiles by TMA, page by page, each into a ring of
+//                   slots of its own.
+//   warp 11         loads Q, the next item's while the last one still ends.
+//   warp 10         allocates TMEM and issues the MMAs.  It and the loaders run whole
+//                   and elect a lane for each instruction, so that the operands stay
+//                   in uniform registers: under a branch on the lane an MMA took 110
+//                   cycles to issue and a load 500, more than they take to run.
 // Every wait is bounded (2 s); one that expires sets error 10 and all roles end.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -55,31 +62,32 @@ int sm_count_cached(int dev);
 namespace ta {
 using namespace tcx;
 
-constexpr int kThreads = 320;
-constexpr int kTmaWarp = 8, kMmaWarp = 9;
-constexpr int kMaxSlots = 12;
+constexpr int kThreads = 384;
+constexpr int kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kQWarp = 11;
+constexpr int kMaxSlots = 12;   // of one ring
 constexpr int kHeader = 3072;   // barriers and the exchange of the two groups
 constexpr uint32_t kTmemCols = 512;
 
 // DP: head_dim padded to 64, 128 or 256.
 template <int DP>
 struct Cfg {
-    static constexpr int kTok = DP == 256 ? 64 : 128;      // tokens of a tile
     static constexpr bool kOne = DP == 256;                // one O, one softmax group
+    static constexpr int kTok = kOne ? 64 : 128;           // tokens of a tile
     static constexpr int kChunks = DP / 64;                // 128-byte columns of a tile
     static constexpr int kSlotBytes = kTok * DP * 2;       // 16 or 32 KB
     static constexpr int kQBytes = 128 * DP * 2;           // one 128-row Q tile
-    static constexpr uint32_t kSCol = kTok;                // columns of one S buffer
-    static constexpr uint32_t kOCol = 256;                 // first column of O
-    static constexpr int kRowTile = kOne ? 128 : 256;      // most rows of an item
+    static constexpr uint32_t kOCol = 256;                 // first column of O; before it two S buffers
 };
 
 struct Params {
     SparkTreeAttention a;
     int* err;
-    float* part;            // [2 * grid][rows][DP] O of cut items
+    float4* part;           // [2 * grid][DP / 4][rows] O of cut items
     float2* part_ml;        // [2 * grid][rows] their m, l
-    int rows_total, rows_item, row_tiles, group, box_rows, slots, by_rows;
+    int* count;             // [grid][2] warps that left their part of the item cut first in a CTA, that added it
+    int rows_item, row_tiles, group, box_rows, by_rows, tok, per_seq;   // per_seq: items of a sequence
+    int tile_nodes, item_nodes;   // nodes of a 128-row tile, of an item (two tiles by_rows)
+    int slots[2];           // of K, of V
     float scale;            // times log2 e
 };
 
@@ -101,28 +109,26 @@ __device__ __forceinline__ int context_len(const Params& p, int64_t b) {
     return (int)(len < 0 ? 0 : (len > room ? room : len));
 }
 
-__device__ __forceinline__ int64_t tiles_of(const Params& p, int64_t b, int tok) {
-    return b < p.a.batch ? (context_len(p, b) + tok - 1) / tok + 1 : 0;
+// (tiles of all items are below 2^31: the host checks it by the longest context the pages hold)
+__device__ __forceinline__ int tiles_of(const Params& p, int b) {
+    return b < (int)p.a.batch ? (context_len(p, b) + p.tok - 1) / p.tok + 1 : 0;
 }
 // Number of tiles of all items, by one warp.
-__device__ __forceinline__ int64_t count_tiles(const Params& p, int tok, int lane) {
-    int64_t total = 0;
-    for (int64_t b = lane; b < p.a.batch; b += 32) total += tiles_of(p, b, tok);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    return total * p.a.cache.kv_heads * p.row_tiles;
+__device__ __forceinline__ int count_tiles(const Params& p, int lane) {
+    int total = 0;
+    for (int b = lane; b < (int)p.a.batch; b += 32) total += tiles_of(p, b);
+    return (int)__reduce_add_sync(0xffffffffu, (unsigned)total) * p.per_seq;
 }
 // The sequence that holds tile `pos` of all, and the tile's place among its tiles, by one warp.
-__device__ __forceinline__ void locate(const Params& p, int tok, int lane, int64_t pos, int64_t& b, int64_t& off) {
-    const int64_t per = p.a.cache.kv_heads * p.row_tiles;
-    int64_t at = 0;
-    b = p.a.batch, off = 0;
-    for (int64_t base = 0; base < p.a.batch; base += 32) {
-        const int64_t n = tiles_of(p, base + lane, tok) * per;
-        int64_t sum = n;
+__device__ __forceinline__ void locate(const Params& p, int lane, int pos, int& b, int& off) {
+    int at = 0;
+    b = (int)p.a.batch, off = 0;
+    for (int base = 0; base < (int)p.a.batch; base += 32) {
+        const int n = tiles_of(p, base + lane) * p.per_seq;
+        int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += v;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && pos < at + sum);
@@ -138,40 +144,70 @@ __device__ __forceinline__ void locate(const Params& p, int tok, int lane, int64
 
 // A run of tiles of one item.
 struct Segment {
-    int64_t b;
-    int head, rt, t0, t1, tiles, len;   // tiles t0..t1-1 of `tiles`; the last is the tree
+    int b, head, rt, t0, t1, tiles, len;   // tiles t0..t1-1 of `tiles`; the last is the tree
 };
 
-// Walks the CTA's range of tiles.
-template <int TOK>
+// Walks `left` tiles from place `off` of sequence b on.
 struct Walker {
     const Params& p;
-    int64_t b, off, left;
-    __device__ Walker(const Params& q, int64_t b0, int64_t off0, int64_t n) : p(q), b(b0), off(off0), left(n) {}
+    int b, off, left;
+    __device__ Walker(const Params& q, int b0, int off0, int n) : p(q), b(b0), off(off0), left(n) {}
     __device__ bool next(Segment& s) {
-        if (left <= 0 || b >= p.a.batch) return false;
+        if (left <= 0 || b >= (int)p.a.batch) return false;
         s.len = context_len(p, b);
-        s.tiles = (s.len + TOK - 1) / TOK + 1;
-        const int item = (int)(off / s.tiles);
+        s.tiles = (s.len + p.tok - 1) / p.tok + 1;
+        const int item = off / s.tiles;
         s.b = b;
         s.head = item / p.row_tiles;
         s.rt = item - s.head * p.row_tiles;
-        s.t0 = (int)(off - (int64_t)item * s.tiles);
-        s.t1 = (int)min((int64_t)s.tiles, s.t0 + left);
+        s.t0 = off - item * s.tiles;
+        s.t1 = min(s.tiles, s.t0 + left);
         off += s.t1 - s.t0;
         left -= s.t1 - s.t0;
-        if (off == (int64_t)s.tiles * p.a.cache.kv_heads * p.row_tiles) off = 0, ++b;
+        if (off == s.tiles * p.per_seq) off = 0, ++b;
         return true;
     }
 };
 
-template <int DP>
+// A bounded wait that reads the clock only every 64 tries.
+__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity) {
+    uint64_t deadline = 0;
+    for (int i = 1;; ++i) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 63) == 0) {
+            const uint64_t now = globaltimer_ns();
+            if (deadline == 0) deadline = now + kWaitNs;
+            if (now > deadline) return false;
+        }
+    }
+}
+
+// 64 consecutive entries of a sequence's page table in a warp's registers, the
+// later half loaded ahead of its use: a load's page number costs no round trip
+// to memory (that alone was 0.8 us per K or V tile).
+struct Pages {
+    const int* table;
+    int n, base, cur, nxt;
+    __device__ int entry(int i) const { return i < n ? table[i] : 0; }
+    __device__ void start(const int* t, int entries, int first, int lane) {
+        table = t, n = entries, base = first;
+        cur = entry(base + lane), nxt = entry(base + 32 + lane);
+    }
+    // makes entries first .. first + 32 available
+    __device__ void advance(int first, int lane) {
+        while (first >= base + 32) base += 32, cur = nxt, nxt = entry(base + 32 + lane);
+    }
+    __device__ int at(int i) const {   // every lane of the warp, i within the window
+        const int o = i - base, a = __shfl_sync(0xffffffffu, cur, o & 31), b = __shfl_sync(0xffffffffu, nxt, o & 31);
+        return o < 32 ? a : b;
+    }
+};
+
 struct Smem {
-    uint64_t full[kMaxSlots], empty[kMaxSlots];
-    uint64_t q_full, s_full[2], p_full[2], pv_done, merge, done;
-    int64_t b0, off0, count;
+    uint64_t full[2][kMaxSlots], empty[2][kMaxSlots];   // [K, V]
+    uint64_t q_full, q_free, s_full[2], p_full[2], pv_done[2], merge, done, ended;   // [score buffer], pv_done [stream]
     uint32_t tmem;
-    int bad_v;               // the segment whose tree values hold an infinity or NaN
+    int bad_v[2];            // the segment (one of each parity) whose tree values hold an infinity or NaN
     float2 ml[2][128];
 };
 
@@ -183,28 +219,33 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
         : "memory");
 }
-// D (+)= A B, both from shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// D (+)= A B, both from shared memory; the descriptors' high halves are constant
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
 // D (+)= A B, A from TMEM
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t hi, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b_lo), "r"(hi), "r"(idesc), "r"((uint32_t)acc)
         : "memory");
 }
-// N-major B operand, 128-byte swizzle: 64-column chunks `chunk_bytes` apart
-// (leading offset), groups of eight K rows 1024 bytes apart (stride offset).
-__device__ __forceinline__ uint64_t sdesc_mn128(uint32_t addr, uint32_t chunk_bytes) {
-    return (uint64_t)((addr >> 4) & 0x3fffu) | ((uint64_t)(chunk_bytes >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) |
-           ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
 }
+// Halves of a shared-memory operand descriptor, 128-byte swizzle.  Low: address
+// and leading offset; high: stride offset (groups of eight rows 1024 bytes apart),
+// version and swizzle mode.  K-major (Q, K) does not use the leading offset; for
+// N-major V it is the distance of the 64-column chunks.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t chunk_bytes) { return (addr >> 4) | (chunk_bytes >> 4) << 16; }
 // 32 consecutive TMEM columns of this warp's 32 lanes; wait with tmem_wait_ld
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
     uint32_t* r = reinterpret_cast<uint32_t*>(v);
@@ -237,37 +278,160 @@ __device__ __forceinline__ float exp2_approx(float x) {
 }
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
-// Position of V of the i-th tile (of n) in the ring's order: K0 K1 V0 K2 V1 ...
-// where the groups take tiles in turn, K0 V0 K1 V1 ... where both take each.
-__device__ __forceinline__ int v_ordinal(int i, int n, bool by_rows) {
-    return by_rows ? 2 * i + 1 : min(2, n) + i + min(i, max(n - 2, 0));
+__device__ __forceinline__ void add_release(int* p, int v) {
+    asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
+}
+__device__ __forceinline__ int load_acquire(const int* p) {
+    int v;
+    asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+
+// CTAs that get tiles (no more than there are), the first tile of one, and the one that has tile `pos`.
+__device__ __forceinline__ int ctas(int total) { return min(total, (int)gridDim.x); }
+__device__ __forceinline__ int first_tile(int total, int cta) { return (int)((uint64_t)total * cta / (unsigned)ctas(total)); }
+__device__ __forceinline__ int cta_of(int total, int pos) {
+    return (int)(((uint64_t)(pos + 1) * ctas(total) - 1) / (unsigned)total);
+}
+
+// Scores that a row does not see: of 64 from column h on, those of the tree outside its mask, of the context from `valid` on.
+__device__ __forceinline__ void hide(float (&x)[64], bool tree, uint64_t mask, int valid, int h) {
+    const uint64_t sees = tree ? (h ? 0 : mask) : (valid >= 64 ? ~0ull : (valid > 0 ? (1ull << valid) - 1 : 0));
+#pragma unroll
+    for (int e = 0; e < 64; ++e)
+        if (!((sees >> e) & 1)) x[e] = -INFINITY;
+}
+
+// The node and query head of a row of an item, -1 where it has none.
+__device__ __forceinline__ int node_of(const Params& p, const Segment& sg, int row, int& head) {
+    const int in = p.by_rows ? row & 127 : row, t = in / p.group;
+    head = sg.head * p.group + in - t * p.group;
+    const int node = sg.rt * p.item_nodes + (p.by_rows ? (row >> 7) * p.tile_nodes : 0) + t;
+    return t < p.tile_nodes && node < (int)p.a.nodes ? node : -1;
+}
+
+// The sum of an item's parts at U of its values at a time (four columns of a
+// row each), PU parts loaded together: the loads' latency is what this costs.
+template <int DP, bool BF, int U, int PU>
+__device__ __forceinline__ void add_values(const Params& p, const Segment& sg, int c0, int parts, int e0, int step, int n) {
+    const SparkTreeAttention& a = p.a;
+    const int rows = p.rows_item;
+    for (; e0 < n; e0 += U * step) {
+        float top[U], sum[U];
+        float4 o[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) top[k] = -INFINITY, sum[k] = 0.f, o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int q = 0; q < parts; q += PU) {
+            float2 ml[PU][U];
+            float4 v[PU][U];
+#pragma unroll
+            for (int i = 0; i < PU; ++i)
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    const int e = e0 + k * step;
+                    ml[i][k] = make_float2(-INFINITY, 0.f);
+                    v[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (q + i < parts && e < n) {
+                        const size_t slot = (size_t)(2 * (c0 + q + i) + (q + i == 0 ? 1 : 0));
+                        ml[i][k] = __ldcg(p.part_ml + slot * rows + e % rows);
+                        v[i][k] = __ldcg(p.part + slot * (DP / 4) * rows + e);
+                    }
+                }
+#pragma unroll
+            for (int i = 0; i < PU; ++i)
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    if (ml[i][k].y == 0.f) continue;
+                    const float m2 = fmaxf(top[k], ml[i][k].x), g = exp2_approx(ml[i][k].x - m2);
+                    const float f = sum[k] == 0.f ? 0.f : exp2_approx(top[k] - m2);
+                    top[k] = m2;
+                    sum[k] = sum[k] * f + ml[i][k].y * g;
+                    o[k].x = o[k].x * f + v[i][k].x * g, o[k].y = o[k].y * f + v[i][k].y * g;
+                    o[k].z = o[k].z * f + v[i][k].z * g, o[k].w = o[k].w * f + v[i][k].w * g;
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            const int e = e0 + k * step;
+            if (e >= n) break;
+            const int col = e / rows, row = e - col * rows;
+            int head;
+            const int node = node_of(p, sg, row, head);
+            if (node < 0) continue;
+            const float norm = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)sg.b * a.out_stride[0] + node * a.out_stride[1] + head * a.out_stride[2];
+            *reinterpret_cast<uint2*>(out + col * 4) =
+                make_uint2(pack2<BF>(o[k].x * norm, o[k].y * norm), pack2<BF>(o[k].z * norm, o[k].w * norm));
+            if (a.lse && col == 0)
+                a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
+                    sum[k] == 0.f ? -INFINITY : (log2f(sum[k]) + top[k]) * 0.6931471805599453f;
+        }
+    }
+}
+
+// This warp's share of an item that CTAs left in parts, `lo` its first tile of
+// all `total`.
+template <int DP, bool BF>
+__device__ __forceinline__ bool add_parts(const Params& p, int total, int lo, const Segment& sg) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int c0 = cta_of(total, lo), parts = cta_of(total, lo + sg.tiles - 1) - c0 + 1;
+    int* count = p.count + 2 * c0;
+    bool ok = true;
+    if (lane == 0) {
+        uint64_t deadline = 0;
+        for (int i = 1; load_acquire(count) < 8 * parts && ok; ++i)
+            if ((i & 63) == 0) {
+                const uint64_t now = globaltimer_ns();
+                if (deadline == 0) deadline = now + kWaitNs;
+                ok = now <= deadline;
+            }
+    }
+    if (!all_ok(ok)) return false;
+    const int n = p.rows_item * (int)((p.a.cache.head_dim + 3) / 4), step = parts * 256;
+    const int e0 = (((int)blockIdx.x - c0) * 8 + warp) * 32 + lane;
+    if (n <= step) add_values<DP, BF, 1, 8>(p, sg, c0, parts, e0, step, n);
+    else add_values<DP, BF, 4, 2>(p, sg, c0, parts, e0, step, n);
+    // the last warp to end clears the counters for the next call
+    __syncwarp();
+    if (lane == 0) {
+        int old;
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(count + 1) : "memory");
+        if (old == 8 * parts - 1) count[0] = 0, count[1] = 0;
+    }
+    return true;
 }
 
 template <int DP, bool BF>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_tree_attention(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+    k_tree_attention(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                     const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ CUtensorMap ktmap, const __grid_constant__ CUtensorMap vtmap,
                      const __grid_constant__ Params p) {
     using C = Cfg<DP>;
-    constexpr int TOK = C::kTok;
+    constexpr int kTok = C::kTok;
     extern __shared__ __align__(1024) uint8_t smem[];
-    Smem<DP>& sm = *reinterpret_cast<Smem<DP>*>(smem + (size_t)p.slots * C::kSlotBytes + (size_t)(p.by_rows ? 2 : 1) * C::kQBytes);
-    uint8_t* q_smem = smem + (size_t)p.slots * C::kSlotBytes;
+    const bool by_rows = p.by_rows;
+    uint8_t* q_smem = smem + (size_t)(p.slots[0] + p.slots[1]) * C::kSlotBytes;   // after the slots of K and of V
+    Smem& sm = *reinterpret_cast<Smem*>(q_smem + (size_t)(by_rows ? 2 : 1) * C::kQBytes);
     const SparkTreeAttention& a = p.a;
     const SparkPagedCache& c = a.cache;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    asm volatile("griddepcontrol.launch_dependents;");
 
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < p.slots; ++i) mbar_init(smem_u32(&sm.full[i]), 1), mbar_init(smem_u32(&sm.empty[i]), 1);
-        mbar_init(smem_u32(&sm.q_full), 8);
-        for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.p_full[i]), 4);
-        mbar_init(smem_u32(&sm.pv_done), 1);
-        mbar_init(smem_u32(&sm.merge), 8);
-        mbar_init(smem_u32(&sm.done), 1);
-        sm.bad_v = 0;
+    if (warp == kKWarp) {
+        if (lane < kMaxSlots)
+            for (int v = 0; v < 2; ++v) mbar_init(smem_u32(&sm.full[v][lane]), 1), mbar_init(smem_u32(&sm.empty[v][lane]), 1);
+        if (lane == 0) {
+            mbar_init(smem_u32(&sm.q_full), 1);
+            mbar_init(smem_u32(&sm.q_free), 1);
+            mbar_init(smem_u32(&sm.ended), 8);
+            for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.p_full[i]), 4);
+            for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.pv_done[i]), 1);
+            mbar_init(smem_u32(&sm.merge), 8);
+            mbar_init(smem_u32(&sm.done), 1);
+            sm.bad_v[0] = sm.bad_v[1] = 0;
+            if ((smem_u32(smem) & 1023) != 0) report_device_error(p.err, 10);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if ((smem_u32(smem) & 1023) != 0) report_device_error(p.err, 10);
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
@@ -275,304 +439,287 @@ __global__ void __launch_bounds__(kThreads, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    if (warp == 0) {
-        // this CTA's range of the tiles
-        if (blockIdx.x == 0)
-            for (int64_t b = lane; b < a.batch; b += 32)
-                if (c.lens[b] < 0 || c.lens[b] > c.max_pages * c.page_size) report_device_error(p.err, 9);
-        const int64_t total = count_tiles(p, TOK, lane);
-        const int64_t first = total * blockIdx.x / gridDim.x, end = total * (blockIdx.x + 1) / gridDim.x;
-        int64_t b0, off0;
-        locate(p, TOK, lane, first, b0, off0);
-        if (lane == 0) sm.b0 = b0, sm.off0 = off0, sm.count = end - first;
-    }
+    if (warp == 0 && blockIdx.x == 0)
+        for (int64_t b = lane; b < a.batch; b += 32)
+            if (c.lens[b] < 0 || c.lens[b] > c.max_pages * c.page_size) report_device_error(p.err, 9);
+    // this CTA's range of the tiles; every warp finds it for itself
+    const int total = count_tiles(p, lane);
+    const bool idle = (int)blockIdx.x >= ctas(total);
+    const int range0 = idle ? total : first_tile(total, blockIdx.x), range1 = idle ? total : first_tile(total, blockIdx.x + 1);
+    int b0, off0;
+    locate(p, lane, range0, b0, off0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    Walker<TOK> walk(p, sm.b0, sm.off0, (smem_u32(smem) & 1023) ? 0 : sm.count);
-    const bool by_rows = p.by_rows;
+    const int count = (smem_u32(smem) & 1023) ? 0 : range1 - range0;
+    Walker walk(p, b0, off0, count);
     Segment sg;
     bool ok = true;
 
-    if (warp == kTmaWarp) {
+    if (warp == kKWarp || warp == kVWarp) {
         // ------------------------------------------------------------ loads
-        int ring = 0, filled = 0;
+        const int v = warp - kKWarp, slots = p.slots[v], page_size = (int)c.page_size;
+        const uint32_t ring = smem_u32(smem) + (uint32_t)(v ? p.slots[0] : 0) * C::kSlotBytes;
+        const CUtensorMap* ctx_map = v ? &vmap : &kmap;
+        const CUtensorMap* tree_map = v ? &vtmap : &ktmap;
+        int at = 0, filled = 0;
         uint32_t phase = 1;
-        auto load = [&](const Segment& s, int tile, bool values) {
-            const uint32_t slot = smem_u32(smem) + (uint32_t)ring * C::kSlotBytes, bar = smem_u32(&sm.full[ring]);
-            ok = all_ok(mbar_wait(smem_u32(&sm.empty[ring]), phase));
-            if (!ok) return;
-            if (++ring == p.slots) ring = 0, phase ^= 1;
-            ++filled;
-            if (tile == s.tiles - 1) {
-                if (lane == 0) mbar_expect_tx(bar, C::kChunks * 64 * 128);
-                __syncwarp();
-                if (lane < C::kChunks)
-                    tma_load_4d(slot + lane * TOK * 128, values ? &vtmap : &ktmap, lane * 64, s.head, 0, (int)s.b, bar);
-                return;
-            }
-            const int tok0 = tile * TOK, valid = min(TOK, s.len - tok0);
-            const int n = (valid + p.box_rows - 1) / p.box_rows * C::kChunks;
-            if (lane == 0) mbar_expect_tx(bar, (uint32_t)n * p.box_rows * 128);
-            __syncwarp();
-            for (int i = lane; i < n; i += 32) {
-                const int box = i / C::kChunks, chunk = i - box * C::kChunks, tok = tok0 + box * p.box_rows;
-                const int page_at = tok / (int)c.page_size, row = tok - page_at * (int)c.page_size;
-                const int page = c.page_table[s.b * c.page_table_stride + page_at];
-                if (page < 0 || page >= c.pages) report_device_error(p.err, 9);   // the load gives zeros
-                tma_load_4d(slot + (uint32_t)(chunk * TOK + box * p.box_rows) * 128, values ? &vmap : &kmap, chunk * 64,
-                            s.head, row, page, bar);
-            }
-        };
         while (ok && walk.next(sg)) {
-            const int n = sg.t1 - sg.t0;
-            const int ahead = by_rows ? 1 : 2;
-            for (int i = 0; i < min(ahead, n) && ok; ++i) load(sg, sg.t0 + i, false);
-            for (int i = 0; i < n && ok; ++i) {
-                load(sg, sg.t0 + i, true);
-                if (ok && i + ahead < n) load(sg, sg.t0 + i + ahead, false);
+            int page_at = sg.t0 * kTok / page_size, row = sg.t0 * kTok - page_at * page_size;
+            Pages pages;
+            pages.start(c.page_table + (int64_t)sg.b * c.page_table_stride, (sg.len + page_size - 1) / page_size, page_at, lane);
+            for (int tile = sg.t0; tile < sg.t1; ++tile) {
+                const uint32_t bar = smem_u32(&sm.full[v][at]), slot = ring + (uint32_t)at * C::kSlotBytes;
+                ok = all_ok(wait_bar(smem_u32(&sm.empty[v][at]), phase));
+                if (!ok) break;
+                if (++at == slots) at = 0, phase ^= 1;
+                ++filled;
+                if (tile == sg.tiles - 1) {
+                    if (elect_one()) {
+                        mbar_expect_tx(bar, 64 * C::kChunks * 128);
+#pragma unroll
+                        for (int k = 0; k < C::kChunks; ++k)
+                            tma_load_4d(slot + k * kTok * 128, tree_map, k * 64, sg.head, 0, sg.b, bar);
+                    }
+                    __syncwarp();
+                    continue;
+                }
+                const int boxes = (min(kTok, sg.len - tile * kTok) + p.box_rows - 1) / p.box_rows;
+                if (elect_one()) mbar_expect_tx(bar, (uint32_t)(boxes * p.box_rows) * (C::kChunks * 128));
+                __syncwarp();
+                pages.advance(page_at, lane);
+                for (int box = 0; box < boxes; ++box) {
+                    const int page = pages.at(page_at);
+                    if (elect_one()) {
+                        if (page < 0 || page >= c.pages) report_device_error(p.err, 9);   // the load gives zeros
+#pragma unroll
+                        for (int k = 0; k < C::kChunks; ++k)
+                            tma_load_4d(slot + (uint32_t)(k * kTok + box * p.box_rows) * 128, ctx_map, k * 64, sg.head, row, page, bar);
+                    }
+                    __syncwarp();
+                    row += p.box_rows;
+                    if (row == page_size) row = 0, ++page_at;
+                }
             }
         }
         if (!ok)   // a wait expired: let the loads in flight land before the CTA ends
-            for (int i = 0; i < min(filled, p.slots); ++i)
-                mbar_wait(smem_u32(&sm.full[i]), (uint32_t)((filled - 1 - i) / p.slots) & 1);
+            for (int i = 0; i < min(filled, slots); ++i)
+                wait_bar(smem_u32(&sm.full[v][i]), (uint32_t)((filled - 1 - i) / slots) & 1);
+    } else if (warp == kQWarp) {
+        // a tile of Q is the heads of the group of tile_nodes nodes, node by node
+        const uint32_t qb = smem_u32(q_smem), bar = smem_u32(&sm.q_full);
+        const uint32_t bytes = (uint32_t)(p.tile_nodes * p.group) * (C::kChunks * 128);
+        int seg = 0;
+        for (; ok && walk.next(sg); ++seg) {
+            ok = all_ok(seg == 0 || wait_bar(smem_u32(&sm.q_free), (seg - 1) & 1));
+            if (!ok) break;
+            if (elect_one()) {
+                mbar_expect_tx(bar, by_rows ? 2 * bytes : bytes);
+                for (int t = 0; t < (by_rows ? 2 : 1); ++t)
+#pragma unroll
+                    for (int k = 0; k < C::kChunks; ++k)
+                        tma_load_4d(qb + t * C::kQBytes + k * 128 * 128, &qmap, k * 64, sg.head * p.group,
+                                    sg.rt * p.item_nodes + t * p.tile_nodes, sg.b, bar);
+            }
+            __syncwarp();
+        }
+        if (!ok && seg > 0) wait_bar(bar, (seg - 1) & 1);
     } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------ products
         constexpr uint32_t kFmt = BF ? (1u << 7) | (1u << 10) : 0u;
-        constexpr uint32_t kIdescS = (1u << 4) | kFmt | ((uint32_t)(TOK >> 3) << 17) | (8u << 24);
+        constexpr uint32_t kIdescS = (1u << 4) | kFmt | ((uint32_t)(kTok >> 3) << 17) | (8u << 24);
         constexpr uint32_t kIdescO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | (8u << 24);
-        if (lane == 0) {
-            const uint32_t base = smem_u32(smem), qb = smem_u32(q_smem);
-            const int ksteps = (int)(c.head_dim + 15) / 16;
-            int ring = 0, seg = 0;
-            uint32_t phase = 0, p_phase[2] = {0, 0};
-            uint32_t k_slot[2], v_slot, v_bar;
-            // next slot of the ring, once its tile has landed
-            auto take = [&](uint32_t& slot, uint32_t& bar) {
-                slot = base + (uint32_t)ring * C::kSlotBytes;
-                bar = smem_u32(&sm.empty[ring]);
-                ok = mbar_wait(smem_u32(&sm.full[ring]), phase);
-                tc_fence_after();
-                if (++ring == p.slots) ring = 0, phase ^= 1;
-                return ok;
-            };
-            auto scores = [&](int s, int qt, uint32_t slot) {
-                for (int k = 0; k < ksteps; ++k) {
-                    const uint32_t o = (uint32_t)(k & 3) * 32;
-                    mma_ss(tmem + (uint32_t)s * C::kSCol, sdesc_sw128(qb + (uint32_t)qt * C::kQBytes + (k >> 2) * 128 * 128 + o),
-                           sdesc_sw128(slot + (k >> 2) * TOK * 128 + o), kIdescS, k != 0);
-                }
-                mma_commit(smem_u32(&sm.s_full[s]));
-            };
-            auto values = [&](int s, uint32_t slot, int valid, bool acc) {
-                const int n = (valid + 15) / 16;
-                const uint32_t o = tmem + C::kOCol + (C::kOne ? 0u : (uint32_t)s * DP);
-                for (int k = 0; k < n; ++k)
-                    mma_ts(o, tmem + (uint32_t)s * C::kSCol + k * 8, sdesc_mn128(slot + k * 2048, TOK * 128), kIdescO, acc || k);
-            };
-            while (ok && walk.next(sg)) {
-                const int n = sg.t1 - sg.t0;
-                auto valid = [&](int i) {
-                    const int t = sg.t0 + i;
-                    return t == sg.tiles - 1 ? (int)a.nodes : min(TOK, sg.len - t * TOK);
-                };
-                ok = mbar_wait(smem_u32(&sm.q_full), seg & 1);
-                if (!ok) break;
-                tc_fence_after();
-                uint32_t bar;
-                if (by_rows) {
-                    if (!take(k_slot[0], bar)) break;
-                    scores(0, 0, k_slot[0]);
-                    scores(1, 1, k_slot[0]);
-                    mma_commit(bar);
-                    for (int i = 0; i < n && ok; ++i) {
-                        uint32_t k_bar = 0;
-                        if (!take(v_slot, v_bar)) break;
-                        for (int s = 0; s < 2 && ok; ++s) {
-                            ok = mbar_wait(smem_u32(&sm.p_full[s]), p_phase[s]);
-                            p_phase[s] ^= 1;
-                            if (!ok) break;
-                            tc_fence_after();
-                            values(s, v_slot, valid(i), i > 0);
-                            if (s == 1) mma_commit(v_bar);
-                            if (i + 1 < n) {
-                                if (s == 0 && !take(k_slot[0], k_bar)) break;
-                                scores(s, s, k_slot[0]);
-                                if (s == 1) mma_commit(k_bar);
-                            }
-                        }
-                    }
-                } else {
-                    for (int i = 0; i < min(2, n) && ok; ++i) {
-                        if (!take(k_slot[i], bar)) break;
-                        scores(i, 0, k_slot[i]);
-                        mma_commit(bar);
-                    }
-                    for (int i = 0; i < n && ok; ++i) {
-                        const int s = i & 1;
-                        if (!take(v_slot, v_bar)) break;
-                        ok = mbar_wait(smem_u32(&sm.p_full[s]), p_phase[s]);
-                        p_phase[s] ^= 1;
+        const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + (uint32_t)p.slots[0] * C::kSlotBytes, qb = smem_u32(q_smem);
+        const int ksteps = (int)(c.head_dim + 15) / 16;
+        const int streams = by_rows ? 2 : 1;           // that take each tile
+        const int ahead = by_rows ? 1 : 2;             // tiles whose scores come before the first weights
+        int k_at = 0, v_at = 0, seg = 0;
+        uint32_t k_phase = 0, v_phase = 0, p_phase = 0;   // p_phase: a bit for each buffer
+        auto scores = [&](int buf, uint32_t slot) {
+            const uint32_t ql = desc_lo(qb + (by_rows ? (uint32_t)buf * C::kQBytes : 0u), 16), kl = desc_lo(slot, 16);
+            const uint32_t d = tmem + (uint32_t)buf * kTok;
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k)
+                if (k < ksteps)
+                    mma_ss(d, ql + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, kl + (k >> 2) * (kTok * 128 / 16) + (k & 3) * 2,
+                           kDescHi, kIdescS, k != 0);
+            mma_commit(smem_u32(&sm.s_full[buf]));
+        };
+        auto values = [&](int buf, uint32_t slot, int valid, bool acc) {
+            const int s = C::kOne ? 0 : buf;
+            const uint32_t vl = desc_lo(slot, kTok * 128), d = tmem + C::kOCol + (uint32_t)s * DP, w = tmem + (uint32_t)buf * kTok;
+#pragma unroll
+            for (int k = 0; k < kTok / 16; ++k)
+                if (k * 16 < valid) mma_ts(d, w + k * 8, vl + k * (2048 / 16), kDescHi, kIdescO, acc || k);
+            mma_commit(smem_u32(&sm.pv_done[s]));
+        };
+        while (ok && walk.next(sg)) {
+            const int n = sg.t1 - sg.t0;
+            ok = all_ok(wait_bar(smem_u32(&sm.q_full), seg & 1));
+            if (!ok) break;
+            tc_fence_after();
+            // scores run `ahead` tiles ahead of the second products
+            for (int i = -ahead; i < n; ++i) {
+                const bool more = i + ahead < n;
+                const int tile = sg.t0 + i, valid = tile == sg.tiles - 1 ? (int)a.nodes : min(kTok, sg.len - tile * kTok);
+                const uint32_t k_slot = k_ring + (uint32_t)k_at * C::kSlotBytes, v_slot = v_ring + (uint32_t)v_at * C::kSlotBytes;
+                for (int t = 0; t < streams; ++t) {
+                    const int buf = by_rows ? t : i & 1;      // score buffer = stream, but for kOne
+                    if (i >= 0) {
+                        if (t == 0) ok = wait_bar(smem_u32(&sm.full[1][v_at]), v_phase);
+                        ok = all_ok(ok && wait_bar(smem_u32(&sm.p_full[buf]), p_phase >> buf & 1));
+                        p_phase ^= 1u << buf;
                         if (!ok) break;
                         tc_fence_after();
-                        values(s, v_slot, valid(i), C::kOne ? i > 0 : i > 1);
-                        if (C::kOne) mma_commit(smem_u32(&sm.pv_done));
-                        mma_commit(v_bar);
-                        if (i + 2 < n) {
-                            if (!take(k_slot[s], bar)) break;
-                            scores(s, 0, k_slot[s]);
-                            mma_commit(bar);
+                        if (elect_one()) {
+                            values(buf, v_slot, valid, by_rows || C::kOne ? i > 0 : i > 1);
+                            if (t == streams - 1) mma_commit(smem_u32(&sm.empty[1][v_at]));
                         }
+                        __syncwarp();
+                    }
+                    if (more) {
+                        if (t == 0) ok = all_ok(wait_bar(smem_u32(&sm.full[0][k_at]), k_phase));
+                        if (!ok) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+                            scores(buf, k_slot);
+                            if (t == streams - 1) mma_commit(smem_u32(&sm.empty[0][k_at]));
+                            if (t == streams - 1 && i + ahead == n - 1) mma_commit(smem_u32(&sm.q_free));
+                        }
+                        __syncwarp();
                     }
                 }
                 if (!ok) break;
-                mma_commit(smem_u32(&sm.done));
-                ++seg;
+                if (i >= 0 && ++v_at == p.slots[1]) v_at = 0, v_phase ^= 1;
+                if (more && ++k_at == p.slots[0]) k_at = 0, k_phase ^= 1;
             }
-            if (!ok) {   // a wait expired: let the products in flight end before TMEM is freed
-                mma_commit(smem_u32(&sm.done));
-                mbar_wait(smem_u32(&sm.done), seg & 1);
-            }
+            if (!ok) break;
+            if (elect_one()) mma_commit(smem_u32(&sm.done));
+            __syncwarp();
+            ++seg;
+        }
+        if (!ok) {   // a wait expired: let the products in flight end before TMEM is freed
+            if (elect_one()) mma_commit(smem_u32(&sm.done));
+            __syncwarp();
+            wait_bar(smem_u32(&sm.done), seg & 1);
         }
     } else {
         // ------------------------------------------------------------ softmax
-        const int g = warp >> 2, quad = warp & 3, row_in = quad * 32 + lane;   // group, lane quadrant, row = TMEM lane
+        const int g = warp >> 2, quad = warp & 3, row_in = quad * 32 + lane;   // stream, lane quadrant, row = TMEM lane
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const int dim = (int)c.head_dim;
-        int seg = 0, ring0 = 0;          // ring position of the segment's first tile, counted on
-        uint32_t s_phase[2] = {0, 0};
-        int pv = 0;                      // second products so far (kOne)
+        int seg = 0, tile0 = 0;          // tiles of the segments so far: places in the ring of V
+        int j = 0;                       // tiles of this stream so far
+        uint32_t s_phase = 0;            // a bit for each score buffer
         while (ok && walk.next(sg)) {
             const int n = sg.t1 - sg.t0;
-            const int row_base = sg.rt * C::kRowTile;
-            const int rows = min(p.rows_total - row_base, C::kRowTile);   // of this item
-            // Q: rows in the order of nodes, then the heads of the group
-            {
-                const int units = DP / 8, first = by_rows ? g * 128 : 0;
-                const int n_rows = by_rows ? min(max(rows - first, 0), 128) : rows;
-                const int tid = by_rows ? (int)threadIdx.x & 127 : (int)threadIdx.x, nt = by_rows ? 128 : 256;
-                uint8_t* qs = q_smem + (by_rows ? g : 0) * C::kQBytes;
-                for (int i = tid; i < n_rows * units; i += nt) {
-                    const int r = i / units, u = i - r * units, rr = row_base + first + r;
-                    const int t = rr / p.group, h = sg.head * p.group + rr - t * p.group;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (u * 8 < dim)
-                        v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + sg.b * a.q_stride[0] +
-                                                            t * a.q_stride[1] + h * a.q_stride[2] + u * 8);
-                    *reinterpret_cast<uint4*>(qs + (u >> 3) * 128 * 128 + r * 128 + (((u & 7) ^ (r & 7)) << 4)) = v;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&sm.q_full));
-            }
-            // (a group without tiles may not run ahead of the other's last item either)
-            ok = all_ok(mbar_wait(smem_u32(&sm.q_full), seg & 1));
-            if (!ok) break;
             const int row = (by_rows ? g * 128 : 0) + row_in;     // of the item
-            const bool mine = row < rows;
-            const bool work = (by_rows ? g * 128 : 0) + quad * 32 < rows;   // any row of this warp
-            const int node = mine ? (row_base + row) / p.group : 0;
-            const uint64_t mask = mine ? ancestors(a.parents + sg.b * a.parents_stride, node) : 0;
+            int head;
+            const int node = node_of(p, sg, row, head);
+            const bool mine = node >= 0;
+            const bool work = __any_sync(0xffffffffu, mine);
+            const uint64_t mask = mine ? ancestors(a.parents + (int64_t)sg.b * a.parents_stride, node) : 0;
             float m = -INFINITY, l = 0.f;
             int my_tiles = 0;
             if (!(C::kOne && g == 1)) {
                 const int step = by_rows || C::kOne ? 1 : 2;
-                for (int i = by_rows || C::kOne ? 0 : g; i < n; i += step) {
-                    const int s = by_rows ? g : (i & 1);          // S buffer
-                    const int tile = sg.t0 + i;
+                const uint32_t o_t = tmem + lane_off + C::kOCol + (uint32_t)g * DP;
+                for (int i = by_rows ? 0 : g; i < n; i += step) {
+                    const int buf = C::kOne ? i & 1 : g, tile = sg.t0 + i;
                     const bool tree = tile == sg.tiles - 1;
-                    const int valid = tree ? (int)a.nodes : min(TOK, sg.len - tile * TOK);
-                    ok = all_ok(mbar_wait(smem_u32(&sm.s_full[s]), s_phase[s]));
-                    s_phase[s] ^= 1;
+                    const int valid = tree ? (int)a.nodes : min(kTok, sg.len - tile * kTok);
+                    ok = all_ok(wait_bar(smem_u32(&sm.s_full[buf]), s_phase >> buf & 1));
+                    s_phase ^= 1u << buf;
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t st = tmem + lane_off + (uint32_t)s * C::kSCol;
-                    float x[TOK];
+                    const bool masked = tree || valid < kTok;
                     if (work) {
+                        const uint32_t st = tmem + lane_off + (uint32_t)buf * kTok;
+                        // scores are read twice, 64 at a time: kept, 128 would not fit the registers (next to no
+                        // first-level cache is left beside the tiles, a spill costs more than the second read)
+                        float x[64], top = -INFINITY;
+#pragma unroll 1
+                        for (int h = 0; h < kTok; h += 64) {
+                            tmem_ld32(st + h, x);
+                            tmem_ld32(st + h + 32, x + 32);
+                            tmem_wait_ld();
+                            if (masked) hide(x, tree, mask, valid - h, h);
 #pragma unroll
-                        for (int j = 0; j < TOK; j += 32) tmem_ld32(st + j, x + j);
-                        tmem_wait_ld();
-                        if (tree) {
-#pragma unroll
-                            for (int j = 0; j < TOK; ++j)
-                                if (j >= 64 || !((mask >> (j & 63)) & 1)) x[j] = -INFINITY;
-                        } else if (valid < TOK) {
-#pragma unroll
-                            for (int j = 0; j < TOK; ++j)
-                                if (j >= valid) x[j] = -INFINITY;
+                            for (int e = 0; e < 64; ++e) top = fmaxf(top, x[e]);
                         }
-                        float top = x[0];
-#pragma unroll
-                        for (int j = 1; j < TOK; ++j) top = fmaxf(top, x[j]);
                         top *= p.scale;
-                        if (C::kOne && pv > 0) {
-                            ok = all_ok(mbar_wait(smem_u32(&sm.pv_done), (uint32_t)(pv - 1) & 1));
-                            if (!ok) break;
-                            tc_fence_after();
-                        }
                         const bool grow = mine && top > m + 8.f;
                         if (my_tiles == 0) {
                             m = top;
                         } else if (__any_sync(0xffffffffu, grow)) {
+                            // O holds the tiles so far once the last of their products has ended
+                            ok = all_ok(wait_bar(smem_u32(&sm.pv_done[g]), (uint32_t)(j - 1) & 1));
+                            if (!ok) break;
+                            tc_fence_after();
                             const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
                             if (grow) m = top, l *= f;
-                            const uint32_t ot = tmem + lane_off + C::kOCol + (C::kOne ? 0u : (uint32_t)(by_rows ? g : s) * DP);
-#pragma unroll
-                            for (int j = 0; j < DP; j += 32) {
+#pragma unroll 1
+                            for (int e0 = 0; e0 < DP; e0 += 32) {
                                 float o[32];
-                                tmem_ld32(ot + j, o);
+                                tmem_ld32(o_t + e0, o);
                                 tmem_wait_ld();
 #pragma unroll
                                 for (int e = 0; e < 32; ++e) o[e] *= f;
-                                tmem_st16(ot + j, reinterpret_cast<const uint32_t*>(o));
-                                tmem_st16(ot + j + 16, reinterpret_cast<const uint32_t*>(o) + 16);
+                                tmem_st16(o_t + e0, reinterpret_cast<const uint32_t*>(o));
+                                tmem_st16(o_t + e0 + 16, reinterpret_cast<const uint32_t*>(o) + 16);
                             }
                         }
                         const float ref = m == -INFINITY ? 0.f : m;
                         float sum = 0.f;
-#pragma unroll
-                        for (int j = 0; j < TOK; j += 32) {
-                            uint32_t w[16];
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                const float u = exp2_approx(fmaf(x[j + 2 * e], p.scale, -ref));
-                                const float v = exp2_approx(fmaf(x[j + 2 * e + 1], p.scale, -ref));
-                                sum += u + v;
-                                w[e] = pack2<BF>(u, v);
+#pragma unroll 1
+                        for (int h = 0; h < kTok; h += 64) {
+                            if (kTok > 64) {
+                                tmem_ld32(st + h, x);
+                                tmem_ld32(st + h + 32, x + 32);
+                                tmem_wait_ld();
+                                if (masked) hide(x, tree, mask, valid - h, h);
                             }
-                            tmem_st16(st + j / 2, w);
+                            // the weights of h.. take the columns of the scores h / 2.., which are done with
+#pragma unroll
+                            for (int e0 = 0; e0 < 64; e0 += 32) {
+                                uint32_t w[16];
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) {
+                                    const float u = exp2_approx(fmaf(x[e0 + 2 * e], p.scale, -ref));
+                                    const float v = exp2_approx(fmaf(x[e0 + 2 * e + 1], p.scale, -ref));
+                                    sum += u + v;
+                                    w[e] = pack2<BF>(u, v);
+                                }
+                                tmem_st16(st + (h + e0) / 2, w);
+                            }
                         }
                         l += sum;
                         tmem_wait_st();
-                    } else if (C::kOne && pv > 0) {
-                        ok = all_ok(mbar_wait(smem_u32(&sm.pv_done), (uint32_t)(pv - 1) & 1));
-                        if (!ok) break;
                     }
                     ++my_tiles;
-                    ++pv;
+                    ++j;
                     // values that meet weights of zero must be finite: clear what lies behind the context in the last
                     // group of 16, and the infinities and NaN of the tree (added back below)
                     if ((tree || (valid & 15)) && !(by_rows && g == 1)) {
-                        const int at = ring0 + v_ordinal(i, n, by_rows), slot_i = at % p.slots;
-                        ok = all_ok(mbar_wait(smem_u32(&sm.full[slot_i]), (uint32_t)(at / p.slots) & 1));
+                        const int pos = tile0 + i, slot_i = pos % p.slots[1];
+                        ok = all_ok(wait_bar(smem_u32(&sm.full[1][slot_i]), (uint32_t)(pos / p.slots[1]) & 1));
                         if (!ok) break;
-                        uint8_t* slot = smem + (size_t)slot_i * C::kSlotBytes;
+                        uint8_t* slot = smem + (size_t)(p.slots[0] + slot_i) * C::kSlotBytes;
                         const int tid = (int)threadIdx.x & 127;
                         if (!tree) {
                             const int n_rows = ((valid + 15) & ~15) - valid;
                             for (int e = tid; e < n_rows * C::kChunks * 8; e += 128) {
                                 const int r = e / (C::kChunks * 8), u = e % (C::kChunks * 8);
-                                *reinterpret_cast<uint4*>(slot + (u >> 3) * TOK * 128 + (valid + r) * 128 + (u & 7) * 16) =
+                                *reinterpret_cast<uint4*>(slot + (u >> 3) * kTok * 128 + (valid + r) * 128 + (u & 7) * 16) =
                                     make_uint4(0, 0, 0, 0);
                             }
                         } else {
                             constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
                             for (int e = tid; e < valid * C::kChunks * 8; e += 128) {
                                 const int r = e / (C::kChunks * 8), u = e % (C::kChunks * 8);
-                                uint32_t* w = reinterpret_cast<uint32_t*>(slot + (u >> 3) * TOK * 128 + r * 128 + (u & 7) * 16);
-                                uint4 q4 = *reinterpret_cast<uint4*>(w);
+                                uint4* w = reinterpret_cast<uint4*>(slot + (u >> 3) * kTok * 128 + r * 128 + (u & 7) * 16);
+                                const uint4 q4 = *w;
                                 uint32_t v4[4] = {q4.x, q4.y, q4.z, q4.w};
                                 bool hit = false;
 #pragma unroll
@@ -581,101 +728,127 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     if ((v4[k] & kExp & 0xffff0000u) == (kExp & 0xffff0000u)) v4[k] &= 0xffffu, hit = true;
                                 }
                                 if (hit) {
-                                    *reinterpret_cast<uint4*>(w) = make_uint4(v4[0], v4[1], v4[2], v4[3]);
-                                    sm.bad_v = seg + 1;
+                                    *w = make_uint4(v4[0], v4[1], v4[2], v4[3]);
+                                    sm.bad_v[seg & 1] = seg + 1;
                                 }
                             }
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
+                    // the first product of an item starts O anew: all warps have read the last one's
+                    if (my_tiles == 1 && seg > 0) {
+                        ok = all_ok(wait_bar(smem_u32(&sm.ended), (seg - 1) & 1));
+                        if (!ok) break;
+                    }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[s]));
+                    if (lane == 0) mbar_arrive(smem_u32(&sm.p_full[buf]));
                 }
             }
             if (!ok) break;
             // the item's end (or the range's): O of both groups, added
-            if (!by_rows) sm.ml[g][row_in] = make_float2(m, my_tiles ? l : 0.f);
+            if (!by_rows) {
+                ok = all_ok(seg == 0 || wait_bar(smem_u32(&sm.ended), (seg - 1) & 1));
+                if (!ok) break;
+                sm.ml[g][row_in] = make_float2(m, my_tiles ? l : 0.f);
+            }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sm.merge));
-            ok = all_ok(mbar_wait(smem_u32(&sm.merge), seg & 1) && mbar_wait(smem_u32(&sm.done), seg & 1));
+            ok = all_ok(wait_bar(smem_u32(&sm.merge), seg & 1) && wait_bar(smem_u32(&sm.done), seg & 1));
             if (!ok) break;
             tc_fence_after();
             if (work) {
+                const bool whole = n == sg.tiles;
                 float2 ml[2];
                 uint32_t o_col[2];
-                int c0 = 0, c1 = DP;
+                int col0 = 0, col1 = DP;
                 if (by_rows) {
                     ml[0] = make_float2(m, l), ml[1] = make_float2(-INFINITY, 0.f);
-                    o_col[0] = o_col[1] = C::kOCol + (C::kOne ? 0u : (uint32_t)g * DP);
+                    o_col[0] = o_col[1] = C::kOCol + (uint32_t)g * DP;
                 } else {
                     ml[0] = sm.ml[0][row_in], ml[1] = sm.ml[1][row_in];
                     o_col[0] = C::kOCol, o_col[1] = C::kOCol + (C::kOne ? 0u : DP);
-                    c0 = g * (DP / 2), c1 = c0 + DP / 2;           // each group half of the columns
+                    col0 = g * (DP / 2), col1 = col0 + DP / 2;       // each group half of the columns
                 }
                 const float top = fmaxf(ml[0].x, ml[1].x);
-                const float f0 = ml[0].y == 0.f ? 0.f : exp2_approx(ml[0].x - top);
-                const float f1 = ml[1].y == 0.f ? 0.f : exp2_approx(ml[1].x - top);
+                float f0 = ml[0].y == 0.f ? 0.f : exp2_approx(ml[0].x - top);
+                float f1 = ml[1].y == 0.f ? 0.f : exp2_approx(ml[1].x - top);
                 const float sum = mask ? ml[0].y * f0 + ml[1].y * f1 : 0.f;
-                const bool whole = n == sg.tiles;
-                const float norm = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
                 const bool second = __any_sync(0xffffffffu, f1 != 0.f);
-                const bool fix = sm.bad_v == seg + 1;
-                const int slot = 2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0);
-                float* part = p.part + ((size_t)slot * p.rows_item + row) * DP;
-                const int head = sg.head * p.group + (row_base + row) - node * p.group;
-                uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + sg.b * a.out_stride[0] + node * a.out_stride[1] +
+                if (whole) {
+                    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+                    f0 *= norm, f1 *= norm;
+                }
+                const bool fix = sm.bad_v[seg & 1] == seg + 1;
+                float4* part = p.part + (size_t)(2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0)) * (DP / 4) * p.rows_item + row;
+                uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)sg.b * a.out_stride[0] + node * a.out_stride[1] +
                                 head * a.out_stride[2];
-                const uint16_t* tv = reinterpret_cast<const uint16_t*>(a.v) + sg.b * a.vn_stride[0] + sg.head * a.vn_stride[2];
-                for (int j = c0; j < c1 && j < dim; j += 16) {
-                    float o[16];
-                    tmem_ld16(tmem + lane_off + o_col[0] + j, o);
+                const uint16_t* tv = reinterpret_cast<const uint16_t*>(a.v) + (int64_t)sg.b * a.vn_stride[0] + sg.head * a.vn_stride[2];
+#pragma unroll 1
+                for (int e0 = col0; e0 < col1 && e0 < dim; e0 += 32) {
+                    float o[32], o1[32];
+                    tmem_ld32(tmem + lane_off + o_col[0] + e0, o);
+                    if (second) tmem_ld32(tmem + lane_off + o_col[1] + e0, o1);
+                    tmem_wait_ld();
+                    // (O of a stream without tiles is not defined)
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = f0 == 0.f ? 0.f : o[e] * f0;
+                    for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0.f : o[e] * f0;
                     if (second) {
-                        float o1[16];
-                        tmem_ld16(tmem + lane_off + o_col[1] + j, o1);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] += f1 == 0.f ? 0.f : o1[e] * f1;
+                        for (int e = 0; e < 32; ++e) o[e] += f1 == 0.f ? 0.f : o1[e] * f1;
                     }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = sum == 0.f ? 0.f : o[e] * norm;
                     if (fix) {
                         for (uint64_t left = mask; left; left &= left - 1) {
-                            const int t = __ffsll((long long)left) - 1;
+                            const uint16_t* v = tv + (__ffsll((long long)left) - 1) * a.vn_stride[1] + e0;
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                if (j + e >= dim) continue;
-                                const float v = load_as_float(tv, (int)c.dtype, t * a.vn_stride[1] + j + e);
-                                if (!isfinite(v)) o[e] += v;
+                            for (int e = 0; e < 32; ++e) {
+                                if (e0 + e >= dim) continue;
+                                const uint16_t h = v[e];
+                                if ((h & (BF ? 0x7f80 : 0x7c00)) != (BF ? 0x7f80 : 0x7c00)) continue;
+                                o[e] += BF ? __uint_as_float((uint32_t)h << 16) : __half2float(__ushort_as_half(h));
                             }
                         }
                     }
                     if (!mine) {
                         // a lane without a row only takes part in the loads
                     } else if (whole) {
-                        uint32_t w[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) w[e] = pack2<BF>(o[2 * e], o[2 * e + 1]);
-                        *reinterpret_cast<uint4*>(out + j) = make_uint4(w[0], w[1], w[2], w[3]);
-                        if (j + 8 < dim) *reinterpret_cast<uint4*>(out + j + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                        for (int e = 0; e < 32; e += 8)
+                            if (e0 + e < dim)
+                                *reinterpret_cast<uint4*>(out + e0 + e) =
+                                    make_uint4(pack2<BF>(o[e], o[e + 1]), pack2<BF>(o[e + 2], o[e + 3]),
+                                               pack2<BF>(o[e + 4], o[e + 5]), pack2<BF>(o[e + 6], o[e + 7]));
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            *reinterpret_cast<float4*>(part + j + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                        for (int e = 0; e < 32; e += 4)
+                            part[(size_t)((e0 + e) / 4) * p.rows_item] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                     }
                     __syncwarp();
                 }
-                if (mine && c0 == 0) {
+                if (mine && col0 == 0) {
                     if (!whole)
-                        p.part_ml[(size_t)slot * p.rows_item + row] = make_float2(top, sum);
+                        p.part_ml[(size_t)(2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0)) * p.rows_item + row] = make_float2(top, sum);
                     else if (a.lse)
-                        a.lse[(sg.b * a.nodes + node) * a.q_heads + head] =
+                        a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
                             sum == 0.f ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
                 }
             }
-            ring0 += 2 * n;
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sm.ended));
+            tile0 += n;
             ++seg;
+        }
+        // items in parts, at most the range's first and its last: say that this warp's share is there, then add
+        for (int pass = 0; pass < 2 && ok; ++pass) {
+            Walker again(p, b0, off0, count);
+            for (int at = range0; ok && again.next(sg); at += sg.t1 - sg.t0) {
+                if (sg.t1 - sg.t0 == sg.tiles) continue;
+                const int lo = at - sg.t0;
+                if (pass == 1) ok = add_parts<DP, BF>(p, total, lo, sg);
+                else if (lane == 0) add_release(p.count + 2 * cta_of(total, lo), 1);
+            }
+            __syncwarp();
         }
     }
     if (!ok) report_device_error(p.err, 10);
@@ -685,62 +858,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
-    }
-}
-
-// Adds the parts of the items that several CTAs worked on, in the CTAs' order.
-// Block y stands for the cut between CTAs y and y + 1 of the first kernel (of
-// `grid` CTAs) and does the item it cuts, unless an earlier cut has that item.
-// A warp adds a row.
-constexpr int kCombineRows = 32;
-template <int DP>
-__global__ void __launch_bounds__(256) k_tree_combine(const __grid_constant__ Params p, int grid) {
-    constexpr int TOK = Cfg<DP>::kTok, kRowTile = Cfg<DP>::kRowTile;
-    const SparkTreeAttention& a = p.a;
-    const SparkPagedCache& c = a.cache;
-    const int lane = threadIdx.x & 31;
-    const int64_t total = count_tiles(p, TOK, lane);
-    const int64_t cut = total * (blockIdx.y + 1) / grid;
-    int64_t b, off;
-    locate(p, TOK, lane, cut, b, off);
-    const int64_t tiles = tiles_of(p, b, TOK);
-    const int item = tiles ? (int)(off / tiles) : 0;
-    const int64_t lo = cut - (off - (int64_t)item * tiles), hi = lo + tiles;   // the item's tiles among all
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (b >= a.batch || cut == lo || total * blockIdx.y / grid > lo) return;
-    const int head = item / p.row_tiles, rt = item - head * p.row_tiles;
-    const int c0 = (int)blockIdx.y, c1 = (int)((hi * grid - 1) / total);   // first and last CTA of the item
-    for (int r = threadIdx.x >> 5; r < kCombineRows; r += 8) {
-        const int row = blockIdx.x * kCombineRows + r, rr = rt * kRowTile + row;
-        if (row >= p.rows_item || rr >= p.rows_total) break;
-        float top = -INFINITY, sum = 0.f, o[DP / 32];
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) o[i] = 0.f;
-        for (int cta = c0; cta <= c1; ++cta) {
-            const int64_t first = total * cta / grid;
-            if (first == total * (cta + 1) / grid) continue;
-            const size_t at = (size_t)(2 * cta + (lo >= first ? 1 : 0)) * p.rows_item + row;
-            const float2 ml = p.part_ml[at];
-            if (ml.y == 0.f) continue;
-            const float m2 = fmaxf(top, ml.x), f = top == -INFINITY ? 0.f : exp2_approx(top - m2);
-            const float g = exp2_approx(ml.x - m2);
-            top = m2;
-            sum = sum * f + ml.y * g;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const int d = lane + 32 * i;
-                if (d < c.head_dim) o[i] = (f == 0.f ? 0.f : o[i] * f) + p.part[at * DP + d] * g;
-            }
-        }
-        const int node = rr / p.group, h = head * p.group + rr - node * p.group;
-        const int64_t out = b * a.out_stride[0] + node * a.out_stride[1] + h * a.out_stride[2];
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) {
-            const int d = lane + 32 * i;
-            if (d < c.head_dim) store_from_float(a.out, (int)c.dtype, out + d, sum == 0.f ? 0.f : o[i] / sum);
-        }
-        if (a.lse && lane == 0)
-            a.lse[(b * a.nodes + node) * a.q_heads + h] = sum == 0.f ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
     }
 }
 
@@ -758,6 +875,9 @@ int check(const SparkTreeAttention* a) {
                   "spark_tree_attention: bf16 or f16");
     SPARK_REQUIRE(a->cache.head_dim % 8 == 0 && a->cache.head_dim <= 256, SPARK_ERR_UNSUPPORTED,
                   "spark_tree_attention: head_dim %lld is no multiple of 8 up to 256", (long long)a->cache.head_dim);
+    SPARK_REQUIRE(a->q_heads / a->cache.kv_heads <= 128, SPARK_ERR_UNSUPPORTED,
+                  "spark_tree_attention: %lld query heads per kv head, at most 128",
+                  (long long)(a->q_heads / a->cache.kv_heads));
     SPARK_REQUIRE(a->cache.page_size % 8 == 0, SPARK_ERR_UNSUPPORTED,
                   "spark_tree_attention: page_size %lld is no multiple of 8", (long long)a->cache.page_size);
     SPARK_REQUIRE(a->scale > 0 && a->scale < 1e30, SPARK_ERR_INVALID, "spark_tree_attention: scale must be positive");
@@ -768,8 +888,8 @@ int padded_dim(int64_t d) { return d <= 64 ? 64 : (d <= 128 ? 128 : 256); }
 
 // Sizes that follow from the shapes alone; the workspace's layout.
 struct Plan {
-    int dp, grid, rows_total, rows_item, row_tiles;
-    size_t part, part_ml, bytes;
+    int dp, grid, group, by_rows, tile_nodes, item_nodes, rows_item, row_tiles;
+    size_t count, part, part_ml, bytes;
 };
 Plan plan(const SparkTreeAttention* a) {
     Plan q;
@@ -777,11 +897,14 @@ Plan plan(const SparkTreeAttention* a) {
     cudaGetDevice(&dev);
     q.grid = tc::sm_count_cached(dev);
     q.dp = padded_dim(a->cache.head_dim);
-    const int tile = q.dp == 256 ? 128 : 256;
-    q.rows_total = (int)(a->nodes * (a->q_heads / a->cache.kv_heads));
-    q.row_tiles = (q.rows_total + tile - 1) / tile;
-    q.rows_item = std::min(q.rows_total, tile);
-    q.part_ml = 256;
+    q.group = (int)(a->q_heads / a->cache.kv_heads);
+    q.tile_nodes = std::min(128 / q.group, (int)a->nodes);
+    q.by_rows = q.dp < 256 && q.tile_nodes < a->nodes;
+    q.item_nodes = q.by_rows ? 2 * q.tile_nodes : q.tile_nodes;
+    q.row_tiles = (int)((a->nodes + q.item_nodes - 1) / q.item_nodes);
+    q.rows_item = q.by_rows ? 256 : q.tile_nodes * q.group;
+    q.count = 256;
+    q.part_ml = (q.count + (size_t)2 * q.grid * sizeof(int) + 255) / 256 * 256;
     q.part = (q.part_ml + (size_t)2 * q.grid * q.rows_item * sizeof(float2) + 255) / 256 * 256;
     q.bytes = q.part + (size_t)2 * q.grid * q.rows_item * q.dp * sizeof(float);
     return q;
@@ -794,50 +917,53 @@ int launch(const SparkTreeAttention* a, const Plan& q, uint8_t* ws, cudaStream_t
     Params p;
     p.a = *a;
     p.err = reinterpret_cast<int*>(ws);
-    p.part = reinterpret_cast<float*>(ws + q.part);
+    p.count = reinterpret_cast<int*>(ws + q.count);
+    p.part = reinterpret_cast<float4*>(ws + q.part);
     p.part_ml = reinterpret_cast<float2*>(ws + q.part_ml);
-    p.rows_total = q.rows_total, p.rows_item = q.rows_item, p.row_tiles = q.row_tiles;
-    p.group = (int)(a->q_heads / c.kv_heads);
-    p.by_rows = !C::kOne && q.rows_total > 128;
+    p.rows_item = q.rows_item, p.row_tiles = q.row_tiles, p.group = q.group;
+    p.by_rows = q.by_rows, p.tile_nodes = q.tile_nodes, p.item_nodes = q.item_nodes;
     p.scale = (float)(a->scale * 1.4426950408889634);
     // a box of a TMA load lies within a page and within a tile
+    p.tok = C::kTok;
+    p.per_seq = (int)c.kv_heads * q.row_tiles;
     p.box_rows = 8;
     while (p.box_rows < C::kTok && c.page_size % (2 * p.box_rows) == 0) p.box_rows *= 2;
     const int q_tiles = p.by_rows ? 2 : 1;
-    p.slots = std::min(kMaxSlots, (232448 - kHeader - q_tiles * C::kQBytes) / C::kSlotBytes);
-    const size_t smem = (size_t)p.slots * C::kSlotBytes + (size_t)q_tiles * C::kQBytes + kHeader;
-    static_assert(sizeof(Smem<DP>) <= kHeader, "shared header");
+    const int slots = std::min(2 * kMaxSlots, (232448 - kHeader - q_tiles * C::kQBytes) / C::kSlotBytes);
+    p.slots[0] = slots / 2, p.slots[1] = slots - slots / 2;
+    const size_t smem = (size_t)slots * C::kSlotBytes + (size_t)q_tiles * C::kQBytes + kHeader;
+    static_assert(sizeof(Smem) <= kHeader, "shared header");
 
     int rc = tc::get_encoder();
     if (rc) return rc;
-    CUtensorMap map[4];
+    CUtensorMap map[5];
     const CUtensorMapDataType dt = BF ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    for (int i = 0; i < 4; ++i) {
-        const bool tree = i >= 2, v = i & 1;
-        const int64_t* st = tree ? (v ? a->vn_stride : a->kn_stride) : (v ? c.v_stride : c.k_stride);   // outer, row, head
-        const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.kv_heads, (uint64_t)(tree ? a->nodes : c.page_size),
-                                  (uint64_t)(tree ? a->batch : c.pages)};
+    auto encode = [&](CUtensorMap* m, const void* base, int64_t heads, int64_t rows, int64_t outer, const int64_t* st, int box_heads,
+                      int box_rows) {
+        const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)heads, (uint64_t)rows, (uint64_t)outer};
         const uint64_t strides[3] = {(uint64_t)st[2] * 2, (uint64_t)st[1] * 2, (uint64_t)st[0] * 2};
-        const uint32_t box[4] = {64, 1, (uint32_t)(tree ? 64 : p.box_rows), 1};
-        rc = tc::encode_4d(&map[i], dt, tree ? (v ? a->v : a->k) : (v ? c.v : c.k), dims, strides, box,
-                           CU_TENSOR_MAP_SWIZZLE_128B);
-        if (rc) return rc;
-    }
+        const uint32_t box[4] = {64, (uint32_t)box_heads, (uint32_t)box_rows, 1};
+        return tc::encode_4d(m, dt, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    rc = encode(&map[0], a->q, a->q_heads, a->nodes, a->batch, a->q_stride, q.group, q.tile_nodes);
+    if (!rc) rc = encode(&map[1], c.k, c.kv_heads, c.page_size, c.pages, c.k_stride, 1, p.box_rows);
+    if (!rc) rc = encode(&map[2], c.v, c.kv_heads, c.page_size, c.pages, c.v_stride, 1, p.box_rows);
+    if (!rc) rc = encode(&map[3], a->k, c.kv_heads, a->nodes, a->batch, a->kn_stride, 1, 64);
+    if (!rc) rc = encode(&map[4], a->v, c.kv_heads, a->nodes, a->batch, a->vn_stride, 1, 64);
+    if (rc) return rc;
     cudaError_t e = cudaFuncSetAttribute(k_tree_attention<DP, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
     if (e != cudaSuccess) return set_error((int)e, "spark_tree_attention: %s", cudaGetErrorString(e));
-    k_tree_attention<DP, BF><<<q.grid, kThreads, smem, s>>>(map[0], map[1], map[2], map[3], p);
-    rc = check_launch("spark_tree_attention");
-    if (rc) return rc;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((q.rows_item + kCombineRows - 1) / kCombineRows), (unsigned)(q.grid - 1));
-    cfg.blockDim = dim3(256);
+    cfg.gridDim = dim3((unsigned)q.grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[0].id = cudaLaunchAttributeCooperative;
+    at[0].val.cooperative = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_tree_combine<DP>, p, q.grid);
+    e = cudaLaunchKernelEx(&cfg, k_tree_attention<DP, BF>, map[0], map[1], map[2], map[3], map[4], p);
     if (e != cudaSuccess) return set_error((int)e, "spark_tree_attention: launch failed: %s", cudaGetErrorString(e));
     return check_launch("spark_tree_attention");
 }
@@ -879,6 +1005,9 @@ int spark_tree_attention(const SparkTreeAttention* args, void* workspace, size_t
     SPARK_REQUIRE(a->q && a->k && a->v && a->out && a->parents && c.k && c.v && c.lens && (c.page_table || c.max_pages == 0),
                   SPARK_ERR_INVALID, "spark_tree_attention: null pointer");
     const Plan q = plan(a);
+    const int tok = q.dp == 256 ? 64 : 128;
+    SPARK_REQUIRE((double)a->batch * c.kv_heads * q.row_tiles * ((double)c.max_pages * c.page_size / tok + 2) < 2147483647.0,
+                  SPARK_ERR_UNSUPPORTED, "spark_tree_attention: 2^31 tiles of %d tokens or more", tok);
     SPARK_REQUIRE(workspace && workspace_bytes >= q.bytes, SPARK_ERR_WORKSPACE,
                   "spark_tree_attention: the workspace has %zu of %zu bytes", workspace_bytes, q.bytes);
     bool al = aligned(workspace, 256);

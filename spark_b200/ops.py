@@ -485,7 +485,12 @@ def check_device_errors(device=None) -> None:
     for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()):
         if device is not None and dev != device:
             continue
-        call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
+        try:
+            call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
+        except _lib.SparkError:
+            if _tree_ws.get((dev, sh)) is buf:
+                buf.zero_()    # an expired wait may leave its counters behind
+            raise
 
 
 def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
@@ -665,7 +670,7 @@ def tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, 
     -1 hangs a node on the context, j < i node i on node j, -2 marks it unused (a zero
     row).  Each node sees the context, itself and its ancestors.  scale defaults to
     head_dim ** -0.5, it must be positive.  page_size and head_dim (up to 256) must be
-    multiples of 8.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
+    multiples of 8, q_heads at most 128 times kv_heads.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
     also the natural log of the softmax sums, fp32 [batch, nodes, q_heads]."""
     if not q.is_cuda:
         raise RuntimeError("spark_b200.tree_attention: q must be a CUDA tensor")
