@@ -87,6 +87,7 @@ struct Params {
     int* count;             // [grid][2] warps that left their part of the item cut first in a CTA, that added it
     int rows_item, row_tiles, group, box_rows, by_rows, tok, per_seq;   // per_seq: items of a sequence
     int tile_nodes, item_nodes;   // nodes of a 128-row tile, of an item (two tiles by_rows)
+    float inv_group, inv_rows;    // 1 / group, 1 / rows_item: (n + 0.5) times them is exact enough to divide n < 2^16
     int slots[2];           // of K, of V
     float scale;            // times log2 e
 };
@@ -203,10 +204,18 @@ struct Pages {
     }
 };
 
+// An item that this CTA has a part of, with CTAs c0 .. c0 + parts - 1.
+struct Cut {
+    Segment sg;
+    int c0, parts;
+};
+
 struct Smem {
     uint64_t full[2][kMaxSlots], empty[2][kMaxSlots];   // [K, V]
-    uint64_t q_full, q_free, s_full[2], p_full[2], pv_done[2], merge, done, ended;   // [score buffer], pv_done [stream]
+    uint64_t q_full, q_free, s_full[2], p_full[2], pv_done, merge, done, ended, cuts_known;   // [score buffer]; pv_done: kOne
     uint32_t tmem;
+    int cuts;                // items in parts: at most the range's first and its last
+    Cut cut[2];
     int bad_v[2];            // the segment (one of each parity) whose tree values hold an infinity or NaN
     float2 ml[2][128];
 };
@@ -276,6 +285,41 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+// 2^t for t <= 8 on the FMA pipe: t = j + f, |f| <= 1/2, a polynomial of degree 4
+// in f with value 1 at 0 whose largest relative error on the interval is smallest
+// (2.9e-6, fitted by linear programming), and j added to its exponent.  At and
+// below -127 the result is exactly 0: 1.0 loses all of its exponent.  The
+// exponential unit gives 16 results a clock to an SM, this is what the row of 128
+// weights waits for, so that a part of them is computed here.
+__device__ __forceinline__ float2 exp2_poly(float2 t) {
+    const float kRound = 12582912.f;   // 1.5 2^23: the sum's low bits are the nearest integer
+    t = make_float2(fmaxf(t.x, -127.f), fmaxf(t.y, -127.f));
+    const float2 z = add2(t, make_float2(kRound, kRound));
+    const float2 f = add2(t, fma2(z, make_float2(-1.f, -1.f), make_float2(kRound, kRound)));
+    float2 q = fma2(f, make_float2(0.00958538242f, 0.00958538242f), make_float2(0.0559066273f, 0.0559066273f));
+    q = fma2(q, f, make_float2(0.24024038f, 0.24024038f));
+    q = fma2(q, f, make_float2(0.693124175f, 0.693124175f));
+    q = fma2(q, f, make_float2(1.f, 1.f));
+    return make_float2(__uint_as_float((__float_as_uint(z.x) << 23) + __float_as_uint(q.x)),
+                       __uint_as_float((__float_as_uint(z.y) << 23) + __float_as_uint(q.y)));
+}
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 __device__ __forceinline__ void add_release(int* p, int v) {
@@ -304,78 +348,15 @@ __device__ __forceinline__ void hide(float (&x)[64], bool tree, uint64_t mask, i
 
 // The node and query head of a row of an item, -1 where it has none.
 __device__ __forceinline__ int node_of(const Params& p, const Segment& sg, int row, int& head) {
-    const int in = p.by_rows ? row & 127 : row, t = in / p.group;
+    const int in = p.by_rows ? row & 127 : row, t = (int)((in + 0.5f) * p.inv_group);
     head = sg.head * p.group + in - t * p.group;
     const int node = sg.rt * p.item_nodes + (p.by_rows ? (row >> 7) * p.tile_nodes : 0) + t;
     return t < p.tile_nodes && node < (int)p.a.nodes ? node : -1;
 }
 
-// The sum of an item's parts at U of its values at a time (four columns of a
-// row each), PU parts loaded together: the loads' latency is what this costs.
-template <int DP, bool BF, int U, int PU>
-__device__ __forceinline__ void add_values(const Params& p, const Segment& sg, int c0, int parts, int e0, int step, int n) {
-    const SparkTreeAttention& a = p.a;
-    const int rows = p.rows_item;
-    for (; e0 < n; e0 += U * step) {
-        float top[U], sum[U];
-        float4 o[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) top[k] = -INFINITY, sum[k] = 0.f, o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int q = 0; q < parts; q += PU) {
-            float2 ml[PU][U];
-            float4 v[PU][U];
-#pragma unroll
-            for (int i = 0; i < PU; ++i)
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    const int e = e0 + k * step;
-                    ml[i][k] = make_float2(-INFINITY, 0.f);
-                    v[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (q + i < parts && e < n) {
-                        const size_t slot = (size_t)(2 * (c0 + q + i) + (q + i == 0 ? 1 : 0));
-                        ml[i][k] = __ldcg(p.part_ml + slot * rows + e % rows);
-                        v[i][k] = __ldcg(p.part + slot * (DP / 4) * rows + e);
-                    }
-                }
-#pragma unroll
-            for (int i = 0; i < PU; ++i)
-#pragma unroll
-                for (int k = 0; k < U; ++k) {
-                    if (ml[i][k].y == 0.f) continue;
-                    const float m2 = fmaxf(top[k], ml[i][k].x), g = exp2_approx(ml[i][k].x - m2);
-                    const float f = sum[k] == 0.f ? 0.f : exp2_approx(top[k] - m2);
-                    top[k] = m2;
-                    sum[k] = sum[k] * f + ml[i][k].y * g;
-                    o[k].x = o[k].x * f + v[i][k].x * g, o[k].y = o[k].y * f + v[i][k].y * g;
-                    o[k].z = o[k].z * f + v[i][k].z * g, o[k].w = o[k].w * f + v[i][k].w * g;
-                }
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int e = e0 + k * step;
-            if (e >= n) break;
-            const int col = e / rows, row = e - col * rows;
-            int head;
-            const int node = node_of(p, sg, row, head);
-            if (node < 0) continue;
-            const float norm = sum[k] == 0.f ? 0.f : 1.f / sum[k];
-            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)sg.b * a.out_stride[0] + node * a.out_stride[1] + head * a.out_stride[2];
-            *reinterpret_cast<uint2*>(out + col * 4) =
-                make_uint2(pack2<BF>(o[k].x * norm, o[k].y * norm), pack2<BF>(o[k].z * norm, o[k].w * norm));
-            if (a.lse && col == 0)
-                a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
-                    sum[k] == 0.f ? -INFINITY : (log2f(sum[k]) + top[k]) * 0.6931471805599453f;
-        }
-    }
-}
-
-// This warp's share of an item that CTAs left in parts, `lo` its first tile of
-// all `total`.
-template <int DP, bool BF>
-__device__ __forceinline__ bool add_parts(const Params& p, int total, int lo, const Segment& sg) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int c0 = cta_of(total, lo), parts = cta_of(total, lo + sg.tiles - 1) - c0 + 1;
-    int* count = p.count + 2 * c0;
+// Waits until all parts of an item are there, and says that this warp knows.
+// The last warp to know clears the counters for the next call.
+__device__ __forceinline__ bool await_parts(int* count, int parts, int lane) {
     bool ok = true;
     if (lane == 0) {
         uint64_t deadline = 0;
@@ -385,20 +366,78 @@ __device__ __forceinline__ bool add_parts(const Params& p, int total, int lo, co
                 if (deadline == 0) deadline = now + kWaitNs;
                 ok = now <= deadline;
             }
+        if (ok && atomicAdd(count + 1, 1) == 8 * parts - 1) count[0] = 0, count[1] = 0;
     }
-    if (!all_ok(ok)) return false;
-    const int n = p.rows_item * (int)((p.a.cache.head_dim + 3) / 4), step = parts * 256;
-    const int e0 = (((int)blockIdx.x - c0) * 8 + warp) * 32 + lane;
-    if (n <= step) add_values<DP, BF, 1, 8>(p, sg, c0, parts, e0, step, n);
-    else add_values<DP, BF, 4, 2>(p, sg, c0, parts, e0, step, n);
-    // the last warp to end clears the counters for the next call
-    __syncwarp();
-    if (lane == 0) {
-        int old;
-        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(old) : "l"(count + 1) : "memory");
-        if (old == 8 * parts - 1) count[0] = 0, count[1] = 0;
+    return all_ok(ok);
+}
+
+// This warp's share of the sum of an item's parts.  A lane adds four columns of
+// four rows at a time, four parts loaded together: the loads' latency is what
+// this costs.
+template <int DP, bool BF>
+__device__ __forceinline__ void add_parts(const Params& p, const Segment& sg, int c0, int parts) {
+    const SparkTreeAttention& a = p.a;
+    constexpr int U = 4, PU = 4;
+    const int rows = p.rows_item, n = rows * (int)((a.cache.head_dim + 3) / 4), step = parts * 256;
+#pragma unroll 1
+    for (int e0 = ((int)blockIdx.x - c0) * 256 + (int)threadIdx.x; e0 < n; e0 += U * step) {
+        float top[U], sum[U];
+        float4 o[U];
+        int row[U], col[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            top[k] = -INFINITY, sum[k] = 0.f, o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            col[k] = (int)((e0 + k * step + 0.5f) * p.inv_rows);
+            row[k] = e0 + k * step - col[k] * rows;
+        }
+#pragma unroll 1
+        for (int q = 0; q < parts; q += PU) {
+            float2 ml[PU][U];
+            float4 v[PU][U];
+#pragma unroll
+            for (int i = 0; i < PU; ++i)
+#pragma unroll
+                for (int k = 0; k < U; ++k) {
+                    ml[i][k] = make_float2(-INFINITY, 0.f);
+                    v[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (q + i < parts && e0 + k * step < n) {
+                        const int slot = 2 * (c0 + q + i) + (q + i == 0 ? 1 : 0);
+                        ml[i][k] = __ldcg(p.part_ml + slot * rows + row[k]);
+                        v[i][k] = __ldcg(p.part + (slot * (DP / 4) + col[k]) * rows + row[k]);
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                float m2 = top[k];
+#pragma unroll
+                for (int i = 0; i < PU; ++i) m2 = ml[i][k].y == 0.f ? m2 : fmaxf(m2, ml[i][k].x);
+                const float f = sum[k] == 0.f ? 0.f : exp2_approx(top[k] - m2);
+                top[k] = m2;
+                sum[k] *= f;
+                o[k].x *= f, o[k].y *= f, o[k].z *= f, o[k].w *= f;
+#pragma unroll
+                for (int i = 0; i < PU; ++i) {
+                    const float g = ml[i][k].y == 0.f ? 0.f : exp2_approx(ml[i][k].x - m2);
+                    sum[k] += ml[i][k].y * g;
+                    if (g == 0.f) v[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);   // (an infinity of no weight)
+                    o[k].x += v[i][k].x * g, o[k].y += v[i][k].y * g, o[k].z += v[i][k].z * g, o[k].w += v[i][k].w * g;
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+            int head;
+            const int node = e0 + k * step < n ? node_of(p, sg, row[k], head) : -1;
+            if (node < 0) continue;
+            const float norm = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+            uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)sg.b * a.out_stride[0] + node * a.out_stride[1] + head * a.out_stride[2];
+            *reinterpret_cast<uint2*>(out + col[k] * 4) =
+                make_uint2(pack2<BF>(o[k].x * norm, o[k].y * norm), pack2<BF>(o[k].z * norm, o[k].w * norm));
+            if (a.lse && col[k] == 0)
+                a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
+                    sum[k] == 0.f ? -INFINITY : (log2f(sum[k]) + top[k]) * 0.6931471805599453f;
+        }
     }
-    return true;
 }
 
 template <int DP, bool BF>
@@ -423,15 +462,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             mbar_init(smem_u32(&sm.q_full), 1);
             mbar_init(smem_u32(&sm.q_free), 1);
+            mbar_init(smem_u32(&sm.cuts_known), 1);
             mbar_init(smem_u32(&sm.ended), 8);
             for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.s_full[i]), 1), mbar_init(smem_u32(&sm.p_full[i]), 4);
-            for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sm.pv_done[i]), 1);
+            mbar_init(smem_u32(&sm.pv_done), 1);
             mbar_init(smem_u32(&sm.merge), 8);
             mbar_init(smem_u32(&sm.done), 1);
             sm.bad_v[0] = sm.bad_v[1] = 0;
             if ((smem_u32(smem) & 1023) != 0) report_device_error(p.err, 10);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (lane == 0 && warp >= kKWarp) {
+        const CUtensorMap* mine = warp == kKWarp ? &kmap : warp == kVWarp ? &vmap : warp == kQWarp ? &qmap : &ktmap;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(mine) : "memory");
+        if (warp == kMmaWarp) asm volatile("prefetch.tensormap [%0];" ::"l"(&vtmap) : "memory");
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)),
@@ -510,8 +555,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a tile of Q is the heads of the group of tile_nodes nodes, node by node
         const uint32_t qb = smem_u32(q_smem), bar = smem_u32(&sm.q_full);
         const uint32_t bytes = (uint32_t)(p.tile_nodes * p.group) * (C::kChunks * 128);
-        int seg = 0;
+        int seg = 0, cuts = 0, at = range0;
         for (; ok && walk.next(sg); ++seg) {
+            if (sg.t1 - sg.t0 < sg.tiles) {
+                const int lo = at - sg.t0, c0 = cta_of(total, lo), c1 = cta_of(total, lo + sg.tiles - 1);
+                if (lane == 0) sm.cut[cuts] = Cut{sg, c0, c1 - c0 + 1};
+                ++cuts;
+            }
+            at += sg.t1 - sg.t0;
             ok = all_ok(seg == 0 || wait_bar(smem_u32(&sm.q_free), (seg - 1) & 1));
             if (!ok) break;
             if (elect_one()) {
@@ -524,35 +575,41 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncwarp();
         }
+        if (lane == 0) {
+            sm.cuts = cuts;
+            mbar_arrive(smem_u32(&sm.cuts_known));
+        }
         if (!ok && seg > 0) wait_bar(bar, (seg - 1) & 1);
     } else if (warp == kMmaWarp) {
         // ------------------------------------------------------------ products
         constexpr uint32_t kFmt = BF ? (1u << 7) | (1u << 10) : 0u;
         constexpr uint32_t kIdescS = (1u << 4) | kFmt | ((uint32_t)(kTok >> 3) << 17) | (8u << 24);
         constexpr uint32_t kIdescO = (1u << 4) | kFmt | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | (8u << 24);
-        const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + (uint32_t)p.slots[0] * C::kSlotBytes, qb = smem_u32(q_smem);
-        const int ksteps = (int)(c.head_dim + 15) / 16;
+        const int ksteps = (int)(c.head_dim + 15) / 16, k_slots = p.slots[0], v_slots = p.slots[1];
         const int streams = by_rows ? 2 : 1;           // that take each tile
         const int ahead = by_rows ? 1 : 2;             // tiles whose scores come before the first weights
+        const uint32_t k_ring = desc_lo(smem_u32(smem), 16), v_ring = desc_lo(smem_u32(smem) + (uint32_t)k_slots * C::kSlotBytes, kTok * 128);
+        const uint32_t q_lo = desc_lo(smem_u32(q_smem), 16);
+        const uint32_t k_full = smem_u32(&sm.full[0][0]), v_full = smem_u32(&sm.full[1][0]);
+        const uint32_t k_empty = smem_u32(&sm.empty[0][0]), v_empty = smem_u32(&sm.empty[1][0]);
+        const uint32_t s_full = smem_u32(&sm.s_full[0]), p_full = smem_u32(&sm.p_full[0]);
         int k_at = 0, v_at = 0, seg = 0;
         uint32_t k_phase = 0, v_phase = 0, p_phase = 0;   // p_phase: a bit for each buffer
-        auto scores = [&](int buf, uint32_t slot) {
-            const uint32_t ql = desc_lo(qb + (by_rows ? (uint32_t)buf * C::kQBytes : 0u), 16), kl = desc_lo(slot, 16);
-            const uint32_t d = tmem + (uint32_t)buf * kTok;
+        auto scores = [&](int buf, uint32_t kl) {
+            const uint32_t ql = q_lo + (by_rows && buf ? C::kQBytes / 16 : 0), d = tmem + (uint32_t)buf * kTok;
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k)
                 if (k < ksteps)
                     mma_ss(d, ql + (k >> 2) * (128 * 128 / 16) + (k & 3) * 2, kl + (k >> 2) * (kTok * 128 / 16) + (k & 3) * 2,
                            kDescHi, kIdescS, k != 0);
-            mma_commit(smem_u32(&sm.s_full[buf]));
+            mma_commit(s_full + 8 * buf);
         };
-        auto values = [&](int buf, uint32_t slot, int valid, bool acc) {
-            const int s = C::kOne ? 0 : buf;
-            const uint32_t vl = desc_lo(slot, kTok * 128), d = tmem + C::kOCol + (uint32_t)s * DP, w = tmem + (uint32_t)buf * kTok;
+        auto values = [&](int buf, uint32_t vl, int valid, bool acc) {
+            const uint32_t d = tmem + C::kOCol + (C::kOne ? 0u : (uint32_t)buf * DP), w = tmem + (uint32_t)buf * kTok;
 #pragma unroll
             for (int k = 0; k < kTok / 16; ++k)
                 if (k * 16 < valid) mma_ts(d, w + k * 8, vl + k * (2048 / 16), kDescHi, kIdescO, acc || k);
-            mma_commit(smem_u32(&sm.pv_done[s]));
+            if (C::kOne) mma_commit(smem_u32(&sm.pv_done));
         };
         while (ok && walk.next(sg)) {
             const int n = sg.t1 - sg.t0;
@@ -561,38 +618,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_after();
             // scores run `ahead` tiles ahead of the second products
             for (int i = -ahead; i < n; ++i) {
-                const bool more = i + ahead < n;
+                const bool more = i + ahead < n, first = i < (by_rows || C::kOne ? 1 : 2);
                 const int tile = sg.t0 + i, valid = tile == sg.tiles - 1 ? (int)a.nodes : min(kTok, sg.len - tile * kTok);
-                const uint32_t k_slot = k_ring + (uint32_t)k_at * C::kSlotBytes, v_slot = v_ring + (uint32_t)v_at * C::kSlotBytes;
+                const uint32_t kl = k_ring + (uint32_t)k_at * (C::kSlotBytes / 16), vl = v_ring + (uint32_t)v_at * (C::kSlotBytes / 16);
+                // K and V are waited for before the weights, where K is not late
+                if (i >= 0) ok = wait_bar(v_full + 8 * v_at, v_phase);
+                bool k_there = more && mbar_try(k_full + 8 * k_at, k_phase);
+                k_there = __all_sync(0xffffffffu, k_there);
                 for (int t = 0; t < streams; ++t) {
                     const int buf = by_rows ? t : i & 1;      // score buffer = stream, but for kOne
                     if (i >= 0) {
-                        if (t == 0) ok = wait_bar(smem_u32(&sm.full[1][v_at]), v_phase);
-                        ok = all_ok(ok && wait_bar(smem_u32(&sm.p_full[buf]), p_phase >> buf & 1));
+                        ok = all_ok(ok && wait_bar(p_full + 8 * buf, p_phase >> buf & 1));
                         p_phase ^= 1u << buf;
                         if (!ok) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-                            values(buf, v_slot, valid, by_rows || C::kOne ? i > 0 : i > 1);
-                            if (t == streams - 1) mma_commit(smem_u32(&sm.empty[1][v_at]));
-                        }
-                        __syncwarp();
                     }
-                    if (more) {
-                        if (t == 0) ok = all_ok(wait_bar(smem_u32(&sm.full[0][k_at]), k_phase));
+                    tc_fence_after();
+                    if (elect_one()) {
+                        if (i >= 0) values(buf, vl, valid, !first);
+                        if (k_there) scores(buf, kl);
+                    }
+                    __syncwarp();
+                    if (more && !k_there) {
+                        k_there = ok = all_ok(wait_bar(k_full + 8 * k_at, k_phase));
                         if (!ok) break;
                         tc_fence_after();
-                        if (elect_one()) {
-                            scores(buf, k_slot);
-                            if (t == streams - 1) mma_commit(smem_u32(&sm.empty[0][k_at]));
-                            if (t == streams - 1 && i + ahead == n - 1) mma_commit(smem_u32(&sm.q_free));
-                        }
+                        if (elect_one()) scores(buf, kl);
                         __syncwarp();
                     }
                 }
                 if (!ok) break;
-                if (i >= 0 && ++v_at == p.slots[1]) v_at = 0, v_phase ^= 1;
-                if (more && ++k_at == p.slots[0]) k_at = 0, k_phase ^= 1;
+                if (elect_one()) {
+                    if (i >= 0) mma_commit(v_empty + 8 * v_at);
+                    if (more) mma_commit(k_empty + 8 * k_at);
+                    if (i + ahead == n - 1) mma_commit(smem_u32(&sm.q_free));
+                }
+                __syncwarp();
+                if (i >= 0 && ++v_at == v_slots) v_at = 0, v_phase ^= 1;
+                if (more && ++k_at == k_slots) k_at = 0, k_phase ^= 1;
             }
             if (!ok) break;
             if (elect_one()) mma_commit(smem_u32(&sm.done));
@@ -638,7 +700,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t st = tmem + lane_off + (uint32_t)buf * kTok;
                         // scores are read twice, 64 at a time: kept, 128 would not fit the registers (next to no
                         // first-level cache is left beside the tiles, a spill costs more than the second read)
-                        float x[64], top = -INFINITY;
+                        float x[64], most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
                         for (int h = 0; h < kTok; h += 64) {
                             tmem_ld32(st + h, x);
@@ -646,17 +708,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_wait_ld();
                             if (masked) hide(x, tree, mask, valid - h, h);
 #pragma unroll
-                            for (int e = 0; e < 64; ++e) top = fmaxf(top, x[e]);
+                            for (int e = 0; e < 64; e += 8)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) most[k] = fmaxf(most[k], fmaxf(x[e + 2 * k], x[e + 2 * k + 1]));
                         }
-                        top *= p.scale;
+                        const float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * p.scale;
                         const bool grow = mine && top > m + 8.f;
                         if (my_tiles == 0) {
                             m = top;
                         } else if (__any_sync(0xffffffffu, grow)) {
-                            // O holds the tiles so far once the last of their products has ended
-                            ok = all_ok(wait_bar(smem_u32(&sm.pv_done[g]), (uint32_t)(j - 1) & 1));
-                            if (!ok) break;
-                            tc_fence_after();
+                            // O holds the tiles so far: these scores come after their products, but for kOne, whose
+                            // scores run ahead of them
+                            if (C::kOne) {
+                                ok = all_ok(wait_bar(smem_u32(&sm.pv_done), (uint32_t)(j - 1) & 1));
+                                if (!ok) break;
+                                tc_fence_after();
+                            }
                             const float f = grow ? (m == -INFINITY ? 0.f : exp2_approx(m - top)) : 1.f;
                             if (grow) m = top, l *= f;
 #pragma unroll 1
@@ -671,7 +738,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                         const float ref = m == -INFINITY ? 0.f : m;
-                        float sum = 0.f;
+                        const float2 scale2 = make_float2(p.scale, p.scale), ref2 = make_float2(-ref, -ref);
+                        float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
                         for (int h = 0; h < kTok; h += 64) {
                             if (kTok > 64) {
@@ -686,15 +754,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 uint32_t w[16];
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) {
-                                    const float u = exp2_approx(fmaf(x[e0 + 2 * e], p.scale, -ref));
-                                    const float v = exp2_approx(fmaf(x[e0 + 2 * e + 1], p.scale, -ref));
-                                    sum += u + v;
-                                    w[e] = pack2<BF>(u, v);
+                                    float2 t = fma2(make_float2(x[e0 + 2 * e], x[e0 + 2 * e + 1]), scale2, ref2);
+                                    t = e % 8 == 1 || e % 8 == 4 || e % 8 == 6 ? exp2_poly(t) : make_float2(exp2_approx(t.x), exp2_approx(t.y));
+                                    sums[e & 1] = add2(sums[e & 1], t);
+                                    w[e] = pack2<BF>(t.x, t.y);
                                 }
                                 tmem_st16(st + (h + e0) / 2, w);
                             }
                         }
-                        l += sum;
+                        sums[0] = add2(sums[0], sums[1]);
+                        l += sums[0].x + sums[0].y;
                         tmem_wait_st();
                     }
                     ++my_tiles;
@@ -839,17 +908,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tile0 += n;
             ++seg;
         }
-        // items in parts, at most the range's first and its last: say that this warp's share is there, then add
-        for (int pass = 0; pass < 2 && ok; ++pass) {
-            Walker again(p, b0, off0, count);
-            for (int at = range0; ok && again.next(sg); at += sg.t1 - sg.t0) {
-                if (sg.t1 - sg.t0 == sg.tiles) continue;
-                const int lo = at - sg.t0;
-                if (pass == 1) ok = add_parts<DP, BF>(p, total, lo, sg);
-                else if (lane == 0) add_release(p.count + 2 * cta_of(total, lo), 1);
-            }
-            __syncwarp();
-        }
+        // items in parts: say that this warp's share is there, wait for the others', add
+        ok = ok && all_ok(wait_bar(smem_u32(&sm.cuts_known), 0));
+        const int cuts = ok ? sm.cuts : 0;
+        if (lane < cuts) add_release(p.count + 2 * sm.cut[lane].c0, 1);
+        for (int k = 0; k < cuts && ok; ++k) ok = await_parts(p.count + 2 * sm.cut[k].c0, sm.cut[k].parts, lane);
+#pragma unroll 1
+        for (int k = 0; k < cuts && ok; ++k) add_parts<DP, BF>(p, sm.cut[k].sg, sm.cut[k].c0, sm.cut[k].parts);
     }
     if (!ok) report_device_error(p.err, 10);
     __syncwarp();
@@ -921,6 +986,7 @@ int launch(const SparkTreeAttention* a, const Plan& q, uint8_t* ws, cudaStream_t
     p.part = reinterpret_cast<float4*>(ws + q.part);
     p.part_ml = reinterpret_cast<float2*>(ws + q.part_ml);
     p.rows_item = q.rows_item, p.row_tiles = q.row_tiles, p.group = q.group;
+    p.inv_group = 1.f / (float)q.group, p.inv_rows = 1.f / (float)q.rows_item;
     p.by_rows = q.by_rows, p.tile_nodes = q.tile_nodes, p.item_nodes = q.item_nodes;
     p.scale = (float)(a->scale * 1.4426950408889634);
     // a box of a TMA load lies within a page and within a tile
