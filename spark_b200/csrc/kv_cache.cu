@@ -20,34 +20,50 @@ struct Params {
     int elem;   // bytes of a value
 };
 
-template <typename T>
+// T: what is moved at a time, `per_head` of them a head.  A block moves K and V
+// of kTokens tokens, so that many loads are on the way together.
+constexpr int kTokens = 4;
+template <typename T, int E>   // E values in a T
 __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Params p) {
     const int64_t b = blockIdx.y;
     const int64_t len = p.c.lens[b];
     const int64_t room = p.c.max_pages * p.c.page_size - len;
     int64_t n = p.counts ? p.counts[b] : p.width;
     bool bad = n < 0 || n > p.width || len < 0 || n > room;
-    if (len < 0) n = 0;
-    n = n < 0 ? 0 : n;
+    n = len < 0 || n < 0 ? 0 : n;
     n = n > p.width ? p.width : n;
     n = n > room ? (room < 0 ? 0 : room) : n;
-    const int row = (int)(p.c.kv_heads * p.c.head_dim);
     if (blockIdx.x == 0 && threadIdx.x == 0) p.new_lens[b] = (int)(len + n);
-    for (int64_t j = blockIdx.x; j < n; j += gridDim.x) {
-        const int64_t src = p.index ? p.index[b * p.width + j] : j, at = len + j;
-        const int64_t page = p.c.page_table[b * p.c.page_table_stride + at / p.c.page_size];
-        if (src < 0 || src >= p.tokens || page < 0 || page >= p.c.pages) {
-            bad = true;
-            continue;
-        }
-        const int64_t r = at % p.c.page_size;
-        for (int i = threadIdx.x; i < row; i += blockDim.x) {
-            const int64_t h = i / p.c.head_dim, d = i % p.c.head_dim;
-            reinterpret_cast<T*>(p.c.k)[page * p.c.k_stride[0] + r * p.c.k_stride[1] + h * p.c.k_stride[2] + d] =
-                reinterpret_cast<const T*>(p.k)[b * p.ks[0] + src * p.ks[1] + h * p.ks[2] + d];
-            reinterpret_cast<T*>(p.c.v)[page * p.c.v_stride[0] + r * p.c.v_stride[1] + h * p.c.v_stride[2] + d] =
-                reinterpret_cast<const T*>(p.v)[b * p.vs[0] + src * p.vs[1] + h * p.vs[2] + d];
-        }
+    const int per_head = (int)p.c.head_dim / E, row = (int)p.c.kv_heads * per_head;
+    const int64_t j0 = (int64_t)blockIdx.x * kTokens;
+    const T *kx[kTokens], *vx[kTokens];
+    T *ky[kTokens], *vy[kTokens];
+    bool move[kTokens];
+#pragma unroll
+    for (int q = 0; q < kTokens; ++q) {
+        const int64_t j = j0 + q, at = len + j;
+        move[q] = j < n;
+        if (!move[q]) continue;
+        const int64_t src = p.index ? p.index[b * p.width + j] : j;
+        const int64_t page = p.c.page_table[b * p.c.page_table_stride + at / p.c.page_size], r = at % p.c.page_size;
+        move[q] = src >= 0 && src < p.tokens && page >= 0 && page < p.c.pages;
+        bad |= !move[q];
+        kx[q] = reinterpret_cast<const T*>(p.k) + (b * p.ks[0] + src * p.ks[1]) / E;
+        vx[q] = reinterpret_cast<const T*>(p.v) + (b * p.vs[0] + src * p.vs[1]) / E;
+        ky[q] = reinterpret_cast<T*>(p.c.k) + (page * p.c.k_stride[0] + r * p.c.k_stride[1]) / E;
+        vy[q] = reinterpret_cast<T*>(p.c.v) + (page * p.c.v_stride[0] + r * p.c.v_stride[1]) / E;
+    }
+    for (int i = threadIdx.x; i < row; i += 256) {
+        const int h = i / per_head, d = i - h * per_head;
+        const int64_t xk = h * (p.ks[2] / E) + d, xv = h * (p.vs[2] / E) + d;
+        const int64_t yk = h * (p.c.k_stride[2] / E) + d, yv = h * (p.c.v_stride[2] / E) + d;
+        T a[kTokens], c[kTokens];
+#pragma unroll
+        for (int q = 0; q < kTokens; ++q)
+            if (move[q]) a[q] = kx[q][xk], c[q] = vx[q][xv];
+#pragma unroll
+        for (int q = 0; q < kTokens; ++q)
+            if (move[q]) ky[q][yk] = a[q], vy[q][yv] = c[q];
     }
     if (bad && threadIdx.x == 0) report_device_error(p.err, 9);
 }
@@ -93,12 +109,24 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     for (int i = 0; i < 3 && k_stride && v_stride; ++i) p.ks[i] = k_stride[i], p.vs[i] = v_stride[i];
     p.batch = batch, p.tokens = tokens, p.width = width, p.index = index, p.counts = counts;
     p.new_lens = new_lens, p.err = err;
-    const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(width, 1), 2048), (unsigned)batch);
+    const int64_t blocks = std::max<int64_t>((width + kTokens - 1) / kTokens, 1);
+    SPARK_REQUIRE(blocks < (1ll << 31), SPARK_ERR_INVALID, "spark_kv_append: bad size");
+    const dim3 grid((unsigned)blocks, (unsigned)batch);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (cache->dtype == SPARK_DTYPE_F32)
-        k_kv_append<float><<<grid, 256, 0, s>>>(p);
+    // 16 bytes at a time where sizes, addresses and strides let it
+    const int vec = cache->dtype == SPARK_DTYPE_F32 ? 4 : 8;
+    bool fits = cache->head_dim % vec == 0;
+    for (const void* ptr : {k, v, (const void*)cache->k, (const void*)cache->v}) fits = fits && aligned(ptr, 16);
+    for (const int64_t* st : {(const int64_t*)p.ks, (const int64_t*)p.vs, cache->k_stride, cache->v_stride})
+        for (int i = 0; i < 3; ++i) fits = fits && st[i] % vec == 0;
+    if (fits && vec == 4)
+        k_kv_append<uint4, 4><<<grid, 256, 0, s>>>(p);
+    else if (fits)
+        k_kv_append<uint4, 8><<<grid, 256, 0, s>>>(p);
+    else if (vec == 4)
+        k_kv_append<float, 1><<<grid, 256, 0, s>>>(p);
     else
-        k_kv_append<uint16_t><<<grid, 256, 0, s>>>(p);
+        k_kv_append<uint16_t, 1><<<grid, 256, 0, s>>>(p);
     return check_launch("spark_kv_append");
 }
 
