@@ -461,7 +461,7 @@ SPARK_API int spark_tree_attention(const SparkTreeAttention* a, void* workspace,
  * nodes from node 0 on, then -1; accepted [batch] their number; next [batch].
  * A row of logits without a distribution (a NaN, +inf, or no value above -inf)
  * ends the sequence with next = -1.  A token id outside the vocabulary is never
- * accepted and sets error 11 in *err. */
+ * accepted and sets error 11 in *err.  nodes <= 1024, vocab <= 425,984. */
 typedef struct {
     int64_t batch, nodes, vocab;
     const void* logits;

@@ -8,11 +8,16 @@
 // probability proportional to r(v).
 //
 // One thread-block cluster per sequence, each CTA a contiguous slice of the
-// vocabulary whose r stays in shared memory, so that a row of logits is read
-// once.  The walk is a chain of row passes; after each the CTAs exchange their
-// partial sums through distributed shared memory (one cluster barrier) and add
-// them in rank order, so all of them take the same decisions.  Rows of nodes
-// that the walk does not reach are not read.
+// vocabulary that it keeps in shared memory, so that a row is read from memory
+// once.  The walk is a chain of row passes, its bound their latency (about 2 us
+// each): one reduction in the CTA, one exchange of partial sums through
+// distributed shared memory with one cluster barrier; all CTAs add them in rank
+// order and so take the same decisions.  r at a single token needs no exchange:
+// every CTA computes it from the token's logit and the sums.  Without draft
+// probabilities a rejection needs no pass either, it takes one exponential out
+// of the sum.  Rows of nodes that the walk does not reach are not read, but for
+// the row of the first child, which is brought into L2 while its parent's is
+// worked on, as the noise is from the start.
 #include <math.h>
 
 #include <algorithm>
@@ -24,7 +29,9 @@ namespace tv {
 
 constexpr int kThreads = 512;
 constexpr int kMaxCluster = 8;
-constexpr int kSliceMax = 52 * 1024;   // values of r in a CTA's shared memory (208 KB)
+constexpr int kMaxNodes = 1024;
+constexpr int kSliceMax = 52 * 1024;   // values in a CTA's shared memory (208 KB)
+constexpr int kBatch = 8;              // loads of a thread on the way together
 
 struct Params {
     SparkTreeVerify a;
@@ -34,13 +41,18 @@ struct Params {
 
 // What a CTA tells the others after a pass.
 struct Note {
-    float a, b, c;
-    int i;
+    float a, b;
+    int i, pad;
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+struct Shared {
+    Note note[2][kMaxCluster];
+    Note red[kThreads / 32];
+    float mass[kMaxNodes];   // sums of what was left after each rejection at this node, 0 where nothing was
+};
+
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_size() {
     uint32_t n;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
@@ -51,68 +63,80 @@ __device__ __forceinline__ uint32_t cluster_rank() {
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
+// Asks for bytes [p, p + n) in L2.
+__device__ __forceinline__ void to_l2(const void* p, int64_t n) {
+    const uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t(15);
+    const int64_t m = (reinterpret_cast<intptr_t>(p) + n - (intptr_t)a) & ~int64_t(15);
+    if (m > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"((uint32_t)m) : "memory");
+}
 
-struct Shared {
-    Note note[2][kMaxCluster];
-    float red[kThreads / 32], red2[kThreads / 32];
-    int redi[kThreads / 32];
-    float x, x2;   // r at the next token tried, written by the thread that holds it
+// Integers in the order of the floats (no NaN), and back.
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(x);
+    return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+__device__ __forceinline__ float max_of_warp(float x) { return unordered(__reduce_max_sync(0xffffffffu, ordered(x))); }
+// (both lanes of a pair compute the same: an addition commutes)
+__device__ __forceinline__ float sum_of_warp(float x) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+
+// How the notes of a warp's lanes become one.
+// Largest value a with its lowest index i (-1 where there is none); b: any.
+struct Best {
+    static __device__ Note none() { return Note{-INFINITY, 0.f, -1, 0}; }
+    static __device__ Note warp(Note v) {
+        const float top = max_of_warp(v.i < 0 ? -INFINITY : v.a);
+        const uint32_t first = __reduce_min_sync(0xffffffffu, v.i >= 0 && v.a == top ? (uint32_t)v.i : 0xffffffffu);
+        return Note{top, __any_sync(0xffffffffu, v.b != 0.f) ? 1.f : 0.f, (int)first, 0};
+    }
+    static __device__ void add(Note& v, float a, int i) {
+        if (v.i < 0 || a > v.a) v.a = a, v.i = i;     // indexes come in increasing order
+    }
+};
+// Maximum a and the sum b of exponentials over it.
+struct Softmax {
+    static __device__ Note none() { return Note{-INFINITY, 0.f, 0, 0}; }
+    static __device__ Note warp(Note v) {
+        const float top = max_of_warp(v.a);
+        return Note{top, sum_of_warp(v.b * expf(v.a - (top == -INFINITY ? 0.f : top))), 0, 0};
+    }
+};
+struct Sum {
+    static __device__ Note none() { return Note{0.f, 0.f, 0, 0}; }
+    static __device__ Note warp(Note v) { return Note{sum_of_warp(v.a), 0.f, 0, 0}; }
 };
 
-// Sends (a, b, c, i) to every CTA of the cluster and waits for theirs.
-__device__ __forceinline__ const Note* exchange(Shared& s, int& step, Note mine) {
+// Joins the notes of all threads of the cluster; every thread gets the result.
+// The order is fixed: by lanes, warps and CTAs.
+template <typename J>
+__device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int n = (int)cluster_size();
+    v = J::warp(v);
+    if (lane == 0) s.red[warp] = v;
+    __syncthreads();
     Note* slot = s.note[step & 1];
+    if (step == 0) cluster_wait();     // every CTA of the cluster has started: its shared memory may be written
     ++step;
-    const uint32_t n = cluster_size();
-    if (threadIdx.x < n) {
-        uint32_t local = (uint32_t)__cvta_generic_to_shared(&slot[cluster_rank()]), remote;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(threadIdx.x));
-        asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(__float_as_uint(mine.a)),
-                     "r"(__float_as_uint(mine.b)), "r"(__float_as_uint(mine.c)), "r"(mine.i)
-                     : "memory");
+    if (warp == 0) {
+        v = J::warp(lane < kThreads / 32 ? s.red[lane] : J::none());
+        if (lane < n) {
+            const uint32_t local = (uint32_t)__cvta_generic_to_shared(&slot[cluster_rank()]);
+            uint32_t remote;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(lane));
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(remote), "r"(__float_as_uint(v.a)),
+                         "r"(__float_as_uint(v.b)), "r"(v.i), "r"(0)
+                         : "memory");
+        }
     }
-    cluster_barrier();
-    return slot;
-}
-
-__device__ __forceinline__ float block_sum(Shared& s, float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.f;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) t += s.red[w];
-    return t;
-}
-__device__ __forceinline__ float block_max(Shared& s, float v) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = s.red[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) t = fmaxf(t, s.red[w]);
-    return t;
-}
-// The largest value and its lowest index (-1 where there is none).
-__device__ __forceinline__ void better(float& v, int& i, float v2, int i2) {
-    if (i2 >= 0 && (i < 0 || v2 > v || (v2 == v && i2 < i))) v = v2, i = i2;
-}
-__device__ __forceinline__ void block_best(Shared& s, float& v, int& i) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float v2 = __shfl_xor_sync(0xffffffffu, v, o);
-        const int i2 = __shfl_xor_sync(0xffffffffu, i, o);
-        better(v, i, v2, i2);
-    }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s.red2[threadIdx.x >> 5] = v, s.redi[threadIdx.x >> 5] = i;
-    __syncthreads();
-    v = s.red2[0], i = s.redi[0];
-    for (int w = 1; w < kThreads / 32; ++w) better(v, i, s.red2[w], s.redi[w]);
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
+    return J::warp(lane < n ? slot[lane] : J::none());
 }
 
 // The first child of `cur` after node `from`, or -1.
@@ -126,127 +150,169 @@ __device__ __forceinline__ int next_child(const int* parents, int nodes, int cur
     return -1;
 }
 
+template <typename L, typename D>   // types of logits and draft probabilities
 __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant__ Params p) {
-    extern __shared__ float raw[];   // r of this slice up to the factor `f`; below zero: nothing left of -raw
+    extern __shared__ float raw[];   // logits over T, after a rejection with draft probabilities r; below zero: nothing is left of -raw
     __shared__ Shared s;
     const SparkTreeVerify& a = p.a;
-    const uint32_t rank = cluster_rank(), csize = cluster_size();
-    const int64_t b = blockIdx.x / csize;
+    const uint32_t rank = cluster_rank();
+    const int64_t b = blockIdx.x / cluster_size();
     const int nodes = (int)a.nodes, tid = threadIdx.x;
     const int64_t v0 = (int64_t)rank * p.slice;
     const int n = (int)max((int64_t)0, min((int64_t)p.slice, a.vocab - v0));
-    const int* parents = a.parents + b * a.parents_stride;
-    const int64_t* tokens = a.tokens + b * a.tokens_stride;
+    // the tree, in shared memory after the slice: from here on a child costs no round trip but for its logit
+    int* parents = reinterpret_cast<int*>(raw + p.slice);
+    int* tokens = parents + nodes;        // -1: outside the vocabulary
+    float* uniforms = reinterpret_cast<float*>(tokens + nodes);
     const float* noise = a.noise + b * a.noise_stride + v0;
+    const L* logits = reinterpret_cast<const L*>(a.logits) + b * a.logits_stride[0];
+    const D* draft = a.draft ? reinterpret_cast<const D*>(a.draft) + b * a.draft_stride[0] : nullptr;
     const float temp = a.temperature ? a.temperature[b] : 1.f;
     const bool lead = rank == 0 && tid == 0;
     int step = 0, cur = 0, accepted = 1;
     int64_t last = -1;
-    cluster_barrier();   // every CTA of the cluster has started: its shared memory may be written
+    cluster_arrive();
     if (lead) a.path[b * nodes] = 0;
+    if (tid == 0 && temp != 0.f) to_l2(noise, (int64_t)n * 4);
+    if (tid == 0) to_l2(logits + v0, (int64_t)n * sizeof(L));
+    for (int i = tid; i < nodes; i += kThreads) {
+        const int64_t x = a.tokens[b * a.tokens_stride + i];
+        parents[i] = a.parents[b * a.parents_stride + i];
+        tokens[i] = x >= 0 && x < a.vocab ? (int)x : -1;
+        uniforms[i] = a.uniforms[b * a.uniforms_stride + i];
+    }
+    __syncthreads();
 
     while (true) {
-        const int64_t row = b * a.logits_stride[0] + cur * a.logits_stride[1] + v0;
+        const L* row = logits + cur * a.logits_stride[1];
         int child = next_child(parents, nodes, cur, cur);
-        if (temp == 0.f) {
-            float best = -INFINITY;
-            int at = -1;
-            bool nan = false;
-            for (int i = tid; i < n; i += kThreads) {
-                const float x = load_as_float(a.logits, (int)a.logits_dtype, row + i);
-                nan |= x != x;
-                if (x > best) best = x, at = i + (int)v0;
+        if (child >= 0 && tid == 0) to_l2(logits + child * a.logits_stride[1] + v0, (int64_t)n * sizeof(L));
+        // the child's logit and draft probability are on their way during the pass
+        const D* q_row = draft ? draft + cur * a.draft_stride[1] : nullptr;
+        if (child >= 0 && draft && tid == 32) to_l2(q_row + v0, (int64_t)n * sizeof(D));
+        int x = child >= 0 ? tokens[child] : -1;
+        float lx = x >= 0 ? (float)row[x] : 0.f, qx = x >= 0 && draft ? (float)q_row[x] : 1.f;
+        float m = -INFINITY;
+        int at = -1;
+        bool nan = false;
+        for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
+            float x[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * kThreads;
+                x[k] = i < n ? (float)row[v0 + i] : -INFINITY;
             }
-            nan = __syncthreads_or(nan);
-            block_best(s, best, at);
-            const Note* got = exchange(s, step, Note{best, nan ? 1.f : 0.f, 0.f, at});
-            best = -INFINITY, at = -1;
-            for (uint32_t r = 0; r < csize; ++r) better(best, at, got[r].a, got[r].i), nan |= got[r].b != 0.f;
-            if (nan || at < 0 || best == INFINITY) break;
-            while (child >= 0 && tokens[child] != at) child = next_child(parents, nodes, cur, child);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * kThreads;
+                if (i >= n) break;
+                if (temp == 0.f) {
+                    nan |= x[k] != x[k];
+                    if (x[k] > m) m = x[k], at = i + (int)v0;
+                } else {
+                    raw[i] = x[k] = temp == 1.f ? x[k] : x[k] / temp;
+                    m = fmaxf(m, x[k]);
+                }
+            }
+        }
+        if (temp == 0.f) {
+            const Note got = join_all<Best>(s, step, Note{m, nan ? 1.f : 0.f, at, 0});
+            if (got.b != 0.f || got.i < 0 || got.a == INFINITY) break;   // no distribution here
+            while (child >= 0 && tokens[child] != got.i) child = next_child(parents, nodes, cur, child);
             if (child < 0) {
-                last = at;
+                last = got.i;
                 break;
             }
         } else {
-            // r(v) = raw(v) f: the maximum, then exponentials and their sum
-            int64_t x = child >= 0 ? tokens[child] : -1;
-            if (tid == 0) s.x = 0.f, s.x2 = 0.f;
-            float m = -INFINITY, z = 0.f;
-            for (int i = tid; i < n; i += kThreads) {
-                const float v = load_as_float(a.logits, (int)a.logits_dtype, row + i) / temp;
-                raw[i] = v;
-                m = fmaxf(m, v);
-            }
-            m = block_max(s, m);
-            for (int i = tid; i < n; i += kThreads) {
-                const float e = m == -INFINITY && raw[i] == m ? 0.f : expf(raw[i] - m);
-                raw[i] = e;
-                z += e;
-                if (v0 + i == x) s.x = e;
-            }
-            z = block_sum(s, z);
-            const Note* got = exchange(s, step, Note{m, z, s.x, 0});
-            float top = -INFINITY, sum = 0.f, rx = 0.f;
-            for (uint32_t r = 0; r < csize; ++r) top = fmaxf(top, got[r].a);
-            for (uint32_t r = 0; r < csize; ++r) {
-                const float g = got[r].b == 0.f ? 0.f : expf(got[r].a - top);
-                sum += got[r].b * g;
-                rx += got[r].c * g;
-            }
+            float z = 0.f;
+            const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+            for (int i = tid; i < n; i += kThreads) z += expf(raw[i] - ref);
+            const Note got = join_all<Softmax>(s, step, Note{m, z, 0, 0});
+            const float top = got.a;
+            float sum = got.b;
             if (!(sum > 0.f && sum < INFINITY)) break;   // no distribution here
-            float f = m == -INFINITY ? 0.f : expf(m - top) / sum;
-            rx /= sum;
+            int rejected = 0;          // children whose rejection changed r; with draft probabilities raw is r then
+            float f = 1.f;             // r = raw f
             // the children in turn
             while (child >= 0) {
-                const bool valid = x >= 0 && x < a.vocab;
+                const bool valid = x >= 0;
                 if (!valid && lead) report_device_error(p.err, 11);
-                const int64_t dr = b * a.draft_stride[0] + cur * a.draft_stride[1];
-                const float qx = !valid ? 0.f : a.draft ? load_as_float(a.draft, (int)a.draft_dtype, dr + x) : 1.f;
-                if (valid && a.uniforms[b * a.uniforms_stride + child] * qx < rx) break;
-                child = next_child(parents, nodes, cur, child);
-                const int64_t x2 = child >= 0 ? tokens[child] : -1;
-                __syncthreads();
-                if (tid == 0) s.x = 0.f, s.x2 = 0.f;
-                __syncthreads();
-                float left = 0.f;
-                for (int i = tid; i < n; i += kThreads) {
-                    const float old = fmaxf(raw[i], 0.f) * f;
-                    float t = old;
-                    if (!valid) t = old;
-                    else if (a.draft) t = fmaxf(old - load_as_float(a.draft, (int)a.draft_dtype, dr + v0 + i), 0.f);
-                    else if (v0 + i == x) t = 0.f;
-                    raw[i] = t > 0.f ? t : -old;
-                    left += t;
-                    if (v0 + i == x2) s.x = t, s.x2 = old;
+                const int next = next_child(parents, nodes, cur, child), x2 = next >= 0 ? tokens[next] : -1;
+                const float lx2 = x2 >= 0 ? (float)row[x2] : 0.f, qx2 = x2 >= 0 && draft ? (float)q_row[x2] : 1.f;
+                bool known = false;    // rejected already under another number
+                if (valid && !draft)
+                    for (int base = cur + 1; base < child; base += 32) {
+                        const int c = base + (tid & 31);
+                        known |= __any_sync(0xffffffffu, c < child && parents[c] == cur && tokens[c] == x);
+                    }
+                if (valid && !known) {
+                    const float e = expf((temp == 1.f ? lx : lx / temp) - top);
+                    float rx = e / sum;
+                    for (int k = 0; k < rejected && draft; ++k)
+                        if (s.mass[k] > 0.f) rx = fmaxf(rx - qx, 0.f) / s.mass[k];
+                    if (uniforms[child] * qx < rx) break;
+                    if (!draft) {
+                        // without x: its exponential leaves the sum, its owner forgets it
+                        if (sum - e > 0.f) {
+                            sum -= e;
+                            const int64_t i = (int64_t)x - v0;
+                            if (i >= 0 && i < n && i % kThreads == tid) raw[i] = -INFINITY;
+                        }
+                    } else {
+                        float left = 0.f;
+                        for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
+                            float q[kBatch];
+#pragma unroll
+                            for (int k = 0; k < kBatch; ++k) {
+                                const int i = i0 + k * kThreads;
+                                q[k] = i < n ? (float)q_row[v0 + i] : 0.f;
+                            }
+#pragma unroll
+                            for (int k = 0; k < kBatch; ++k) {
+                                const int i = i0 + k * kThreads;
+                                if (i >= n) break;
+                                const float old = rejected ? fmaxf(raw[i], 0.f) * f : expf(raw[i] - top) / sum;
+                                const float t = fmaxf(old - q[k], 0.f);
+                                raw[i] = t > 0.f ? t : -old;
+                                left += t;
+                            }
+                        }
+                        const float mass = join_all<Sum>(s, step, Note{left, 0.f, 0, 0}).a;
+                        if (mass > 0.f) {
+                            f = 1.f / mass;
+                        } else {
+                            // nothing is left: the distribution stays what it was
+                            for (int i = tid; i < n; i += kThreads) raw[i] = -raw[i];
+                            f = 1.f;
+                        }
+                        if (tid == 0) s.mass[rejected] = mass;
+                        __syncthreads();
+                        ++rejected;
+                    }
                 }
-                left = block_sum(s, left);
-                got = exchange(s, step, Note{left, s.x, s.x2, 0});
-                float mass = 0.f, rn = 0.f, ro = 0.f;
-                for (uint32_t r = 0; r < csize; ++r) mass += got[r].a, rn += got[r].b, ro += got[r].c;
-                if (mass > 0.f) {
-                    f = 1.f / mass;
-                    rx = rn / mass;
-                } else {
-                    // nothing is left: the distribution stays what it was
-                    for (int i = tid; i < n; i += kThreads) raw[i] = -raw[i];
-                    f = 1.f;
-                    rx = ro;
-                }
-                x = x2;
+                child = next, x = x2, lx = lx2, qx = qx2;
             }
             if (child < 0) {
-                float best = -INFINITY;
-                int at = -1;
-                for (int i = tid; i < n; i += kThreads) {
-                    const float r = fmaxf(raw[i], 0.f) * f;
-                    if (r > 0.f) better(best, at, r / noise[i], i + (int)v0);
+                Note best = Best::none();
+                for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
+                    float e[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int i = i0 + k * kThreads;
+                        e[k] = i < n ? noise[i] : 1.f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int i = i0 + k * kThreads;
+                        if (i >= n) break;
+                        // (a common factor of r does not change which quotient is the largest; the quotient is good
+                        // to two units in its last place)
+                        const float r = rejected ? raw[i] : expf(raw[i] - top);
+                        if (r > 0.f) Best::add(best, __fdividef(r, e[k]), i + (int)v0);
+                    }
                 }
-                block_best(s, best, at);
-                got = exchange(s, step, Note{best, 0.f, 0.f, at});
-                best = -INFINITY, at = -1;
-                for (uint32_t r = 0; r < csize; ++r) better(best, at, got[r].a, got[r].i);
-                last = at;
+                last = join_all<Best>(s, step, best).i;
                 break;
             }
         }
@@ -254,10 +320,38 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
         ++accepted;
         cur = child;
     }
+    if (step == 0) cluster_wait();
     if (rank == 0) {
         for (int i = accepted + tid; i < nodes; i += kThreads) a.path[b * nodes + i] = -1;
         if (tid == 0) a.accepted[b] = accepted, a.next[b] = last;
     }
+}
+
+template <typename L, typename D>
+int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(k_tree_verify<L, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)((kSliceMax + 3 * kMaxNodes) * sizeof(float)));
+    if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: %s", cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(batch * cs));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = ((size_t)p.slice + 3 * (size_t)p.a.nodes) * sizeof(float);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, k_tree_verify<L, D>, p);
+    if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: launch failed: %s", cudaGetErrorString(e));
+    return check_launch("spark_tree_verify");
+}
+
+template <typename L>
+int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
+    if (p.a.draft && p.a.draft_dtype == SPARK_DTYPE_BF16) return launch<L, __nv_bfloat16>(p, batch, cs, s);
+    if (p.a.draft && p.a.draft_dtype == SPARK_DTYPE_F16) return launch<L, __half>(p, batch, cs, s);
+    return launch<L, float>(p, batch, cs, s);
 }
 
 }  // namespace tv
@@ -269,8 +363,10 @@ int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream) {
     using namespace spark;
     using namespace spark::tv;
     SPARK_REQUIRE(a, SPARK_ERR_INVALID, "spark_tree_verify: null pointer");
-    SPARK_REQUIRE(a->batch >= 0 && a->batch < (1 << 24) && a->nodes >= 1 && a->nodes < (1 << 20) && a->vocab >= 1,
+    SPARK_REQUIRE(a->batch >= 0 && a->batch < (1 << 24) && a->nodes >= 1 &&  a->vocab >= 1,
                   SPARK_ERR_INVALID, "spark_tree_verify: bad size");
+    SPARK_REQUIRE(a->nodes <= kMaxNodes, SPARK_ERR_UNSUPPORTED, "spark_tree_verify: %lld nodes, at most %d",
+                  (long long)a->nodes, kMaxNodes);
     SPARK_REQUIRE(a->logits_dtype >= 0 && a->logits_dtype <= 2 && (!a->draft || (a->draft_dtype >= 0 && a->draft_dtype <= 2)),
                   SPARK_ERR_INVALID, "spark_tree_verify: bad dtype");
     SPARK_REQUIRE(a->vocab <= (int64_t)kMaxCluster * kSliceMax, SPARK_ERR_UNSUPPORTED,
@@ -284,23 +380,10 @@ int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream) {
     p.err = err;
     const int cs = kMaxCluster;
     p.slice = (int)((a->vocab + cs - 1) / cs + 7) / 8 * 8;
-    const size_t smem = (size_t)p.slice * sizeof(float);
-    cudaError_t e = cudaFuncSetAttribute(k_tree_verify, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)(kSliceMax * sizeof(float)));
-    if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: %s", cudaGetErrorString(e));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(a->batch * cs));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, k_tree_verify, p);
-    if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: launch failed: %s", cudaGetErrorString(e));
-    return check_launch("spark_tree_verify");
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (a->logits_dtype == SPARK_DTYPE_BF16) return launch<__nv_bfloat16>(p, a->batch, cs, st);
+    if (a->logits_dtype == SPARK_DTYPE_F16) return launch<__half>(p, a->batch, cs, st);
+    return launch<float>(p, a->batch, cs, st);
 }
 
 }  // extern "C"
