@@ -513,6 +513,8 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------ tree decoding
+MAX_TREE_NODES = 64    # of one sequence in tree_attention (SPARK_MAX_TREE_NODES)
+
 _tree_ws: dict[tuple[int, int], torch.Tensor] = {}
 _pack_heads = _lib.packer(_lib.SparkRopeHeads)
 _pack_cache = _lib.packer(_lib.SparkPagedCache)
