@@ -110,9 +110,12 @@ __device__ __forceinline__ int context_len(const Params& p, int64_t b) {
     return (int)(len < 0 ? 0 : (len > room ? room : len));
 }
 
-// (tiles of all items are below 2^31: the host checks it by the longest context the pages hold)
+// Starting an item (loading Q, filling the pipeline, writing O) costs as much as
+// this many tiles: the cut into ranges counts them in front of the item's own.
+constexpr int kStart = 3;
+// Places of an item of sequence b (all items' are below 2^31: the host checks it by the longest context the pages hold)
 __device__ __forceinline__ int tiles_of(const Params& p, int b) {
-    return b < (int)p.a.batch ? (context_len(p, b) + p.tok - 1) / p.tok + 1 : 0;
+    return b < (int)p.a.batch ? (context_len(p, b) + p.tok - 1) / p.tok + 1 + kStart : 0;
 }
 // Number of tiles of all items, by one warp.
 __device__ __forceinline__ int count_tiles(const Params& p, int lane) {
@@ -146,27 +149,34 @@ __device__ __forceinline__ void locate(const Params& p, int lane, int pos, int& 
 // A run of tiles of one item.
 struct Segment {
     int b, head, rt, t0, t1, tiles, len;   // tiles t0..t1-1 of `tiles`; the last is the tree
+    int lo;                                // place of tile 0 among all
 };
 
-// Walks `left` tiles from place `off` of sequence b on.
+// Walks `left` places from place `off` of sequence b on; a run may be empty
+// where the range ends in front of an item's own tiles.
 struct Walker {
     const Params& p;
-    int b, off, left;
-    __device__ Walker(const Params& q, int b0, int off0, int n) : p(q), b(b0), off(off0), left(n) {}
+    int b, off, left, pos;
+    __device__ Walker(const Params& q, int b0, int off0, int n, int first) : p(q), b(b0), off(off0), left(n), pos(first) {}
     __device__ bool next(Segment& s) {
-        if (left <= 0 || b >= (int)p.a.batch) return false;
-        s.len = context_len(p, b);
-        s.tiles = (s.len + p.tok - 1) / p.tok + 1;
-        const int item = off / s.tiles;
-        s.b = b;
-        s.head = item / p.row_tiles;
-        s.rt = item - s.head * p.row_tiles;
-        s.t0 = off - item * s.tiles;
-        s.t1 = min(s.tiles, s.t0 + left);
-        off += s.t1 - s.t0;
-        left -= s.t1 - s.t0;
-        if (off == s.tiles * p.per_seq) off = 0, ++b;
-        return true;
+        while (left > 0 && b < (int)p.a.batch) {
+            s.len = context_len(p, b);
+            s.tiles = (s.len + p.tok - 1) / p.tok + 1;
+            const int places = s.tiles + kStart, item = off / places;
+            s.b = b;
+            s.head = item / p.row_tiles;
+            s.rt = item - s.head * p.row_tiles;
+            const int at = off - item * places, n = min(places - at, left);
+            s.t0 = max(at - kStart, 0);
+            s.t1 = at + n - kStart;
+            off += n;
+            left -= n;
+            pos += n;
+            s.lo = pos - n - at + kStart;
+            if (off == places * p.per_seq) off = 0, ++b;
+            if (s.t1 > s.t0) return true;
+        }
+        return false;
     }
 };
 
@@ -302,24 +312,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-// 2^t for t <= 8 on the FMA pipe: t = j + f, |f| <= 1/2, a polynomial of degree 4
-// in f with value 1 at 0 whose largest relative error on the interval is smallest
-// (2.9e-6, fitted by linear programming), and j added to its exponent.  At and
-// below -127 the result is exactly 0: 1.0 loses all of its exponent.  The
-// exponential unit gives 16 results a clock to an SM, this is what the row of 128
-// weights waits for, so that a part of them is computed here.
-__device__ __forceinline__ float2 exp2_poly(float2 t) {
-    const float kRound = 12582912.f;   // 1.5 2^23: the sum's low bits are the nearest integer
-    t = make_float2(fmaxf(t.x, -127.f), fmaxf(t.y, -127.f));
-    const float2 z = add2(t, make_float2(kRound, kRound));
-    const float2 f = add2(t, fma2(z, make_float2(-1.f, -1.f), make_float2(kRound, kRound)));
-    float2 q = fma2(f, make_float2(0.00958538242f, 0.00958538242f), make_float2(0.0559066273f, 0.0559066273f));
-    q = fma2(q, f, make_float2(0.24024038f, 0.24024038f));
-    q = fma2(q, f, make_float2(0.693124175f, 0.693124175f));
-    q = fma2(q, f, make_float2(1.f, 1.f));
-    return make_float2(__uint_as_float((__float_as_uint(z.x) << 23) + __float_as_uint(q.x)),
-                       __uint_as_float((__float_as_uint(z.y) << 23) + __float_as_uint(q.y)));
-}
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 __device__ __forceinline__ void add_release(int* p, int v) {
@@ -331,7 +323,7 @@ __device__ __forceinline__ int load_acquire(const int* p) {
     return v;
 }
 
-// CTAs that get tiles (no more than there are), the first tile of one, and the one that has tile `pos`.
+// CTAs that get places (no more than there are), the first place of one, and the one that has place `pos`.
 __device__ __forceinline__ int ctas(int total) { return min(total, (int)gridDim.x); }
 __device__ __forceinline__ int first_tile(int total, int cta) { return (int)((uint64_t)total * cta / (unsigned)ctas(total)); }
 __device__ __forceinline__ int cta_of(int total, int pos) {
@@ -498,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
     const int count = (smem_u32(smem) & 1023) ? 0 : range1 - range0;
-    Walker walk(p, b0, off0, count);
+    Walker walk(p, b0, off0, count, range0);
     Segment sg;
     bool ok = true;
 
@@ -555,14 +547,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         // a tile of Q is the heads of the group of tile_nodes nodes, node by node
         const uint32_t qb = smem_u32(q_smem), bar = smem_u32(&sm.q_full);
         const uint32_t bytes = (uint32_t)(p.tile_nodes * p.group) * (C::kChunks * 128);
-        int seg = 0, cuts = 0, at = range0;
+        int seg = 0, cuts = 0;
         for (; ok && walk.next(sg); ++seg) {
             if (sg.t1 - sg.t0 < sg.tiles) {
-                const int lo = at - sg.t0, c0 = cta_of(total, lo), c1 = cta_of(total, lo + sg.tiles - 1);
+                const int c0 = cta_of(total, sg.lo), c1 = cta_of(total, sg.lo + sg.tiles - 1);
                 if (lane == 0) sm.cut[cuts] = Cut{sg, c0, c1 - c0 + 1};
                 ++cuts;
             }
-            at += sg.t1 - sg.t0;
             ok = all_ok(seg == 0 || wait_bar(smem_u32(&sm.q_free), (seg - 1) & 1));
             if (!ok) break;
             if (elect_one()) {
@@ -755,7 +746,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                                 for (int e = 0; e < 16; ++e) {
                                     float2 t = fma2(make_float2(x[e0 + 2 * e], x[e0 + 2 * e + 1]), scale2, ref2);
-                                    t = e % 8 == 1 || e % 8 == 4 || e % 8 == 6 ? exp2_poly(t) : make_float2(exp2_approx(t.x), exp2_approx(t.y));
+                                    t = make_float2(exp2_approx(t.x), exp2_approx(t.y));
                                     sums[e & 1] = add2(sums[e & 1], t);
                                     w[e] = pack2<BF>(t.x, t.y);
                                 }
@@ -1072,7 +1063,7 @@ int spark_tree_attention(const SparkTreeAttention* args, void* workspace, size_t
                   SPARK_ERR_INVALID, "spark_tree_attention: null pointer");
     const Plan q = plan(a);
     const int tok = q.dp == 256 ? 64 : 128;
-    SPARK_REQUIRE((double)a->batch * c.kv_heads * q.row_tiles * ((double)c.max_pages * c.page_size / tok + 2) < 2147483647.0,
+    SPARK_REQUIRE((double)a->batch * c.kv_heads * q.row_tiles * ((double)c.max_pages * c.page_size / tok + 2 + kStart) < 2147483647.0,
                   SPARK_ERR_UNSUPPORTED, "spark_tree_attention: 2^31 tiles of %d tokens or more", tok);
     SPARK_REQUIRE(workspace && workspace_bytes >= q.bytes, SPARK_ERR_WORKSPACE,
                   "spark_tree_attention: the workspace has %zu of %zu bytes", workspace_bytes, q.bytes);
