@@ -108,18 +108,6 @@ __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params
     const int half = p.rot / 2, d = copy ? p.rot + (unit - turned) * N : unit * N;
     const int64_t pos = p.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(p.positions)[tok]
                                          : reinterpret_cast<const int*>(p.positions)[tok];
-    const bool good = pos >= 0 && pos < p.table_rows;
-    if (!good && unit == 0 && h0 == 0) report_device_error(p.err, 8);
-    float c[PAIRS], sn[PAIRS];
-    if (!copy) {
-        const float* row = p.table + (good ? pos : 0) * p.rot + (INTER ? d / 2 : d);
-#pragma unroll
-        for (int k = 0; k < PAIRS; k += 2) {
-            const float2 cc = *reinterpret_cast<const float2*>(row + k), ss = *reinterpret_cast<const float2*>(row + half + k);
-            c[k] = cc.x, c[k + 1] = cc.y;
-            sn[k] = p.inverse ? -ss.x : ss.x, sn[k + 1] = p.inverse ? -ss.y : ss.y;
-        }
-    }
     uint4 va[kHeads], vb[kHeads];
     T* y[kHeads];
 #pragma unroll
@@ -134,6 +122,18 @@ __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params
         y[k] = reinterpret_cast<T*>(s.y) + b * s.ys[0] + t * s.ys[1] + h * s.ys[2] + d;
         va[k] = *reinterpret_cast<const uint4*>(x);
         if (!INTER && !copy) vb[k] = *reinterpret_cast<const uint4*>(x + half);
+    }
+    const bool good = pos >= 0 && pos < p.table_rows;
+    if (!good && unit == 0 && h0 == 0) report_device_error(p.err, 8);
+    float c[PAIRS], sn[PAIRS];
+    if (!copy) {
+        const float* row = p.table + (good ? pos : 0) * p.rot + (INTER ? d / 2 : d);
+#pragma unroll
+        for (int k = 0; k < PAIRS; k += 2) {
+            const float2 cc = *reinterpret_cast<const float2*>(row + k), ss = *reinterpret_cast<const float2*>(row + half + k);
+            c[k] = cc.x, c[k + 1] = cc.y;
+            sn[k] = p.inverse ? -ss.x : ss.x, sn[k + 1] = p.inverse ? -ss.y : ss.y;
+        }
     }
 #pragma unroll
     for (int k = 0; k < kHeads; ++k) {
