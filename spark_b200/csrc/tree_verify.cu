@@ -139,17 +139,6 @@ __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
     return J::warp(lane < n ? slot[lane] : J::none());
 }
 
-// The first child of `cur` after node `from`, or -1.
-__device__ __forceinline__ int next_child(const int* parents, int nodes, int cur, int from) {
-    const int lane = threadIdx.x & 31;
-    for (int base = from + 1; base < nodes; base += 32) {
-        const int c = base + lane;
-        const unsigned hit = __ballot_sync(0xffffffffu, c < nodes && parents[c] == cur);
-        if (hit) return base + __ffs(hit) - 1;
-    }
-    return -1;
-}
-
 template <typename L, typename D>   // types of logits and draft probabilities
 __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant__ Params p) {
     extern __shared__ float raw[];   // logits over T, after a rejection with draft probabilities r; below zero: nothing is left of -raw
@@ -157,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
     const SparkTreeVerify& a = p.a;
     const uint32_t rank = cluster_rank();
     const int64_t b = blockIdx.x / cluster_size();
-    const int nodes = (int)a.nodes, tid = threadIdx.x;
+    const int nodes = (int)a.nodes, tid = threadIdx.x, lane = tid & 31;
     const int64_t v0 = (int64_t)rank * p.slice;
     const int n = (int)max((int64_t)0, min((int64_t)p.slice, a.vocab - v0));
     // the tree, in shared memory after the slice: from here on a child costs no round trip but for its logit
@@ -185,49 +174,81 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
 
     while (true) {
         const L* row = logits + cur * a.logits_stride[1];
-        int child = next_child(parents, nodes, cur, cur);
-        if (child >= 0 && tid == 0) to_l2(logits + child * a.logits_stride[1] + v0, (int64_t)n * sizeof(L));
-        // the child's logit and draft probability are on their way during the pass
         const D* q_row = draft ? draft + cur * a.draft_stride[1] : nullptr;
+        // The children in index order.  A lane has one of 32 nodes: logits and draft probabilities of all children among
+        // them are on their way together, and during the pass.
+        int base = cur + 1, child = -1, x = -1, xl;
+        unsigned waiting;
+        float lx = 0.f, qx = 1.f, lxl, qxl;
+        auto gather = [&]() {
+            const int c = base + lane;
+            const bool is = c < nodes && parents[c] == cur;
+            xl = is ? tokens[c] : -1;
+            lxl = xl >= 0 ? (float)row[xl] : 0.f, qxl = xl >= 0 && draft ? (float)q_row[xl] : 1.f;
+            waiting = __ballot_sync(0xffffffffu, is);
+        };
+        auto next = [&]() {
+            while (!waiting) {
+                base += 32;
+                if (base >= nodes) {
+                    child = -1;
+                    return;
+                }
+                gather();
+            }
+            const int at = __ffs(waiting) - 1;
+            waiting &= waiting - 1;
+            child = base + at;
+            x = __shfl_sync(0xffffffffu, xl, at), lx = __shfl_sync(0xffffffffu, lxl, at), qx = __shfl_sync(0xffffffffu, qxl, at);
+        };
+        gather();
+        next();
+        if (child >= 0 && tid == 0) to_l2(logits + child * a.logits_stride[1] + v0, (int64_t)n * sizeof(L));
         if (child >= 0 && draft && tid == 32) to_l2(q_row + v0, (int64_t)n * sizeof(D));
-        int x = child >= 0 ? tokens[child] : -1;
-        float lx = x >= 0 ? (float)row[x] : 0.f, qx = x >= 0 && draft ? (float)q_row[x] : 1.f;
-        float m = -INFINITY;
+        // one pass: running maximum m and sum z of exponentials over it (a NaN stays in z), or the argmax
+        float m = -INFINITY, z = 0.f;
         int at = -1;
         bool nan = false;
         for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
-            float x[kBatch];
+            float l[kBatch];
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const int i = i0 + k * kThreads;
-                x[k] = i < n ? (float)row[v0 + i] : -INFINITY;
+                l[k] = i < n ? (float)row[v0 + i] : -INFINITY;
             }
+            if (temp == 0.f) {
 #pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const int i = i0 + k * kThreads;
-                if (i >= n) break;
-                if (temp == 0.f) {
-                    nan |= x[k] != x[k];
-                    if (x[k] > m) m = x[k], at = i + (int)v0;
-                } else {
-                    raw[i] = x[k] = temp == 1.f ? x[k] : x[k] / temp;
-                    m = fmaxf(m, x[k]);
+                for (int k = 0; k < kBatch; ++k) {
+                    nan |= l[k] != l[k];
+                    if (l[k] > m) m = l[k], at = i0 + k * kThreads + (int)v0;
                 }
+                continue;
             }
+            if (temp != 1.f)
+#pragma unroll
+                for (int k = 0; k < kBatch; ++k) l[k] /= temp;
+            float most = m;
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) {
+                const int i = i0 + k * kThreads;
+                if (i < n) raw[i] = l[k];
+                most = fmaxf(most, l[k]);
+            }
+            const float ref = most == -INFINITY ? 0.f : most;
+            z *= __expf(m - ref);
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) z += __expf(l[k] - ref);
+            m = most;
         }
         if (temp == 0.f) {
             const Note got = join_all<Best>(s, step, Note{m, nan ? 1.f : 0.f, at, 0});
             if (got.b != 0.f || got.i < 0 || got.a == INFINITY) break;   // no distribution here
-            while (child >= 0 && tokens[child] != got.i) child = next_child(parents, nodes, cur, child);
+            while (child >= 0 && x != got.i) next();
             if (child < 0) {
                 last = got.i;
                 break;
             }
         } else {
-            float z = 0.f;
-            const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-            for (int i = tid; i < n; i += kThreads) z += expf(raw[i] - ref);
             const Note got = join_all<Softmax>(s, step, Note{m, z, 0, 0});
             const float top = got.a;
             float sum = got.b;
@@ -238,14 +259,12 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
             while (child >= 0) {
                 const bool valid = x >= 0;
                 if (!valid && lead) report_device_error(p.err, 11);
-                const int next = next_child(parents, nodes, cur, child), x2 = next >= 0 ? tokens[next] : -1;
-                const float lx2 = x2 >= 0 ? (float)row[x2] : 0.f, qx2 = x2 >= 0 && draft ? (float)q_row[x2] : 1.f;
                 bool known = false;    // rejected already under another number
-                if (valid && !draft)
-                    for (int base = cur + 1; base < child; base += 32) {
-                        const int c = base + (tid & 31);
-                        known |= __any_sync(0xffffffffu, c < child && parents[c] == cur && tokens[c] == x);
-                    }
+                if (valid && !draft) {
+                    known = __any_sync(0xffffffffu, base + lane < child && xl == x);
+                    for (int c = cur + 1 + lane; c - lane < base; c += 32)
+                        known |= __any_sync(0xffffffffu, parents[c] == cur && tokens[c] == x);
+                }
                 if (valid && !known) {
                     const float e = expf((temp == 1.f ? lx : lx / temp) - top);
                     float rx = e / sum;
@@ -291,7 +310,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
                         ++rejected;
                     }
                 }
-                child = next, x = x2, lx = lx2, qx = qx2;
+                next();
             }
             if (child < 0) {
                 Note best = Best::none();
@@ -308,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
                         if (i >= n) break;
                         // (a common factor of r does not change which quotient is the largest; the quotient is good
                         // to two units in its last place)
-                        const float r = rejected ? raw[i] : expf(raw[i] - top);
+                        const float r = rejected ? raw[i] : __expf(raw[i] - top);
                         if (r > 0.f) Best::add(best, __fdividef(r, e[k]), i + (int)v0);
                     }
                 }
