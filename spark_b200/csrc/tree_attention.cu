@@ -523,20 +523,29 @@ __global__ void __launch_bounds__(kThreads, 1)
                     continue;
                 }
                 const int boxes = (min(kTok, sg.len - tile * kTok) + p.box_rows - 1) / p.box_rows;
-                if (elect_one()) mbar_expect_tx(bar, (uint32_t)(boxes * p.box_rows) * (C::kChunks * 128));
-                __syncwarp();
                 pages.advance(page_at, lane);
-                for (int box = 0; box < boxes; ++box) {
-                    const int page = pages.at(page_at);
-                    if (elect_one()) {
-                        if (page < 0 || page >= c.pages) report_device_error(p.err, 9);   // the load gives zeros
+                // four boxes at a time under one election
+#pragma unroll 1
+                for (int box = 0; box < boxes; box += 4) {
+                    int page[4], first[4];
 #pragma unroll
-                        for (int k = 0; k < C::kChunks; ++k)
-                            tma_load_4d(slot + (uint32_t)(k * kTok + box * p.box_rows) * 128, ctx_map, k * 64, sg.head, row, page, bar);
+                    for (int i = 0; i < 4; ++i) {
+                        page[i] = pages.at(page_at), first[i] = row;
+                        if (box + i < boxes && (row += p.box_rows) == page_size) row = 0, ++page_at;
+                    }
+                    if (elect_one()) {
+                        if (box == 0) mbar_expect_tx(bar, (uint32_t)(boxes * p.box_rows) * (C::kChunks * 128));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            if (box + i >= boxes) break;
+                            if (page[i] < 0 || page[i] >= c.pages) report_device_error(p.err, 9);   // the load gives zeros
+#pragma unroll
+                            for (int k = 0; k < C::kChunks; ++k)
+                                tma_load_4d(slot + (uint32_t)(k * kTok + (box + i) * p.box_rows) * 128, ctx_map, k * 64, sg.head, first[i],
+                                            page[i], bar);
+                        }
                     }
                     __syncwarp();
-                    row += p.box_rows;
-                    if (row == page_size) row = 0, ++page_at;
                 }
             }
         }
