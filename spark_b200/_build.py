@@ -2,7 +2,8 @@
 
 Each .cu compiles in parallel with nvcc; the objects link into one shared
 library next to this file, so it travels with the source tree.  Importing the
-package never compiles.
+package never compiles.  torch_binding.cpp becomes the extension module
+spark_b200._native beside it, linked to the library.
 """
 from __future__ import annotations
 
@@ -11,12 +12,15 @@ import glob
 import os
 import shutil
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "libspark_b200.so")
 OBJ_DIR = os.path.join(HERE, "_build")
+BINDING_SRC = os.path.join(CSRC, "torch_binding.cpp")
+BINDING = os.path.join(HERE, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -49,7 +53,33 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in _deps())
 
 
+def build_binding(force: bool = False) -> str:
+    """spark_b200._native: torch_binding.cpp on torch's headers, linked to LIB."""
+    newest = max(os.path.getmtime(p) for p in [BINDING_SRC] + glob.glob(os.path.join(INCLUDE, "*.h")))
+    if not force and os.path.exists(BINDING) and os.path.getmtime(BINDING) >= newest:
+        return BINDING
+    import torch
+    from torch.utils import cpp_extension as ext
+    tmp = BINDING + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           *(f"-isystem{p}" for p in [*ext.include_paths(), sysconfig.get_path("include")]), BINDING_SRC, "-o", tmp,
+           *(f"-L{p}" for p in ext.library_paths()), "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           LIB, "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {BINDING_SRC}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
+    _build_lib(force, verbose)
+    build_binding(force)
+    return LIB
+
+
+def _build_lib(force: bool, verbose: bool) -> str:
     if not force and up_to_date():
         return LIB
     nvcc = _nvcc()
@@ -71,7 +101,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         objs = list(ex.map(compile_one, _sources()))
     tmp = LIB + ".tmp"
-    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-o", tmp, *objs]
+    cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-shared", "-Xlinker", "-soname,libspark_b200.so", "-o", tmp,
+           *objs]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")

@@ -9,7 +9,6 @@ from __future__ import annotations
 import ctypes
 import os
 import re
-import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libspark_b200.so")
@@ -79,21 +78,6 @@ class SparkTreeVerify(ctypes.Structure):
                 ("parents_stride", ctypes.c_int64), ("uniforms", ctypes.c_void_p), ("uniforms_stride", ctypes.c_int64),
                 ("noise", ctypes.c_void_p), ("noise_stride", ctypes.c_int64), ("temperature", ctypes.c_void_p),
                 ("path", ctypes.c_void_p), ("accepted", ctypes.c_void_p), ("next", ctypes.c_void_p)]
-
-
-def packer(cls):
-    """A function from a structure's flat list of values to its bytes: packing
-    them at once takes a few microseconds less than setting the fields one by one."""
-    codes = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_double: "d"}
-
-    def flat(c):
-        if issubclass(c, ctypes.Structure):
-            return "".join(flat(t) for _, t in c._fields_)
-        return flat(c._type_) * c._length_ if issubclass(c, ctypes.Array) else codes[c]
-
-    s = struct.Struct("@" + flat(cls))
-    assert s.size == ctypes.sizeof(cls)
-    return s.pack
 
 
 class SparkError(RuntimeError):

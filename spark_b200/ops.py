@@ -8,7 +8,6 @@ the functions can stand in for the reference emulators that take CPU tensors.
 from __future__ import annotations
 
 import ctypes
-import struct
 import threading
 
 import torch
@@ -516,11 +515,26 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 MAX_TREE_NODES = 64    # of one sequence in tree_attention (SPARK_MAX_TREE_NODES)
 
 _tree_ws: dict[tuple[int, int], torch.Tensor] = {}
-_pack_heads = _lib.packer(_lib.SparkRopeHeads)
-_pack_cache = _lib.packer(_lib.SparkPagedCache)
-_pack_attention = _lib.packer(_lib.SparkTreeAttention)
-_pack_verify = _lib.packer(_lib.SparkTreeVerify)
-_pack_strides = struct.Struct("@qqq").pack
+_native_module = None
+
+
+def _native():
+    """spark_b200._native: checks, outputs and the C call of the functions below."""
+    global _native_module
+    if _native_module is None:
+        _lib.lib()
+        try:
+            from . import _native as module
+        except ImportError as e:
+            raise RuntimeError("spark_b200._native is missing or does not load: build it with "
+                               "`python -c 'import __graft_entry__ as g; g.build()'`") from e
+        _native_module = module
+    return _native_module
+
+
+def _check(name: str, rc: int) -> None:
+    if rc != _lib.OK:
+        raise _lib.SparkError(name, rc, _lib.last_error())
 
 
 def _tree_workspace(device: torch.device, stream: int, nbytes: int = 256) -> torch.Tensor:
@@ -537,30 +551,15 @@ def _tree_workspace(device: torch.device, stream: int, nbytes: int = 256) -> tor
     return buf
 
 
-def _raw_stream(index: int) -> int:
-    """The current stream's handle (torch.cuda.current_stream builds an object, 2 us)."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-def _on_gpu(what: str, index: int, **tensors) -> None:
-    """Names the tensor that is not on device `index`."""
-    for name, t in tensors.items():
-        if t is not None and t.get_device() != index:
-            raise RuntimeError(f"spark_b200.{what}: {name} must be on cuda:{index}, it is on {t.device}")
-
-
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
-
-
-def _tma(t: torch.Tensor) -> torch.Tensor:
-    """A 4-D t, or a copy of it where the kernels' 16-byte loads do not fit its address or strides."""
-    s0, s1, s2, s3 = t.stride()
-    if s3 == 1 and not (t.data_ptr() & 15) and not ((s0 | s1 | s2) & 7):
-        return t
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip((s0, s1, s2), t.shape) if n > 1):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+def _place(what: str, t: torch.Tensor, nbytes: int = 256):
+    """(workspace, its address, the current stream's handle) on t's device."""
+    index = t.get_device()
+    if index < 0:
+        raise RuntimeError(f"spark_b200.{what}: expected a CUDA tensor, got one on {t.device}")
+    # (torch.cuda.current_stream builds an object for it, 2 us)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws = _tree_workspace(t.device, stream, nbytes)
+    return ws, ws.data_ptr(), stream
 
 
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
@@ -573,70 +572,12 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
     one leading (batch) dimension; strided views are read in place.  out: (q', k')
     tensors to write to, q and k themselves among them.  A position outside the
     table gives a zero row and an error that check_device_errors() raises."""
-    index = q.get_device()
-    if index < 0:
-        raise RuntimeError("spark_b200.rope: q must be a CUDA tensor")
-    if positions.get_device() != index or table.get_device() != index or (k is not None and k.get_device() != index):
-        _on_gpu("rope", index, k=k, positions=positions, table=table)
-    shape = q.shape
-    if len(shape) not in (3, 4) or (k is not None and (k.shape[:-2] != shape[:-2] or k.shape[-1] != shape[-1])):
-        raise ValueError(f"rope: q and k must be [(batch,) tokens, heads, head_dim] of the same tokens, got "
-                         f"{list(shape)} and {None if k is None else list(k.shape)}")
-    dtype = q.dtype
-    if k is not None and k.dtype is not dtype:
-        raise TypeError(f"rope: q is {dtype}, k is {k.dtype}")
-    if positions.shape != shape[:-2]:
-        raise ValueError(f"rope: positions are {list(positions.shape)}, the tokens {list(shape[:-2])}")
-    if positions.dtype is not torch.int64 and positions.dtype is not torch.int32:
-        raise TypeError(f"rope: positions must be int32 or int64, got {positions.dtype}")
-    if table.dim() != 2 or table.dtype is not torch.float32 or not table.is_contiguous():
-        raise TypeError("rope: table must be a contiguous float32 [rows, rot_dim]")
-    dt = _dt(q)
-    q_out, q_part = _rope_part(q, None if out is None else out[0])
-    k_out, k_part = (None, None) if k is None else _rope_part(k, None if out is None else out[1])
-    batch, tokens = (1, shape[0]) if len(shape) == 3 else shape[:2]
-    positions = positions.contiguous()
-    rows, rot = table.shape
-    s = _raw_stream(index)
-    ws = _tree_workspace(q.device, s)
-    call("spark_rope", q_part, k_part, dt, batch, tokens, shape[-1], rot, interleaved, inverse, positions.data_ptr(),
-         positions.element_size(), table.data_ptr(), rows, ws.data_ptr(), s)
+    _, ws, stream = _place("rope", q)
+    q_out, k_out = (None, None) if out is None else out
+    q_out, k_out, rc = _native().rope(q, k, positions, table, interleaved, inverse, q_out, k_out, ws, stream)
+    if rc:
+        _check("spark_rope", rc)
     return q_out, k_out
-
-
-def _rope_part(x: torch.Tensor, y: torch.Tensor | None):
-    """(output, packed SparkRopeHeads) of q or k."""
-    x = _unit(x)
-    if y is None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    elif y.shape != x.shape or y.dtype != x.dtype or y.device != x.device or y.stride(-1) != 1:
-        raise ValueError("rope: out must have the shapes, type and device of q and k, with unit stride along the head")
-    if x.dim() == 4:
-        x0, x1, x2, _ = x.stride()
-        y0, y1, y2, _ = y.stride()
-    else:
-        x0 = y0 = 0
-        x1, x2, _ = x.stride()
-        y1, y2, _ = y.stride()
-    return y, _pack_heads(x.data_ptr(), y.data_ptr(), x.shape[-2], x0, x1, x2, y0, y1, y2)
-
-
-def _cache_args(what: str, index: int, k_cache, v_cache, page_table, lens, dtype) -> tuple:
-    """The values of a SparkPagedCache after its checks."""
-    if (k_cache.get_device() != index or v_cache.get_device() != index or page_table.get_device() != index
-            or lens.get_device() != index):
-        _on_gpu(what, index, k_cache=k_cache, v_cache=v_cache, page_table=page_table, context_lens=lens)
-    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
-    if len(shape) != 4 or v_cache.shape != shape or ks[3] != 1 or vs[3] != 1:
-        raise ValueError(f"{what}: k_cache and v_cache must be [pages, page_size, kv_heads, head_dim] with unit stride "
-                         "along the head")
-    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
-        raise TypeError(f"{what}: the cache is {k_cache.dtype} and {v_cache.dtype}, the tokens are {dtype}")
-    if (page_table.dtype is not torch.int32 or lens.dtype is not torch.int32 or page_table.dim() != 2
-            or page_table.stride(1) != 1 or not lens.is_contiguous() or lens.shape != page_table.shape[:1]):
-        raise TypeError(f"{what}: page_table must be int32 [batch, max_pages], context_lens a contiguous int32 [batch]")
-    return (k_cache.data_ptr(), v_cache.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], *shape,
-            page_table.data_ptr(), page_table.stride(0), page_table.shape[1], lens.data_ptr(), _DT[dtype])
 
 
 def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -648,39 +589,10 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
     index (int32 [batch, n]): which tokens, in order, e.g. tree_verify's path; counts
     (int32 [batch]): how many of them.  Without both, all tokens go in.  What does not
     fit a sequence's pages is left out and reported by check_device_errors()."""
-    shape = k_new.shape
-    if len(shape) != 4 or v_new.shape != shape or shape[2:] != k_cache.shape[2:]:
-        raise ValueError(f"kv_append: k_new and v_new must be [batch, tokens, {', '.join(map(str, k_cache.shape[2:]))}], "
-                         f"got {list(shape)} and {list(v_new.shape)}")
-    dtype = k_new.dtype
-    if dtype not in _DT or v_new.dtype is not dtype:
-        raise TypeError(f"kv_append: float32, bfloat16 or float16 tokens, got {dtype} and {v_new.dtype}")
-    at = k_cache.get_device()
-    if at < 0:
-        raise RuntimeError("spark_b200.kv_append: the cache must be on a CUDA device")
-    cache = _cache_args("kv_append", at, k_cache, v_cache, page_table, context_lens, dtype)
-    if (k_new.get_device() != at or v_new.get_device() != at or (index is not None and index.get_device() != at)
-            or (counts is not None and counts.get_device() != at)):
-        _on_gpu("kv_append", at, k_new=k_new, v_new=v_new, index=index, counts=counts)
-    batch, tokens = shape[:2]
-    if context_lens.shape[0] != batch:
-        raise ValueError(f"kv_append: {batch} sequences of tokens, {context_lens.shape[0]} in the page table")
-    width, index_ptr, counts_ptr = tokens, None, None
-    if index is not None:
-        if index.dtype is not torch.int32 or index.dim() != 2 or index.shape[0] != batch:
-            raise TypeError("kv_append: index must be int32 [batch, n]")
-        index = index.contiguous()
-        width, index_ptr = index.shape[1], index.data_ptr()
-    if counts is not None:
-        if counts.dtype is not torch.int32 or counts.shape != (batch,) or not counts.is_contiguous():
-            raise TypeError("kv_append: counts must be a contiguous int32 [batch]")
-        counts_ptr = counts.data_ptr()
-    k, v = _unit(k_new), _unit(v_new)
-    new_lens = torch.empty(batch, dtype=torch.int32, device=k_cache.device)
-    s = _raw_stream(at)
-    ws = _tree_workspace(k_cache.device, s)
-    call("spark_kv_append", _pack_cache(*cache), batch, tokens, k.data_ptr(), _pack_strides(*k.stride()[:3]),
-         v.data_ptr(), _pack_strides(*v.stride()[:3]), index_ptr, width, counts_ptr, new_lens.data_ptr(), ws.data_ptr(), s)
+    _, ws, stream = _place("kv_append", k_cache)
+    new_lens, rc = _native().kv_append(k_new, v_new, k_cache, v_cache, page_table, context_lens, index, counts, ws, stream)
+    if rc:
+        _check("spark_kv_append", rc)
     return new_lens
 
 
@@ -698,51 +610,14 @@ def tree_attention(q: torch.Tensor, k_tree: torch.Tensor, v_tree: torch.Tensor, 
     head_dim ** -0.5, it must be positive.  page_size and head_dim (up to 256) must be
     multiples of 8, q_heads at most 128 times kv_heads.  Returns out [batch, nodes, q_heads, head_dim], with return_lse
     also the natural log of the softmax sums, fp32 [batch, nodes, q_heads]."""
-    index = q.get_device()
-    if index < 0:
-        raise RuntimeError("spark_b200.tree_attention: q must be a CUDA tensor")
-    shape, ks = q.shape, k_tree.shape
-    if len(shape) != 4 or len(ks) != 4 or v_tree.shape != ks or ks[:2] != shape[:2]:
-        raise ValueError(f"tree_attention: q must be [batch, nodes, q_heads, head_dim], k_tree and v_tree the same with "
-                         f"kv_heads, got {list(shape)}, {list(ks)}, {list(v_tree.shape)}")
-    batch, nodes, heads, dim = shape
-    if ks[2:] != k_cache.shape[2:] or dim != ks[3]:
-        raise ValueError("tree_attention: q, k_tree, v_tree and the cache differ in heads or head_dim")
-    dtype = q.dtype
-    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k_tree.dtype is not dtype or v_tree.dtype is not dtype:
-        raise TypeError(f"tree_attention: bfloat16 or float16 throughout, got {dtype}, {k_tree.dtype}, {v_tree.dtype}")
-    cache = _cache_args("tree_attention", index, k_cache, v_cache, page_table, context_lens, dtype)
-    if k_tree.get_device() != index or v_tree.get_device() != index or parents.get_device() != index:
-        _on_gpu("tree_attention", index, k_tree=k_tree, v_tree=v_tree, parents=parents)
-    if context_lens.shape[0] != batch:
-        raise ValueError(f"tree_attention: {batch} sequences of queries, {context_lens.shape[0]} in the page table")
-    if parents.dtype is not torch.int32 or (parents.shape != shape[:2] and parents.shape != (nodes,)):
-        raise TypeError(f"tree_attention: parents must be int32 [{nodes}] or [{batch}, {nodes}]")
-    parents = _unit(parents)
-    device = q.device
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
-    elif out.shape != shape or out.dtype != dtype or out.device != device or out.stride(3) != 1:
-        raise ValueError("tree_attention: out must have q's shape, type and device, with unit stride along the head")
-    q, k, v = _tma(q), _tma(k_tree), _tma(v_tree)
-    lse = torch.empty(batch, nodes, heads, dtype=torch.float32, device=device) if return_lse else None
-    q0, q1, q2, _ = q.stride()
-    k0, k1, k2, _ = k.stride()
-    v0, v1, v2, _ = v.stride()
-    o0, o1, o2, _ = out.stride()
-    a = _pack_attention(*cache, batch, nodes, heads, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                        q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2, parents.data_ptr(),
-                        parents.stride(0) if parents.dim() == 2 else 0, lse.data_ptr() if return_lse else 0,
-                        dim ** -0.5 if scale is None else scale)
-    s = _raw_stream(index)
-    ws = _tree_workspace(device, s)
-    try:
-        call("spark_tree_attention", a, ws.data_ptr(), ws.numel(), s)
-    except _lib.SparkError as e:
-        if e.code != _lib.ERR_WORKSPACE:
-            raise
-        ws = _tree_workspace(device, s, int(_lib.lib().spark_tree_attention_workspace_size(a)))
-        call("spark_tree_attention", a, ws.data_ptr(), ws.numel(), s)
+    ws, ptr, stream = _place("tree_attention", q)
+    args = (q, k_tree, v_tree, k_cache, v_cache, page_table, context_lens, parents, scale)
+    out, lse, rc, need = _native().tree_attention(*args, out, return_lse, ptr, ws.numel(), stream)
+    if rc == _lib.ERR_WORKSPACE and need > ws.numel():
+        ws, ptr, stream = _place("tree_attention", q, need)
+        out, lse, rc, need = _native().tree_attention(*args, out, return_lse, ptr, ws.numel(), stream)
+    if rc:
+        _check("spark_tree_attention", rc)
     return (out, lse) if return_lse else out
 
 
@@ -759,50 +634,11 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     path int32 [batch, nodes] (accepted nodes from node 0, then -1), accepted int32
     [batch] (how many) and next int64 [batch], the token after them (-1 where the
     logits give no distribution)."""
-    index = logits.get_device()
-    if index < 0:
-        raise RuntimeError("spark_b200.tree_verify: logits must be a CUDA tensor")
-    shape = logits.shape
-    if len(shape) != 3:
-        raise ValueError(f"tree_verify: logits must be [batch, nodes, vocab], got {list(shape)}")
-    batch, nodes, vocab = shape
-    if (tokens.get_device() != index or parents.get_device() != index or uniforms.get_device() != index
-            or noise.get_device() != index or (draft_probs is not None and draft_probs.get_device() != index)):
-        _on_gpu("tree_verify", index, tokens=tokens, parents=parents, uniforms=uniforms, noise=noise,
-                draft_probs=draft_probs)
-    per_node = shape[:2]
-    if draft_probs is not None and draft_probs.shape != shape:
-        raise ValueError(f"tree_verify: draft_probs are {list(draft_probs.shape)}, logits {list(shape)}")
-    if tokens.shape != per_node or uniforms.shape != per_node or noise.shape != (batch, vocab):
-        raise ValueError(f"tree_verify: tokens and uniforms must be [{batch}, {nodes}], noise [{batch}, {vocab}]")
-    if tokens.dtype is not torch.int64 or uniforms.dtype is not torch.float32 or noise.dtype is not torch.float32:
-        raise TypeError("tree_verify: tokens must be int64, uniforms and noise float32")
-    if parents.dtype is not torch.int32 or (parents.shape != per_node and parents.shape != (nodes,)):
-        raise TypeError(f"tree_verify: parents must be int32 [{nodes}] or [{batch}, {nodes}]")
-    device = logits.device
+    _, ws, stream = _place("tree_verify", logits)
     if not isinstance(temperature, torch.Tensor):
-        temperature = None if temperature == 1.0 else torch.full((batch,), float(temperature), device=device)
-    elif temperature.dtype is not torch.float32 or temperature.shape != (batch,) or temperature.get_device() != index:
-        raise TypeError(f"tree_verify: temperature must be a number or float32 [{batch}] on {device}")
-    else:
-        temperature = temperature.contiguous()
-    x = _unit(logits)
-    x0, x1, _ = x.stride()
-    d_ptr, d_type, d0, d1 = 0, 0, 0, 0
-    if draft_probs is not None:
-        draft_probs = _unit(draft_probs)
-        d_ptr, d_type = draft_probs.data_ptr(), _dt(draft_probs)
-        d0, d1, _ = draft_probs.stride()
-    tokens, parents, uniforms, noise = _unit(tokens), _unit(parents), _unit(uniforms), _unit(noise)
-    path = torch.empty(per_node, dtype=torch.int32, device=device)
-    accepted = torch.empty(batch, dtype=torch.int32, device=device)
-    last = torch.empty(batch, dtype=torch.int64, device=device)
-    a = _pack_verify(batch, nodes, vocab, x.data_ptr(), _dt(x), x0, x1, d_ptr, d_type, d0, d1, tokens.data_ptr(),
-                     tokens.stride(0), parents.data_ptr(), parents.stride(0) if parents.dim() == 2 else 0,
-                     uniforms.data_ptr(), uniforms.stride(0), noise.data_ptr(), noise.stride(0),
-                     temperature.data_ptr() if temperature is not None else 0, path.data_ptr(), accepted.data_ptr(),
-                     last.data_ptr())
-    s = _raw_stream(index)
-    ws = _tree_workspace(device, s)
-    call("spark_tree_verify", a, ws.data_ptr(), s)
+        temperature = None if temperature == 1.0 else torch.full((logits.shape[0],), float(temperature), device=logits.device)
+    path, accepted, last, rc = _native().tree_verify(logits, tokens, parents, uniforms, noise, draft_probs, temperature, ws,
+                                                     stream)
+    if rc:
+        _check("spark_tree_verify", rc)
     return path, accepted, last

@@ -637,11 +637,17 @@ def test_refusals():
                     (ValueError, {"q": q[..., :32]}), (ValueError, {"v_cache": vc[:, :8]}),
                     (ValueError, {"out": q[:, :1].clone()}), (RuntimeError, {"q": q.cpu()}),
                     (RuntimeError, {"page_table": table.cpu()}), (RuntimeError, {"k_cache": kc.cpu()}),
-                    (SparkError, {"q": q[:, :, :7]})):
+                    (SparkError, {"q": q[:, :, :7]}), (SparkError, {"scale": 0.0}), (SparkError, {"scale": -1.0})):
         with pytest.raises(err):
             attention(**kw)
     y = make(g, 1, 65, 2, 2, 64, [30], 16, BF)
     with pytest.raises(SparkError, match="64 nodes"):
+        o.tree_attention(*y)
+    y = make(g, 1, 2, 129, 1, 64, [30], 16, BF)
+    with pytest.raises(SparkError, match="at most 128"):
+        o.tree_attention(*y)
+    y = make(g, 1, 2, 2, 2, 64, [30], 12, BF)
+    with pytest.raises(SparkError, match="page_size"):
         o.tree_attention(*y)
     y = make(g, 1, 2, 2, 2, 264, [30], 16, BF)
     with pytest.raises(SparkError, match="head_dim"):

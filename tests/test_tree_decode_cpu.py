@@ -107,13 +107,24 @@ def test_verify_checks():
     assert _lib.lib().spark_tree_verify(None, None, None) == _lib.ERR_INVALID
 
 
-def test_packed_structures_are_what_ctypes_lays_out():
-    a = attention(lse=7777, parents_stride=4)
-    c = a.cache
-    flat = (c.k, c.v, *c.k_stride, *c.v_stride, c.pages, c.page_size, c.kv_heads, c.head_dim, c.page_table,
-            c.page_table_stride, c.max_pages, c.lens, c.dtype, a.batch, a.nodes, a.q_heads, a.q, a.k, a.v, a.out,
-            *a.q_stride, *a.kn_stride, *a.vn_stride, *a.out_stride, a.parents, a.parents_stride, a.lse, a.scale)
-    assert _lib.packer(_lib.SparkTreeAttention)(*flat) == bytes(a)
+def test_the_torch_binding_loads_and_refuses_cpu_tensors():
+    from spark_b200 import ops
+    x = torch.zeros(2, 3, 64)
+    i = torch.zeros(2, 2, dtype=torch.int32)
+    for call in (lambda: ops.rope(x, None, i[0], torch.zeros(4, 8)),
+                 lambda: ops.kv_append(x[None], x[None], x[None], x[None], i, i[0]),
+                 lambda: ops.tree_attention(x[None], x[None], x[None], x[None], x[None], i, i[0], i),
+                 lambda: ops.tree_verify(x, i, i, x[..., 0], x[:, 0])):
+        with pytest.raises(RuntimeError, match="CUDA tensor"):
+            call()
+    n = ops._native()
+    with pytest.raises(RuntimeError, match="q must be a CUDA tensor"):
+        n.rope(x, None, i[0], torch.zeros(4, 8), False, False, None, None, 0, 0)
+    # the checks before the device's, by their kinds
+    with pytest.raises(ValueError, match="kv_append"):
+        n.kv_append(x, x, x, x, i, i[0], None, None, 0, 0)
+    with pytest.raises(TypeError, match="differ in type"):
+        n.kv_append(x[None], x[None].half(), x[None], x[None], i, i[0], None, None, 0, 0)
 
 
 def test_rope_frequencies():
