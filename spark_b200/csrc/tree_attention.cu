@@ -363,13 +363,12 @@ __device__ __forceinline__ bool await_parts(int* count, int parts, int lane) {
     return all_ok(ok);
 }
 
-// This warp's share of the sum of an item's parts.  A lane adds four columns of
-// four rows at a time, four parts loaded together: the loads' latency is what
-// this costs.
-template <int DP, bool BF>
+// This warp's share of the sum of an item's parts.  A lane adds U times four
+// columns of a row, PU parts loaded together: the loads' latency is what this
+// costs, about a microsecond a round.
+template <int DP, bool BF, int U, int PU>
 __device__ __forceinline__ void add_parts(const Params& p, const Segment& sg, int c0, int parts) {
     const SparkTreeAttention& a = p.a;
-    constexpr int U = 4, PU = 4;
     const int rows = p.rows_item, n = rows * (int)((a.cache.head_dim + 3) / 4), step = parts * 256;
 #pragma unroll 1
     for (int e0 = ((int)blockIdx.x - c0) * 256 + (int)threadIdx.x; e0 < n; e0 += U * step) {
@@ -914,7 +913,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < cuts) add_release(p.count + 2 * sm.cut[lane].c0, 1);
         for (int k = 0; k < cuts && ok; ++k) ok = await_parts(p.count + 2 * sm.cut[k].c0, sm.cut[k].parts, lane);
 #pragma unroll 1
-        for (int k = 0; k < cuts && ok; ++k) add_parts<DP, BF>(p, sm.cut[k].sg, sm.cut[k].c0, sm.cut[k].parts);
+        for (int k = 0; k < cuts && ok; ++k) {
+            const Cut& cut = sm.cut[k];
+            // one value a lane: few rows, often many parts
+            if (p.rows_item * DP <= cut.parts * 1024) add_parts<DP, BF, 1, 16>(p, cut.sg, cut.c0, cut.parts);
+            else add_parts<DP, BF, 4, 4>(p, cut.sg, cut.c0, cut.parts);
+        }
     }
     if (!ok) report_device_error(p.err, 10);
     __syncwarp();
