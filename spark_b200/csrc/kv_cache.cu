@@ -2,7 +2,10 @@
 //
 // Position n of sequence b is row n % page_size of page page_table[b, n /
 // page_size].  The kernel moves rows of kv_heads x head_dim values; its bound
-// is HBM (each value is read and written once).
+// is HBM (each value is read and written once).  A block moves K and V of two
+// tokens, four 16-byte loads of a thread on the way together: 8192 tokens of 32
+// heads of 128 in bf16 44 us (6.1 TB/s; four tokens a block, whose pointers take
+// half as many registers again, 47 us).
 #include <algorithm>
 
 #include "common.cuh"
@@ -20,9 +23,8 @@ struct Params {
     int elem;   // bytes of a value
 };
 
-// T: what is moved at a time, `per_head` of them a head.  A block moves K and V
-// of kTokens tokens, so that many loads are on the way together.
-constexpr int kTokens = 4;
+// T: what is moved at a time.
+constexpr int kTokens = 2;   // of a block
 template <typename T, int E>   // E values in a T
 __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Params p) {
     const int64_t b = blockIdx.y;

@@ -39,6 +39,20 @@
 //                   and elect a lane for each instruction, so that the operands stay
 //                   in uniform registers: under a branch on the lane an MMA took 110
 //                   cycles to issue and a load 500, more than they take to run.
+// What bounds it.  A tile of 128 tokens x 128 values is 64 KB of K and V: 2670
+// cycles of an SM's share of HBM at 1.8 GHz, against 1024 of tensor cores for a
+// stream's 128 rows (an MMA of 128 x 128 x 16 takes 64, also with Q from shared
+// memory; 128 x 64 from shared memory takes 48, so that tiles of 64 tokens cost
+// more) and about 2100 of softmax (1024 of them the exponential unit's).  In turns
+// two streams hide each other's chains and HBM bounds: 16 sequences of up to 32k
+// tokens, 128 rows, 2430 cycles a tile, 287 us (5.8 TB/s).  By rows a tile is
+// 2 x (1024 + 2100) cycles of work on two engines that wait for each other: 64
+// nodes x 8 heads over 65k tokens, 3990 cycles a tile, 132 us (0.91 PFLOP/s), where
+// neither is full.  Both run into the power cap when repeated (1000 W at 1.4 GHz:
+// 313 us, 153 us).  Small calls are their start (5 us to the first scores: lengths,
+// page numbers and the first tile are three round trips to memory) and their end
+// (about 6 us: the parts' stores made visible, counted, read and added).
+//
 // Every wait is bounded (2 s); one that expires sets error 10 and all roles end.
 #include <cuda.h>
 #include <cudaTypedefs.h>
