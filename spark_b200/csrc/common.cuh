@@ -26,6 +26,26 @@ int check_launch(const char* what);
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
+// Launches `kernel` so that its blocks may be set up while the previous kernel of
+// the stream still ends (programmatic stream serialization); the kernel has to
+// call grid_wait() before it touches memory.
+template <typename... P, typename... A>
+inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+// Lets the next such kernel be set up, then waits for the previous one's results.
+__device__ __forceinline__ void grid_wait() {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ dtypes
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t i) {
     if (dtype == SPARK_DTYPE_F32) return reinterpret_cast<const float*>(p)[i];

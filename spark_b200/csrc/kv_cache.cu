@@ -27,6 +27,7 @@ struct Params {
 constexpr int kTokens = 2;   // of a block
 template <typename T, int E>   // E values in a T
 __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Params p) {
+    grid_wait();
     const int64_t b = blockIdx.y;
     const int64_t len = p.c.lens[b];
     const int64_t room = p.c.max_pages * p.c.page_size - len;
@@ -122,13 +123,13 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     for (const int64_t* st : {(const int64_t*)p.ks, (const int64_t*)p.vs, cache->k_stride, cache->v_stride})
         for (int i = 0; i < 3; ++i) fits = fits && st[i] % vec == 0;
     if (fits && vec == 4)
-        k_kv_append<uint4, 4><<<grid, 256, 0, s>>>(p);
+        launch_overlapped(k_kv_append<uint4, 4>, grid, 256, 0, s, p);
     else if (fits)
-        k_kv_append<uint4, 8><<<grid, 256, 0, s>>>(p);
+        launch_overlapped(k_kv_append<uint4, 8>, grid, 256, 0, s, p);
     else if (vec == 4)
-        k_kv_append<float, 1><<<grid, 256, 0, s>>>(p);
+        launch_overlapped(k_kv_append<float, 1>, grid, 256, 0, s, p);
     else
-        k_kv_append<uint16_t, 1><<<grid, 256, 0, s>>>(p);
+        launch_overlapped(k_kv_append<uint16_t, 1>, grid, 256, 0, s, p);
     return check_launch("spark_kv_append");
 }
 

@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params
     using V = Vec<T, N>;
     using R = typename V::type;
     constexpr int PAIRS = INTER ? N / 2 : N;
+    grid_wait();
     const int heads = p.part[0].heads + p.part[1].heads, groups = (heads + kHeads - 1) / kHeads;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t rest = i / units, tok = rest / groups;
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params
 
 // What not even a pair's access fits (interleaved pairs at an odd address): a thread a pair.
 __global__ void __launch_bounds__(256) k_rope(const __grid_constant__ Params p) {
+    grid_wait();
     const int half = p.rot / 2, items = half + (p.dim - p.rot);   // pairs, then copied values
     const int heads = p.part[0].heads + p.part[1].heads;
     const int64_t n = p.n_tokens * heads * items;
@@ -189,11 +191,11 @@ template <typename T, int N>
 void launch(const Params& p, unsigned grid, int units, int turned, cudaStream_t s) {
     if constexpr (N > 1) {
         if (p.interleaved) {
-            k_rope_vec<T, N, true><<<grid, 256, 0, s>>>(p, units, turned);
+            launch_overlapped(k_rope_vec<T, N, true>, grid, 256, 0, s, p, units, turned);
             return;
         }
     }
-    k_rope_vec<T, N, false><<<grid, 256, 0, s>>>(p, units, turned);
+    launch_overlapped(k_rope_vec<T, N, false>, grid, 256, 0, s, p, units, turned);
 }
 template <typename T>
 void launch(const Params& p, int vec, unsigned grid, int units, int turned, cudaStream_t s) {
@@ -270,7 +272,7 @@ int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int dtype, int6
     }
     const int64_t n = p.n_tokens * heads * (rot_dim / 2 + head_dim - rot_dim);
     const int grid = (int)std::min<int64_t>((n + 255) / 256, 148 * 16);
-    k_rope<<<grid, 256, 0, s>>>(p);
+    launch_overlapped(k_rope, grid, 256, 0, s, p);
     return check_launch("spark_rope");
 }
 

@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant_
     const float* noise = a.noise + b * a.noise_stride + v0;
     const L* logits = reinterpret_cast<const L*>(a.logits) + b * a.logits_stride[0];
     const D* draft = a.draft ? reinterpret_cast<const D*>(a.draft) + b * a.draft_stride[0] : nullptr;
+    grid_wait();
     const float temp = a.temperature ? a.temperature[b] : 1.f;
     const bool lead = rank == 0 && tid == 0;
     int step = 0, cur = 0, accepted = 1;
@@ -360,11 +361,13 @@ int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = ((size_t)p.slice + 3 * (size_t)p.a.nodes) * sizeof(float);
     cfg.stream = s;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)cs, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     e = cudaLaunchKernelEx(&cfg, k_tree_verify<L, D>, p);
     if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: launch failed: %s", cudaGetErrorString(e));
     return check_launch("spark_tree_verify");
