@@ -344,12 +344,15 @@ __device__ __forceinline__ int cta_of(int total, int pos) {
     return (int)(((uint64_t)(pos + 1) * ctas(total) - 1) / (unsigned)total);
 }
 
-// Scores that a row does not see: of 64 from column h on, those of the tree outside its mask, of the context from `valid` on.
-__device__ __forceinline__ void hide(float (&x)[64], bool tree, uint64_t mask, int valid, int h) {
-    const uint64_t sees = tree ? (h ? 0 : mask) : (valid >= 64 ? ~0ull : (valid > 0 ? (1ull << valid) - 1 : 0));
+// Scores that a row does not see: of 64, those of the tree outside its mask, of the context from `valid` (> 0) on.
+__device__ __forceinline__ void hide(float (&x)[64], bool tree, uint64_t mask, int valid) {
+    const uint64_t sees = tree ? mask : (valid >= 64 ? ~0ull : (1ull << valid) - 1);   // (h < valid; the tree has one run of 64)
+    const uint32_t lo = (uint32_t)sees, hi = (uint32_t)(sees >> 32);
 #pragma unroll
-    for (int e = 0; e < 64; ++e)
-        if (!((sees >> e) & 1)) x[e] = -INFINITY;
+    for (int e = 0; e < 32; ++e) {
+        if (!(lo & (1u << e))) x[e] = -INFINITY;
+        if (!(hi & (1u << e))) x[e + 32] = -INFINITY;
+    }
 }
 
 // The node and query head of a row of an item, -1 where it has none.
@@ -708,18 +711,20 @@ __global__ void __launch_bounds__(kThreads, 1)
                     s_phase ^= 1u << buf;
                     if (!ok) break;
                     tc_fence_after();
-                    const bool masked = tree || valid < kTok;
                     if (work) {
                         const uint32_t st = tmem + lane_off + (uint32_t)buf * kTok;
                         // scores are read twice, 64 at a time: kept, 128 would not fit the registers (next to no
                         // first-level cache is left beside the tiles, a spill costs more than the second read)
+                        // Columns behind the last group of 16 that has a token are not multiplied: a tile of up to 64
+                        // tokens, as every tree is, is done after the first 64 (many short contexts 49 -> 46 us).
+                        const int cols = kTok > 64 && valid <= 64 ? 64 : kTok;
                         float x[64], most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-                        for (int h = 0; h < kTok; h += 64) {
+                        for (int h = 0; h < cols; h += 64) {
                             tmem_ld32(st + h, x);
                             tmem_ld32(st + h + 32, x + 32);
                             tmem_wait_ld();
-                            if (masked) hide(x, tree, mask, valid - h, h);
+                            if (tree || valid < h + 64) hide(x, tree, mask, valid - h);
 #pragma unroll
                             for (int e = 0; e < 64; e += 8)
 #pragma unroll
@@ -754,12 +759,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const float2 scale2 = make_float2(p.scale, p.scale), ref2 = make_float2(-ref, -ref);
                         float2 sums[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll 1
-                        for (int h = 0; h < kTok; h += 64) {
+                        for (int h = 0; h < cols; h += 64) {
                             if (kTok > 64) {
                                 tmem_ld32(st + h, x);
                                 tmem_ld32(st + h + 32, x + 32);
                                 tmem_wait_ld();
-                                if (masked) hide(x, tree, mask, valid - h, h);
+                                if (tree || valid < h + 64) hide(x, tree, mask, valid - h);
                             }
                             // the weights of h.. take the columns of the scores h / 2.., which are done with
 #pragma unroll
