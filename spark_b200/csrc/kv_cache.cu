@@ -2,10 +2,13 @@
 //
 // Position n of sequence b is row n % page_size of page page_table[b, n /
 // page_size].  The kernel moves rows of kv_heads x head_dim values; its bound
-// is HBM (each value is read and written once).  A block moves K and V of two
-// tokens, four 16-byte loads of a thread on the way together: 8192 tokens of 32
-// heads of 128 in bf16 44 us (6.1 TB/s; four tokens a block, whose pointers take
-// half as many registers again, 47 us).
+// is HBM (each value is read and written once).  A group of threads, as many as
+// a row has 16-byte pieces (a power of two of 8 to 256), moves K and V of two
+// tokens, four loads of a thread on the way together: 8192 tokens of 32 heads of
+// 128 in bf16 44 us (6.1 TB/s; four tokens a group, whose pointers take half as
+// many registers again, 47 us).  A block has as many groups as fit: with one of
+// 256 threads, most of them idle in short rows, 8192 tokens of one head of 80 in
+// fp32 took 14.6 us, now 4.4, and of 8 heads of 64 8.6, now 4.6.
 #include <algorithm>
 
 #include "common.cuh"
@@ -20,11 +23,11 @@ struct Params {
     int64_t batch, tokens, width;
     const int *index, *counts;
     int *new_lens, *err;
-    int elem;   // bytes of a value
+    int group;   // threads that move a row, a power of two
 };
 
 // T: what is moved at a time.
-constexpr int kTokens = 2;   // of a block
+constexpr int kTokens = 2;   // of a group
 template <typename T, int E>   // E values in a T
 __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Params p) {
     grid_wait();
@@ -36,9 +39,10 @@ __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Param
     n = len < 0 || n < 0 ? 0 : n;
     n = n > p.width ? p.width : n;
     n = n > room ? (room < 0 ? 0 : room) : n;
+    const int slot = (int)threadIdx.x / p.group, lane = (int)threadIdx.x % p.group;
     if (blockIdx.x == 0 && threadIdx.x == 0) p.new_lens[b] = (int)(len + n);
     const int per_head = (int)p.c.head_dim / E, row = (int)p.c.kv_heads * per_head;
-    const int64_t j0 = (int64_t)blockIdx.x * kTokens;
+    const int64_t j0 = ((int64_t)blockIdx.x * (256 / p.group) + slot) * kTokens;
     const T *kx[kTokens], *vx[kTokens];
     T *ky[kTokens], *vy[kTokens];
     bool move[kTokens];
@@ -56,7 +60,7 @@ __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Param
         ky[q] = reinterpret_cast<T*>(p.c.k) + (page * p.c.k_stride[0] + r * p.c.k_stride[1]) / E;
         vy[q] = reinterpret_cast<T*>(p.c.v) + (page * p.c.v_stride[0] + r * p.c.v_stride[1]) / E;
     }
-    for (int i = threadIdx.x; i < row; i += 256) {
+    for (int i = lane; i < row; i += p.group) {
         const int h = i / per_head, d = i - h * per_head;
         const int64_t xk = h * (p.ks[2] / E) + d, xv = h * (p.vs[2] / E) + d;
         const int64_t yk = h * (p.c.k_stride[2] / E) + d, yv = h * (p.c.v_stride[2] / E) + d;
@@ -68,7 +72,7 @@ __global__ void __launch_bounds__(256) k_kv_append(const __grid_constant__ Param
         for (int q = 0; q < kTokens; ++q)
             if (move[q]) ky[q][yk] = a[q], vy[q][yv] = c[q];
     }
-    if (bad && threadIdx.x == 0) report_device_error(p.err, 9);
+    if (bad && lane == 0) report_device_error(p.err, 9);
 }
 
 }  // namespace kv
@@ -112,9 +116,6 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     for (int i = 0; i < 3 && k_stride && v_stride; ++i) p.ks[i] = k_stride[i], p.vs[i] = v_stride[i];
     p.batch = batch, p.tokens = tokens, p.width = width, p.index = index, p.counts = counts;
     p.new_lens = new_lens, p.err = err;
-    const int64_t blocks = std::max<int64_t>((width + kTokens - 1) / kTokens, 1);
-    SPARK_REQUIRE(blocks < (1ll << 31), SPARK_ERR_INVALID, "spark_kv_append: bad size");
-    const dim3 grid((unsigned)blocks, (unsigned)batch);
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     // 16 bytes at a time where sizes, addresses and strides let it
     const int vec = cache->dtype == SPARK_DTYPE_F32 ? 4 : 8;
@@ -122,6 +123,13 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     for (const void* ptr : {k, v, (const void*)cache->k, (const void*)cache->v}) fits = fits && aligned(ptr, 16);
     for (const int64_t* st : {(const int64_t*)p.ks, (const int64_t*)p.vs, cache->k_stride, cache->v_stride})
         for (int i = 0; i < 3; ++i) fits = fits && st[i] % vec == 0;
+    const int64_t row = cache->kv_heads * cache->head_dim / (fits ? vec : 1);
+    p.group = 256;
+    while (p.group > 8 && p.group / 2 >= row) p.group /= 2;
+    const int64_t per_block = kTokens * (256 / p.group);
+    const int64_t blocks = std::max<int64_t>((width + per_block - 1) / per_block, 1);
+    SPARK_REQUIRE(blocks < (1ll << 31), SPARK_ERR_INVALID, "spark_kv_append: bad size");
+    const dim3 grid((unsigned)blocks, (unsigned)batch);
     if (fits && vec == 4)
         launch_overlapped(k_kv_append<uint4, 4>, grid, 256, 0, s, p);
     else if (fits)

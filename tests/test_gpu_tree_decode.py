@@ -569,7 +569,7 @@ def test_tree_verify_rows_without_a_distribution():
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [BF, HF, FP])
 @pytest.mark.parametrize("b,t,hkv,d,page,ctx", [(1, 1, 1, 64, 16, 0), (5, 16, 8, 128, 32, 100), (3, 7, 3, 50, 5, 11),
-                                                (2, 300, 4, 80, 24, 1), (4, 9, 2, 8, 1, 17)])
+                                                (2, 300, 4, 80, 24, 1), (4, 9, 2, 8, 1, 17), (2, 45, 1, 8, 7, 3), (2, 70, 3, 24, 16, 9)])
 def test_kv_append(b, t, hkv, d, page, ctx, dtype):
     g = gen(t)
     lens = [(ctx + 13 * i) % (ctx + 40) for i in range(b)]
