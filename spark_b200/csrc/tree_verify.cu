@@ -7,7 +7,8 @@
 // exponential variates e(v) the index of the smallest e(v) / r(v) is v with
 // probability proportional to r(v).
 //
-// One thread-block cluster per sequence, each CTA a contiguous slice of the
+// One thread-block cluster of 8 CTAs (fewer where there are many sequences) per
+// sequence, each CTA a contiguous slice of the
 // vocabulary that it keeps in shared memory, so that a row is read from memory
 // once.  The walk is a chain of row passes, its bound their latency (about 2 us
 // each): one reduction in the CTA, one exchange of partial sums through
@@ -19,9 +20,9 @@
 // the row of the first child, which is brought into L2 while its parent's is
 // worked on, as the noise is from the start.  Measured: a chain of 8 nodes over
 // 32000 entries 15 us (3.4 us a node: 1.2 the row's loads, 1.2 the join, 0.3 the
-// exponentials), 64 trees of 16 nodes over 100003 entries 60 us -- the longest
-// walk, whose rows take 3.5 us with four CTAs to an SM.  256 or 1024 threads a CTA
-// and clusters of 4 were 5 to 40% slower.
+// exponentials), 64 trees of 16 nodes over 100003 entries 59 us.  256 or 1024
+// threads a CTA were 5 to 40% slower; three or four CTAs to an SM, which takes
+// spilled registers, 7 to 35% for few sequences and no faster for many.
 #include <math.h>
 
 #include <algorithm>
@@ -29,6 +30,10 @@
 #include "common.cuh"
 
 namespace spark {
+namespace tc {
+int sm_count_cached(int dev);
+}
+
 namespace tv {
 
 constexpr int kThreads = 512;
@@ -36,6 +41,11 @@ constexpr int kMaxCluster = 8;
 constexpr int kMaxNodes = 1024;
 constexpr int kSliceMax = 52 * 1024;   // values in a CTA's shared memory (208 KB)
 constexpr int kBatch = 8;              // loads of a thread on the way together
+
+constexpr int kSmemSm = 228 * 1024;    // shared memory of an SM
+
+// Vocabulary entries of each of cs CTAs.
+inline int64_t slice_of(int64_t vocab, int cs) { return ((vocab + cs - 1) / cs + 7) / 8 * 8; }
 
 struct Params {
     SparkTreeVerify a;
@@ -144,7 +154,7 @@ __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
 }
 
 template <typename L, typename D>   // types of logits and draft probabilities
-__global__ void __launch_bounds__(kThreads) k_tree_verify(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_constant__ Params p) {
     extern __shared__ float raw[];   // logits over T, after a rejection with draft probabilities r; below zero: nothing is left of -raw
     __shared__ Shared s;
     const SparkTreeVerify& a = p.a;
@@ -380,6 +390,26 @@ int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
     return launch<L, float>(p, batch, cs, s);
 }
 
+// CTAs of a cluster.  When the sequences' clusters do not fit the GPU at once they run one after another; smaller
+// clusters then have more at work, each with longer rows, fewer barriers and less waiting.  The time goes with (sequences
+// at a time, at least one filling) x (a pass's fixed part + a thread's share of the row), the fixed part worth 8 entries a
+// thread.  Measured with 8 / 4 / 2 / 1 CTAs: 32 trees of 8 nodes over 32000 entries 20 / 26 / 37 / 57 us, 64 37 / 30 / 45 /
+// 71, 512 224 / 151 / 125 / 175; over 100003 entries (2 at least) 64 78 / 79 / 115, 512 461 / 367 / 509; over 1000 entries
+// 512 186 / 95 / 56 / 34.
+int cluster_ctas(int64_t batch, int64_t vocab, int64_t nodes, int sms) {
+    int best = kMaxCluster;
+    double least = 0;
+    for (int cs = kMaxCluster; cs >= 1; cs /= 2) {
+        const int64_t slice = slice_of(vocab, cs);
+        if (slice > kSliceMax) break;
+        const size_t bytes = sizeof(Shared) + (slice + 3 * nodes) * sizeof(float) + 1024;
+        const double at_once = (double)sms * (2 * bytes <= kSmemSm ? 2 : 1) / cs;
+        const double time = std::max(1.0, batch / at_once) * (8 * kThreads + slice);
+        if (cs == kMaxCluster || time < least) best = cs, least = time;
+    }
+    return best;
+}
+
 }  // namespace tv
 }  // namespace spark
 
@@ -404,8 +434,11 @@ int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream) {
     Params p;
     p.a = *a;
     p.err = err;
-    const int cs = kMaxCluster;
-    p.slice = (int)((a->vocab + cs - 1) / cs + 7) / 8 * 8;
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return set_error((int)e, "spark_tree_verify: %s", cudaGetErrorString(e));
+    const int cs = cluster_ctas(a->batch, a->vocab, a->nodes, tc::sm_count_cached(dev));
+    p.slice = (int)slice_of(a->vocab, cs);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (a->logits_dtype == SPARK_DTYPE_BF16) return launch<__nv_bfloat16>(p, a->batch, cs, st);
     if (a->logits_dtype == SPARK_DTYPE_F16) return launch<__half>(p, a->batch, cs, st);

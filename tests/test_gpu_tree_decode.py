@@ -482,7 +482,8 @@ def check_verify(x, got, temperature):
 
 @pytest.mark.parametrize("dtype", [FP, BF, HF])
 @pytest.mark.parametrize("sampled", [True, False])
-@pytest.mark.parametrize("b,t,v", [(1, 1, 5), (3, 8, 1), (40, 12, 33), (5, 16, 1000), (7, 9, 32001), (2, 64, 4099), (1, 5, 160000)])
+@pytest.mark.parametrize("b,t,v", [(1, 1, 5), (3, 8, 1), (40, 12, 33), (5, 16, 1000), (7, 9, 32001), (2, 64, 4099), (1, 5, 160000),
+                                   (70, 6, 2001), (130, 4, 509), (300, 3, 77)])
 def test_tree_verify(b, t, v, sampled, dtype):
     g = gen(b + t + v)
     x = verify_inputs(g, b, t, v, dtype, sampled)
