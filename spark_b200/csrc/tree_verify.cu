@@ -20,7 +20,8 @@
 // the row of the first child, which is brought into L2 while its parent's is
 // worked on, as the noise is from the start.  Measured: a chain of 8 nodes over
 // 32000 entries 15 us (3.4 us a node: 1.2 the row's loads, 1.2 the join, 0.3 the
-// exponentials), 64 trees of 16 nodes over 100003 entries 59 us.  256 or 1024
+// exponentials), 64 trees of 16 nodes over 100003 entries 44 us
+// (46 without the next entries' loads during the work on the last).  256 or 1024
 // threads a CTA were 5 to 40% slower; three or four CTAs to an SM, which takes
 // spilled registers, 7 to 35% for few sequences and no faster for many.
 #include <float.h>
@@ -228,13 +229,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
         float m = -INFINITY, z = 0.f;
         int at = -1;
         bool nan = false;
-        for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
-            float l[kBatch];
+        L ahead[kBatch];      // the next entries, on their way during the work on these
+        auto load = [&](int i0) {
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const int i = i0 + k * kThreads;
-                l[k] = i < n ? (float)row[v0 + i] : -INFINITY;
+                ahead[k] = i < n ? row[v0 + i] : L(-INFINITY);
             }
+        };
+        load(tid);
+        for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {
+            float l[kBatch];
+#pragma unroll
+            for (int k = 0; k < kBatch; ++k) l[k] = (float)ahead[k];
+            load(i0 + kBatch * kThreads);
             if (temp == 0.f) {
 #pragma unroll
                 for (int k = 0; k < kBatch; ++k) {
@@ -395,9 +403,9 @@ int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
 // CTAs of a cluster.  When the sequences' clusters do not fit the GPU at once they run one after another; smaller
 // clusters then have more at work, each with longer rows, fewer barriers and less waiting.  The time goes with (sequences
 // at a time, at least one filling) x (a pass's fixed part + a thread's share of the row), the fixed part worth 8 entries a
-// thread.  Measured with 8 / 4 / 2 / 1 CTAs: 32 trees of 8 nodes over 32000 entries 20 / 26 / 37 / 57 us, 64 37 / 30 / 45 /
-// 71, 512 224 / 151 / 125 / 175; over 100003 entries (2 at least) 64 78 / 79 / 115, 512 461 / 367 / 509; over 1000 entries
-// 512 186 / 95 / 56 / 34.
+// thread.  Measured with 8 / 4 / 2 / 1 CTAs: 32 trees of 8 nodes over 32000 entries 19 / 24 / 32 / 57 us, 64 35 / 28 / 39 /
+// 71, 512 219 / 140 / 114 / 175; over 100003 entries (2 at least) 64 62 / 62 / 88, 512 373 / 293 / 387; over 1000 entries
+// 512 165 / 82 / 45 / 28.
 int cluster_ctas(int64_t batch, int64_t vocab, int64_t nodes, int sms) {
     int best = kMaxCluster;
     double least = 0;
