@@ -68,6 +68,7 @@ std::tuple<Tensor, OptTensor, int> rope(Tensor q, OptTensor k, Tensor positions,
     on_device("rope", "positions", positions, q);
     on_device("rope", "table", table, q);
     if (k) on_device("rope", "k", *k, q);
+    const at::DeviceGuard guard(q.device());
     const int64_t dim = q.dim();
     TORCH_CHECK_VALUE((dim == 3 || dim == 4) && (!k || (k->dim() == dim && k->sizes().slice(0, dim - 2) == q.sizes().slice(0, dim - 2) &&
                                                         k->size(-1) == q.size(-1))),
@@ -92,6 +93,53 @@ std::tuple<Tensor, OptTensor, int> rope(Tensor q, OptTensor k, Tensor positions,
                               inverse, positions.data_ptr(), (int)positions.element_size(), table.const_data_ptr<float>(),
                               table.size(0), reinterpret_cast<int*>(ws), reinterpret_cast<void*>(stream));
     return {*q_out, k ? k_out : std::nullopt, rc};
+}
+
+// The differentiable form.  Turning is linear, its transpose is the turn back: the gradients are turned back by this
+// function, so that gradients of gradients are right too.  A step backward runs on its forward's stream, with its workspace (which
+// stays for as long as the process).
+struct Turn : torch::autograd::Function<Turn> {
+    static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const Tensor& positions,
+                                       const Tensor& table, bool interleaved, bool inverse, uint64_t ws, uint64_t stream, int* status) {
+        auto [y, z, rc] = rope(q, k, positions, table, interleaved, inverse, std::nullopt, std::nullopt, ws, stream);
+        *status = rc;
+        ctx->save_for_backward({positions, table});
+        ctx->saved_data["how"] = (int64_t)(k.has_value() * 4 + interleaved * 2 + inverse);
+        ctx->saved_data["ws"] = (int64_t)ws, ctx->saved_data["stream"] = (int64_t)stream;
+        ctx->set_materialize_grads(false);
+        return z ? std::vector<Tensor>{y, *z} : std::vector<Tensor>{y};
+    }
+
+    static std::vector<Tensor> backward(torch::autograd::AutogradContext* ctx, std::vector<Tensor> grads) {
+        const auto saved = ctx->get_saved_variables();
+        const int64_t how = ctx->saved_data["how"].toInt();
+        const bool need[2] = {grads[0].defined() && ctx->needs_input_grad(0), (how & 4) && grads[1].defined() && ctx->needs_input_grad(1)};
+        std::vector<Tensor> out(9);
+        if (!need[0] && !need[1]) return out;
+        const int first = need[0] ? 0 : 1;
+        int rc = SPARK_OK;
+        const auto turned = turn(grads[first], need[0] && need[1] ? OptTensor(grads[1]) : std::nullopt, saved[0], saved[1], how & 2, !(how & 1),
+                                 (uint64_t)ctx->saved_data["ws"].toInt(), (uint64_t)ctx->saved_data["stream"].toInt(), &rc);
+        TORCH_CHECK(rc == SPARK_OK, "spark_rope: ", spark_last_error());
+        for (size_t i = 0; i < turned.size(); ++i) out[first + i] = turned[i];
+        return out;
+    }
+
+    static std::vector<Tensor> turn(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& table, bool interleaved,
+                                    bool inverse, uint64_t ws, uint64_t stream, int* rc) {
+        if (at::GradMode::is_enabled() && (q.requires_grad() || (k && k->requires_grad())))
+            return apply(q, k, positions, table, interleaved, inverse, ws, stream, rc);
+        auto [y, z, status] = rope(q, k, positions, table, interleaved, inverse, std::nullopt, std::nullopt, ws, stream);
+        *rc = status;
+        return z ? std::vector<Tensor>{y, *z} : std::vector<Tensor>{y};
+    }
+};
+
+std::tuple<Tensor, OptTensor, int> apply_rope(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& table,
+                                              bool interleaved, uint64_t ws, uint64_t stream) {
+    int rc = SPARK_OK;
+    const auto out = Turn::turn(q, k, positions, table, interleaved, false, ws, stream, &rc);
+    return {out[0], k ? OptTensor(out[1]) : std::nullopt, rc};
 }
 
 // ------------------------------------------------------------------ the cache
@@ -146,6 +194,7 @@ std::tuple<Tensor, int> kv_append(const Tensor& k_new, const Tensor& v_new, cons
         TORCH_CHECK_TYPE(counts->scalar_type() == at::kInt && counts->dim() == 1 && counts->size(0) == batch && counts->is_contiguous(),
                          "kv_append: counts must be a contiguous int32 [batch]");
     }
+    const at::DeviceGuard guard(k_cache.device());
     const Tensor k = unit(k_new), v = unit(v_new);
     Tensor out = at::empty({batch}, lens.options());
     int64_t ks[3], vs[3];
@@ -176,6 +225,7 @@ std::tuple<Tensor, OptTensor, int, size_t> tree_attention(const Tensor& q_, cons
                      "tree_attention: bfloat16 or float16 throughout, got ", type, ", ", k_tree.scalar_type(), ", ",
                      v_tree.scalar_type());
     on_device(what, "k_cache", k_cache, q_);
+    const at::DeviceGuard guard(q_.device());
     SparkTreeAttention a;
     a.cache = paged(what, k_cache, v_cache, page_table, lens, q_);
     on_device(what, "k_tree", k_tree, q_);
@@ -228,6 +278,7 @@ std::tuple<Tensor, Tensor, Tensor, int> tree_verify(const Tensor& logits, Tensor
     TORCH_CHECK_TYPE(parents.scalar_type() == at::kInt && (per_sequence ? parents.size(0) == batch : parents.dim() == 1) &&
                          parents.size(-1) == nodes,
                      "tree_verify: parents must be int32 [", nodes, "] or [", batch, ", ", nodes, "]");
+    const at::DeviceGuard guard(logits.device());
     SparkTreeVerify a{};
     a.batch = batch, a.nodes = nodes, a.vocab = vocab;
     const Tensor x = unit(logits);
@@ -274,6 +325,7 @@ PYBIND11_MODULE(_native, m) {
         }
     });
     m.def("rope", &rope);
+    m.def("apply_rope", &apply_rope);
     m.def("kv_append", &kv_append);
     m.def("tree_attention", &tree_attention);
     m.def("tree_verify", &tree_verify);

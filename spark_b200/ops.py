@@ -482,13 +482,13 @@ def linear_batch_allreduce(batch: list[BatchOp], op: int, world: int, rank: int,
 
 def check_device_errors(device=None) -> None:
     """Raise if a kernel left an error in a workspace (synchronises)."""
-    for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()):
+    for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()) + _tree_outgrown:
         if device is not None and dev != device:
             continue
         try:
             call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
         except _lib.SparkError:
-            if _tree_ws.get((dev, sh)) is buf:
+            if any(buf is other for _, other in [*_tree_ws.items(), *_tree_outgrown]):
                 buf.zero_()    # an expired wait may leave its counters behind
             raise
 
@@ -515,6 +515,7 @@ def silu_mul(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 MAX_TREE_NODES = 64    # of one sequence in tree_attention (SPARK_MAX_TREE_NODES)
 
 _tree_ws: dict[tuple[int, int], torch.Tensor] = {}
+_tree_outgrown: list[tuple[tuple[int, int], torch.Tensor]] = []
 _native_module = None
 
 
@@ -539,13 +540,18 @@ def _check(name: str, rc: int) -> None:
 
 def _tree_workspace(device: torch.device, stream: int, nbytes: int = 256) -> torch.Tensor:
     """Scratch of the tree-decoding calls, one per (device, stream): an error word,
-    counters that are zero between calls, then partial results."""
+    counters that are zero between calls, then partial results.  A larger one takes its
+    place when a call needs it; the old one stays, with the errors left in it, for the
+    CUDA graphs and backward passes that have its address."""
     key = (device.index, stream)
     buf = _tree_ws.get(key)
     if buf is None or buf.numel() < nbytes:
         with _ws_lock:
             buf = _tree_ws.get(key)
             if buf is None or buf.numel() < nbytes:
+                if buf is not None:
+                    _tree_outgrown.append((key, buf))
+                    nbytes = max(nbytes, 2 * buf.numel())     # (all the old ones together are no larger)
                 buf = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
                 _tree_ws[key] = buf
     return buf

@@ -53,29 +53,12 @@ def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device=None,
     return (torch.cat([angle.cos(), angle.sin()], 1) * factor).float().to(device or "cuda")
 
 
-class RoPE(torch.autograd.Function):
-    """q and k turned to their positions; the gradients are turned back."""
-
-    @staticmethod
-    def forward(ctx, q, k, positions, table, interleaved):
-        ctx.save_for_backward(positions, table)
-        ctx.interleaved, ctx.has_k = interleaved, k is not None
-        return ops.rope(q, k, positions, table, interleaved=interleaved)
-
-    @staticmethod
-    def backward(ctx, dq, dk):
-        positions, table = ctx.saved_tensors
-        need_q, need_k = ctx.needs_input_grad[0], ctx.has_k and ctx.needs_input_grad[1]
-        if need_q:
-            dq, dk = ops.rope(dq, dk if need_k else None, positions, table, interleaved=ctx.interleaved, inverse=True)
-            return dq, dk, None, None, None
-        if need_k:
-            return None, ops.rope(dk, None, positions, table, interleaved=ctx.interleaved, inverse=True)[0], None, None, None
-        return None, None, None, None, None
-
-
 def apply_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
                interleaved: bool = False):
-    """Differentiable ops.rope: (q', k').  The gradient of the positions and of the
-    table is not computed."""
-    return RoPE.apply(q, k, positions, table, interleaved)
+    """Differentiable ops.rope: (q', k'), gradients of gradients too.  The gradient of the
+    positions and of the table is not computed."""
+    _, ws, stream = ops._place("rope", q)
+    y, z, rc = ops._native().apply_rope(q, k, positions, table, interleaved, ws, stream)
+    if rc:
+        ops._check("spark_rope", rc)
+    return y, z

@@ -139,6 +139,50 @@ def test_rope_gradient(interleaved):
     assert z is None and torch.equal(torch.autograd.grad(y, q, wq)[0], dq)
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_gradient_of_a_gradient(interleaved):
+    """The gradient is linear in what comes back: its own gradient turns forward again."""
+    from spark_b200.rotary import apply_rope, rope_table
+    g = gen(6)
+    table = rope_table(50, 8, scaling="yarn", factor=4.0)
+    q, k = (randn(g, 7, n, 8).requires_grad_() for n in (3, 2))
+    wq, wk = (randn(g, 7, n, 8).requires_grad_() for n in (3, 2))
+    pos = torch.randint(0, 50, (7,), generator=g, device="cuda")
+    with torch.no_grad():
+        y, z = apply_rope(q, k, pos, table, interleaved)
+    assert not y.requires_grad and not z.requires_grad
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y, z = apply_rope(q, k, pos, table, interleaved)
+        dq, dk = torch.autograd.grad((y, z), (q, k), (wq, wk), create_graph=True)
+        vq, vk = randn(g, *q.shape), randn(g, *k.shape)
+        hq, hk = torch.autograd.grad((dq, dk), (wq, wk), (vq, vk))
+    torch.cuda.current_stream().wait_stream(s)
+    check_rope(q, y, rope64(q, pos, table, interleaved, False))
+    check_rope(wk, dk, rope64(wk, pos, table, interleaved, True))
+    check_rope(vq, hq, rope64(vq, pos, table, interleaved, False))
+    check_rope(vk, hk, rope64(vk, pos, table, interleaved, False))
+    ops().check_device_errors()
+
+
+def test_errors_outlast_a_larger_workspace():
+    from spark_b200 import SparkError
+    from spark_b200.rotary import rope_table
+    g = gen(8)
+    q, kt, vt, kc, vc, table, lens, _ = make(g, 8, 16, 32, 8, 128, [4000] * 8, 16, BF)
+    parents = torch.arange(-1, 15, dtype=torch.int32, device="cuda")
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        bad = torch.full((8, 16), 99, device="cuda")
+        ops().rope(q, None, bad, rope_table(10, 16))
+        ops().tree_attention(q, kt, vt, kc, vc, table, lens, parents)
+    with pytest.raises(SparkError, match="rotary table"):
+        ops().check_device_errors()
+    ops().check_device_errors()
+
+
 def test_rope_position_outside_the_table_is_reported():
     from spark_b200.rotary import rope_table
     q = randn(gen(1), 4, 2, 64, dtype=BF)
