@@ -437,13 +437,13 @@ __device__ __forceinline__ void add_parts(const Params& p, const Segment& sg, in
             int head;
             const int node = e0 + k * step < n ? node_of(p, sg, row[k], head) : -1;
             if (node < 0) continue;
-            const float norm = sum[k] == 0.f ? 0.f : 1.f / sum[k];
+            const float norm = sum[k] == 0.f ? 0.f : __fdividef(1.f, sum[k]);
             uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + (int64_t)sg.b * a.out_stride[0] + node * a.out_stride[1] + head * a.out_stride[2];
             *reinterpret_cast<uint2*>(out + col[k] * 4) =
                 make_uint2(pack2<BF>(o[k].x * norm, o[k].y * norm), pack2<BF>(o[k].z * norm, o[k].w * norm));
             if (a.lse && col[k] == 0)
                 a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
-                    sum[k] == 0.f ? -INFINITY : (log2f(sum[k]) + top[k]) * 0.6931471805599453f;
+                    sum[k] == 0.f ? -INFINITY : (__log2f(sum[k]) + top[k]) * 0.6931471805599453f;
         }
     }
 }
@@ -690,6 +690,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         int seg = 0, tile0 = 0;          // tiles of the segments so far: places in the ring of V
         int j = 0;                       // tiles of this stream so far
         uint32_t s_phase = 0;            // a bit for each score buffer
+        uint64_t mask = 0;
+        int mask_of = -1;                // the nodes that it belongs to: the next head of the sequence has the same
         while (ok && walk.next(sg)) {
             const int n = sg.t1 - sg.t0;
             const int row = (by_rows ? g * 128 : 0) + row_in;     // of the item
@@ -697,7 +699,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int node = node_of(p, sg, row, head);
             const bool mine = node >= 0;
             const bool work = __any_sync(0xffffffffu, mine);
-            const uint64_t mask = mine ? ancestors(a.parents + (int64_t)sg.b * a.parents_stride, node) : 0;
+            const int nodes_of = sg.b * p.row_tiles + sg.rt;
+            if (nodes_of != mask_of) mask = mine ? ancestors(a.parents + (int64_t)sg.b * a.parents_stride, node) : 0;
+            mask_of = nodes_of;
             float m = -INFINITY, l = 0.f;
             int my_tiles = 0;
             if (!(C::kOne && g == 1)) {
@@ -863,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const float sum = mask ? ml[0].y * f0 + ml[1].y * f1 : 0.f;
                 const bool second = __any_sync(0xffffffffu, f1 != 0.f);
                 if (whole) {
-                    const float norm = sum == 0.f ? 0.f : 1.f / sum;
+                    const float norm = sum == 0.f ? 0.f : __fdividef(1.f, sum);   // (two units in fp32's last place)
                     f0 *= norm, f1 *= norm;
                 }
                 const bool fix = sm.bad_v[seg & 1] == seg + 1;
@@ -917,7 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         p.part_ml[(size_t)(2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0)) * p.rows_item + row] = make_float2(top, sum);
                     else if (a.lse)
                         a.lse[((int64_t)sg.b * a.nodes + node) * a.q_heads + head] =
-                            sum == 0.f ? -INFINITY : (log2f(sum) + top) * 0.6931471805599453f;
+                            sum == 0.f ? -INFINITY : (__log2f(sum) + top) * 0.6931471805599453f;
                 }
             }
             tc_fence_before();
