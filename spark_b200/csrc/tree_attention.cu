@@ -137,12 +137,12 @@ __device__ __forceinline__ int count_tiles(const Params& p, int lane) {
     for (int b = lane; b < (int)p.a.batch; b += 32) total += tiles_of(p, b);
     return (int)__reduce_add_sync(0xffffffffu, (unsigned)total) * p.per_seq;
 }
-// The sequence that holds tile `pos` of all, and the tile's place among its tiles, by one warp.
-__device__ __forceinline__ void locate(const Params& p, int lane, int pos, int& b, int& off) {
+// The sequence and its item that hold place `pos` of all, and the place in the item, by one warp.
+__device__ __forceinline__ void locate(const Params& p, int lane, int pos, int& b, int& item, int& off) {
     int at = 0;
-    b = (int)p.a.batch, off = 0;
+    b = (int)p.a.batch, item = off = 0;
     for (int base = 0; base < (int)p.a.batch; base += 32) {
-        const int n = tiles_of(p, base + lane) * p.per_seq;
+        const int places = tiles_of(p, base + lane), n = places * p.per_seq;
         int sum = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -154,6 +154,9 @@ __device__ __forceinline__ void locate(const Params& p, int lane, int pos, int& 
             const int l = __ffs(hit) - 1;
             b = base + l;
             off = pos - (at + __shfl_sync(0xffffffffu, sum - n, l));
+            const int of_item = __shfl_sync(0xffffffffu, places, l);
+            item = off / of_item;
+            off -= item * of_item;
             return;
         }
         at += __shfl_sync(0xffffffffu, sum, 31);
@@ -166,28 +169,29 @@ struct Segment {
     int lo;                                // place of tile 0 among all
 };
 
-// Walks `left` places from place `off` of sequence b on; a run may be empty
-// where the range ends in front of an item's own tiles.
+// Walks `left` places from place `at` of an item of sequence b on; a run may be
+// empty where the range ends in front of an item's own tiles.
 struct Walker {
     const Params& p;
-    int b, off, left, pos;
-    __device__ Walker(const Params& q, int b0, int off0, int n, int first) : p(q), b(b0), off(off0), left(n), pos(first) {}
+    int b, head, rt, at, left, pos;
+    __device__ Walker(const Params& q, int b0, int item, int off, int n, int first)
+        : p(q), b(b0), head(item / q.row_tiles), rt(item - head * q.row_tiles), at(off), left(n), pos(first) {}
     __device__ bool next(Segment& s) {
         while (left > 0 && b < (int)p.a.batch) {
             s.len = context_len(p, b);
             s.tiles = (s.len + p.tok - 1) / p.tok + 1;
-            const int places = s.tiles + kStart, item = off / places;
-            s.b = b;
-            s.head = item / p.row_tiles;
-            s.rt = item - s.head * p.row_tiles;
-            const int at = off - item * places, n = min(places - at, left);
+            s.b = b, s.head = head, s.rt = rt;
+            const int n = min(s.tiles + kStart - at, left);
             s.t0 = max(at - kStart, 0);
             s.t1 = at + n - kStart;
-            off += n;
-            left -= n;
+            s.lo = pos - at + kStart;
             pos += n;
-            s.lo = pos - n - at + kStart;
-            if (off == places * p.per_seq) off = 0, ++b;
+            left -= n;
+            at = 0;
+            if (++rt == p.row_tiles) {
+                rt = 0;
+                if (++head == (int)p.a.cache.kv_heads) head = 0, ++b;
+            }
             if (s.t1 > s.t0) return true;
         }
         return false;
@@ -499,14 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int total = count_tiles(p, lane);
     const bool idle = (int)blockIdx.x >= ctas(total);
     const int range0 = idle ? total : first_tile(total, blockIdx.x), range1 = idle ? total : first_tile(total, blockIdx.x + 1);
-    int b0, off0;
-    locate(p, lane, range0, b0, off0);
+    int b0, item0, off0;
+    locate(p, lane, range0, b0, item0, off0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
     const int count = (smem_u32(smem) & 1023) ? 0 : range1 - range0;
-    Walker walk(p, b0, off0, count, range0);
+    Walker walk(p, b0, item0, off0, count, range0);
     Segment sg;
     bool ok = true;
 
