@@ -330,6 +330,14 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ bool all_ok(bool ok) { return __all_sync(0xffffffffu, ok); }
 
 __device__ __forceinline__ void add_release(int* p, int v) {
@@ -869,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float f0 = ml[0].y == 0.f ? 0.f : exp2_approx(ml[0].x - top);
                 float f1 = ml[1].y == 0.f ? 0.f : exp2_approx(ml[1].x - top);
                 const float sum = mask ? ml[0].y * f0 + ml[1].y * f1 : 0.f;
-                const bool second = __any_sync(0xffffffffu, f1 != 0.f);
+                const bool second = __any_sync(0xffffffffu, f1 != 0.f), none = __any_sync(0xffffffffu, mine && (f0 == 0.f || (second && f1 == 0.f)));
                 if (whole) {
                     const float norm = sum == 0.f ? 0.f : __fdividef(1.f, sum);   // (two units in fp32's last place)
                     f0 *= norm, f1 *= norm;
@@ -886,11 +894,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (second) tmem_ld32(tmem + lane_off + o_col[1] + e0, o1);
                     tmem_wait_ld();
                     // (O of a stream without tiles is not defined)
+                    if (none) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = f0 == 0.f ? 0.f : o[e] * f0;
+                        for (int e = 0; e < 32; ++e) {
+                            if (f0 == 0.f) o[e] = 0.f;
+                            if (second && f1 == 0.f) o1[e] = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 t = mul2(make_float2(o[e], o[e + 1]), make_float2(f0, f0));
+                        o[e] = t.x, o[e + 1] = t.y;
+                    }
                     if (second) {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] += f1 == 0.f ? 0.f : o1[e] * f1;
+                        for (int e = 0; e < 32; e += 2) {
+                            const float2 t = fma2(make_float2(o1[e], o1[e + 1]), make_float2(f1, f1), make_float2(o[e], o[e + 1]));
+                            o[e] = t.x, o[e + 1] = t.y;
+                        }
                     }
                     if (fix) {
                         for (uint64_t left = mask; left; left &= left - 1) {
