@@ -699,6 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int g = warp >> 2, quad = warp & 3, row_in = quad * 32 + lane;   // stream, lane quadrant, row = TMEM lane
         const uint32_t lane_off = (uint32_t)(quad * 32) << 16;
         const int dim = (int)c.head_dim;
+        // items of few rows leave warps without a row: those clear values (below), while the others work
+        const int cleaner = p.rows_item <= 96 ? (p.rows_item + 31) / 32 : 0;
         int seg = 0, tile0 = 0;          // tiles of the segments so far: places in the ring of V
         int j = 0;                       // tiles of this stream so far
         uint32_t s_phase = 0;            // a bit for each score buffer
@@ -804,22 +806,22 @@ __global__ void __launch_bounds__(kThreads, 1)
                     ++j;
                     // values that meet weights of zero must be finite: clear what lies behind the context in the last
                     // group of 16, and the infinities and NaN of the tree (added back below)
-                    if ((tree || (valid & 15)) && !(by_rows && g == 1)) {
+                    if ((tree || (valid & 15)) && !(by_rows && g == 1) && quad >= cleaner) {
                         const int pos = tile0 + i, slot_i = pos % p.slots[1];
                         ok = all_ok(wait_bar(smem_u32(&sm.full[1][slot_i]), (uint32_t)(pos / p.slots[1]) & 1));
                         if (!ok) break;
                         uint8_t* slot = smem + (size_t)(p.slots[0] + slot_i) * C::kSlotBytes;
-                        const int tid = (int)threadIdx.x & 127;
+                        const int tid = row_in - cleaner * 32, step = 128 - cleaner * 32;
                         if (!tree) {
                             const int n_rows = ((valid + 15) & ~15) - valid;
-                            for (int e = tid; e < n_rows * C::kChunks * 8; e += 128) {
+                            for (int e = tid; e < n_rows * C::kChunks * 8; e += step) {
                                 const int r = e / (C::kChunks * 8), u = e % (C::kChunks * 8);
                                 *reinterpret_cast<uint4*>(slot + (u >> 3) * kTok * 128 + (valid + r) * 128 + (u & 7) * 16) =
                                     make_uint4(0, 0, 0, 0);
                             }
                         } else {
                             constexpr uint32_t kExp = BF ? 0x7f807f80u : 0x7c007c00u;
-                            for (int e = tid; e < valid * C::kChunks * 8; e += 128) {
+                            for (int e = tid; e < valid * C::kChunks * 8; e += step) {
                                 const int r = e / (C::kChunks * 8), u = e % (C::kChunks * 8);
                                 uint4* w = reinterpret_cast<uint4*>(slot + (u >> 3) * kTok * 128 + r * 128 + (u & 7) * 16);
                                 const uint4 q4 = *w;
