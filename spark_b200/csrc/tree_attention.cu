@@ -82,7 +82,7 @@ using namespace tcx;
 constexpr int kThreads = 384;
 constexpr int kKWarp = 8, kVWarp = 9, kMmaWarp = 10, kQWarp = 11;
 constexpr int kMaxSlots = 12;   // of one ring
-constexpr int kHeader = 3072;   // barriers and the exchange of the two groups
+constexpr int kHeader = 3 * 1024;   // barriers and the exchange of the two groups
 constexpr uint32_t kTmemCols = 512;
 
 // DP: head_dim padded to 64, 128 or 256.
