@@ -23,7 +23,10 @@ class PagedKVCache:
     """K and V of `layers` layers in pages of `page_size` tokens that sequences
     take from a common pool; the page table and the lengths are shared by the
     layers.  k[l], v[l]: [pages, page_size, kv_heads, head_dim]; page_table int32
-    [batch, max_pages]; lens int32 [batch]."""
+    [batch, max_pages], -1 where a sequence has no page (nothing is written or read
+    there: an append beyond what is reserved is reported); lens int32 [batch]; held
+    int32 [batch], 1 where a sequence has pages: a batch's other rows take part in a
+    step, but nothing of theirs is kept."""
 
     def __init__(self, layers: int, batch: int, max_tokens: int, kv_heads: int, head_dim: int, page_size: int = 64,
                  pages: int | None = None, dtype=torch.bfloat16, device="cuda"):
@@ -34,8 +37,9 @@ class PagedKVCache:
         shape = (pages, page_size, kv_heads, head_dim)
         self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
         self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
-        self.page_table = torch.zeros(batch, self.max_pages, dtype=torch.int32, device=device)
+        self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.held = torch.zeros(batch, dtype=torch.int32, device=device)
         self._free = list(range(pages - 1, -1, -1))
         self._taken: list[list[int]] = [[] for _ in range(batch)]
 
@@ -52,20 +56,25 @@ class PagedKVCache:
         new = [self._free.pop() for _ in range(need)]
         self._taken[sequence] += new
         self.page_table[sequence, at:at + need] = torch.tensor(new, dtype=torch.int32, device=self.page_table.device)
+        self.held[sequence] = 1
 
     def release(self, sequence: int) -> None:
         """Takes the sequence's pages back and empties it."""
         self._free += reversed(self._taken[sequence])
         self._taken[sequence] = []
-        self.lens[sequence] = 0
+        self.page_table[sequence] = -1
+        self.lens[sequence] = self.held[sequence] = 0
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, parents: torch.Tensor, **kw):
         return ops.tree_attention(q, k, v, self.k[layer], self.v[layer], self.page_table, self.lens, parents, **kw)
 
     def append(self, new: list, index: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
         """Every layer's (k, v) of a step [batch, nodes, kv_heads, head_dim]: the rows
-        that index and counts name (ops.kv_append) go behind each sequence's tokens."""
+        that index and counts name (ops.kv_append) go behind each sequence's tokens; none
+        of a sequence without pages."""
         lens = self.lens
+        width = (new[0][0] if index is None else index).shape[1]
+        counts = self.held * (width if counts is None else counts)
         for layer, (k, v) in enumerate(new):
             lens = ops.kv_append(k, v, self.k[layer], self.v[layer], self.page_table, self.lens, index=index, counts=counts)
         self.lens = lens
@@ -138,7 +147,8 @@ class TreeDecoder(nn.Module):
     def step(self, tokens: torch.Tensor, parents: torch.Tensor, depths: torch.Tensor, cache: PagedKVCache,
              uniforms: torch.Tensor, noise: torch.Tensor, draft_probs: torch.Tensor | None = None, temperature=1.0):
         """One step: forward, verification, append of the accepted nodes.  Returns
-        ops.tree_verify's (path, accepted, next)."""
+        ops.tree_verify's (path, accepted, next); those of a row whose sequence has no
+        pages mean nothing."""
         logits, new = self(tokens, parents, depths, cache)
         path, accepted, last = ops.tree_verify(logits, tokens, parents, uniforms, noise, draft_probs=draft_probs,
                                                temperature=temperature)

@@ -1,0 +1,79 @@
+"""The tree-decoding operators where their inputs are at the edge of what they
+take: unused nodes, workspaces shared by graphs, sequences without pages, draws
+from what little a rejection leaves, temperatures and contexts at the ends.
+
+Tolerances as in test_gpu_tree_decode: u the unit roundoff of the tensors' type,
+attention within 3 u max|v| and, over all values, within u of the norm.
+"""
+from __future__ import annotations
+
+import importlib.util
+import os
+
+import pytest
+import torch
+
+from test_gpu_tree_decode import BF, gen, ops, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ the cache
+def example():
+    spec = importlib.util.spec_from_file_location(
+        "example_tree_decode", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "tree_decode.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    return ex
+
+
+def test_rows_without_pages_leave_the_others_alone():
+    """A batch whose first sequence is gone, and whose last never came, decodes what the
+    second decodes by itself, and its pages are the same to the bit."""
+    from spark_b200.tree_decode import PagedKVCache, tree_depths
+    ex = example()
+    model = ex.build()
+    tree = torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda")
+    depths = tree_depths(tree.tolist()).cuda()
+    prompt = torch.randint(0, 2048, (1, 21), generator=gen(1), device="cuda").expand(3, -1)
+    tokens = torch.randint(0, 2048, (1, 4), generator=gen(2), device="cuda").expand(3, -1)
+    u, noise = torch.full((3, 4), 0.5, device="cuda"), torch.ones(3, 2048, device="cuda")
+    got = []
+    for before in (True, False):
+        c = PagedKVCache(2, 3, 64, 2, 64, page_size=8, pages=8)
+        if before:
+            c.reserve(0, 64)
+            c.release(0)
+        c.reserve(1, 40)
+        model.prefill(prompt, c)
+        if before:
+            c.reserve(0, 16)
+            c.release(0)
+        pages = c.page_table[1, :5].long()
+        path, n, last = model.step(tokens, tree, depths, c, u, noise, temperature=0.0)
+        assert c.lens.tolist() == [0, 21 + int(n[1]), 0]
+        got.append([path[1], last[1]] + [x[pages].clone() for x in c.k + c.v])
+        others = torch.ones(8, dtype=torch.bool, device="cuda").index_fill_(0, pages, False)
+        assert all((x[others] == 0).all() for x in c.k + c.v)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ops().check_device_errors()
+
+
+def test_an_append_beyond_the_reserved_pages_is_reported():
+    from spark_b200 import SparkError
+    from spark_b200.tree_decode import PagedKVCache
+    g = gen(3)
+    c = PagedKVCache(1, 2, 64, 2, 64, page_size=8)
+    c.reserve(0, 16)
+    c.reserve(1, 32)
+    k = randn(g, 2, 20, 2, 64, dtype=BF)
+    c.append([(k, k)])
+    with pytest.raises(SparkError, match="outside the cache"):
+        ops().check_device_errors()
+    for i, n in ((0, 16), (1, 20)):
+        rows = c.k[0][c.page_table[i, :-(-n // 8)].long()].flatten(0, 1)
+        assert torch.equal(rows[:n], k[i, :n]) and (rows[n:] == 0).all()
+    kept = torch.zeros(16, dtype=torch.bool, device="cuda")
+    kept[c.page_table[c.page_table >= 0].long()] = True
+    assert (c.k[0][~kept] == 0).all()
+    ops().check_device_errors()
