@@ -879,8 +879,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     col0 = g * (DP / 2), col1 = col0 + DP / 2;       // each group half of the columns
                 }
                 const float top = fmaxf(ml[0].x, ml[1].x);
-                float f0 = ml[0].y == 0.f ? 0.f : exp2_approx(ml[0].x - top);
-                float f1 = ml[1].y == 0.f ? 0.f : exp2_approx(ml[1].x - top);
+                // (an unused node: whatever its scores and the values are, a row of zeros)
+                float f0 = !mask || ml[0].y == 0.f ? 0.f : exp2_approx(ml[0].x - top);
+                float f1 = !mask || ml[1].y == 0.f ? 0.f : exp2_approx(ml[1].x - top);
                 const float sum = mask ? ml[0].y * f0 + ml[1].y * f1 : 0.f;
                 const bool second = __any_sync(0xffffffffu, f1 != 0.f), none = __any_sync(0xffffffffu, mine && (f0 == 0.f || (second && f1 == 0.f)));
                 if (whole) {

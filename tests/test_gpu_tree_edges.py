@@ -8,14 +8,45 @@ attention within 3 u max|v| and, over all values, within u of the norm.
 from __future__ import annotations
 
 import importlib.util
+import math
 import os
 
 import pytest
 import torch
 
-from test_gpu_tree_decode import BF, gen, ops, randn
+from test_gpu_tree_decode import BF, HF, attention64, check_attention, gen, make, ops, randn, sees
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("b,t,hq,hkv,d,n", [
+    (40, 6, 8, 8, 128, 60), (2, 6, 8, 2, 128, 900),       # most items whole; all in parts
+    (60, 20, 32, 4, 64, 60), (3, 20, 32, 4, 64, 700),     # more than 128 rows an item
+    (40, 5, 8, 8, 256, 70), (1, 5, 4, 4, 256, 900),
+])
+def test_unused_nodes_give_zero_rows(b, t, hq, hkv, d, n, dtype):
+    """Whatever their queries and the values that others see hold."""
+    g = gen(t)
+    q, kt, vt, kc, vc, table, lens, parents = make(g, b, t, hq, hkv, d, [n] * b, 16, dtype)
+    parents[:, t - 1] = -2
+    want, want_lse = attention64(q, kt, vt, kc, vc, table, lens, parents, d ** -0.5)
+    used = torch.tensor([[len(chain) > 0 for chain in sees(p)] for p in parents.tolist()], device="cuda")
+    vmax = max(vt.abs().max().item(), vc.abs().max().item())
+    for bad in (math.nan, math.inf, -math.inf):
+        q2 = q.clone()
+        q2[~used] = bad
+        out, lse = ops().tree_attention(q2, kt, vt, kc, vc, table, lens, parents, return_lse=True)
+        check_attention(out, lse, want, want_lse, vmax)
+        # a value of the context that the used nodes see: theirs is what the formula gives, no number
+        v2 = vc.clone()
+        v2[table[:, 0].long(), 5, :, 3] = bad
+        out, lse = ops().tree_attention(q, kt, vt, kc, v2, table, lens, parents, return_lse=True)
+        assert (out[~used] == 0).all() and (lse[~used] == -math.inf).all()
+        assert not torch.isfinite(out[..., 3][used]).any()
+        assert torch.isfinite(out[..., 4:]).all() and torch.isfinite(lse[used]).all()
+    ops().check_device_errors()
 
 
 # ------------------------------------------------------------------ the cache
