@@ -328,6 +328,13 @@ SPARK_API int spark_tile_weights(int fmt, const uint8_t* wq, const uint8_t* scal
  * bounded waits expires; synchronises `stream`.  Returns SPARK_OK or SPARK_ERR_DEVICE. */
 SPARK_API int spark_workspace_check(void* workspace, void* stream);
 
+/* Exchanges *mode and the calling thread's stream-capture mode (0 global, 1 thread
+ * local, 2 relaxed; cudaThreadExchangeStreamCaptureMode).  A workspace that a call
+ * under capture needs is allocated and zeroed in mode 2, on a stream that is not
+ * captured: a fill on the captured one would be a node of the graph, done by no
+ * launch but its replays, and by each of them. */
+SPARK_API int spark_capture_mode(int* mode);
+
 /* Elementwise SiLU(gate) * up for the MLP between the gate/up and down projections
  * (the activation the reference model applies between its MLP linears). */
 SPARK_API int spark_silu_mul(const void* gate, const void* up, void* out, int dtype, int64_t n, void* stream);

@@ -129,6 +129,7 @@ _SIGNATURES = {
     "spark_linear_chain": (_i, [_p, _i, _i64, _p, _sz, _p]),
     "spark_linear_noalloc": (_i, [_i, _p, _p, _p, _i, _i64, _i64, _i64, _i64, _p, _i, _p, _i, _i64, _p]),
     "spark_workspace_check": (_i, [_p, _p]),
+    "spark_capture_mode": (_i, [ctypes.POINTER(_i)]),
     "spark_tiled_bytes": (_sz, [_i, _i64, _i64]),
     "spark_tile_weights": (_i, [_i, _p, _p, _i64, _i64, _p, _p]),
     "spark_silu_mul": (_i, [_p, _p, _p, _i, _i64, _p]),

@@ -1754,6 +1754,15 @@ int spark_workspace_check(void* workspace, void* stream) {
     return SPARK_OK;
 }
 
+int spark_capture_mode(int* mode) {
+    SPARK_REQUIRE(mode && *mode >= 0 && *mode <= 2, SPARK_ERR_INVALID, "spark_capture_mode: mode 0, 1 or 2");
+    cudaStreamCaptureMode m = (cudaStreamCaptureMode)*mode;
+    const cudaError_t e = cudaThreadExchangeStreamCaptureMode(&m);
+    if (e != cudaSuccess) return set_error((int)e, "spark_capture_mode: %s", cudaGetErrorString(e));
+    *mode = (int)m;
+    return SPARK_OK;
+}
+
 }  // extern "C"
 
 // ====================================================================== no-allocation entry point

@@ -273,6 +273,28 @@ _ws_lock = threading.Lock()
 _ws: dict[tuple[int, int], torch.Tensor] = {}
 
 
+def _zeroed(nbytes: int, device: torch.device) -> torch.Tensor:
+    """Zeros to keep between calls.  Where the current stream is being captured the fill
+    would be a node of that graph, which its replays alone run, and each of them, and the
+    memory the graph's, shared with its other tensors: there they are allocated and
+    filled on another stream at once."""
+    with torch.cuda.device(device):
+        if not torch.cuda.is_current_stream_capturing():
+            return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        mode = ctypes.c_int(2)      # relaxed: this thread may allocate and wait beside the capture
+        call("spark_capture_mode", ctypes.byref(mode))
+        try:
+            while True:
+                side = torch.cuda.Stream()      # (of a pool, in turn: the captured stream is one of them)
+                with torch.cuda.stream(side):
+                    if not torch.cuda.is_current_stream_capturing():
+                        buf = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+                        side.synchronize()
+                        return buf
+        finally:
+            call("spark_capture_mode", ctypes.byref(mode))
+
+
 def workspace(device: torch.device, nbytes: int, stream=None) -> torch.Tensor:
     """Zero-initialised scratch for spark_linear, one per (device, stream)."""
     s = stream if stream is not None else torch.cuda.current_stream(device)
@@ -280,7 +302,7 @@ def workspace(device: torch.device, nbytes: int, stream=None) -> torch.Tensor:
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
-            buf = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+            buf = _zeroed(max(nbytes, 1 << 20), device)
             _ws[key] = buf
     return buf
 
@@ -398,7 +420,7 @@ def linear_chain(chain: list[ChainOp], stream=None) -> None:
     key = (x0.device.index, st.cuda_stream)
     ws = _chain_ws.get(key)
     if ws is None or ws.numel() < n:
-        ws = torch.zeros(n, dtype=torch.uint8, device=x0.device)
+        ws = _zeroed(n, x0.device)
         _chain_ws[key] = ws
     call("spark_linear_chain", ctypes.cast(arr, ctypes.c_void_p), len(chain), M, _p(ws), ws.numel(),
          ctypes.c_void_p(st.cuda_stream))
@@ -552,7 +574,7 @@ def _tree_workspace(device: torch.device, stream: int, nbytes: int = 256) -> tor
                 if buf is not None:
                     _tree_outgrown.append((key, buf))
                     nbytes = max(nbytes, 2 * buf.numel())     # (all the old ones together are no larger)
-                buf = torch.zeros(max(nbytes, 1 << 16), dtype=torch.uint8, device=device)
+                buf = _zeroed(max(nbytes, 1 << 16), device)
                 _tree_ws[key] = buf
     return buf
 

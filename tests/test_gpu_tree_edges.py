@@ -19,6 +19,62 @@ from test_gpu_tree_decode import BF, HF, attention64, check_attention, gen, make
 pytestmark = pytest.mark.gpu
 
 
+# ------------------------------------------------------------------ workspaces
+def test_workspaces_born_in_a_capture(monkeypatch):
+    """Their zeros are there before any replay, and no replay makes them anew: graphs of
+    one stream are replayed in any order, and errors stay."""
+    from spark_b200 import SparkError
+    from spark_b200.rotary import rope_table
+    g = gen(21)
+    for name in ("_ws", "_chain_ws", "_tree_ws"):
+        monkeypatch.setattr(ops(), name, {})
+    stream = torch.cuda.Stream()
+    rope_in, table = (randn(g, 4, 2, 64, dtype=BF), torch.tensor([3, 10, -1, 9], device="cuda")), rope_table(10, 32)
+    cases, graphs = [], []
+    for b, hq, n in ((2, 8, 900), (3, 8, 2000), (8, 32, 700)):
+        x = make(g, b, 8, hq, 2, 128, [n] * b, 32, BF)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            turned = ops().rope(rope_in[0], None, rope_in[1], table)[0] if len(graphs) == 1 else None
+            out, lse = ops().tree_attention(*x, return_lse=True)
+            if not graphs:
+                scratch = ops().workspace(x[0].device, 1 << 20)
+        cases.append((x, out, lse, turned))
+        graphs.append(graph)
+    tree = [v for (_, s), v in [*ops()._tree_ws.items(), *ops()._tree_outgrown] if s == stream.cuda_stream]
+    assert len(tree) >= 2 and all(int(v.count_nonzero()) == 0 for v in tree + [scratch])
+    for i in (2, 1, 0, 1, 0, 2):
+        x, out, lse, _ = cases[i]
+        out.zero_()
+        graphs[i].replay()
+        want, want_lse = attention64(*x, 128 ** -0.5)
+        check_attention(out, lse, want, want_lse, 5.0)
+    # the second graph's bad positions, with a replay of each graph since
+    with pytest.raises(SparkError, match="rotary table"):
+        ops().check_device_errors()
+    ops().check_device_errors()
+
+
+def test_two_streams_at_once():
+    """Each with a workspace of its own, their launches between one another's."""
+    g = gen(22)
+    cases = [make(g, 2, 8, 8, 2, 128, [900, 3000], 32, BF), make(g, 3, 20, 16, 4, 64, [1500, 10, 400], 16, BF)]
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for s, x, to in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                to.append(ops().tree_attention(*x, return_lse=True))
+    for s, x, to in zip(streams, cases, got):
+        torch.cuda.current_stream().wait_stream(s)
+        want, want_lse = attention64(*x, x[0].shape[-1] ** -0.5)
+        check_attention(*to[0], want, want_lse, 5.0)
+        assert all(torch.equal(a, b) for other in to for a, b in zip(to[0], other))
+    ops().check_device_errors()
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("b,t,hq,hkv,d,n", [

@@ -2,6 +2,9 @@
 sequence has, rotary scalings, sizes that the C entry points refuse."""
 from __future__ import annotations
 
+import ctypes
+
+from spark_b200 import _lib
 from spark_b200.tree_decode import PagedKVCache
 
 
@@ -21,3 +24,10 @@ def test_a_page_is_in_one_sequence_only():
     c.release(1)
     c.release(2)
     assert sorted(c._free) == list(range(6)) and (c.page_table == -1).all() and c.held.tolist() == [0, 0, 0]
+
+
+def test_capture_mode_refuses_other_modes():
+    for mode in (None, -1, 3):
+        m = ctypes.c_int(mode or 0)
+        assert _lib.lib().spark_capture_mode(None if mode is None else ctypes.byref(m)) == _lib.ERR_INVALID
+        assert "spark_capture_mode" in _lib.last_error()
