@@ -511,7 +511,9 @@ def check_device_errors(device=None) -> None:
             call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
         except _lib.SparkError:
             if any(buf is other for _, other in [*_tree_ws.items(), *_tree_outgrown]):
-                buf.zero_()    # an expired wait may leave its counters behind
+                # an expired wait may leave its counters behind; on the stream that uses them, before its next launch
+                with torch.cuda.stream(torch.cuda.ExternalStream(sh, device=buf.device)):
+                    buf.zero_()
             raise
 
 

@@ -75,6 +75,29 @@ def test_two_streams_at_once():
     ops().check_device_errors()
 
 
+def test_errors_are_cleared_on_the_workspace_s_own_stream():
+    """Work that the current stream still has to do neither holds the clearing back nor
+    lets it fall on a later launch of the workspace's stream."""
+    from spark_b200 import SparkError
+    from spark_b200.rotary import rope_table
+    q, bad, table = randn(gen(4), 4, 2, 64, dtype=BF), torch.full((4,), 99, device="cuda"), rope_table(10, 32)
+    for stream in (torch.cuda.Stream(), torch.cuda.default_stream()):
+        with torch.cuda.stream(stream):
+            stream.wait_stream(torch.cuda.default_stream())
+            ops().rope(q, None, bad, table)
+        other = torch.cuda.Stream()
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(200_000_000)       # about 0.1 s
+            with pytest.raises(SparkError, match="rotary table"):
+                ops().check_device_errors()
+        with torch.cuda.stream(stream):
+            ops().rope(q, None, bad, table)
+        other.synchronize()
+        with pytest.raises(SparkError, match="rotary table"):
+            ops().check_device_errors()
+        ops().check_device_errors()
+
+
 # ------------------------------------------------------------------ attention
 @pytest.mark.parametrize("dtype", [BF, HF])
 @pytest.mark.parametrize("b,t,hq,hkv,d,n", [
