@@ -137,6 +137,8 @@ struct Turn : torch::autograd::Function<Turn> {
 
 std::tuple<Tensor, OptTensor, int> apply_rope(const Tensor& q, const OptTensor& k, const Tensor& positions, const Tensor& table,
                                               bool interleaved, uint64_t ws, uint64_t stream) {
+    for (const Tensor* t : {&q, k ? &*k : &q, &table})
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), "apply_rope: no forward-mode differentiation");
     int rc = SPARK_OK;
     const auto out = Turn::turn(q, k, positions, table, interleaved, false, ws, stream, &rc);
     return {out[0], k ? OptTensor(out[1]) : std::nullopt, rc};
@@ -320,6 +322,8 @@ PYBIND11_MODULE(_native, m) {
             PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
         } catch (const c10::ValueError& e) {
             PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+        } catch (const c10::NotImplementedError& e) {
+            PyErr_SetString(PyExc_NotImplementedError, e.what_without_backtrace());
         } catch (const c10::Error& e) {
             PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
         }

@@ -55,8 +55,8 @@ def rope_table(positions: int, rot_dim: int, base: float = 10000.0, device=None,
 
 def apply_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
                interleaved: bool = False):
-    """Differentiable ops.rope: (q', k'), gradients of gradients too.  The gradient of the
-    positions and of the table is not computed."""
+    """Differentiable ops.rope: (q', k'), gradients of gradients too.  The gradients of the
+    positions and of the table are not computed; forward-mode differentiation is refused."""
     _, ws, stream = ops._place("rope", q)
     y, z, rc = ops._native().apply_rope(q, k, positions, table, interleaved, ws, stream)
     if rc:

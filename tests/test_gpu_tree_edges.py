@@ -187,3 +187,20 @@ def test_an_append_beyond_the_reserved_pages_is_reported():
     kept[c.page_table[c.page_table >= 0].long()] = True
     assert (c.k[0][~kept] == 0).all()
     ops().check_device_errors()
+
+
+def test_forward_mode_is_refused():
+    """No tangent is lost in silence, with and without a gradient in reverse."""
+    import torch.autograd.forward_ad as fwd
+    from spark_b200.rotary import apply_rope, rope_table
+    g = gen(3)
+    table, pos = rope_table(20, 16), torch.arange(5, device="cuda")
+    q, k, tangent = randn(g, 5, 2, 16), randn(g, 5, 1, 16), randn(g, 5, 2, 16)
+    with fwd.dual_level():
+        for x in (q, q.clone().requires_grad_()):
+            dual = fwd.make_dual(x, tangent)
+            for args in ((dual, k), (dual, None), (k, dual)):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    apply_rope(*args, pos, table)
+        apply_rope(q, k, pos, table)
+        apply_rope(q, None, pos, table)
