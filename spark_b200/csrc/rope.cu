@@ -86,7 +86,8 @@ struct Vec {
 };
 
 // units: places in a head that a thread may take -- the vectors of the turned part
-// (half layout: of its first half), then those that are copied (none in place).
+// (half layout: of its first half), then those that are copied (none in place, where
+// the first unit clears them if the position is bad).
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params p, int units, int turned) {
     using V = Vec<T, N>;
@@ -119,7 +120,12 @@ __global__ void __launch_bounds__(256) k_rope_vec(const __grid_constant__ Params
         if (!INTER && !copy) vb[k] = *reinterpret_cast<const R*>(x + half);
     }
     const bool good = pos >= 0 && pos < p.table_rows;
-    if (!good && unit == 0 && h0 == 0) report_device_error(p.err, 8);
+    if (!good && unit == 0) {
+        if (h0 == 0) report_device_error(p.err, 8);
+#pragma unroll
+        for (int k = 0; k < kHeads; ++k)
+            for (int e = p.rot; units == turned && y[k] && e < p.dim; e += N) *reinterpret_cast<R*>(y[k] + e) = V::zero();
+    }
     float c[PAIRS], sn[PAIRS];
     if (!copy) {
         const float* row = p.table + (good ? pos : 0) * p.rot + (INTER ? d / 2 : d);

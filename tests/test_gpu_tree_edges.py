@@ -14,9 +14,31 @@ import os
 import pytest
 import torch
 
-from test_gpu_tree_decode import BF, HF, attention64, check_attention, gen, make, ops, randn, sees
+from test_gpu_tree_decode import BF, FP, HF, attention64, check_attention, gen, make, ops, randn, sees
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ rope
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot", [(64, 32), (256, 64), (112, 28), (66, 6), (64, 64)])
+def test_rope_in_place_outside_the_table_gives_zero_rows(d, rot, interleaved, dtype):
+    from spark_b200 import SparkError
+    from spark_b200.rotary import rope_table
+    g = gen(2)
+    table, pos = rope_table(10, rot), torch.tensor([3, 10, -1, 9], device="cuda")
+    for both in (False, True):
+        for shift in (0, 1):      # an address of whole 16 bytes, one that is none
+            q, k = (torch.empty(4 * n * d + shift, dtype=dtype, device="cuda")[shift:].view(4, n, d).copy_(randn(g, 4, n, d, dtype=dtype))
+                    for n in (6, 3))
+            y, z = ops().rope(q, k if both else None, pos, table, interleaved)
+            ops().rope(q, k if both else None, pos, table, interleaved, out=(q, k if both else None))
+            assert torch.equal(q, y) and (q[1:3] == 0).all()
+            assert not both or (torch.equal(k, z) and (k[1:3] == 0).all())
+            with pytest.raises(SparkError, match="rotary table"):
+                ops().check_device_errors()
+    ops().check_device_errors()
 
 
 # ------------------------------------------------------------------ workspaces
