@@ -268,7 +268,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
         if (temp == 0.f) {
             const Note got = join_all<Best>(s, step, Note{m, nan ? 1.f : 0.f, at, 0});
             if (got.b != 0.f || got.i < 0 || got.a == INFINITY) break;   // no distribution here
-            while (child >= 0 && x != got.i) next();
+            while (child >= 0 && x != got.i) {
+                if (x < 0 && lead) report_device_error(p.err, 11);
+                next();
+            }
             if (child < 0) {
                 last = got.i;
                 break;

@@ -226,3 +226,20 @@ def test_forward_mode_is_refused():
                     apply_rope(*args, pos, table)
         apply_rope(q, k, pos, table)
         apply_rope(q, None, pos, table)
+
+
+def test_bad_token_ids_are_reported_at_any_temperature():
+    from spark_b200 import SparkError
+    g = gen(6)
+    logits, u = torch.randn(1, 3, 300, generator=g, device="cuda"), torch.zeros(1, 3, device="cuda")
+    noise = torch.empty(1, 300, device="cuda").exponential_(generator=g)
+    parents = torch.tensor([-1, 0, 0], dtype=torch.int32, device="cuda")
+    best = int(logits[0, 0].argmax())
+    for temperature in (0.0, 1.0):
+        for bad in (300, -1, 1 << 40, best + (1 << 32)):
+            tokens = torch.tensor([[0, bad, best]], device="cuda")
+            path, n, _ = ops().tree_verify(logits, tokens, parents, u, noise, temperature=temperature)
+            assert path.tolist() == [[0, 2, -1]] and n.tolist() == [2]
+            with pytest.raises(SparkError, match="vocabulary"):
+                ops().check_device_errors()
+    ops().check_device_errors()
