@@ -175,8 +175,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
     grid_wait();
     const float temp = a.temperature ? a.temperature[b] : 1.f;
     // Logits are multiplied by 1 / T: half a unit in the last place more than a division, which took a fifth of the time
-    // (64 trees over 100003 entries 58 us).  (Where 1 / T is no finite number, 0 / T still is 0.)
-    const float per_temp = fminf(fmaxf(1.f / temp, -FLT_MAX), FLT_MAX);
+    // (64 trees over 100003 entries 58 us).  1 / T stays between 2^-126 and 2^100: an infinite T gives equal chances to
+    // all entries above -inf, a T that is all but 0 the argmax, and logits up to 2^27 do not overflow.
+    const float per_temp = temp != temp ? temp : copysignf(fminf(fmaxf(1.f / fabsf(temp), FLT_MIN), 0x1p100f), temp);
     const bool lead = rank == 0 && tid == 0;
     int step = 0, cur = 0, accepted = 1;
     int64_t last = -1;
@@ -255,7 +256,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const int i = i0 + k * kThreads;
-                l[k] *= per_temp;
+                // (rounded alike wherever it is used: not fused with a subtraction)
+                l[k] = i < n ? __fmul_rn(l[k], per_temp) : -INFINITY;
                 if (i < n) raw[i] = l[k];
                 most = fmaxf(most, l[k]);
             }
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
                         known |= __any_sync(0xffffffffu, parents[c] == cur && tokens[c] == x);
                 }
                 if (valid && !known) {
-                    const float e = expf(lx * per_temp - top);
+                    const float e = expf(__fmul_rn(lx, per_temp) - top);
                     float rx = e / sum;
                     for (int k = 0; k < rejected && draft; ++k)
                         if (s.mass[k] > 0.f) rx = fmaxf(rx - qx, 0.f) / s.mass[k];

@@ -14,7 +14,8 @@ import os
 import pytest
 import torch
 
-from test_gpu_tree_decode import BF, FP, HF, attention64, check_attention, gen, make, ops, randn, sees
+from test_gpu_tree_decode import (BF, FP, HF, attention64, check_attention, check_verify, gen,
+                                  make, ops, randn, sees, verify_inputs)
 
 pytestmark = pytest.mark.gpu
 
@@ -242,4 +243,28 @@ def test_bad_token_ids_are_reported_at_any_temperature():
             assert path.tolist() == [[0, 2, -1]] and n.tolist() == [2]
             with pytest.raises(SparkError, match="vocabulary"):
                 ops().check_device_errors()
+    ops().check_device_errors()
+
+
+@pytest.mark.parametrize("sampled", [True, False])
+@pytest.mark.parametrize("v", [5, 300, 4096, 32768])
+def test_temperatures_at_the_ends(v, sampled):
+    """An infinite one is the uniform distribution of what is above -inf, the smallest
+    ones are the argmax, a negative one turns the logits round."""
+    g = gen(v)
+    x = verify_inputs(g, 24, 6, v, FP, sampled)
+    got = ops().tree_verify(*x[:5], draft_probs=x[5], temperature=math.inf)
+    check_verify(x, got, math.inf)
+    assert (got[2] >= 0).all()
+    got = ops().tree_verify(*x[:5], draft_probs=x[5], temperature=-1.5)
+    check_verify(x, got, -1.5)
+    for tiny in (1e-20, 1e-37, 1e-44):
+        check_verify(x, ops().tree_verify(*x[:5], draft_probs=x[5], temperature=tiny), tiny)
+    logits = x[0].clone()
+    logits[..., v // 2:] = -math.inf
+    parents = torch.tensor([-1] + [-2] * 5, dtype=torch.int32, device="cuda")
+    _, _, last = ops().tree_verify(logits, x[1], parents, x[3], x[4], temperature=math.inf)
+    assert torch.equal(last, x[4][:, :v // 2].argmin(-1))
+    got = ops().tree_verify(*x[:5], draft_probs=x[5], temperature=math.nan)
+    assert (got[1] == 1).all() and (got[2] == -1).all()
     ops().check_device_errors()
