@@ -16,7 +16,7 @@
 // order and so take the same decisions.  r at a single token needs no exchange:
 // every CTA computes it from the token's logit and the sums.  Without draft
 // probabilities a rejection needs no pass either, it takes one exponential out
-// of the sum.  Rows of nodes that the walk does not reach are not read, but for
+// of the sum, unless next to nothing is left of that.  Rows of nodes that the walk does not reach are not read, but for
 // the row of the first child, which is brought into L2 while its parent's is
 // worked on, as the noise is from the start.  Measured: a chain of 8 nodes over
 // 32000 entries 15 us (3.4 us a node: 1.2 the row's loads, 1.2 the join, 0.3 the
@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
         } else {
             const Note got = join_all<Softmax>(s, step, Note{m, z, 0, 0});
             const float top = got.a;
-            float sum = got.b;
+            float sum = got.b, added = got.b;    // added: the sum as last added up, sum: that without the rejected ones
             if (!(sum > 0.f && sum < INFINITY)) break;   // no distribution here
             int rejected = 0;          // children whose rejection changed r; with draft probabilities raw is r then
             float f = 1.f;             // r = raw f
@@ -302,12 +302,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
                         if (s.mass[k] > 0.f) rx = fmaxf(rx - qx, 0.f) / s.mass[k];
                     if (uniforms[child] * qx < rx) break;
                     if (!draft) {
-                        // without x: its exponential leaves the sum, its owner forgets it
-                        if (sum - e > 0.f) {
-                            sum -= e;
-                            const int64_t i = (int64_t)x - v0;
-                            if (i >= 0 && i < n && i % kThreads == tid) raw[i] = -INFINITY;
+                        // without x: its exponential leaves the sum, its owner forgets it.  The difference is as good as
+                        // 2^-24 of what was added up: where a sixteenth of that or less is left, it is added up anew.
+                        const int64_t i = (int64_t)x - v0;
+                        const bool owner = i >= 0 && i < n && i % kThreads == tid;
+                        if (owner) raw[i] = -INFINITY;
+                        float rest = sum - e;
+                        if (rest <= added * 0.0625f) {
+                            rest = 0.f;
+                            for (int k = tid; k < n; k += kThreads) rest += expf(raw[k] - top);
+                            rest = join_all<Sum>(s, step, Note{rest, 0.f, 0, 0}).a;
+                            if (rest > 0.f) added = rest;
                         }
+                        if (rest > 0.f) sum = rest;
+                        else if (owner) raw[i] = __fmul_rn(lx, per_temp);    // nothing is left: it stays what it was
                     } else {
                         float left = 0.f;
                         for (int i0 = tid; i0 < n; i0 += kBatch * kThreads) {

@@ -229,6 +229,44 @@ def test_forward_mode_is_refused():
         apply_rope(q, None, pos, table)
 
 
+# ------------------------------------------------------------------ verification
+@pytest.mark.parametrize("dtype", [FP, BF])
+@pytest.mark.parametrize("left,times", [(1e-4, 1), (0.1, 4), (0.02, 2)])
+def test_what_a_rejection_leaves_is_summed_anew(left, times, dtype):
+    """`times` children that leave `left` of the distribution each are rejected; the next
+    one's chance is known to a part in 10000, the draws are that far from it.  (In fp32
+    a chance is off by the rounding of logits below 32, 2^-20, a few times over; 1 minus
+    the rejected ones would be off by 2^-24 / left^times, 6 parts in 10000 and more.)"""
+    g = gen(17)
+    b, v, t = 256, 1000, times + 2
+    logits = torch.randn(b, 1, v, generator=g, device="cuda", dtype=torch.float64)
+    logits[..., :times + 1] -= 20
+    tokens = torch.zeros(b, t, dtype=torch.int64, device="cuda")
+    for i in reversed(range(times)):
+        # token i holds 1 - left of what the tokens after it leave
+        rest = torch.cat([logits[:, 0, i + 1:times], logits[:, 0, times:]], 1) if i + 1 < times else logits[:, 0, times:]
+        logits[:, 0, i] = torch.logsumexp(rest, -1) + math.log((1 - left) / left)
+        tokens[:, 1 + i] = i
+    logits = logits.expand(b, t, v).to(dtype)
+    x = logits[:, 0].double()
+    tokens[:, times + 1] = x[:, times:].argmax(-1) + times
+    rest = x.clone()
+    for i in range(times):
+        rest[:, i] = -math.inf
+    chance = torch.softmax(rest, -1).gather(1, tokens[:, times + 1:])[:, 0]
+    sign = torch.where(torch.arange(b, device="cuda") % 2 == 0, 1.0, -1.0)
+    u = torch.full((b, t), 1 - left / 10, device="cuda")
+    u[:, times + 1] = (chance * (1 + 1e-4 * sign)).float()
+    parents = torch.tensor([-1] + [0] * (t - 1), dtype=torch.int32, device="cuda")
+    noise = torch.empty(b, v, device="cuda").exponential_(generator=g)
+    path, n, _ = ops().tree_verify(logits, tokens, parents, u, noise)
+    taken = sign < 0
+    wrong = (n == 2) != taken
+    assert not wrong.any(), int(wrong.sum())
+    assert (path[:, 1] == torch.where(taken, times + 1, -1)).all()
+    ops().check_device_errors()
+
+
 def test_bad_token_ids_are_reported_at_any_temperature():
     from spark_b200 import SparkError
     g = gen(6)
