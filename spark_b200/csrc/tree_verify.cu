@@ -377,7 +377,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
         ++accepted;
         cur = child;
     }
-    if (step == 0) cluster_wait();
     if (rank == 0) {
         for (int i = accepted + tid; i < nodes; i += kThreads) a.path[b * nodes + i] = -1;
         if (tid == 0) a.accepted[b] = accepted, a.next[b] = last;
