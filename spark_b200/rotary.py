@@ -40,7 +40,8 @@ def rope_frequencies(rot_dim: int, base: float = 10000.0, scaling: str | None = 
         """The (real) index of the pair that turns so often within original_positions."""
         return rot_dim * math.log(original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot_dim // 2 - 1)
+    # (the blend may end behind the last pair, which then keeps a part of its angle)
+    lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot_dim - 1)
     blend = ((torch.arange(rot_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
     return freq * (1 - blend) + freq / factor * blend, (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0)
 

@@ -3,8 +3,12 @@ sequence has, rotary scalings, sizes that the C entry points refuse."""
 from __future__ import annotations
 
 import ctypes
+import math
 
-from spark_b200 import _lib
+import pytest
+import torch
+
+from spark_b200 import _lib, rotary
 from spark_b200.tree_decode import PagedKVCache
 
 
@@ -31,3 +35,21 @@ def test_capture_mode_refuses_other_modes():
         m = ctypes.c_int(mode or 0)
         assert _lib.lib().spark_capture_mode(None if mode is None else ctypes.byref(m)) == _lib.ERR_INVALID
         assert "spark_capture_mode" in _lib.last_error()
+
+
+@pytest.mark.parametrize("rot,base,original", [(128, 10000.0, 65536), (128, 10000.0, 1 << 20), (64, 10000.0, 131072), (64, 500000.0, 4096)])
+def test_yarn_blends_every_pair_between_its_limits(rot, base, original):
+    """Also where even the last pair turns more than `slow` times: it is not divided by
+    the whole factor then."""
+    factor, fast, slow = 8.0, 32.0, 1.0
+    f, _ = rotary.rope_frequencies(rot, base)
+    yarn, _ = rotary.rope_frequencies(rot, base, scaling="yarn", factor=factor, original_positions=original, fast=fast, slow=slow)
+    turns = f * original / (2 * math.pi)
+    # the pair's index (a real number) where a frequency turns n times
+    at = [rot / 2 * math.log(original / (2 * math.pi * n)) / math.log(base) for n in (fast, slow)]
+    lo, hi = math.floor(at[0]), math.ceil(at[1])
+    assert lo >= 0 and hi < rot
+    blend = ((torch.arange(rot // 2, dtype=torch.float64) - lo) / (hi - lo)).clamp(0, 1)
+    assert torch.allclose(yarn, f * (1 - blend) + f / factor * blend, rtol=1e-12)
+    kept = yarn / f
+    assert (kept[turns > slow * 1.5] > 1 / factor).all() and (kept[:-1] >= kept[1:]).all()
