@@ -139,6 +139,8 @@ class TreeDecoder(nn.Module):
 
     def prefill(self, tokens: torch.Tensor, cache: PagedKVCache) -> None:
         """Puts tokens [batch, n] into the cache, 64 at a time as a chain."""
+        if tokens.shape[1] == 0:
+            return
         for part in tokens.split(ops.MAX_TREE_NODES, dim=1):
             chain = torch.arange(-1, part.shape[1] - 1, dtype=torch.int32, device=part.device)
             _, new = self(part, chain, chain + 1, cache)

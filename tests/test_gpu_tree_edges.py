@@ -42,6 +42,53 @@ def test_rope_in_place_outside_the_table_gives_zero_rows(d, rot, interleaved, dt
     ops().check_device_errors()
 
 
+def test_forward_mode_is_refused():
+    """No tangent is lost in silence, with and without a gradient in reverse."""
+    import torch.autograd.forward_ad as fwd
+    from spark_b200.rotary import apply_rope, rope_table
+    g = gen(3)
+    table, pos = rope_table(20, 16), torch.arange(5, device="cuda")
+    q, k, tangent = randn(g, 5, 2, 16), randn(g, 5, 1, 16), randn(g, 5, 2, 16)
+    with fwd.dual_level():
+        for x in (q, q.clone().requires_grad_()):
+            dual = fwd.make_dual(x, tangent)
+            for args in ((dual, k), (dual, None), (k, dual)):
+                with pytest.raises(NotImplementedError, match="forward"):
+                    apply_rope(*args, pos, table)
+        apply_rope(q, k, pos, table)
+        apply_rope(q, None, pos, table)
+
+
+# ------------------------------------------------------------------ attention
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("b,t,hq,hkv,d,n", [
+    (40, 6, 8, 8, 128, 60), (2, 6, 8, 2, 128, 900),       # most items whole; all in parts
+    (60, 20, 32, 4, 64, 60), (3, 20, 32, 4, 64, 700),     # more than 128 rows an item
+    (40, 5, 8, 8, 256, 70), (1, 5, 4, 4, 256, 900),
+])
+def test_unused_nodes_give_zero_rows(b, t, hq, hkv, d, n, dtype):
+    """Whatever their queries and the values that others see hold."""
+    g = gen(t)
+    q, kt, vt, kc, vc, table, lens, parents = make(g, b, t, hq, hkv, d, [n] * b, 16, dtype)
+    parents[:, t - 1] = -2
+    want, want_lse = attention64(q, kt, vt, kc, vc, table, lens, parents, d ** -0.5)
+    used = torch.tensor([[len(chain) > 0 for chain in sees(p)] for p in parents.tolist()], device="cuda")
+    vmax = max(vt.abs().max().item(), vc.abs().max().item())
+    for bad in (math.nan, math.inf, -math.inf):
+        q2 = q.clone()
+        q2[~used] = bad
+        out, lse = ops().tree_attention(q2, kt, vt, kc, vc, table, lens, parents, return_lse=True)
+        check_attention(out, lse, want, want_lse, vmax)
+        # a value of the context that the used nodes see: theirs is what the formula gives, no number
+        v2 = vc.clone()
+        v2[table[:, 0].long(), 5, :, 3] = bad
+        out, lse = ops().tree_attention(q, kt, vt, kc, v2, table, lens, parents, return_lse=True)
+        assert (out[~used] == 0).all() and (lse[~used] == -math.inf).all()
+        assert not torch.isfinite(out[..., 3][used]).any()
+        assert torch.isfinite(out[..., 4:]).all() and torch.isfinite(lse[used]).all()
+    ops().check_device_errors()
+
+
 # ------------------------------------------------------------------ workspaces
 def test_workspaces_born_in_a_capture(monkeypatch):
     """Their zeros are there before any replay, and no replay makes them anew: graphs of
@@ -121,114 +168,6 @@ def test_errors_are_cleared_on_the_workspace_s_own_stream():
         ops().check_device_errors()
 
 
-# ------------------------------------------------------------------ attention
-@pytest.mark.parametrize("dtype", [BF, HF])
-@pytest.mark.parametrize("b,t,hq,hkv,d,n", [
-    (40, 6, 8, 8, 128, 60), (2, 6, 8, 2, 128, 900),       # most items whole; all in parts
-    (60, 20, 32, 4, 64, 60), (3, 20, 32, 4, 64, 700),     # more than 128 rows an item
-    (40, 5, 8, 8, 256, 70), (1, 5, 4, 4, 256, 900),
-])
-def test_unused_nodes_give_zero_rows(b, t, hq, hkv, d, n, dtype):
-    """Whatever their queries and the values that others see hold."""
-    g = gen(t)
-    q, kt, vt, kc, vc, table, lens, parents = make(g, b, t, hq, hkv, d, [n] * b, 16, dtype)
-    parents[:, t - 1] = -2
-    want, want_lse = attention64(q, kt, vt, kc, vc, table, lens, parents, d ** -0.5)
-    used = torch.tensor([[len(chain) > 0 for chain in sees(p)] for p in parents.tolist()], device="cuda")
-    vmax = max(vt.abs().max().item(), vc.abs().max().item())
-    for bad in (math.nan, math.inf, -math.inf):
-        q2 = q.clone()
-        q2[~used] = bad
-        out, lse = ops().tree_attention(q2, kt, vt, kc, vc, table, lens, parents, return_lse=True)
-        check_attention(out, lse, want, want_lse, vmax)
-        # a value of the context that the used nodes see: theirs is what the formula gives, no number
-        v2 = vc.clone()
-        v2[table[:, 0].long(), 5, :, 3] = bad
-        out, lse = ops().tree_attention(q, kt, vt, kc, v2, table, lens, parents, return_lse=True)
-        assert (out[~used] == 0).all() and (lse[~used] == -math.inf).all()
-        assert not torch.isfinite(out[..., 3][used]).any()
-        assert torch.isfinite(out[..., 4:]).all() and torch.isfinite(lse[used]).all()
-    ops().check_device_errors()
-
-
-# ------------------------------------------------------------------ the cache
-def example():
-    spec = importlib.util.spec_from_file_location(
-        "example_tree_decode", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "tree_decode.py"))
-    ex = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(ex)
-    return ex
-
-
-def test_rows_without_pages_leave_the_others_alone():
-    """A batch whose first sequence is gone, and whose last never came, decodes what the
-    second decodes by itself, and its pages are the same to the bit."""
-    from spark_b200.tree_decode import PagedKVCache, tree_depths
-    ex = example()
-    model = ex.build()
-    tree = torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda")
-    depths = tree_depths(tree.tolist()).cuda()
-    prompt = torch.randint(0, 2048, (1, 21), generator=gen(1), device="cuda").expand(3, -1)
-    tokens = torch.randint(0, 2048, (1, 4), generator=gen(2), device="cuda").expand(3, -1)
-    u, noise = torch.full((3, 4), 0.5, device="cuda"), torch.ones(3, 2048, device="cuda")
-    got = []
-    for before in (True, False):
-        c = PagedKVCache(2, 3, 64, 2, 64, page_size=8, pages=8)
-        if before:
-            c.reserve(0, 64)
-            c.release(0)
-        c.reserve(1, 40)
-        model.prefill(prompt, c)
-        if before:
-            c.reserve(0, 16)
-            c.release(0)
-        pages = c.page_table[1, :5].long()
-        path, n, last = model.step(tokens, tree, depths, c, u, noise, temperature=0.0)
-        assert c.lens.tolist() == [0, 21 + int(n[1]), 0]
-        got.append([path[1], last[1]] + [x[pages].clone() for x in c.k + c.v])
-        others = torch.ones(8, dtype=torch.bool, device="cuda").index_fill_(0, pages, False)
-        assert all((x[others] == 0).all() for x in c.k + c.v)
-    assert all(torch.equal(a, b) for a, b in zip(*got))
-    ops().check_device_errors()
-
-
-def test_an_append_beyond_the_reserved_pages_is_reported():
-    from spark_b200 import SparkError
-    from spark_b200.tree_decode import PagedKVCache
-    g = gen(3)
-    c = PagedKVCache(1, 2, 64, 2, 64, page_size=8)
-    c.reserve(0, 16)
-    c.reserve(1, 32)
-    k = randn(g, 2, 20, 2, 64, dtype=BF)
-    c.append([(k, k)])
-    with pytest.raises(SparkError, match="outside the cache"):
-        ops().check_device_errors()
-    for i, n in ((0, 16), (1, 20)):
-        rows = c.k[0][c.page_table[i, :-(-n // 8)].long()].flatten(0, 1)
-        assert torch.equal(rows[:n], k[i, :n]) and (rows[n:] == 0).all()
-    kept = torch.zeros(16, dtype=torch.bool, device="cuda")
-    kept[c.page_table[c.page_table >= 0].long()] = True
-    assert (c.k[0][~kept] == 0).all()
-    ops().check_device_errors()
-
-
-def test_forward_mode_is_refused():
-    """No tangent is lost in silence, with and without a gradient in reverse."""
-    import torch.autograd.forward_ad as fwd
-    from spark_b200.rotary import apply_rope, rope_table
-    g = gen(3)
-    table, pos = rope_table(20, 16), torch.arange(5, device="cuda")
-    q, k, tangent = randn(g, 5, 2, 16), randn(g, 5, 1, 16), randn(g, 5, 2, 16)
-    with fwd.dual_level():
-        for x in (q, q.clone().requires_grad_()):
-            dual = fwd.make_dual(x, tangent)
-            for args in ((dual, k), (dual, None), (k, dual)):
-                with pytest.raises(NotImplementedError, match="forward"):
-                    apply_rope(*args, pos, table)
-        apply_rope(q, k, pos, table)
-        apply_rope(q, None, pos, table)
-
-
 # ------------------------------------------------------------------ verification
 @pytest.mark.parametrize("dtype", [FP, BF])
 @pytest.mark.parametrize("left,times", [(1e-4, 1), (0.1, 4), (0.02, 2)])
@@ -306,3 +245,72 @@ def test_temperatures_at_the_ends(v, sampled):
     got = ops().tree_verify(*x[:5], draft_probs=x[5], temperature=math.nan)
     assert (got[1] == 1).all() and (got[2] == -1).all()
     ops().check_device_errors()
+
+
+# ------------------------------------------------------------------ the cache
+def example():
+    spec = importlib.util.spec_from_file_location(
+        "example_tree_decode", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "tree_decode.py"))
+    ex = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ex)
+    return ex
+
+
+def test_rows_without_pages_leave_the_others_alone():
+    """A batch whose first sequence is gone, and whose last never came, decodes what the
+    second decodes by itself, and its pages are the same to the bit."""
+    from spark_b200.tree_decode import PagedKVCache, tree_depths
+    ex = example()
+    model = ex.build()
+    tree = torch.tensor([-1, 0, 0, 1], dtype=torch.int32, device="cuda")
+    depths = tree_depths(tree.tolist()).cuda()
+    prompt = torch.randint(0, 2048, (1, 21), generator=gen(1), device="cuda").expand(3, -1)
+    tokens = torch.randint(0, 2048, (1, 4), generator=gen(2), device="cuda").expand(3, -1)
+    u, noise = torch.full((3, 4), 0.5, device="cuda"), torch.ones(3, 2048, device="cuda")
+    got = []
+    for before in (True, False):
+        c = PagedKVCache(2, 3, 64, 2, 64, page_size=8, pages=8)
+        if before:
+            c.reserve(0, 64)
+            c.release(0)
+        c.reserve(1, 40)
+        model.prefill(prompt, c)
+        if before:
+            c.reserve(0, 16)
+            c.release(0)
+        pages = c.page_table[1, :5].long()
+        path, n, last = model.step(tokens, tree, depths, c, u, noise, temperature=0.0)
+        assert c.lens.tolist() == [0, 21 + int(n[1]), 0]
+        got.append([path[1], last[1]] + [x[pages].clone() for x in c.k + c.v])
+        others = torch.ones(8, dtype=torch.bool, device="cuda").index_fill_(0, pages, False)
+        assert all((x[others] == 0).all() for x in c.k + c.v)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    ops().check_device_errors()
+
+
+def test_an_append_beyond_the_reserved_pages_is_reported():
+    from spark_b200 import SparkError
+    from spark_b200.tree_decode import PagedKVCache
+    g = gen(3)
+    c = PagedKVCache(1, 2, 64, 2, 64, page_size=8)
+    c.reserve(0, 16)
+    c.reserve(1, 32)
+    k = randn(g, 2, 20, 2, 64, dtype=BF)
+    c.append([(k, k)])
+    with pytest.raises(SparkError, match="outside the cache"):
+        ops().check_device_errors()
+    for i, n in ((0, 16), (1, 20)):
+        rows = c.k[0][c.page_table[i, :-(-n // 8)].long()].flatten(0, 1)
+        assert torch.equal(rows[:n], k[i, :n]) and (rows[n:] == 0).all()
+    kept = torch.zeros(16, dtype=torch.bool, device="cuda")
+    kept[c.page_table[c.page_table >= 0].long()] = True
+    assert (c.k[0][~kept] == 0).all()
+    ops().check_device_errors()
+
+
+def test_a_prompt_of_one_token():
+    """Its prefill has no tokens."""
+    ex = example()
+    model = ex.build()
+    new, steps = ex.generate(model, torch.tensor([[5], [9]], device="cuda"), 6, [-1])
+    assert steps == 6 and [len(t) for t in new] == [6, 6]
