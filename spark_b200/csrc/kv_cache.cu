@@ -103,7 +103,7 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     if (rc) return rc;
     SPARK_REQUIRE(batch >= 0 && batch < 65536 && tokens >= 0 && width >= 0, SPARK_ERR_INVALID,
                   "spark_kv_append: bad size (at most 65535 sequences)");
-    SPARK_REQUIRE(index || width == tokens, SPARK_ERR_INVALID, "spark_kv_append: without an index, width is tokens");
+    SPARK_REQUIRE(index || width == tokens || width == 0, SPARK_ERR_INVALID, "spark_kv_append: without an index, width is tokens");
     if (batch == 0) return SPARK_OK;
     SPARK_REQUIRE(new_lens && new_lens != cache->lens, SPARK_ERR_INVALID,
                   "spark_kv_append: new_lens is null or lens itself");

@@ -314,3 +314,14 @@ def test_a_prompt_of_one_token():
     model = ex.build()
     new, steps = ex.generate(model, torch.tensor([[5], [9]], device="cuda"), 6, [-1])
     assert steps == 6 and [len(t) for t in new] == [6, 6]
+
+
+# ------------------------------------------------------------------ append
+def test_an_index_without_columns_appends_nothing():
+    g = gen(5)
+    _, _, _, kc, vc, table, n, _ = make(g, 2, 1, 2, 2, 64, [30, 20], 16, BF)
+    k = randn(g, 2, 3, 2, 64, dtype=BF)
+    before = kc.clone(), vc.clone()
+    new = ops().kv_append(k, k, kc, vc, table, n, index=torch.zeros(2, 0, dtype=torch.int32, device="cuda"))
+    assert torch.equal(new, n) and torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+    ops().check_device_errors()
