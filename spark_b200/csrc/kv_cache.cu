@@ -82,7 +82,7 @@ int check_cache(const SparkPagedCache* c, const char* who) {
     SPARK_REQUIRE(c, SPARK_ERR_INVALID, "%s: null pointer", who);
     SPARK_REQUIRE(c->pages >= 1 && c->pages < (1ll << 31) && c->page_size >= 1 && c->page_size < (1 << 24) &&
                       c->kv_heads >= 1 && c->kv_heads < (1 << 16) && c->head_dim >= 1 && c->head_dim < (1 << 16) &&
-                      c->max_pages >= 0 && c->page_table_stride >= 0,
+                      c->kv_heads * c->head_dim < (1ll << 31) && c->max_pages >= 0 && c->page_table_stride >= 0,
                   SPARK_ERR_INVALID, "%s: bad cache size", who);
     SPARK_REQUIRE(c->max_pages * c->page_size < (1ll << 31), SPARK_ERR_INVALID,
                   "%s: a sequence's pages hold 2^31 tokens or more", who);

@@ -11,6 +11,8 @@ import torch
 from spark_b200 import _lib, rotary
 from spark_b200.tree_decode import PagedKVCache
 
+from test_tree_decode_cpu import P, cache
+
 
 def test_a_page_is_in_one_sequence_only():
     c = PagedKVCache(1, 3, 64, 1, 64, page_size=16, pages=6, device="cpu")
@@ -53,3 +55,12 @@ def test_yarn_blends_every_pair_between_its_limits(rot, base, original):
     assert torch.allclose(yarn, f * (1 - blend) + f / factor * blend, rtol=1e-12)
     kept = yarn / f
     assert (kept[turns > slow * 1.5] > 1 / factor).all() and (kept[:-1] >= kept[1:]).all()
+
+
+def test_append_refuses_rows_of_two_to_the_31_values():
+    st = (ctypes.c_int64 * 3)(1, 1, 1)
+    for heads, dim in ((65535, 65535), (65535, 32769)):
+        c = cache(kv_heads=heads, head_dim=dim)
+        rc = _lib.lib().spark_kv_append(ctypes.byref(c), 1, 1, P(256), st, P(256), st, None, 1, None, P(512), None, None)
+        assert rc == _lib.ERR_INVALID
+        assert "cache size" in _lib.last_error()
