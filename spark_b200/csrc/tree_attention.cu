@@ -1003,7 +1003,8 @@ int check(const SparkTreeAttention* a) {
                   (long long)(a->q_heads / a->cache.kv_heads));
     SPARK_REQUIRE(a->cache.page_size % 8 == 0, SPARK_ERR_UNSUPPORTED,
                   "spark_tree_attention: page_size %lld is no multiple of 8", (long long)a->cache.page_size);
-    SPARK_REQUIRE(a->scale > 0 && a->scale < 1e30, SPARK_ERR_INVALID, "spark_tree_attention: scale must be positive");
+    SPARK_REQUIRE(a->scale >= 1e-30 && a->scale <= 1e30, SPARK_ERR_INVALID,
+                  "spark_tree_attention: scale must be positive, 1e-30 to 1e30");
     return SPARK_OK;
 }
 

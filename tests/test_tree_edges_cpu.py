@@ -11,7 +11,7 @@ import torch
 from spark_b200 import _lib, rotary
 from spark_b200.tree_decode import PagedKVCache
 
-from test_tree_decode_cpu import P, cache
+from test_tree_decode_cpu import P, attention, cache
 
 
 def test_a_page_is_in_one_sequence_only():
@@ -64,3 +64,12 @@ def test_append_refuses_rows_of_two_to_the_31_values():
         rc = _lib.lib().spark_kv_append(ctypes.byref(c), 1, 1, P(256), st, P(256), st, None, 1, None, P(512), None, None)
         assert rc == _lib.ERR_INVALID
         assert "cache size" in _lib.last_error()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 1e-46, 9e-31, 2e30, math.inf, math.nan])
+def test_attention_refuses_scales_that_fp32_does_not_hold(scale):
+    """A scale that is 0 in fp32 would make a NaN of a masked score."""
+    a = attention(scale=scale)
+    assert _lib.lib().spark_tree_attention_workspace_size(ctypes.byref(a)) == 0
+    assert _lib.lib().spark_tree_attention(ctypes.byref(a), P(1 << 20), 1 << 30, None) == _lib.ERR_INVALID
+    assert "scale" in _lib.last_error()
