@@ -434,7 +434,7 @@ SPARK_API int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64
  * with fp32 scores, sums and accumulation.  An unused node gets a zero row and
  * lse -inf.  nodes <= 64; scale 1e-30 to 1e30; head_dim a multiple of 8, at most 256;
  * page_size a multiple of 8; at most 128 query heads per kv head; tensors 16-byte aligned with strides that are
- * multiples of 8, the workspace 256-byte aligned, its first int zero before the
+ * positive multiples of 8 (any where the extent is 1), the workspace 256-byte aligned, its first int zero before the
  * first use.  One node per sequence is plain decode attention. */
 #define SPARK_MAX_TREE_NODES 64
 typedef struct {

@@ -34,10 +34,10 @@ void need_cuda(const char* what, const char* name, const Tensor& t) {
 }
 Tensor unit(const Tensor& t) { return t.dim() == 0 || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
 
-// t, or a copy where the kernels' 16-byte loads do not fit its address or strides (4-D).
+// t, or a copy where the kernels' 16-byte loads do not fit its address or strides (4-D); a tensor map has no stride 0.
 Tensor tma(const Tensor& t) {
     bool fits = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-    for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+    for (int i = 0; i < 3; ++i) fits = fits && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0));
     return fits ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 void strides(int64_t* to, const Tensor& t) {

@@ -1138,10 +1138,10 @@ int spark_tree_attention(const SparkTreeAttention* args, void* workspace, size_t
     bool al = aligned(workspace, 256);
     for (const void* ptr : {a->q, a->k, a->v, (const void*)a->out, (const void*)c.k, (const void*)c.v}) al = al && aligned(ptr, 16);
     for (const int64_t* st : {(const int64_t*)a->q_stride, a->kn_stride, a->vn_stride, a->out_stride, c.k_stride, c.v_stride})
-        for (int i = 0; i < 3; ++i) al = al && st[i] % 8 == 0 && st[i] >= 0 && st[i] < (1ll << 38);
+        for (int i = 0; i < 3; ++i) al = al && st[i] % 8 == 0 && st[i] > 0 && st[i] < (1ll << 38);
     SPARK_REQUIRE(al, SPARK_ERR_ALIGNMENT,
-                  "spark_tree_attention: 16-byte aligned tensors with strides of a multiple of 8, and a 256-byte aligned "
-                  "workspace");
+                  "spark_tree_attention: 16-byte aligned tensors with strides of a positive multiple of 8, and a 256-byte "
+                  "aligned workspace");
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     const bool bf = c.dtype == SPARK_DTYPE_BF16;

@@ -89,6 +89,24 @@ def test_unused_nodes_give_zero_rows(b, t, hq, hkv, d, n, dtype):
     ops().check_device_errors()
 
 
+def test_tree_attention_of_expanded_inputs():
+    """Queries, keys or values that a batch, the nodes or the heads share (stride 0) give
+    what their copies give; an output or a cache of that kind is refused."""
+    from spark_b200 import SparkError
+    g = gen(14)
+    q, kt, vt, kc, vc, table, lens, parents = make(g, 3, 4, 8, 2, 64, [100, 30, 0], 16, BF)
+    args = (kc, vc, table, lens, parents)
+    for dim in range(3):
+        x, k, v = (t.narrow(dim, 0, 1).expand_as(t) for t in (q, kt, vt))
+        for tree in ((x, kt, vt), (q, k, vt), (q, kt, v), (x, k, v)):
+            assert torch.equal(ops().tree_attention(*tree, *args), ops().tree_attention(*(t.contiguous() for t in tree), *args))
+        with pytest.raises(SparkError, match="strides"):
+            ops().tree_attention(q, kt, vt, *args, out=x)
+        with pytest.raises(SparkError, match="strides"):
+            ops().tree_attention(q, kt, vt, kc.narrow(dim, 0, 1).expand_as(kc), *args[1:])
+    ops().check_device_errors()
+
+
 # ------------------------------------------------------------------ workspaces
 def test_workspaces_born_in_a_capture(monkeypatch):
     """Their zeros are there before any replay, and no replay makes them anew: graphs of

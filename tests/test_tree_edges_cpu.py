@@ -73,3 +73,22 @@ def test_attention_refuses_scales_that_fp32_does_not_hold(scale):
     assert _lib.lib().spark_tree_attention_workspace_size(ctypes.byref(a)) == 0
     assert _lib.lib().spark_tree_attention(ctypes.byref(a), P(1 << 20), 1 << 30, None) == _lib.ERR_INVALID
     assert "scale" in _lib.last_error()
+
+
+def test_attention_refuses_strides_of_zero():
+    """A tensor map takes none; the extents of 1 have no stride."""
+    def run(**kw):
+        a = attention(cache(**{n: v for n, v in kw.items() if n in ("k_stride", "v_stride")}), batch=2)
+        for n, v in kw.items():
+            if n in ("k_stride", "v_stride"):
+                continue
+            setattr(a, n, v)
+        return _lib.lib().spark_tree_attention(ctypes.byref(a), P(1 << 20), 1 << 30, None)
+
+    three = ctypes.c_int64 * 3
+    for name in ("q_stride", "kn_stride", "vn_stride", "out_stride", "k_stride", "v_stride"):
+        for at in range(3):
+            st = [1024, 256, 64]
+            st[at] = 0
+            assert run(**{name: three(*st)}) == _lib.ERR_ALIGNMENT, (name, at)
+            assert "strides" in _lib.last_error()
