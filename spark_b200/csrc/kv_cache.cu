@@ -110,6 +110,10 @@ int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens,
     SPARK_REQUIRE(cache->k && cache->v && cache->lens && (cache->page_table || cache->max_pages == 0), SPARK_ERR_INVALID,
                   "spark_kv_append: null pointer in the cache");
     SPARK_REQUIRE((k && v && k_stride && v_stride) || width == 0, SPARK_ERR_INVALID, "spark_kv_append: null pointer");
+    const int64_t extent[3] = {cache->pages, cache->page_size, cache->kv_heads};
+    for (int i = 0; i < 3; ++i)
+        SPARK_REQUIRE(extent[i] == 1 || (cache->k_stride[i] != 0 && cache->v_stride[i] != 0), SPARK_ERR_INVALID,
+                      "spark_kv_append: rows of the cache in one place");
     Params p{};
     p.c = *cache;
     p.k = k, p.v = v;

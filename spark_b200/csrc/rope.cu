@@ -242,12 +242,18 @@ int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int dtype, int6
         bool same = true;
         for (int i = 0; i < 3; ++i) same = same && s->xs[i] == s->ys[i];
         SPARK_REQUIRE(s->x != s->y || same, SPARK_ERR_INVALID, "spark_rope: in place needs equal strides");
+        const int64_t extent[3] = {batch, tokens, s->heads};
+        for (int i = 0; i < 3; ++i)
+            SPARK_REQUIRE(extent[i] == 1 || s->ys[i] != 0, SPARK_ERR_INVALID, "spark_rope: output rows in one place");
         t.x = s->x, t.y = s->y, t.heads = (int)s->heads;
         for (int i = 0; i < 3; ++i) t.xs[i] = s->xs[i], t.ys[i] = s->ys[i];
     }
     p.tokens = tokens, p.n_tokens = batch * tokens;
     p.dim = head_dim, p.rot = rot_dim, p.dtype = dtype, p.interleaved = interleaved, p.inverse = inverse;
     p.pos_bytes = position_bytes, p.positions = positions, p.table = table, p.table_rows = table_rows, p.err = err;
+    if (p.part[0].heads && p.part[1].heads)
+        SPARK_REQUIRE(p.part[0].y != p.part[1].x && p.part[1].y != p.part[0].x && p.part[0].y != p.part[1].y, SPARK_ERR_INVALID,
+                      "spark_rope: the output of one part is the other's input or output");
     const int64_t heads = p.part[0].heads + p.part[1].heads;
     if (heads == 0) return SPARK_OK;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);

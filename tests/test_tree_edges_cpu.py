@@ -92,3 +92,26 @@ def test_attention_refuses_strides_of_zero():
             st[at] = 0
             assert run(**{name: three(*st)}) == _lib.ERR_ALIGNMENT, (name, at)
             assert "strides" in _lib.last_error()
+
+
+def test_outputs_that_share_their_rows_are_refused():
+    def turn(x, y, ys=(512, 128, 64), heads=2, x2=None, y2=None):
+        q, k = _lib.SparkRopeHeads(x=x, y=y, heads=heads), _lib.SparkRopeHeads(x=x2, y=y2, heads=heads)
+        for h in (q, k):
+            h.xs[:], h.ys[:] = (512, 128, 64), ys
+        return _lib.lib().spark_rope(ctypes.byref(q), ctypes.byref(k) if x2 else None, 1, 2, 4, 64, 32, 0, 0, P(256), 8, P(256), 10,
+                                     None, None)
+
+    for ys in ((0, 128, 64), (512, 0, 64), (512, 128, 0)):
+        assert turn(1 << 20, 1 << 21, ys) == _lib.ERR_INVALID and "spark_rope: output rows" in _lib.last_error()
+    a, b, c = 1 << 20, 1 << 21, 1 << 22
+    for x, y, x2, y2 in ((a, b, b, a), (a, b, b, c), (a, a, b, a), (a, c, b, c)):
+        assert turn(x, y, x2=x2, y2=y2) == _lib.ERR_INVALID and "the other's" in _lib.last_error()
+    st, three = (ctypes.c_int64 * 3)(256, 128, 64), ctypes.c_int64 * 3
+    for name in ("k_stride", "v_stride"):
+        for at in range(3):
+            bad = [2048, 128, 64]
+            bad[at] = 0
+            rc = _lib.lib().spark_kv_append(ctypes.byref(cache(**{name: three(*bad)})), 1, 2, P(256), st, P(256), st, None, 2, None,
+                                            P(512), None, None)
+            assert rc == _lib.ERR_INVALID and "rows of the cache" in _lib.last_error()
