@@ -432,11 +432,17 @@ SPARK_API int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64
  *     out = softmax(scale q k^T) v, lse = log sum exp (fp32 [batch, nodes,
  *     q_heads] contiguous, or NULL)
  * with fp32 scores, sums and accumulation.  An unused node gets a zero row and
- * lse -inf.  nodes <= 64; scale 1e-30 to 1e30; head_dim a multiple of 8, at most 256;
- * page_size a multiple of 8; at most 128 query heads per kv head; tensors 16-byte aligned with strides that are
- * positive multiples of 8 (any where the extent is 1), the workspace 256-byte aligned, its first int zero before the
- * first use.  One node per sequence is plain decode attention. */
+ * lse -inf.  nodes <= 64; scale 1e-30 to 1e30; head_dim a multiple of 8, at most
+ * 256; page_size a multiple of 8; at most 128 query heads per kv head; tensors
+ * 16-byte aligned with strides that are positive multiples of 8 (any where the
+ * extent is 1).  One node per sequence is plain decode attention.
+ * workspace: spark_tree_attention_workspace_size(a) bytes, 256-byte aligned, for
+ * one launch at a time.  Its first SPARK_TREE_ATTENTION_ZEROED bytes (the error
+ * word and counters, which every launch leaves at zero) have to be zero before the
+ * first use, and to be zeroed again after error 10: a wait that expired leaves
+ * its counters behind, and spark_workspace_check clears the error word alone. */
 #define SPARK_MAX_TREE_NODES 64
+#define SPARK_TREE_ATTENTION_ZEROED 4096
 typedef struct {
     SparkPagedCache cache;
     int64_t batch, nodes, q_heads;

@@ -60,6 +60,9 @@ class SparkPagedCache(ctypes.Structure):
                 ("dtype", ctypes.c_int64)]
 
 
+TREE_ATTENTION_ZEROED = 4096    # SPARK_TREE_ATTENTION_ZEROED
+
+
 class SparkTreeAttention(ctypes.Structure):
     """struct SparkTreeAttention of include/spark_b200.h."""
     _fields_ = [("cache", SparkPagedCache), ("batch", ctypes.c_int64), ("nodes", ctypes.c_int64),

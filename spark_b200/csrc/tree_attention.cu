@@ -1019,7 +1019,9 @@ Plan plan(const SparkTreeAttention* a) {
     Plan q;
     int dev = 0;
     cudaGetDevice(&dev);
-    q.grid = tc::sm_count_cached(dev);
+    q.count = 256;
+    // (148 on a B200; two counters each lie in the part that the caller zeroes)
+    q.grid = std::min(tc::sm_count_cached(dev), (int)((SPARK_TREE_ATTENTION_ZEROED - q.count) / (2 * sizeof(int))));
     q.dp = padded_dim(a->cache.head_dim);
     q.group = (int)(a->q_heads / a->cache.kv_heads);
     q.tile_nodes = std::min(128 / q.group, (int)a->nodes);
@@ -1027,8 +1029,7 @@ Plan plan(const SparkTreeAttention* a) {
     q.item_nodes = q.by_rows ? 2 * q.tile_nodes : q.tile_nodes;
     q.row_tiles = (int)((a->nodes + q.item_nodes - 1) / q.item_nodes);
     q.rows_item = q.by_rows ? 256 : q.tile_nodes * q.group;
-    q.count = 256;
-    q.part_ml = (q.count + (size_t)2 * q.grid * sizeof(int) + 255) / 256 * 256;
+    q.part_ml = SPARK_TREE_ATTENTION_ZEROED;
     q.part = (q.part_ml + (size_t)2 * q.grid * q.rows_item * sizeof(float2) + 255) / 256 * 256;
     q.bytes = q.part + (size_t)2 * q.grid * q.rows_item * q.dp * sizeof(float);
     return q;

@@ -513,7 +513,7 @@ def check_device_errors(device=None) -> None:
             if any(buf is other for _, other in [*_tree_ws.items(), *_tree_outgrown]):
                 # an expired wait may leave its counters behind; on the stream that uses them, before its next launch
                 with torch.cuda.stream(torch.cuda.ExternalStream(sh, device=buf.device)):
-                    buf.zero_()
+                    buf[:_lib.TREE_ATTENTION_ZEROED].zero_()
             raise
 
 

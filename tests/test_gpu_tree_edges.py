@@ -107,6 +107,37 @@ def test_tree_attention_of_expanded_inputs():
     ops().check_device_errors()
 
 
+def test_a_workspace_as_the_header_asks_for_it():
+    """Zeros where the C header says so, every bit set behind them, and nothing else done
+    between calls; items in parts of several CTAs."""
+    import ctypes
+    from spark_b200 import _lib
+    L = _lib.lib()
+    g = gen(15)
+    for b, t, hq, hkv, d, n in ((1, 1, 16, 16, 256, 1000), (2, 64, 8, 1, 128, 5000), (3, 9, 4, 2, 64, 900)):
+        x = q, kt, vt, kc, vc, table, lens, parents = make(g, b, t, hq, hkv, d, [n] * b, 16, BF)
+        want, lse = ops().tree_attention(*x, return_lse=True)
+        out, lse2 = torch.empty_like(q), torch.empty_like(lse)
+        c = _lib.SparkPagedCache(k=kc.data_ptr(), v=vc.data_ptr(), pages=kc.shape[0], page_size=16, kv_heads=hkv, head_dim=d,
+                                 page_table=table.data_ptr(), page_table_stride=table.stride(0), max_pages=table.shape[1],
+                                 lens=lens.data_ptr(), dtype=_lib.DTYPE_BF16)
+        c.k_stride[:], c.v_stride[:] = kc.stride()[:3], vc.stride()[:3]
+        a = _lib.SparkTreeAttention(cache=c, batch=b, nodes=t, q_heads=hq, q=q.data_ptr(), k=kt.data_ptr(), v=vt.data_ptr(),
+                                    out=out.data_ptr(), parents=parents.data_ptr(), parents_stride=parents.stride(0),
+                                    lse=lse2.data_ptr(), scale=d ** -0.5)
+        a.q_stride[:], a.out_stride[:] = q.stride()[:3], out.stride()[:3]
+        a.kn_stride[:], a.vn_stride[:] = kt.stride()[:3], vt.stride()[:3]
+        size = L.spark_tree_attention_workspace_size(ctypes.byref(a))
+        ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+        ws[:_lib.TREE_ATTENTION_ZEROED] = 0
+        stream = torch.cuda.current_stream().cuda_stream
+        for _ in range(3):
+            out.zero_()
+            assert L.spark_tree_attention(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), size, ctypes.c_void_p(stream)) == _lib.OK
+            assert torch.equal(out, want) and torch.equal(lse2, lse)
+        assert int(ws[:_lib.TREE_ATTENTION_ZEROED].count_nonzero()) == 0
+
+
 # ------------------------------------------------------------------ workspaces
 def test_workspaces_born_in_a_capture(monkeypatch):
     """Their zeros are there before any replay, and no replay makes them anew: graphs of

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import os
 
 import pytest
 import torch
@@ -115,3 +116,9 @@ def test_outputs_that_share_their_rows_are_refused():
             rc = _lib.lib().spark_kv_append(ctypes.byref(cache(**{name: three(*bad)})), 1, 2, P(256), st, P(256), st, None, 2, None,
                                             P(512), None, None)
             assert rc == _lib.ERR_INVALID and "rows of the cache" in _lib.last_error()
+
+
+def test_the_zeroed_part_of_a_workspace_is_the_header_s():
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "spark_b200.h")).read()
+    assert f"#define SPARK_TREE_ATTENTION_ZEROED {_lib.TREE_ATTENTION_ZEROED}\n" in header
+    assert _lib.lib().spark_tree_attention_workspace_size(ctypes.byref(attention())) > _lib.TREE_ATTENTION_ZEROED
