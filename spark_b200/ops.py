@@ -302,7 +302,8 @@ def workspace(device: torch.device, nbytes: int, stream=None) -> torch.Tensor:
     with _ws_lock:
         buf = _ws.get(key)
         if buf is None or buf.numel() < nbytes:
-            buf = _zeroed(max(nbytes, 1 << 20), device)
+            with torch.cuda.stream(s):
+                buf = _zeroed(max(nbytes, 1 << 20), device)
             _ws[key] = buf
     return buf
 
@@ -420,7 +421,8 @@ def linear_chain(chain: list[ChainOp], stream=None) -> None:
     key = (x0.device.index, st.cuda_stream)
     ws = _chain_ws.get(key)
     if ws is None or ws.numel() < n:
-        ws = _zeroed(n, x0.device)
+        with torch.cuda.stream(st):
+            ws = _zeroed(n, x0.device)
         _chain_ws[key] = ws
     call("spark_linear_chain", ctypes.cast(arr, ctypes.c_void_p), len(chain), M, _p(ws), ws.numel(),
          ctypes.c_void_p(st.cuda_stream))

@@ -217,6 +217,19 @@ def test_errors_are_cleared_on_the_workspace_s_own_stream():
         ops().check_device_errors()
 
 
+def test_a_workspace_is_zero_on_the_stream_it_is_for(monkeypatch):
+    """Not only once the current stream has got there."""
+    monkeypatch.setattr(ops(), "_ws", {})
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+    torch.full((1 << 20,), 255, dtype=torch.uint8, device="cuda")
+    torch.cuda._sleep(200_000_000)       # about 0.1 s
+    ws = ops().workspace(torch.device("cuda", torch.cuda.current_device()), 1 << 20, stream=stream)
+    with torch.cuda.stream(stream):
+        assert int(ws.count_nonzero()) == 0
+
+
 # ------------------------------------------------------------------ verification
 @pytest.mark.parametrize("dtype", [FP, BF])
 @pytest.mark.parametrize("left,times", [(1e-4, 1), (0.1, 4), (0.02, 2)])
