@@ -230,12 +230,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
         float m = -INFINITY, z = 0.f;
         int at = -1;
         bool nan = false;
+        const L none(temp < 0.f ? INFINITY : -INFINITY);   // over T -inf
         L ahead[kBatch];      // the next entries, on their way during the work on these
         auto load = [&](int i0) {
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) {
                 const int i = i0 + k * kThreads;
-                ahead[k] = i < n ? row[v0 + i] : L(-INFINITY);
+                ahead[k] = i < n ? row[v0 + i] : none;
             }
         };
         load(tid);
@@ -257,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
             for (int k = 0; k < kBatch; ++k) {
                 const int i = i0 + k * kThreads;
                 // (rounded alike wherever it is used: not fused with a subtraction)
-                l[k] = i < n ? __fmul_rn(l[k], per_temp) : -INFINITY;
+                l[k] = __fmul_rn(l[k], per_temp);
                 if (i < n) raw[i] = l[k];
                 most = fmaxf(most, l[k]);
             }
