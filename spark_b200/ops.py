@@ -505,17 +505,23 @@ def linear_batch_allreduce(batch: list[BatchOp], op: int, world: int, rank: int,
 
 
 def check_device_errors(device=None) -> None:
-    """Raise if a kernel left an error in a workspace (synchronises)."""
-    for (dev, sh), buf in list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()) + _tree_outgrown:
+    """Raise if a kernel left an error in a workspace.  Synchronises the devices: a
+    workspace is used on its stream, and by the graphs captured there on any."""
+    all_ws = list(_ws.items()) + list(_chain_ws.items()) + list(_tree_ws.items()) + _tree_outgrown
+    for dev in {dev for (dev, _), _ in all_ws if device is None or dev == device}:
+        torch.cuda.synchronize(dev)
+    for (dev, sh), buf in all_ws:
         if device is not None and dev != device:
             continue
         try:
             call("spark_workspace_check", _p(buf), ctypes.c_void_p(sh))
         except _lib.SparkError:
             if any(buf is other for _, other in [*_tree_ws.items(), *_tree_outgrown]):
-                # an expired wait may leave its counters behind; on the stream that uses them, before its next launch
-                with torch.cuda.stream(torch.cuda.ExternalStream(sh, device=buf.device)):
+                # an expired wait may leave its counters behind; cleared before the next launch on any stream
+                stream = torch.cuda.ExternalStream(sh, device=buf.device)
+                with torch.cuda.stream(stream):
                     buf[:_lib.TREE_ATTENTION_ZEROED].zero_()
+                stream.synchronize()
             raise
 
 

@@ -217,6 +217,24 @@ def test_errors_are_cleared_on_the_workspace_s_own_stream():
         ops().check_device_errors()
 
 
+def test_errors_of_a_replay_on_another_stream():
+    """The check waits for the replay, which is not on the stream of its capture."""
+    from spark_b200 import SparkError
+    from spark_b200.rotary import rope_table
+    q, bad, table = randn(gen(4), 4, 2, 64, dtype=BF), torch.full((4,), 99, device="cuda"), rope_table(10, 32)
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    ops().rope(q, None, bad * 0, table)
+    with torch.cuda.graph(graph):
+        ops().rope(q, None, bad, table)
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(200_000_000)       # about 0.1 s
+        graph.replay()
+    with pytest.raises(SparkError, match="rotary table"):
+        ops().check_device_errors()
+    ops().check_device_errors()
+
+
 def test_a_workspace_is_zero_on_the_stream_it_is_for(monkeypatch):
     """Not only once the current stream has got there."""
     monkeypatch.setattr(ops(), "_ws", {})
