@@ -390,7 +390,8 @@ SPARK_API int spark_silu_mul_rows(const void* gate, const void* up, int64_t ld_i
  * of dtype with strides xs (batch, token, head), y with ys; positions
  * [batch, tokens] contiguous, 4- or 8-byte integers; table fp32 [table_rows,
  * rot_dim] (cosines, then sines; any scaling for long contexts is in it).  A
- * position outside the table gives a zero row and error 8 in *err. */
+ * position outside the table gives a zero row and error 8 in *err.  Rows of y are
+ * apart from one another, and from the other part's x and y. */
 typedef struct {
     const void* x;
     void* y;
@@ -418,8 +419,9 @@ typedef struct {
  * row j) of k / v [batch, tokens, kv_heads, head_dim] (strides batch, token, head)
  * goes to position lens[b] + j.  n_b = counts[b] (counts NULL: all `width`
  * columns of index, or all tokens).  new_lens [batch] = lens + n_b; it may not be
- * lens itself.  What does not fit the sequence's pages is left out, a bad page
- * number or index skips its token; both set error 9 in *err. */
+ * lens itself.  What is beyond the table's max_pages is left out, of new_lens too;
+ * a bad page number (as -1 where a sequence has no page) or index skips its token;
+ * both set error 9 in *err. */
 SPARK_API int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64_t tokens, const void* k,
                               const int64_t* k_stride, const void* v, const int64_t* v_stride, const int* index,
                               int64_t width, const int* counts, int* new_lens, int* err, void* stream);
@@ -470,10 +472,11 @@ SPARK_API int spark_tree_attention(const SparkTreeAttention* a, void* workspace,
  * last rejection, or at a leaf, next = argmax_v r(v) / noise[b, v], with
  * exponential variates noise a sample of r; the lowest index wins a tie.
  * Temperature 0: x is accepted when it is the argmax of the logits (the lowest
- * index of a tie), next is that argmax.  Outputs: path [batch, nodes] = accepted
+ * index of a tie), next is that argmax; an infinite one gives what is above -inf
+ * equal chances.  Outputs: path [batch, nodes] = accepted
  * nodes from node 0 on, then -1; accepted [batch] their number; next [batch].
- * A row of logits without a distribution (a NaN, +inf, or no value above -inf)
- * ends the sequence with next = -1.  A token id outside the vocabulary is never
+ * A row of logits without a distribution (a NaN, +inf, no value above -inf, or a
+ * temperature that is NaN) ends the sequence with next = -1.  A token id outside the vocabulary is never
  * accepted and sets error 11 in *err.  nodes <= 1024, vocab <= 425,984. */
 typedef struct {
     int64_t batch, nodes, vocab;

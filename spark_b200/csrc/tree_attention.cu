@@ -12,6 +12,9 @@
 // error, at most 2^-9 in bf16, is independent from weight to weight).  O is
 // rescaled only when m grows by more than 2^8 -- weights up to 2^8 are as exact
 // as those below 1 -- since a rescale is a round trip of O through registers.
+// The tensor cores cut a product off at 2^-25 of the O that it is added to: next
+// to one token, n others of 2^-25 of its weight lose up to n 2^-25 of the sum
+// (262144 of them half of their own 0.3 %).
 //
 // Work: an item is (sequence, kv head, tile of rows), its tiles are the context
 // in steps of 128 tokens (64 for heads above 128 wide) and last the tree.  All tiles of all items form one
@@ -45,11 +48,11 @@
 // memory; 128 x 64 from shared memory takes 48, so that tiles of 64 tokens cost
 // more) and about 2100 of softmax (1024 of them the exponential unit's).  In turns
 // two streams hide each other's chains and HBM bounds: 16 sequences of up to 32k
-// tokens, 128 rows, 2430 cycles a tile, 285 us (5.8 TB/s).  By rows a tile is
+// tokens, 128 rows, 2430 cycles a tile, 290 us (5.7 TB/s).  By rows a tile is
 // 2 x (1024 + 2100) cycles of work on two engines that wait for each other: 64
-// nodes x 8 heads over 65k tokens, 3990 cycles a tile, 132 us (0.91 PFLOP/s), where
+// nodes x 8 heads over 65k tokens, 3990 cycles a tile, 129-135 us (0.9 PFLOP/s), where
 // neither is full.  Both run into the power cap when repeated (1000 W at 1.4 GHz:
-// 313 us, 153 us).  Small calls are their start (5 us to the first scores: lengths,
+// 331-341 us, 155-158 us).  Small calls are their start (5 us to the first scores: lengths,
 // page numbers and the first tile are three round trips to memory) and their end
 // (about 6 us: the parts' stores made visible, counted, read and added).  Many
 // short contexts are a chain for each item (about 8500 cycles for 88 tokens and 8

@@ -20,8 +20,8 @@
 // the row of the first child, which is brought into L2 while its parent's is
 // worked on, as the noise is from the start.  Measured: a chain of 8 nodes over
 // 32000 entries 15 us (3.4 us a node: 1.2 the row's loads, 1.2 the join, 0.3 the
-// exponentials), 64 trees of 16 nodes over 100003 entries 44 us
-// (46 without the next entries' loads during the work on the last).  256 or 1024
+// exponentials), 64 trees of 16 nodes over 100003 entries 45 us
+// (47 without the next entries' loads during the work on the last).  256 or 1024
 // threads a CTA were 5 to 40% slower; three or four CTAs to an SM, which takes
 // spilled registers, 7 to 35% for few sequences and no faster for many.
 #include <float.h>
@@ -263,6 +263,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_tree_verify(const __grid_consta
                 most = fmaxf(most, l[k]);
             }
             const float ref = most == -INFINITY ? 0.f : most;
+            // (__expf(x) is off by up to 2 + 1.2 |x| units in its last place, the rounding of a scaled logit l makes
+            // |l| / 2 of them in any case)
             z *= __expf(m - ref);
 #pragma unroll
             for (int k = 0; k < kBatch; ++k) z += __expf(l[k] - ref);
@@ -416,9 +418,9 @@ int launch(const Params& p, int64_t batch, int cs, cudaStream_t s) {
 // CTAs of a cluster.  When the sequences' clusters do not fit the GPU at once they run one after another; smaller
 // clusters then have more at work, each with longer rows, fewer barriers and less waiting.  The time goes with (sequences
 // at a time, at least one filling) x (a pass's fixed part + a thread's share of the row), the fixed part worth 8 entries a
-// thread.  Measured with 8 / 4 / 2 / 1 CTAs: 32 trees of 8 nodes over 32000 entries 19 / 24 / 32 / 57 us, 64 35 / 28 / 39 /
-// 71, 512 219 / 140 / 114 / 175; over 100003 entries (2 at least) 64 62 / 62 / 88, 512 373 / 293 / 387; over 1000 entries
-// 512 165 / 82 / 45 / 28.
+// thread.  Measured with 8 / 4 / 2 / 1 CTAs, sampled drafts: 32 trees of 8 nodes over 32000 entries 19 / 24 / 33 / 52 us, 64
+// 36 / 29 / 40 / 60, 128 64 / 47 / 49 / 67, 512 225 / 144 / 117 / 155; over 100003 entries (2 at least) 64 64 / 64 / 89, 128
+// 112 / 107 / 143, 512 387 / 303 / 390; over 1000 entries 128 47 / 26 / 16 / 15, 512 169 / 84 / 47 / 28.
 int cluster_ctas(int64_t batch, int64_t vocab, int64_t nodes, int sms) {
     int best = kMaxCluster;
     double least = 0;
