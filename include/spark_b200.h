@@ -440,9 +440,9 @@ SPARK_API int spark_kv_append(const SparkPagedCache* cache, int64_t batch, int64
  * extent is 1).  One node per sequence is plain decode attention.
  * workspace: spark_tree_attention_workspace_size(a) bytes, 256-byte aligned, for
  * one launch at a time.  Its first SPARK_TREE_ATTENTION_ZEROED bytes (the error
- * word and counters, which every launch leaves at zero) have to be zero before the
- * first use, and to be zeroed again after error 10: a wait that expired leaves
- * its counters behind, and spark_workspace_check clears the error word alone. */
+ * word, and counters that a launch leaves at zero) have to be zero before the first
+ * use, and to be zeroed again after error 10: a wait that expired leaves counters
+ * behind, and spark_workspace_check clears the error word alone. */
 #define SPARK_MAX_TREE_NODES 64
 #define SPARK_TREE_ATTENTION_ZEROED 4096
 typedef struct {
@@ -473,11 +473,11 @@ SPARK_API int spark_tree_attention(const SparkTreeAttention* a, void* workspace,
  * exponential variates noise a sample of r; the lowest index wins a tie.
  * Temperature 0: x is accepted when it is the argmax of the logits (the lowest
  * index of a tie), next is that argmax; an infinite one gives what is above -inf
- * equal chances.  Outputs: path [batch, nodes] = accepted
- * nodes from node 0 on, then -1; accepted [batch] their number; next [batch].
- * A row of logits without a distribution (a NaN, +inf, no value above -inf, or a
- * temperature that is NaN) ends the sequence with next = -1.  A token id outside the vocabulary is never
- * accepted and sets error 11 in *err.  nodes <= 1024, vocab <= 425,984. */
+ * equal chances.  Outputs: path [batch, nodes] = accepted nodes from node 0 on, then
+ * -1; accepted [batch] their number; next [batch].  A row of logits without a
+ * distribution (a NaN, +inf, no value above -inf, or a NaN as temperature) ends the
+ * sequence with next = -1.  A token id outside the vocabulary is never accepted and
+ * sets error 11 in *err.  nodes <= 1024, vocab <= 425,984. */
 typedef struct {
     int64_t batch, nodes, vocab;
     const void* logits;

@@ -14,7 +14,8 @@
 // as those below 1 -- since a rescale is a round trip of O through registers.
 // The tensor cores cut a product off at 2^-25 of the O that it is added to: next
 // to one token, n others of 2^-25 of its weight lose up to n 2^-25 of the sum
-// (262144 of them half of their own 0.3 %).
+// (two tokens and 262144 others of 2^-25.3 of them: half of the others' 0.3 % of
+// the sum).
 //
 // Work: an item is (sequence, kv head, tile of rows), its tiles are the context
 // in steps of 128 tokens (64 for heads above 128 wide) and last the tree.  All tiles of all items form one

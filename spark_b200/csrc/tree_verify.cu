@@ -16,9 +16,10 @@
 // order and so take the same decisions.  r at a single token needs no exchange:
 // every CTA computes it from the token's logit and the sums.  Without draft
 // probabilities a rejection needs no pass either, it takes one exponential out
-// of the sum, unless next to nothing is left of that.  Rows of nodes that the walk does not reach are not read, but for
-// the row of the first child, which is brought into L2 while its parent's is
-// worked on, as the noise is from the start.  Measured: a chain of 8 nodes over
+// of the sum, unless a sixteenth or less is left of that.  Rows of nodes that the
+// walk does not reach are not read, but for the row of the first child, which is
+// brought into L2 while its parent's is worked on, as the noise is from the start.
+// Measured: a chain of 8 nodes over
 // 32000 entries 15 us (3.4 us a node: 1.2 the row's loads, 1.2 the join, 0.3 the
 // exponentials), 64 trees of 16 nodes over 100003 entries 45 us
 // (47 without the next entries' loads during the work on the last).  256 or 1024
