@@ -402,6 +402,40 @@ SPARK_API int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int d
                          int head_dim, int rot_dim, int interleaved, int inverse, const void* positions,
                          int position_bytes, const float* table, int64_t table_rows, int* err, void* stream);
 
+/* RMS norms of q and k for each head, with the rotary positions of spark_rope in
+ * the same pass (either part may have no heads).  For a head x at position p, with
+ * the rotation R(p) of its first rot_dim values:
+ *     s = (mean x^2 + eps)^-1/2,  y = R(p) (s x weight)
+ * in fp32, rounded once; weight NULL: ones.  x and y [batch, tokens, heads,
+ * head_dim] of dtype, weight [head_dim] of weight_dtype; y may be x with equal
+ * strides.  head_dim is even, at most 256; interleaved pairs lie on two values'
+ * bytes.  A position outside the table gives a zero row and error 8 in *err.
+ *
+ * spark_qk_norm_rope_backward: dy is the gradient of y (strides dys), y takes that
+ * of x, dweight that of weight (weight_dtype; NULL: not wanted), from sums in fp32
+ * whose order depends on the sizes alone.  A row of a bad position has none.
+ * workspace: where a dweight is wanted, spark_qk_norm_rope_backward_workspace_size
+ * bytes on the current device, 16-byte aligned; what is in it does not matter. */
+typedef struct {
+    const void *x, *dy;
+    void* y;
+    const void* weight;
+    void* dweight;
+    int64_t weight_dtype, heads;
+    int64_t xs[3], dys[3], ys[3];
+} SparkNormRopeHeads;
+typedef struct {
+    SparkNormRopeHeads part[2];
+    int64_t dtype, batch, tokens, head_dim, rot_dim, interleaved, position_bytes, table_rows;
+    double eps;
+    const void* positions;
+    const float* table;
+} SparkNormRope;
+SPARK_API int spark_qk_norm_rope(const SparkNormRope* a, int* err, void* stream);
+SPARK_API size_t spark_qk_norm_rope_backward_workspace_size(int64_t head_dim);
+SPARK_API int spark_qk_norm_rope_backward(const SparkNormRope* a, void* workspace, size_t workspace_bytes, int* err,
+                                          void* stream);
+
 /* A paged K/V cache: token n of sequence b lies in page page_table[b, n /
  * page_size], row n % page_size.  k and v: element (page, row, head, 0) with
  * strides (page, row, head) k_stride / v_stride; lens [batch]: tokens in it. */

@@ -51,6 +51,21 @@ class SparkRopeHeads(ctypes.Structure):
                 ("xs", ctypes.c_int64 * 3), ("ys", ctypes.c_int64 * 3)]
 
 
+class SparkNormRopeHeads(ctypes.Structure):
+    """struct SparkNormRopeHeads of include/spark_b200.h."""
+    _fields_ = [("x", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("y", ctypes.c_void_p), ("weight", ctypes.c_void_p),
+                ("dweight", ctypes.c_void_p), ("weight_dtype", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("xs", ctypes.c_int64 * 3), ("dys", ctypes.c_int64 * 3), ("ys", ctypes.c_int64 * 3)]
+
+
+class SparkNormRope(ctypes.Structure):
+    """struct SparkNormRope of include/spark_b200.h."""
+    _fields_ = [("part", SparkNormRopeHeads * 2), ("dtype", ctypes.c_int64), ("batch", ctypes.c_int64),
+                ("tokens", ctypes.c_int64), ("head_dim", ctypes.c_int64), ("rot_dim", ctypes.c_int64),
+                ("interleaved", ctypes.c_int64), ("position_bytes", ctypes.c_int64), ("table_rows", ctypes.c_int64),
+                ("eps", ctypes.c_double), ("positions", ctypes.c_void_p), ("table", ctypes.c_void_p)]
+
+
 class SparkPagedCache(ctypes.Structure):
     """struct SparkPagedCache of include/spark_b200.h."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_stride", ctypes.c_int64 * 3),
@@ -146,6 +161,9 @@ _SIGNATURES = {
     "spark_ipc_open": (_i, [_p, _i64, ctypes.POINTER(ctypes.c_void_p)]),
     "spark_ipc_close": (_i, [_p, _i64]),
     "spark_rope": (_i, [_p, _p, _i, _i64, _i64, _i, _i, _i, _i, _p, _i, _p, _i64, _p, _p]),
+    "spark_qk_norm_rope": (_i, [_p, _p, _p]),
+    "spark_qk_norm_rope_backward_workspace_size": (_sz, [_i64]),
+    "spark_qk_norm_rope_backward": (_i, [_p, _p, _sz, _p, _p]),
     "spark_kv_append": (_i, [_p, _i64, _i64, _p, _p, _p, _p, _p, _i64, _p, _p, _p, _p]),
     "spark_tree_attention_workspace_size": (_sz, [_p]),
     "spark_tree_attention": (_i, [_p, _p, _sz, _p]),

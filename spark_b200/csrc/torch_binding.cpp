@@ -144,6 +144,216 @@ std::tuple<Tensor, OptTensor, int> apply_rope(const Tensor& q, const OptTensor& 
     return {out[0], k ? OptTensor(out[1]) : std::nullopt, rc};
 }
 
+// ------------------------------------------------------------------ norms of q and k with rope
+// What the parts' heads are read from: x with unit stride along the head, interleaved pairs on their bytes.
+Tensor pairs(const Tensor& x_, bool interleaved) {
+    const Tensor x = unit(x_);
+    bool fits = !interleaved || reinterpret_cast<uintptr_t>(x.data_ptr()) % (2 * x.element_size()) == 0;
+    for (int64_t i = 0; interleaved && i < x.dim() - 1; ++i) fits = fits && (x.size(i) <= 1 || x.stride(i) % 2 == 0);
+    return fits ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+// strides of [(batch,) tokens, heads, head_dim]; without a batch its stride is 0
+void head_strides(int64_t* to, const Tensor& x) {
+    const int first = x.dim() == 4 ? 0 : 1;
+    to[0] = 0;
+    for (int i = first; i < 3; ++i) to[i] = x.stride(i - first);
+}
+struct NormInputs {
+    Tensor q;
+    OptTensor k, q_weight, k_weight;
+    Tensor positions, table;
+    double eps;
+    bool interleaved;
+};
+// The arguments of both passes, checked; what had to be copied is held by `in`.
+SparkNormRope norm_args(NormInputs& in) {
+    const char* what = "qk_norm_rope";
+    need_cuda(what, "q", in.q);
+    on_device(what, "positions", in.positions, in.q);
+    on_device(what, "table", in.table, in.q);
+    const int64_t dim = in.q.dim();
+    TORCH_CHECK_VALUE((dim == 3 || dim == 4) && (!in.k || (in.k->dim() == dim && in.k->sizes().slice(0, dim - 2) == in.q.sizes().slice(0, dim - 2) &&
+                                                           in.k->size(-1) == in.q.size(-1))),
+                      "qk_norm_rope: q and k must be [(batch,) tokens, heads, head_dim] of the same tokens, got ", in.q.sizes(), " and ",
+                      in.k ? in.k->sizes() : at::IntArrayRef());
+    if (in.k) on_device(what, "k", *in.k, in.q);
+    TORCH_CHECK_TYPE(!in.k || in.k->scalar_type() == in.q.scalar_type(), "qk_norm_rope: q and k differ in type");
+    TORCH_CHECK_VALUE(in.k || !in.k_weight, "qk_norm_rope: k_weight without k");
+    TORCH_CHECK_VALUE(in.positions.sizes() == in.q.sizes().slice(0, dim - 2), "qk_norm_rope: positions are ", in.positions.sizes(),
+                      ", the tokens ", in.q.sizes().slice(0, dim - 2));
+    TORCH_CHECK_TYPE(in.positions.scalar_type() == at::kInt || in.positions.scalar_type() == at::kLong,
+                     "qk_norm_rope: positions must be int32 or int64, got ", in.positions.scalar_type());
+    TORCH_CHECK_TYPE(in.table.dim() == 2 && in.table.scalar_type() == at::kFloat && in.table.is_contiguous(),
+                     "qk_norm_rope: table must be a contiguous float32 [rows, rot_dim]");
+    SparkNormRope a{};
+    a.dtype = dtype_of(in.q, what, "q");
+    a.batch = dim == 4 ? in.q.size(0) : 1, a.tokens = in.q.size(dim - 3);
+    a.head_dim = in.q.size(-1), a.rot_dim = in.table.size(1), a.interleaved = in.interleaved;
+    for (int w = 0; w < 2; ++w) {
+        if (w && !in.k) continue;
+        Tensor& x = w ? *in.k : in.q;
+        OptTensor& weight = w ? in.k_weight : in.q_weight;
+        const char* name = w ? "k_weight" : "q_weight";
+        x = pairs(x, in.interleaved);
+        SparkNormRopeHeads& part = a.part[w];
+        part.x = x.data_ptr(), part.heads = x.size(-2);
+        head_strides(part.xs, x);
+        if (!weight) continue;
+        on_device(what, name, *weight, in.q);
+        TORCH_CHECK_VALUE(weight->dim() == 1 && weight->size(0) == a.head_dim, "qk_norm_rope: ", name, " must be [", a.head_dim, "], got ",
+                          weight->sizes());
+        weight = weight->contiguous();
+        part.weight = weight->data_ptr(), part.weight_dtype = dtype_of(*weight, what, name);
+    }
+    in.positions = in.positions.contiguous();
+    a.positions = in.positions.data_ptr(), a.position_bytes = (int64_t)in.positions.element_size();
+    a.table = in.table.const_data_ptr<float>(), a.table_rows = in.table.size(0);
+    a.eps = in.eps;
+    return a;
+}
+
+std::tuple<Tensor, OptTensor, int> qk_norm_rope(Tensor q, OptTensor k, OptTensor q_weight, OptTensor k_weight, Tensor positions,
+                                                const Tensor& table, double eps, bool interleaved, OptTensor q_out, OptTensor k_out,
+                                                uint64_t ws, uint64_t stream) {
+    need_cuda("qk_norm_rope", "q", q);
+    const at::DeviceGuard guard(q.device());
+    TORCH_CHECK_VALUE(k || !k_out, "qk_norm_rope: an output for k without k");
+    NormInputs in{q, k, q_weight, k_weight, positions, table, eps, interleaved};
+    SparkNormRope a = norm_args(in);
+    for (int w = 0; w < 2; ++w) {
+        if (w && !k) continue;
+        const Tensor& x = w ? *k : q;
+        OptTensor& y = w ? k_out : q_out;
+        if (!y) {
+            y = at::empty(x.sizes(), x.options());
+        } else {
+            TORCH_CHECK_VALUE(y->sizes() == x.sizes() && y->scalar_type() == x.scalar_type() && y->device() == x.device() &&
+                                  (y->stride(-1) == 1 || y->size(-1) == 1),
+                              "qk_norm_rope: out must have the shapes, type and device of q and k, with unit stride along the head");
+        }
+        a.part[w].y = y->data_ptr();
+        head_strides(a.part[w].ys, *y);
+    }
+    const int rc = spark_qk_norm_rope(&a, reinterpret_cast<int*>(ws), reinterpret_cast<void*>(stream));
+    return {*q_out, k ? k_out : std::nullopt, rc};
+}
+
+// The gradients of q, k and the weights (undefined where not wanted), from those of the outputs (undefined: none).
+std::vector<Tensor> norm_gradients(NormInputs in, const Tensor& dq, const Tensor& dk, std::array<bool, 4> want, uint64_t ws,
+                                   uint64_t stream) {
+    const at::DeviceGuard guard(in.q.device());
+    SparkNormRope a = norm_args(in);
+    std::vector<Tensor> out(4), held;
+    bool weights = false;
+    for (int w = 0; w < 2; ++w) {
+        SparkNormRopeHeads& part = a.part[w];
+        if (!(w ? dk : dq).defined() || !(want[w] || want[2 + w])) {
+            part = SparkNormRopeHeads{};
+            continue;
+        }
+        const Tensor& x = w ? *in.k : in.q;
+        const Tensor g = pairs((w ? dk : dq).to(x.scalar_type()), in.interleaved);
+        const Tensor dx = at::empty(x.sizes(), x.options());
+        part.dy = g.data_ptr(), part.y = dx.data_ptr();
+        head_strides(part.dys, g), head_strides(part.ys, dx);
+        held.push_back(g), held.push_back(dx);
+        if (want[w]) out[w] = dx;
+        if (!want[2 + w]) continue;
+        const Tensor& weight = w ? *in.k_weight : *in.q_weight;
+        out[2 + w] = at::empty(weight.sizes(), weight.options());
+        part.dweight = out[2 + w].data_ptr();
+        weights = true;
+    }
+    Tensor partial;
+    const size_t bytes = weights ? spark_qk_norm_rope_backward_workspace_size(a.head_dim) : 0;
+    if (weights) partial = at::empty({(int64_t)bytes}, in.q.options().dtype(at::kByte));
+    const int rc = spark_qk_norm_rope_backward(&a, weights ? partial.data_ptr() : nullptr, bytes, reinterpret_cast<int*>(ws),
+                                               reinterpret_cast<void*>(stream));
+    TORCH_CHECK(rc == SPARK_OK, "spark_qk_norm_rope_backward: ", spark_last_error());
+    return out;
+}
+
+// Gradients that a graph was asked for (create_graph): they have none of their own.
+struct NormGradients : torch::autograd::Function<NormGradients> {
+    static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& q_weight,
+                                       const OptTensor& k_weight, const OptTensor& dq, const OptTensor& dk, const NormInputs* in,
+                                       std::array<bool, 4> want, uint64_t ws, uint64_t stream, int64_t* where) {
+        NormInputs now = *in;
+        now.q = q, now.k = k, now.q_weight = q_weight, now.k_weight = k_weight;
+        const auto out = norm_gradients(now, dq ? *dq : Tensor(), dk ? *dk : Tensor(), want, ws, stream);
+        std::vector<Tensor> defined;
+        for (int i = 0; i < 4; ++i) {
+            where[i] = out[i].defined() ? (int64_t)defined.size() : -1;
+            if (out[i].defined()) defined.push_back(out[i]);
+        }
+        return defined;
+    }
+    static std::vector<Tensor> backward(torch::autograd::AutogradContext*, std::vector<Tensor>) {
+        TORCH_CHECK_NOT_IMPLEMENTED(false, "apply_qk_norm_rope: no gradients of gradients");
+        return {};
+    }
+};
+
+// The differentiable form.  A step backward runs on its forward's stream, with its error word (which stays for as long as
+// the process).
+struct NormRope : torch::autograd::Function<NormRope> {
+    static std::vector<Tensor> forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const OptTensor& k, const OptTensor& q_weight,
+                                       const OptTensor& k_weight, const Tensor& positions, const Tensor& table, double eps,
+                                       bool interleaved, uint64_t ws, uint64_t stream, int* status) {
+        auto [y, z, rc] = qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, std::nullopt, std::nullopt, ws, stream);
+        *status = rc;
+        ctx->save_for_backward({q, k ? *k : Tensor(), q_weight ? *q_weight : Tensor(), k_weight ? *k_weight : Tensor(), positions, table});
+        ctx->saved_data["eps"] = eps, ctx->saved_data["interleaved"] = interleaved;
+        ctx->saved_data["ws"] = (int64_t)ws, ctx->saved_data["stream"] = (int64_t)stream;
+        ctx->set_materialize_grads(false);
+        return z ? std::vector<Tensor>{y, *z} : std::vector<Tensor>{y};
+    }
+
+    static std::vector<Tensor> backward(torch::autograd::AutogradContext* ctx, std::vector<Tensor> grads) {
+        const auto saved = ctx->get_saved_variables();
+        auto optional = [](const Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; };
+        NormInputs in{saved[0], optional(saved[1]), optional(saved[2]), optional(saved[3]), saved[4], saved[5],
+                      ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool()};
+        const uint64_t ws = (uint64_t)ctx->saved_data["ws"].toInt(), stream = (uint64_t)ctx->saved_data["stream"].toInt();
+        // (only tensors that were given have an edge)
+        std::array<bool, 4> want{};
+        int64_t edge = 0;
+        for (int i : {0, 1, 2, 3})
+            if (saved[i].defined()) want[i] = ctx->needs_input_grad(edge++);
+        const Tensor dq = grads[0], dk = grads.size() > 1 ? grads[1] : Tensor();
+        std::vector<Tensor> out(11);
+        if (!dq.defined() && !dk.defined()) return out;
+        if (at::GradMode::is_enabled()) {
+            int64_t where[4];
+            const auto got = NormGradients::apply(in.q, in.k, in.q_weight, in.k_weight, optional(dq), optional(dk), &in, want, ws, stream,
+                                                  &where[0]);
+            for (int i = 0; i < 4; ++i)
+                if (where[i] >= 0) out[i] = got[where[i]];
+            return out;
+        }
+        const auto got = norm_gradients(in, dq, dk, want, ws, stream);
+        for (int i = 0; i < 4; ++i) out[i] = got[i];
+        return out;
+    }
+};
+
+std::tuple<Tensor, OptTensor, int> apply_qk_norm_rope(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
+                                                      const Tensor& positions, const Tensor& table, double eps, bool interleaved,
+                                                      uint64_t ws, uint64_t stream) {
+    bool grad = q.requires_grad();
+    TORCH_CHECK_NOT_IMPLEMENTED(!q._fw_grad(0).defined() && !table._fw_grad(0).defined(), "apply_qk_norm_rope: no forward-mode differentiation");
+    for (const OptTensor* t : {&k, &q_weight, &k_weight}) {
+        if (!*t) continue;
+        TORCH_CHECK_NOT_IMPLEMENTED(!(*t)->_fw_grad(0).defined(), "apply_qk_norm_rope: no forward-mode differentiation");
+        grad = grad || (*t)->requires_grad();
+    }
+    if (!grad || !at::GradMode::is_enabled())
+        return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, std::nullopt, std::nullopt, ws, stream);
+    int rc = SPARK_OK;
+    const auto out = NormRope::apply(q, k, q_weight, k_weight, positions, table, eps, interleaved, ws, stream, &rc);
+    return {out[0], k ? OptTensor(out[1]) : std::nullopt, rc};
+}
+
 // ------------------------------------------------------------------ the cache
 SparkPagedCache paged(const char* what, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lens,
                       const Tensor& tokens) {
@@ -330,6 +540,8 @@ PYBIND11_MODULE(_native, m) {
     });
     m.def("rope", &rope);
     m.def("apply_rope", &apply_rope);
+    m.def("qk_norm_rope", &qk_norm_rope);
+    m.def("apply_qk_norm_rope", &apply_qk_norm_rope);
     m.def("kv_append", &kv_append);
     m.def("tree_attention", &tree_attention);
     m.def("tree_verify", &tree_verify);

@@ -618,6 +618,23 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table
     return q_out, k_out
 
 
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 positions: torch.Tensor, table: torch.Tensor, eps: float = 1e-6, interleaved: bool = False, out=None):
+    """RMS norms of q and k for each head and their rotary positions in one launch
+    (spark_qk_norm_rope): (q', k'), q' = rope(q / sqrt(mean q^2 + eps) * q_weight).  q [...,
+    tokens, heads, head_dim], k, positions, table, interleaved and out as in rope;
+    head_dim even, up to 256.  The weights [head_dim] are float32, bfloat16 or float16,
+    None for ones.  All in fp32, rounded once.  rotary.apply_qk_norm_rope is the
+    differentiable form."""
+    _, ws, stream = _place("qk_norm_rope", q)
+    q_out, k_out = (None, None) if out is None else out
+    q_out, k_out, rc = _native().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, q_out, k_out,
+                                              ws, stream)
+    if rc:
+        _check("spark_qk_norm_rope", rc)
+    return q_out, k_out
+
+
 def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
               page_table: torch.Tensor, context_lens: torch.Tensor, index: torch.Tensor | None = None,
               counts: torch.Tensor | None = None) -> torch.Tensor:

@@ -1,5 +1,6 @@
 """Rotary positions: the table of cosines and sines, and the differentiable
-application of it to q and k (ops.rope).
+application of it to q and k, alone (ops.rope) or with their norms
+(ops.qk_norm_rope).
 """
 from __future__ import annotations
 
@@ -62,4 +63,17 @@ def apply_rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     y, z, rc = ops._native().apply_rope(q, k, positions, table, interleaved, ws, stream)
     if rc:
         ops._check("spark_rope", rc)
+    return y, z
+
+
+def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor | None,
+                       k_weight: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor, eps: float = 1e-6,
+                       interleaved: bool = False):
+    """Differentiable ops.qk_norm_rope: (q', k'), with gradients for q, k and the weights.
+    Those of positions and table are not computed; gradients of gradients and forward-mode
+    differentiation are refused."""
+    _, ws, stream = ops._place("qk_norm_rope", q)
+    y, z, rc = ops._native().apply_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, ws, stream)
+    if rc:
+        ops._check("spark_qk_norm_rope", rc)
     return y, z
