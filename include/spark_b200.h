@@ -533,6 +533,44 @@ typedef struct {
 } SparkTreeVerify;
 SPARK_API int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream);
 
+/* Sampling with temperature, top-k, top-p and min-p, and the same cut of logits for
+ * what samples later (spark_tree_verify).  logits [batch, nodes, vocab] of dtype.  In
+ * falling order of a row, the lower index first, and with e = exp((logit - largest) /
+ * temperature):
+ *     the first top_k entries stay (0 or below, or vocab and above: all);
+ *     of those the shortest prefix whose sum of e is at least top_p times theirs (1
+ *     and above, or a NaN: all; the first entry always stays);
+ *     of those the entries with e >= min_p (a NaN: all; above 1 as 1).
+ * token [batch] (nodes 1; or NULL) = argmax e / noise[b, v] over what stays, with
+ * exponential variates noise a sample; the lowest index wins a tie.  logprob [batch]
+ * (or NULL): log of the token's share of e.  Temperature 0: the token is the argmax (the
+ * lowest index of a tie), and it alone stays; others count as 1e-30 to 1e30.
+ * out [batch, nodes, vocab] of dtype (or NULL): the logits that stay, -inf for the
+ * others; it may be logits with equal strides.
+ * A row without a distribution (a NaN, +inf, no value above -inf, a temperature below
+ * 0 or NaN) gives token -1 and logprob NaN, and is copied to out.  Sums of e are in
+ * multiples of 2^-44 of the largest, so that results do not depend on any order.
+ * temperature, top_k, top_p, min_p [batch]: NULL for the one value of all.
+ * vocab <= 409,600, fewer than 2^24 rows. */
+typedef struct {
+    int64_t batch, nodes, vocab;
+    const void* logits;
+    int64_t dtype, logits_stride[2];
+    const float* temperature;
+    const int* top_k;
+    const float *top_p, *min_p;
+    double temperature_all;
+    int64_t top_k_all;
+    double top_p_all, min_p_all;
+    const float* noise;
+    int64_t noise_stride;
+    int64_t* token;
+    float* logprob;
+    void* out;
+    int64_t out_stride[2];
+} SparkSample;
+SPARK_API int spark_sample(const SparkSample* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

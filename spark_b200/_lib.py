@@ -98,6 +98,17 @@ class SparkTreeVerify(ctypes.Structure):
                 ("path", ctypes.c_void_p), ("accepted", ctypes.c_void_p), ("next", ctypes.c_void_p)]
 
 
+class SparkSample(ctypes.Structure):
+    """struct SparkSample of include/spark_b200.h."""
+    _fields_ = [("batch", ctypes.c_int64), ("nodes", ctypes.c_int64), ("vocab", ctypes.c_int64),
+                ("logits", ctypes.c_void_p), ("dtype", ctypes.c_int64), ("logits_stride", ctypes.c_int64 * 2),
+                ("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p), ("temperature_all", ctypes.c_double), ("top_k_all", ctypes.c_int64),
+                ("top_p_all", ctypes.c_double), ("min_p_all", ctypes.c_double), ("noise", ctypes.c_void_p),
+                ("noise_stride", ctypes.c_int64), ("token", ctypes.c_void_p), ("logprob", ctypes.c_void_p),
+                ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64 * 2)]
+
+
 class SparkError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 
@@ -168,6 +179,7 @@ _SIGNATURES = {
     "spark_tree_attention_workspace_size": (_sz, [_p]),
     "spark_tree_attention": (_i, [_p, _p, _sz, _p]),
     "spark_tree_verify": (_i, [_p, _p, _p]),
+    "spark_sample": (_i, [_p, _p]),
 }
 
 _lib = None

@@ -8,6 +8,7 @@
 #include <torch/extension.h>
 
 #include <limits>
+#include <variant>
 
 #include "../../include/spark_b200.h"
 
@@ -522,6 +523,78 @@ std::tuple<Tensor, Tensor, Tensor, int> tree_verify(const Tensor& logits, Tensor
     return {path, accepted, next, rc};
 }
 
+// ------------------------------------------------------------------ sampling
+// One setting of all sequences, or a tensor [batch].
+template <typename N>
+using Setting = std::variant<N, Tensor>;
+template <typename T, typename N>
+const T* setting(const char* what, const char* name, Setting<N>& s, N& all, at::ScalarType type, int64_t batch, const Tensor& like) {
+    if (const N* one = std::get_if<N>(&s)) {
+        all = *one;
+        return nullptr;
+    }
+    Tensor& t = std::get<Tensor>(s);
+    TORCH_CHECK_TYPE(t.scalar_type() == type && t.dim() == 1 && t.size(0) == batch && t.device() == like.device(), what, ": ", name,
+                     " must be a number or ", type, " [", batch, "] on ", like.device());
+    t = t.contiguous();
+    return t.const_data_ptr<T>();
+}
+SparkSample sample_args(const char* what, const Tensor& logits, int64_t batch, Setting<double>& temperature, Setting<int64_t>& top_k,
+                        Setting<double>& top_p, Setting<double>& min_p) {
+    SparkSample a{};
+    a.batch = batch, a.nodes = logits.dim() == 3 ? logits.size(1) : 1, a.vocab = logits.size(-1);
+    a.logits = logits.data_ptr(), a.dtype = dtype_of(logits, what, "logits");
+    a.logits_stride[0] = logits.stride(0), a.logits_stride[1] = logits.dim() == 3 ? logits.stride(1) : 0;
+    a.temperature = setting<float>(what, "temperature", temperature, a.temperature_all, at::kFloat, batch, logits);
+    a.top_k = setting<int>(what, "top_k", top_k, a.top_k_all, at::kInt, batch, logits);
+    a.top_p = setting<float>(what, "top_p", top_p, a.top_p_all, at::kFloat, batch, logits);
+    a.min_p = setting<float>(what, "min_p", min_p, a.min_p_all, at::kFloat, batch, logits);
+    TORCH_CHECK_VALUE(a.temperature || a.temperature_all >= 0, what, ": temperature must be 0 or above, got ", a.temperature_all);
+    TORCH_CHECK_VALUE(a.top_k || a.top_k_all >= 0, what, ": top_k must be 0 (all) or above, got ", a.top_k_all);
+    TORCH_CHECK_VALUE(a.top_p || (a.top_p_all >= 0 && a.top_p_all <= 1), what, ": top_p must be in 0..1, got ", a.top_p_all);
+    TORCH_CHECK_VALUE(a.min_p || (a.min_p_all >= 0 && a.min_p_all <= 1), what, ": min_p must be in 0..1, got ", a.min_p_all);
+    return a;
+}
+
+std::tuple<Tensor, OptTensor, int> sample(const Tensor& logits, Tensor noise, Setting<double> temperature, Setting<int64_t> top_k,
+                                          Setting<double> top_p, Setting<double> min_p, bool return_logprob, uint64_t stream) {
+    const char* what = "sample";
+    need_cuda(what, "logits", logits);
+    TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1, "sample: logits must be [batch, vocab], got ", logits.sizes());
+    on_device(what, "noise", noise, logits);
+    TORCH_CHECK_TYPE(noise.scalar_type() == at::kFloat, "sample: noise must be float32");
+    TORCH_CHECK_VALUE(noise.sizes() == logits.sizes(), "sample: noise is ", noise.sizes(), ", logits ", logits.sizes());
+    const at::DeviceGuard guard(logits.device());
+    const Tensor x = unit(logits);
+    noise = unit(noise);
+    SparkSample a = sample_args(what, x, x.size(0), temperature, top_k, top_p, min_p);
+    a.noise = noise.const_data_ptr<float>(), a.noise_stride = noise.stride(0);
+    Tensor token = at::empty({a.batch}, x.options().dtype(at::kLong));
+    OptTensor logprob;
+    if (return_logprob) logprob = at::empty({a.batch}, x.options().dtype(at::kFloat));
+    a.token = token.data_ptr<int64_t>(), a.logprob = logprob ? logprob->data_ptr<float>() : nullptr;
+    return {token, logprob, spark_sample(&a, reinterpret_cast<void*>(stream))};
+}
+
+std::tuple<Tensor, int> filter_logits(const Tensor& logits, Setting<double> temperature, Setting<int64_t> top_k, Setting<double> top_p,
+                                      Setting<double> min_p, OptTensor out, uint64_t stream) {
+    const char* what = "filter_logits";
+    need_cuda(what, "logits", logits);
+    TORCH_CHECK_VALUE((logits.dim() == 2 || logits.dim() == 3) && logits.size(-1) >= 1,
+                      "filter_logits: logits must be [batch, (nodes,) vocab], got ", logits.sizes());
+    const at::DeviceGuard guard(logits.device());
+    const Tensor x = unit(logits);
+    if (!out)
+        out = at::empty(x.sizes(), x.options());
+    else
+        TORCH_CHECK_VALUE(out->sizes() == x.sizes() && out->scalar_type() == x.scalar_type() && out->device() == x.device() &&
+                              (out->stride(-1) == 1 || out->size(-1) == 1),
+                          "filter_logits: out must have the logits' shape, type and device, with unit stride along the vocabulary");
+    SparkSample a = sample_args(what, x, x.size(0), temperature, top_k, top_p, min_p);
+    a.out = out->data_ptr(), a.out_stride[0] = out->stride(0), a.out_stride[1] = out->dim() == 3 ? out->stride(1) : 0;
+    return {*out, spark_sample(&a, reinterpret_cast<void*>(stream))};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -545,4 +618,6 @@ PYBIND11_MODULE(_native, m) {
     m.def("kv_append", &kv_append);
     m.def("tree_attention", &tree_attention);
     m.def("tree_verify", &tree_verify);
+    m.def("sample", &sample);
+    m.def("filter_logits", &filter_logits);
 }

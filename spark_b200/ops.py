@@ -600,6 +600,14 @@ def _place(what: str, t: torch.Tensor, nbytes: int = 256):
     return ws, ws.data_ptr(), stream
 
 
+def _stream_of(what: str, t: torch.Tensor) -> int:
+    """The current stream's handle on t's device."""
+    index = t.get_device()
+    if index < 0:
+        raise RuntimeError(f"spark_b200.{what}: expected a CUDA tensor, got one on {t.device}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def rope(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, table: torch.Tensor,
          interleaved: bool = False, inverse: bool = False, out=None):
     """Rotary positions of q [..., tokens, heads, head_dim] and k (the same with its
@@ -697,3 +705,34 @@ def tree_verify(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     if rc:
         _check("spark_tree_verify", rc)
     return path, accepted, last
+
+
+# ------------------------------------------------------------------ sampling
+def sample(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor | float = 1.0, top_k: torch.Tensor | int = 0,
+           top_p: torch.Tensor | float = 1.0, min_p: torch.Tensor | float = 0.0, return_logprob: bool = False):
+    """Tokens drawn from logits [batch, vocab] with the given random numbers (spark_sample):
+    int64 [batch]; with return_logprob also the log of the probability that each was drawn
+    with, fp32 [batch].  noise fp32 [batch, vocab]: exponential variates, as tree_verify's;
+    equal ones give equal tokens.  Of the distribution at the temperature stay the top_k
+    likeliest tokens (0: all), of those the fewest that have top_p of their mass, of those
+    the ones at least min_p as likely as the likeliest.  Temperature 0 takes the argmax.
+    Settings are numbers or tensors [batch], top_k int32, the others fp32.  A row without a
+    distribution (a NaN, +inf, nothing above -inf) gives -1 and NaN."""
+    stream = _stream_of("sample", logits)
+    token, logprob, rc = _native().sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob, stream)
+    if rc:
+        _check("spark_sample", rc)
+    return (token, logprob) if return_logprob else token
+
+
+def filter_logits(logits: torch.Tensor, temperature: torch.Tensor | float = 1.0, top_k: torch.Tensor | int = 0,
+                  top_p: torch.Tensor | float = 1.0, min_p: torch.Tensor | float = 0.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """logits [batch, (nodes,) vocab] with -inf in place of what sample's settings leave out:
+    tree_verify of these at the same temperature samples from the cut distribution.  out: a
+    tensor to write to, logits themselves for instance.  A row without a distribution is
+    copied."""
+    stream = _stream_of("filter_logits", logits)
+    out, rc = _native().filter_logits(logits, temperature, top_k, top_p, min_p, out, stream)
+    if rc:
+        _check("spark_sample", rc)
+    return out

@@ -73,3 +73,40 @@ def test_cpu_tensors_are_refused():
     q = torch.zeros(1, 2, 2, 64)
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.qk_norm_rope(q, None, None, None, torch.zeros(1, 2, dtype=torch.int64), torch.zeros(4, 64))
+
+
+def sampling(**kw):
+    a = _lib.SparkSample()
+    both = dict(batch=2, nodes=1, vocab=100, logits=4096, dtype=_lib.DTYPE_F32, logits_stride=(100, 0), temperature_all=1.0,
+                top_p_all=1.0, noise=8192, noise_stride=100, token=16384, out=None, out_stride=(100, 100))
+    both.update(kw)
+    for name, v in both.items():
+        setattr(a, name, (ctypes.c_int64 * 2)(*v) if isinstance(v, tuple) else v)
+    return a
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(batch=-1), INVALID), (dict(nodes=-1), INVALID), (dict(vocab=0), INVALID), (dict(dtype=3), INVALID),
+    (dict(vocab=409601), UNSUPPORTED), (dict(batch=1 << 24), UNSUPPORTED), (dict(batch=1 << 13, nodes=1 << 13), UNSUPPORTED),
+    (dict(logits=None), INVALID), (dict(token=None), INVALID), (dict(noise=None), INVALID), (dict(nodes=2), INVALID),
+    (dict(token=None, out=4096, logprob=256), INVALID), (dict(token=None, out=4096, out_stride=(101, 0)), INVALID),
+    (dict(token=None, out=8192, out_stride=(0, 0)), INVALID), (dict(token=None, nodes=3, out=8192, out_stride=(300, 0)), INVALID),
+])
+def test_sample_refuses(kw, status):
+    a = sampling(**kw)
+    assert _lib.lib().spark_sample(ctypes.byref(a), None) == status
+    assert "spark_sample" in _lib.last_error()
+
+
+def test_sample_of_nothing():
+    assert _lib.lib().spark_sample(None, None) == INVALID
+    for kw in (dict(batch=0), dict(nodes=0)):
+        assert _lib.lib().spark_sample(ctypes.byref(sampling(**kw)), None) == _lib.OK
+
+
+def test_sampling_refuses_cpu_tensors():
+    x = torch.zeros(2, 10)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.sample(x, torch.ones(2, 10))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.filter_logits(x)
