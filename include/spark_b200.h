@@ -571,6 +571,29 @@ typedef struct {
 } SparkSample;
 SPARK_API int spark_sample(const SparkSample* a, void* stream);
 
+/* ---------------------------------------------------------------- adapters
+ * Low-rank adapters of many requests beside a shared projection:
+ *     out[t] = y[t] + scale[i] B[i] (A[i] x[t]),   i = adapter[t / repeat];
+ * a negative i: no adapter, out[t] = y[t]; i >= adapters counts as none and sets error
+ * 12 in *err.  x [tokens, ic], a [adapters, rank, ic] and b [adapters, oc, rank] of
+ * dtype (bf16 or f16), a and b contiguous; y and out [tokens, oc] of y_dtype (dtype, or
+ * fp32), out may be y with equal strides; ldx, ldy, ldo: elements between rows; scale
+ * fp32 [adapters], or NULL: scale_all.  adapter int32 [tokens / repeat, rounded up].
+ * Products and sums are fp32, A x to 2^-17 of it (fp32 y: 2^-22), the result is rounded
+ * once.  rank <= 256.  workspace: spark_lora_workspace_size bytes on the current device,
+ * 16-byte aligned; what is in it does not matter. */
+typedef struct {
+    int64_t tokens, ic, oc, rank, adapters, repeat, dtype, y_dtype;
+    const void *x, *a, *b, *y;
+    void* out;
+    int64_t ldx, ldy, ldo;
+    const int* adapter;
+    const float* scale;
+    double scale_all;
+} SparkLora;
+SPARK_API size_t spark_lora_workspace_size(int64_t tokens, int64_t ic, int64_t rank);
+SPARK_API int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int* err, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -109,6 +109,16 @@ class SparkSample(ctypes.Structure):
                 ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64 * 2)]
 
 
+class SparkLora(ctypes.Structure):
+    """struct SparkLora of include/spark_b200.h."""
+    _fields_ = [("tokens", ctypes.c_int64), ("ic", ctypes.c_int64), ("oc", ctypes.c_int64), ("rank", ctypes.c_int64),
+                ("adapters", ctypes.c_int64), ("repeat", ctypes.c_int64), ("dtype", ctypes.c_int64),
+                ("y_dtype", ctypes.c_int64), ("x", ctypes.c_void_p), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("y", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("ldy", ctypes.c_int64),
+                ("ldo", ctypes.c_int64), ("adapter", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("scale_all", ctypes.c_double)]
+
+
 class SparkError(RuntimeError):
     """A C-ABI call returned a non-zero status."""
 
@@ -180,6 +190,8 @@ _SIGNATURES = {
     "spark_tree_attention": (_i, [_p, _p, _sz, _p]),
     "spark_tree_verify": (_i, [_p, _p, _p]),
     "spark_sample": (_i, [_p, _p]),
+    "spark_lora_workspace_size": (_sz, [_i64, _i64, _i64]),
+    "spark_lora": (_i, [_p, _p, _sz, _p, _p]),
 }
 
 _lib = None

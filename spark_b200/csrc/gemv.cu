@@ -1749,6 +1749,7 @@ int spark_workspace_check(void* workspace, void* stream) {
                          : flag == 8  ? "position outside the rotary table"
                          : flag == 9  ? "page, length or index outside the cache"
                          : flag == 11 ? "token id outside the vocabulary"
+                         : flag == 12 ? "adapter outside the pool"
                                       : "bounded wait expired");
     }
     return SPARK_OK;

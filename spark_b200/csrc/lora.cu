@@ -1,0 +1,476 @@
+// lora.cu -- low-rank adapters of many requests beside a shared projection:
+//     out[t] = y[t] + scale[a] B[a] (A[a] x[t]),   a = the adapter of token t.
+//
+// Two launches: h = A x (fp32, split over the input's columns), then B h on top of y.
+// Tokens are taken in tiles of consecutive rows; a tile's items are its distinct
+// adapters: mma.sync of all its rows with that adapter's weights, of which the rows
+// that have the adapter are kept.  Tokens of a request lie together, so that a
+// prompt's tile has one or two of them, and a decoding batch's sixteen cost no more
+// than reading each adapter once: no sorting, and what a row gets does not depend on
+// its neighbours.  The work is bound by memory (r <= 128 needs at most 2 r flop a byte of y), which
+// mma.sync can feed; tcgen05 would want 128 rows of one adapter.
+//
+// Fragments come straight from memory: the order of a contraction's terms is free, so
+// that a lane takes 8 consecutive values of a row (16 bytes) as its share of two
+// steps, and in the second product the columns of a lane are 8 consecutive ones of y.
+//
+// h is in fp32 and meets B in 16 bits: it is split into two (y in 16 bits) or three
+// (fp32) terms of B's type, which together are good to 2^-17 or 2^-23 of it; for f16,
+// whose exponents are few, a row is brought to 2^14 by a power of 2 first.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace spark {
+namespace tc {
+int sm_count_cached(int dev);
+}
+
+namespace lora {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+constexpr int kMaxRank = 256;
+constexpr int kColumns = 32;   // of y, by one warp at a time
+
+struct Params {
+    const void *x, *a, *b, *y;
+    void* out;
+    const int* adapter;
+    const float* scale;
+    float scale_all;
+    int64_t tokens, ic, oc, ldx, ldy, ldo;
+    int64_t adapters;
+    int rank, repeat;            // tokens of an entry of `adapter`
+    int splits, slots;           // of the input's columns; of a tile's items, worked on side by side
+    int rank_blocks, columns;    // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y
+    int a_time;                  // second product: column blocks of a CTA
+    int wide_y;                  // rows of y and out on 16 bytes
+    float* h;                    // [splits, tokens, rank]
+    int* err;
+};
+
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__nv_bfloat16> {
+    static __device__ __forceinline__ void run(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+};
+template <>
+struct Mma<__half> {
+    static __device__ __forceinline__ void run(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+};
+
+// Values k..k + 7 of a row of n, zeros behind its end; VEC: rows on 16 bytes, n a multiple of 8.
+template <typename T, bool VEC>
+__device__ __forceinline__ uint4 load8(const T* row, int64_t k, int64_t n) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if constexpr (VEC) {
+        if (k < n) v = *reinterpret_cast<const uint4*>(row + k);
+    } else {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t lo = k + 2 * j < n ? p[k + 2 * j] : 0, hi = k + 2 * j + 1 < n ? p[k + 2 * j + 1] : 0;
+            w[j] = lo | hi << 16;
+        }
+        v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return v;
+}
+
+// A tile's adapters: ids[row] (-1: none, or no such token), and the distinct ones in order of their first rows.
+template <int ROWS>
+struct Tile {
+    int ids[ROWS];
+    int distinct[ROWS];
+    int count;
+    unsigned first[2];
+};
+template <int ROWS>
+__device__ __forceinline__ void load_tile(Tile<ROWS>& s, const Params& p, int64_t t0, bool report) {
+    const int i = threadIdx.x;
+    if (i < ROWS) {
+        int id = t0 + i < p.tokens ? p.adapter[(t0 + i) / p.repeat] : -1;
+        if (id >= p.adapters) {
+            if (report) report_device_error(p.err, 12);
+            id = -1;
+        }
+        s.ids[i] = id < 0 ? -1 : id;
+    }
+    if (i == 0) s.count = 0;
+    __syncthreads();
+    if (i < (ROWS + 31) / 32 * 32) {
+        bool lead = i < ROWS && t0 + i < p.tokens;
+        for (int j = 0; j < i && lead; ++j) lead = s.ids[j] != s.ids[i];
+        const unsigned leads = __ballot_sync(0xffffffffu, lead);
+        if ((i & 31) == 0) s.first[i >> 5] = leads;
+    }
+    __syncthreads();
+    if (i < ROWS) {
+        const unsigned mine = s.first[i >> 5];
+        const int before = (i >= 32 ? __popc(s.first[0]) : 0) + __popc(mine & ((1u << (i & 31)) - 1));
+        if (mine >> (i & 31) & 1) s.distinct[before] = s.ids[i];
+        if (i == ROWS - 1) s.count = before + (int)(mine >> (i & 31) & 1);
+    }
+    __syncthreads();
+}
+
+// h[split, t, :] = A[a] x[t] over the split's columns.  The warps of a CTA take chunks of 32 columns in turn.
+template <typename T, int MT, int NT, bool VEC>
+__global__ void __launch_bounds__(kThreads) k_lora_down(const __grid_constant__ Params p) {
+    constexpr int ROWS = 16 * MT, RANKS = 8 * NT;
+    __shared__ Tile<ROWS> s;
+    extern __shared__ float part[];   // [kWarps, ROWS, RANKS]
+    // the next launch reads what was ready before this one: it may begin when this one may
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int64_t t0 = (int64_t)blockIdx.x * ROWS;
+    const int split = blockIdx.y, r0 = (int)(blockIdx.z % p.rank_blocks) * RANKS, slot = blockIdx.z / p.rank_blocks;
+    load_tile(s, p, t0, split == 0 && r0 == 0 && slot == 0);
+    const T* x = reinterpret_cast<const T*>(p.x);
+    for (int d = slot; d < s.count; d += p.slots) {
+        const int id = s.distinct[d];
+        if (id < 0) continue;
+        const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)id * p.rank * p.ic;
+        float acc[MT][NT][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
+#pragma unroll 2
+        for (int64_t k = ((int64_t)split * kWarps + warp) * 32 + 8 * t; k - 8 * t < p.ic; k += (int64_t)p.splits * kWarps * 32) {
+            uint4 u[MT][2], w[NT];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int64_t row = t0 + m * 16 + e * 8 + g;
+                    u[m][e] = load8<T, VEC>(x + (row < p.tokens ? row : 0) * p.ldx, k, row < p.tokens ? p.ic : 0);
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = r0 + n * 8 + g;
+                w[n] = load8<T, VEC>(a + (int64_t)(r < p.rank ? r : 0) * p.ic, k, r < p.rank ? p.ic : 0);
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    Mma<T>::run(acc[m][n], u[m][0].x, u[m][1].x, u[m][0].y, u[m][1].y, w[n].x, w[n].y);
+                    Mma<T>::run(acc[m][n], u[m][0].z, u[m][1].z, u[m][0].w, u[m][1].w, w[n].z, w[n].w);
+                }
+        }
+        float* mine = part + warp * ROWS * RANKS;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    *reinterpret_cast<float2*>(mine + (m * 16 + e * 8 + g) * RANKS + n * 8 + 2 * t) =
+                        make_float2(acc[m][n][2 * e], acc[m][n][2 * e + 1]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < ROWS * RANKS; i += kThreads) {
+            const int row = i / RANKS, r = r0 + i % RANKS;
+            if (s.ids[row] != id || r >= p.rank) continue;
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) sum += part[w * ROWS * RANKS + i];
+            p.h[((int64_t)split * p.tokens + t0 + row) * p.rank + r] = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// 8 values of a row of y as floats, and back.
+template <typename Y>
+struct Eight;
+template <>
+struct Eight<float> {
+    float v[8];
+    __device__ __forceinline__ void load(const float* p) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    __device__ __forceinline__ float get(int j) const { return v[j]; }
+    static __device__ __forceinline__ void store(float* p, const float* f) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    }
+};
+template <typename Y>
+struct Eight {
+    union {
+        uint4 raw;
+        Y v[8];
+    };
+    __device__ __forceinline__ Eight() {}
+    __device__ __forceinline__ void load(const Y* p) { raw = *reinterpret_cast<const uint4*>(p); }
+    __device__ __forceinline__ float get(int j) const { return (float)v[j]; }
+    static __device__ __forceinline__ void store(Y* p, const float* f) {
+        Eight e;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e.v[j] = Mma<Y>::round(f[j]);
+        *reinterpret_cast<uint4*>(p) = e.raw;
+    }
+};
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+template <typename Y>
+__device__ __forceinline__ void put(Y* p, float v) { *p = Mma<Y>::round(v); }
+
+// out[t, :] = y[t, :] + scale B[a] h[t].  A warp has kColumns columns at a time.
+template <typename T, typename Y, int MT, bool VEC>
+__global__ void __launch_bounds__(kThreads) k_lora_up(const __grid_constant__ Params p) {
+    constexpr int ROWS = 16 * MT, TERMS = sizeof(Y) == 4 ? 3 : 2;
+    __shared__ Tile<ROWS> s;
+    __shared__ float row_scale[ROWS];
+    extern __shared__ __align__(16) unsigned char raw[];
+    T* terms = reinterpret_cast<T*>(raw);   // [TERMS, ROWS, width]
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int chunks = (p.rank + 31) / 32, width = chunks * 32 + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int per_tile = (p.columns + p.a_time - 1) / p.a_time;
+    const int64_t t0 = (int64_t)(blockIdx.x / per_tile) * ROWS;
+    const int c0 = (int)(blockIdx.x % per_tile) * p.a_time, c1 = min(c0 + p.a_time, p.columns), slot = blockIdx.y;
+    // (what was ready before the first product may be read before it ends)
+    load_tile(s, p, t0, false);
+    if (slot >= s.count) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (int row = warp; row < ROWS; row += kWarps) {
+        const bool is = s.ids[row] >= 0;
+        float v[kMaxRank / 32], most = 0.f;
+#pragma unroll
+        for (int c = 0; c < kMaxRank / 32; ++c) {
+            const int r = c * 32 + lane;
+            v[c] = 0.f;
+            if (c < chunks && is && r < p.rank)
+                for (int k = 0; k < p.splits; ++k) v[c] += p.h[((int64_t)k * p.tokens + t0 + row) * p.rank + r];
+            most = fmaxf(most, fabsf(v[c]));
+        }
+        float up = 1.f, down = 1.f;
+        if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            // (zeros and infinities stay what they are)
+            if (most > 0.f && most < INFINITY) {
+                const int e = min(max(14 - ilogbf(most), -100), 100);
+                up = ldexpf(1.f, e), down = ldexpf(1.f, -e);
+            }
+        }
+        const float scale = is ? (p.scale ? p.scale[s.ids[row]] : p.scale_all) : 0.f;
+        if (lane == 0) row_scale[row] = down * scale;
+#pragma unroll
+        for (int c = 0; c < kMaxRank / 32; ++c) {
+            if (c >= chunks) break;
+            float rest = v[c] * up;
+#pragma unroll
+            for (int k = 0; k < TERMS; ++k) {
+                const T q = Mma<T>::round(rest);
+                terms[(k * ROWS + row) * width + c * 32 + lane] = q;
+                const float f = (float)q;
+                rest = fabsf(f) < INFINITY ? rest - f : 0.f;
+            }
+        }
+    }
+    __syncthreads();
+    const Y* y = reinterpret_cast<const Y*>(p.y);
+    Y* out = reinterpret_cast<Y*>(p.out);
+    for (int d = slot; d < s.count; d += p.slots) {
+        const int id = s.distinct[d];
+        if (id < 0 && p.y == p.out) continue;
+        const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.oc * p.rank;
+        for (int c = c0; c < c1; ++c) {
+            const int64_t o0 = ((int64_t)c * kWarps + warp) * kColumns;
+            if (o0 >= p.oc) break;
+            const int64_t mine = o0 + 8 * t;                 // this lane's columns
+            const bool whole = p.wide_y && mine + 8 <= p.oc;
+            Eight<Y> old[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = m * 16 + e * 8 + g;
+                    if (whole && t0 + row < p.tokens && s.ids[row] == id) old[m][e].load(y + (t0 + row) * p.ldy + mine);
+                }
+            float acc[MT][4][4];
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
+            if (id >= 0) {
+                for (int k = 0; k < chunks; ++k) {
+                    uint4 w[4];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        // column n of a step is one of lane g / 2's eight
+                        const int64_t o = o0 + 8 * (g >> 1) + 2 * n + (g & 1);
+                        w[n] = load8<T, VEC>(b + (o < p.oc ? o : 0) * p.rank, k * 32 + 8 * t, o < p.oc ? p.rank : 0);
+                    }
+#pragma unroll
+                    for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            const T* at = terms + (q * ROWS + m * 16 + g) * width + k * 32 + 8 * t;
+                            const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 8 * width);
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) {
+                                Mma<T>::run(acc[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
+                                Mma<T>::run(acc[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = m * 16 + e * 8 + g;
+                    if (t0 + row >= p.tokens || s.ids[row] != id) continue;
+                    const float f = row_scale[row];
+                    if (whole) {
+                        float v[8];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) v[j] = fmaf(acc[m][j >> 1][2 * e + (j & 1)], f, old[m][e].get(j));
+                        Eight<Y>::store(out + (t0 + row) * p.ldo + mine, v);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (mine + j < p.oc)
+                                put(out + (t0 + row) * p.ldo + mine + j,
+                                    fmaf(acc[m][j >> 1][2 * e + (j & 1)], f, (float)y[(t0 + row) * p.ldy + mine + j]));
+                    }
+                }
+        }
+    }
+}
+
+constexpr int kFew = 64;        // tokens up to which tiles have 16 rows
+// Splits of the input's columns: as many as give two CTAs an SM work, each at least two chunks of 32 columns a warp.
+int splits_of(int64_t tokens, int64_t ic, int64_t rank, int sms) {
+    const int64_t rows = tokens <= kFew ? 16 : 32, tiles = (tokens + rows - 1) / rows * ((rank + 63) / 64);
+    const int64_t most = std::max<int64_t>(1, ic / (2 * 32 * kWarps));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 16), 2 * sms / tiles));
+}
+
+template <typename F>
+cudaError_t start(F kernel, dim3 grid, size_t smem, cudaStream_t s, const Params& p) {
+    if (smem > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_overlapped(kernel, grid, dim3(kThreads), smem, s, p);
+}
+template <typename T, int MT, int NT>
+cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
+    const size_t smem = (size_t)kWarps * 16 * MT * 8 * NT * sizeof(float);
+    return vec ? start(k_lora_down<T, MT, NT, true>, grid, smem, s, p) : start(k_lora_down<T, MT, NT, false>, grid, smem, s, p);
+}
+template <typename T, int MT>
+cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
+    if (p.rank <= 16) return down<T, MT, 2>(p, vec, grid, s);
+    if (p.rank <= 32) return down<T, MT, 4>(p, vec, grid, s);
+    return down<T, MT, 8>(p, vec, grid, s);
+}
+template <typename T, typename Y, int MT>
+cudaError_t up(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
+    const size_t smem = (size_t)(sizeof(Y) == 4 ? 3 : 2) * 16 * MT * ((p.rank + 31) / 32 * 32 + 8) * sizeof(T);
+    return vec ? start(k_lora_up<T, Y, MT, true>, grid, smem, s, p) : start(k_lora_up<T, Y, MT, false>, grid, smem, s, p);
+}
+template <typename T>
+cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t s) {
+    const bool few = p.tokens <= kFew;
+    {
+        const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
+        p.rank_blocks = (p.rank + 63) / 64;
+        p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2 * sms / (tiles * p.splits * p.rank_blocks)));
+        p.slots = (int)std::min<int64_t>(p.slots, p.tokens);
+        const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)(p.slots * p.rank_blocks));
+        const cudaError_t e = few ? down<T, 1>(p, vec_down, grid, s) : down<T, 2>(p, vec_down, grid, s);
+        if (e != cudaSuccess) return e;
+    }
+    const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
+    p.columns = (int)((p.oc + kWarps * kColumns - 1) / (kWarps * kColumns));
+    p.slots = (int)std::min<int64_t>(std::min<int64_t>(rows, p.tokens), std::max<int64_t>(1, 4 * sms / (tiles * p.columns)));
+    p.a_time = (int)std::min<int64_t>(p.columns, std::max<int64_t>(1, tiles * p.columns / (8 * sms)));
+    const dim3 grid((unsigned)(tiles * ((p.columns + p.a_time - 1) / p.a_time)), (unsigned)p.slots);
+    if (few) return wide ? up<T, float, 1>(p, vec_up, grid, s) : up<T, T, 1>(p, vec_up, grid, s);
+    return wide ? up<T, float, 2>(p, vec_up, grid, s) : up<T, T, 2>(p, vec_up, grid, s);
+}
+
+}  // namespace lora
+}  // namespace spark
+
+extern "C" {
+
+size_t spark_lora_workspace_size(int64_t tokens, int64_t ic, int64_t rank) {
+    using namespace spark;
+    int dev = 0;
+    if (tokens <= 0 || ic <= 0 || rank <= 0 || cudaGetDevice(&dev) != cudaSuccess) return 0;
+    return (size_t)lora::splits_of(tokens, ic, rank, tc::sm_count_cached(dev)) * tokens * rank * sizeof(float);
+}
+
+int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
+    using namespace spark;
+    using namespace spark::lora;
+    const char* name = "spark_lora";
+    SPARK_REQUIRE(a, SPARK_ERR_INVALID, "%s: null pointer", name);
+    SPARK_REQUIRE(a->dtype == SPARK_DTYPE_BF16 || a->dtype == SPARK_DTYPE_F16, SPARK_ERR_INVALID, "%s: bad dtype %d", name, (int)a->dtype);
+    SPARK_REQUIRE(a->y_dtype == a->dtype || a->y_dtype == SPARK_DTYPE_F32, SPARK_ERR_INVALID, "%s: y is of dtype or fp32, got %d", name,
+                  (int)a->y_dtype);
+    SPARK_REQUIRE(a->tokens >= 0 && a->ic >= 1 && a->oc >= 0 && a->adapters >= 0 && a->repeat >= 1, SPARK_ERR_INVALID, "%s: bad size", name);
+    SPARK_REQUIRE(a->rank >= 1 && a->rank <= kMaxRank, SPARK_ERR_UNSUPPORTED, "%s: rank %lld is not in 1..%d", name, (long long)a->rank, kMaxRank);
+    SPARK_REQUIRE(a->tokens < (1 << 26) && a->ic < (1 << 26) && a->oc < (1 << 26) && a->adapters < (1ll << 31) && a->repeat < (1ll << 31),
+                  SPARK_ERR_UNSUPPORTED, "%s: size", name);
+    if (a->tokens == 0 || a->oc == 0) return SPARK_OK;
+    SPARK_REQUIRE(a->x && a->y && a->out && a->adapter && ((a->a && a->b) || a->adapters == 0), SPARK_ERR_INVALID, "%s: null pointer", name);
+    SPARK_REQUIRE(a->tokens == 1 || a->ldo >= a->oc, SPARK_ERR_INVALID, "%s: output rows in one place", name);
+    SPARK_REQUIRE(a->out != a->y || a->ldo == a->ldy || a->tokens == 1, SPARK_ERR_INVALID, "%s: in place needs equal strides", name);
+    SPARK_REQUIRE(a->out != a->x, SPARK_ERR_INVALID, "%s: the output is the input", name);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return set_error((int)e, "%s: %s", name, cudaGetErrorString(e));
+    const int sms = tc::sm_count_cached(dev);
+    Params p{};
+    p.splits = splits_of(a->tokens, a->ic, a->rank, sms);
+    const size_t need = (size_t)p.splits * a->tokens * a->rank * sizeof(float);
+    SPARK_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), SPARK_ERR_WORKSPACE,
+                  "%s: workspace of %zu bytes on 16, %zu needed", name, workspace_bytes, need);
+    p.x = a->x, p.a = a->a, p.b = a->b, p.y = a->y, p.out = a->out, p.adapter = a->adapter, p.scale = a->scale;
+    p.scale_all = (float)a->scale_all;
+    p.tokens = a->tokens, p.ic = a->ic, p.oc = a->oc, p.adapters = a->adapters;
+    // (a stride that no second row uses says nothing)
+    p.ldx = a->tokens == 1 ? 0 : a->ldx, p.ldy = a->tokens == 1 ? 0 : a->ldy, p.ldo = a->tokens == 1 ? 0 : a->ldo;
+    p.rank = (int)a->rank, p.repeat = (int)a->repeat;
+    p.h = reinterpret_cast<float*>(workspace), p.err = err;
+    const int items = a->y_dtype == SPARK_DTYPE_F32 ? 4 : 8;   // of y, in 16 bytes
+    p.wide_y = aligned(p.y, 16) && aligned(p.out, 16) && p.ldy % items == 0 && p.ldo % items == 0;
+    const bool vec_down = p.ic % 8 == 0 && p.ldx % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16);
+    const bool vec_up = p.rank % 8 == 0 && aligned(p.b, 16), wide = a->y_dtype == SPARK_DTYPE_F32;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    e = a->dtype == SPARK_DTYPE_BF16 ? run<__nv_bfloat16>(p, vec_down, vec_up, wide, sms, st)
+                                     : run<__half>(p, vec_down, vec_up, wide, sms, st);
+    if (e != cudaSuccess) return set_error((int)e, "%s: launch failed: %s", name, cudaGetErrorString(e));
+    return check_launch(name);
+}
+
+}  // extern "C"

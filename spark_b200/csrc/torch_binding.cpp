@@ -595,6 +595,58 @@ std::tuple<Tensor, int> filter_logits(const Tensor& logits, Setting<double> temp
     return {*out, spark_sample(&a, reinterpret_cast<void*>(stream))};
 }
 
+// ------------------------------------------------------------------ adapters
+// [rows, n] of a tensor [..., n], its rows at one distance.
+Tensor rows_of(const Tensor& t) { return unit(t.reshape({-1, t.size(-1)})); }
+
+std::tuple<Tensor, int> lora_add(const Tensor& y_, const Tensor& x_, const Tensor& a, const Tensor& b, Tensor adapter, Setting<double> scale,
+                                 OptTensor out, uint64_t ws, uint64_t stream) {
+    const char* what = "lora_add";
+    need_cuda(what, "y", y_);
+    for (const auto& [name, t] : {std::pair<const char*, const Tensor*>{"x", &x_}, {"a", &a}, {"b", &b}, {"adapter", &adapter}})
+        on_device(what, name, *t, y_);
+    TORCH_CHECK_VALUE(y_.dim() >= 1 && x_.dim() == y_.dim() && x_.sizes().slice(0, x_.dim() - 1) == y_.sizes().slice(0, y_.dim() - 1),
+                      "lora_add: x must be [..., in_features] and y [..., out_features] of the same tokens, got ", x_.sizes(), " and ",
+                      y_.sizes());
+    const int64_t ic = x_.size(-1), oc = y_.size(-1);
+    TORCH_CHECK_VALUE(a.dim() == 3 && b.dim() == 3 && a.size(0) == b.size(0) && a.size(1) == b.size(2) && a.size(2) == ic && b.size(1) == oc,
+                      "lora_add: a must be [adapters, rank, ", ic, "] and b [adapters, ", oc, ", rank], got ", a.sizes(), " and ", b.sizes());
+    TORCH_CHECK_VALUE(ic >= 1 && a.size(1) >= 1, "lora_add: no features or a rank of 0");
+    const auto type = x_.scalar_type();
+    TORCH_CHECK_TYPE((type == at::kBFloat16 || type == at::kHalf) && a.scalar_type() == type && b.scalar_type() == type &&
+                         (y_.scalar_type() == type || y_.scalar_type() == at::kFloat),
+                     "lora_add: x, a and b must be bfloat16 or float16 alike, y of that type or float32, got ", type, ", ", a.scalar_type(), ", ",
+                     b.scalar_type(), ", ", y_.scalar_type());
+    TORCH_CHECK_TYPE(adapter.scalar_type() == at::kInt, "lora_add: adapter must be int32, got ", adapter.scalar_type());
+    SparkLora p{};
+    p.tokens = 1;
+    for (int64_t i = 0; i < x_.dim() - 1; ++i) p.tokens *= x_.size(i);
+    TORCH_CHECK_VALUE(p.tokens == 0 || (adapter.numel() >= 1 && p.tokens % adapter.numel() == 0), "lora_add: ", adapter.numel(),
+                      " adapter numbers for ", p.tokens, " tokens: their number must divide the tokens'");
+    const at::DeviceGuard guard(y_.device());
+    if (!out) {
+        out = at::empty(y_.sizes(), y_.options());
+    } else {
+        TORCH_CHECK_VALUE(out->sizes() == y_.sizes() && out->scalar_type() == y_.scalar_type() && out->device() == y_.device(),
+                          "lora_add: out must have y's shape, type and device");
+    }
+    if (p.tokens == 0 || oc == 0) return {*out, SPARK_OK};
+    // (a copy of out would take the result with it)
+    const Tensor to = out->view({-1, oc}), x = rows_of(x_), y = out->is_same(y_) ? to : rows_of(y_);
+    TORCH_CHECK_VALUE(to.stride(1) == 1 || oc == 1, "lora_add: out must have unit stride along the features");
+    const Tensor ac = a.contiguous(), bc = b.contiguous();
+    adapter = adapter.contiguous();
+    p.ic = ic, p.oc = oc, p.rank = a.size(1), p.adapters = a.size(0), p.repeat = p.tokens / adapter.numel();
+    p.dtype = dtype_of(x, what, "x"), p.y_dtype = dtype_of(y, what, "y");
+    p.x = x.data_ptr(), p.a = ac.data_ptr(), p.b = bc.data_ptr(), p.y = y.data_ptr(), p.out = to.data_ptr();
+    p.ldx = x.stride(0), p.ldy = y.stride(0), p.ldo = to.stride(0);
+    p.adapter = adapter.const_data_ptr<int>();
+    p.scale = setting<float>(what, "scale", scale, p.scale_all, at::kFloat, p.adapters, y_);
+    const size_t bytes = spark_lora_workspace_size(p.tokens, ic, p.rank);
+    const Tensor h = at::empty({(int64_t)bytes}, y_.options().dtype(at::kByte));
+    return {*out, spark_lora(&p, h.data_ptr(), bytes, reinterpret_cast<int*>(ws), reinterpret_cast<void*>(stream))};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_native, m) {
@@ -620,4 +672,5 @@ PYBIND11_MODULE(_native, m) {
     m.def("tree_verify", &tree_verify);
     m.def("sample", &sample);
     m.def("filter_logits", &filter_logits);
+    m.def("lora_add", &lora_add);
 }

@@ -736,3 +736,22 @@ def filter_logits(logits: torch.Tensor, temperature: torch.Tensor | float = 1.0,
     if rc:
         _check("spark_sample", rc)
     return out
+
+
+# ------------------------------------------------------------------ adapters
+def lora_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, adapter: torch.Tensor,
+             scale: torch.Tensor | float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Low-rank adapters of many requests on top of a shared projection's y (spark_lora):
+    y[t] + scale[i] * b[i] @ (a[i] @ x[t]), i = the token's adapter, a negative one for none.
+    x [..., in_features], y [..., out_features], a pool of a [adapters, rank, in_features] and
+    b [adapters, out_features, rank], bfloat16 or float16 alike, y also float32; smaller ranks
+    padded with zeros, 256 at most.  adapter int32: one for each token, or for each run of as many
+    tokens (of [batch, tokens, ...] one for each sequence).  scale: a number or fp32
+    [adapters].  out: a tensor to write to, y itself for instance; otherwise a new one.
+    An adapter outside the pool counts as none and is reported by
+    check_device_errors().  Not differentiable."""
+    _, ws, stream = _place("lora_add", y)
+    out, rc = _native().lora_add(y, x, a, b, adapter, scale, out, ws, stream)
+    if rc:
+        _check("spark_lora", rc)
+    return out

@@ -110,3 +110,36 @@ def test_sampling_refuses_cpu_tensors():
         ops.sample(x, torch.ones(2, 10))
     with pytest.raises(RuntimeError, match="CUDA"):
         ops.filter_logits(x)
+
+
+def adapters(**kw):
+    a = _lib.SparkLora()
+    both = dict(tokens=4, ic=64, oc=32, rank=8, adapters=2, repeat=1, dtype=_lib.DTYPE_BF16, y_dtype=_lib.DTYPE_BF16, x=4096, a=8192,
+                b=16384, y=32768, out=65536, ldx=64, ldy=32, ldo=32, adapter=256, scale=512)
+    both.update(kw)
+    for name, v in both.items():
+        setattr(a, name, v)
+    return a
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=_lib.DTYPE_F32), INVALID), (dict(dtype=7), INVALID), (dict(y_dtype=_lib.DTYPE_F16), INVALID), (dict(tokens=-1), INVALID),
+    (dict(ic=0), INVALID), (dict(oc=-1), INVALID), (dict(adapters=-1), INVALID), (dict(repeat=0), INVALID), (dict(rank=0), UNSUPPORTED),
+    (dict(rank=257), UNSUPPORTED), (dict(tokens=1 << 26), UNSUPPORTED), (dict(x=None), INVALID), (dict(a=None), INVALID),
+    (dict(b=None), INVALID), (dict(y=None), INVALID), (dict(out=None), INVALID), (dict(adapter=None), INVALID), (dict(ldo=31), INVALID),
+    (dict(ldo=0), INVALID), (dict(out=32768, ldo=40), INVALID), (dict(out=4096), INVALID),
+])
+def test_lora_refuses(kw, status):
+    assert _lib.lib().spark_lora(ctypes.byref(adapters(**kw)), P(256), 1 << 30, None, None) == status
+    assert "spark_lora" in _lib.last_error()
+
+
+def test_lora_of_nothing():
+    L = _lib.lib()
+    assert L.spark_lora(None, None, 0, None, None) == INVALID
+    for kw in (dict(tokens=0), dict(oc=0)):
+        assert L.spark_lora(ctypes.byref(adapters(**kw)), None, 0, None, None) == _lib.OK
+    assert L.spark_lora_workspace_size(0, 64, 8) == 0 and L.spark_lora_workspace_size(4, 64, 0) == 0
+    with pytest.raises(RuntimeError, match="CUDA"):
+        x = torch.zeros(2, 8, dtype=torch.bfloat16)
+        ops.lora_add(x, x, torch.zeros(1, 1, 8), torch.zeros(1, 8, 1), torch.zeros(2, dtype=torch.int32))

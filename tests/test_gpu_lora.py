@@ -1,0 +1,196 @@
+"""Low-rank adapters of many requests (ops.lora_add) against 64 bits.
+
+Tolerances, e = 2^-24, u the unit roundoff of y's type.  h = A x is a sum of n products in
+fp32 on the tensor cores, which may cut instead of round: 2 e a term of a chain of n / (8 splits) + 8 + 16
+at most, bounded here by 2 e (n / 8 + 24) of hh = sum |A| |x|.  Its two terms are good to 2^-17 of h (bf16; f16
+better), three to 2^-23; B h adds r terms (2 or 3 times) in a chain: 2 e (3 r + 4) of |B| hh; the product with
+scale and y: e (|y| + 2 |scale B h|), then u |out|.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_tree_decode import BF, FP, HF, U, gen, randn
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+
+
+def ops():
+    from spark_b200 import ops as _ops
+    return _ops
+
+
+def check(y, x, a, b, adapter, scale, out):
+    assert out.shape == y.shape and out.dtype == y.dtype
+    ic, oc, r = x.shape[-1], y.shape[-1], a.shape[1]
+    X, Y, O = x.reshape(-1, ic).double(), y.reshape(-1, oc).double(), out.reshape(-1, oc).double()
+    ids = adapter.flatten().long().repeat_interleave(X.shape[0] // max(adapter.numel(), 1))
+    want, room = Y.clone(), E * Y.abs()
+    for i in ids.unique().tolist():
+        if i < 0 or i >= a.shape[0]:
+            continue
+        rows = (ids == i).nonzero()[:, 0]
+        A, B = a[i].double(), b[i].double()
+        s = abs(float(scale[i] if isinstance(scale, torch.Tensor) else scale))
+        sign = 1 if float(scale[i] if isinstance(scale, torch.Tensor) else scale) >= 0 else -1
+        h, hh = X[rows] @ A.T, X[rows].abs() @ A.T.abs()
+        term = 2.0 ** -23 if y.dtype == FP else 2.0 ** -17
+        off = (h.abs() * term + 2 * E * (ic / 8 + 24) * hh) @ B.T.abs() + 2 * E * (3 * r + 4) * (hh @ B.T.abs())
+        delta = h @ B.T * s
+        want[rows] += sign * delta
+        room[rows] += s * off + 2 * E * delta.abs()
+    bad = (O - want).abs() - (U[y.dtype] * want.abs() + room) * 1.001
+    assert float(bad.max()) <= (2.0 ** -25 if y.dtype == HF else 0), float(bad.max())
+
+
+def make(seed, tokens, ic, oc, r, pool, dtype, y_dtype=None, ids=None):
+    g = gen(seed)
+    x, y = randn(g, tokens, ic, dtype=dtype), randn(g, tokens, oc, dtype=y_dtype or dtype)
+    a, b = (randn(g, pool, r, ic) * ic ** -0.5).to(dtype), randn(g, pool, oc, r, dtype=dtype)
+    scale = torch.rand(pool, generator=g, device="cuda") * 2 - 0.5
+    if ids is None:
+        ids = torch.randint(-1, pool, (tokens,), generator=g, device="cuda")
+    return y, x, a, b, ids.to(torch.int32), scale
+
+
+SIZES = [  # tokens, ic, oc, r, pool
+    (1, 1, 1, 1, 1), (1, 2560, 4096, 16, 8), (3, 64, 40, 8, 2), (16, 512, 256, 16, 40), (17, 1000, 136, 4, 3), (48, 2560, 1000, 16, 32),
+    (64, 96, 264, 33, 70), (65, 200, 72, 64, 5), (100, 1001, 1030, 12, 5), (130, 4096, 96, 100, 7), (300, 264, 1024, 32, 9),
+    (33, 72, 513, 256, 2), (200, 520, 264, 128, 20), (1000, 512, 520, 24, 3), (7, 31, 9, 7, 4), (2, 8192, 64, 65, 2),
+]
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [(BF, BF), (HF, HF), (BF, FP), (HF, FP)])
+@pytest.mark.parametrize("size", SIZES)
+def test_mixed_adapters(size, dtype, y_dtype):
+    y, x, a, b, ids, scale = make(sum(size), *size, dtype, y_dtype)
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    check(y, x, a, b, ids, scale, out)
+    assert torch.equal(out, ops().lora_add(y, x, a, b, ids, scale=scale))
+    copy = y.clone()
+    assert ops().lora_add(copy, x, a, b, ids, scale=scale, out=copy).data_ptr() == copy.data_ptr()
+    assert torch.equal(copy, out)
+    ops().check_device_errors()
+
+
+@pytest.mark.parametrize("tokens,per", [(1, 1), (64, 4), (96, 16), (4096, 512), (777, 7), (2048, 2048)])
+def test_runs_of_tokens(tokens, per):
+    """One adapter for each run; a row's result does not depend on its neighbours."""
+    y, x, a, b, _, scale = make(tokens, tokens, 264, 272, 16, 5, BF)
+    ids = (torch.arange(tokens // per, device="cuda") * 3 % 6 - 1).to(torch.int32)
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    check(y, x, a, b, ids, scale, out)
+    if tokens % per == 0 and tokens > 1:
+        y3, x3 = y.view(-1, per, 272), x.view(-1, per, 264)
+        assert torch.equal(ops().lora_add(y3, x3, a, b, ids, scale=scale).view(-1, 272), out)
+    mixed = ids.repeat_interleave(per)
+    mixed[1::2] = (mixed[1::2] + 3) % 5
+    other = ops().lora_add(y, x, a, b, mixed, scale=scale)
+    same = mixed == ids.repeat_interleave(per)
+    assert torch.equal(other[same], out[same])
+
+
+def test_no_adapter_and_every_token_its_own():
+    y, x, a, b, _, scale = make(1, 70, 128, 136, 8, 70, HF)
+    none = torch.full((70,), -1, dtype=torch.int32, device="cuda")
+    assert torch.equal(ops().lora_add(y, x, a, b, none, scale=scale), y)
+    assert torch.equal(ops().lora_add(y, x, a, b, none * 7, scale=scale, out=y.clone()), y)
+    own = torch.arange(70, dtype=torch.int32, device="cuda").flip(0)
+    check(y, x, a, b, own, 0.75, ops().lora_add(y, x, a, b, own, scale=0.75))
+    empty = ops().lora_add(y[:0], x[:0], a, b, own[:0])
+    assert empty.shape == (0, 136)
+    assert torch.equal(ops().lora_add(y, x, a[:0], b[:0], none, scale=scale[:0]), y)
+    one = ops().lora_add(y[0], x[0], a, b, own[0])
+    check(y[:1], x[:1], a, b, own[:1], 1.0, one[None])
+
+
+def test_adapter_outside_the_pool():
+    from spark_b200._lib import SparkError
+    y, x, a, b, ids, scale = make(2, 40, 64, 64, 8, 3, BF)
+    ids[5], ids[33] = 3, 2 ** 31 - 1
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    with pytest.raises(SparkError, match="adapter"):
+        ops().check_device_errors()
+    check(y, x, a, b, ids, scale, out)
+    assert torch.equal(out[[5, 33]], y[[5, 33]])
+
+
+@pytest.mark.parametrize("y_dtype", [BF, FP])
+def test_layouts(y_dtype):
+    """Parts of a merged projection's output in place, rows at odd addresses, expanded inputs, weights in another order."""
+    g = gen(3)
+    for lead in (0, 8, 3):
+        y, x, a, b, ids, scale = make(4, 50, 128, 96, 16, 4, BF, y_dtype)
+        wide = randn(g, 50, 96 + 24, dtype=y_dtype)
+        before, part = wide.clone(), wide[:, lead:lead + 96]
+        ops().lora_add(part, x, a, b, ids, scale=scale, out=part)
+        check(before[:, lead:lead + 96], x, a, b, ids, scale, part)
+        assert torch.equal(wide[:, :lead], before[:, :lead]) and torch.equal(wide[:, lead + 96:], before[:, lead + 96:])
+        xx = randn(g, 50, 150, dtype=BF)[:, lead:lead + 128]
+        check(y, xx, a, b, ids, scale, ops().lora_add(y, xx, a, b, ids, scale=scale))
+    check(y[:1].expand(50, 96), x[:1].expand(50, 128), a, b, ids, scale, ops().lora_add(y[:1].expand(50, 96), x[:1].expand(50, 128), a, b, ids, scale=scale))
+    at, bt = a.transpose(1, 2).contiguous().transpose(1, 2), b.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(ops().lora_add(y, x, at, bt, ids, scale=scale), ops().lora_add(y, x, a, b, ids, scale=scale))
+    odd = torch.empty(a.numel() + 1, dtype=BF, device="cuda")[1:].view_as(a).copy_(a)
+    check(y, x, odd, b, ids, scale, ops().lora_add(y, x, odd, b, ids, scale=scale))
+    cols = x.t().contiguous().t()
+    assert torch.equal(ops().lora_add(y, cols, a, b, ids, scale=scale), ops().lora_add(y, x, a, b, ids, scale=scale))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_scales_of_activations(dtype):
+    """A x beyond the range of f16, and tiny: rows of very different sizes."""
+    y, x, a, b, ids, _ = make(5, 40, 256, 128, 16, 3, dtype, FP)
+    size = torch.logspace(-6, 4 if dtype == HF else 8, 40, device="cuda")[:, None]
+    x, a = (x.float() * size).to(dtype), (a.float() * 100).to(dtype)
+    check(y, x, a, b, ids, 1e-3, ops().lora_add(y, x, a, b, ids, scale=1e-3))
+    x = x.clone()
+    x[7, 3], x[9, 0] = float("inf"), float("nan")
+    ids[7] = ids[9] = 1
+    ids[8] = 1
+    out = ops().lora_add(y, x, a, b, ids)
+    assert not torch.isfinite(out[7]).any() and torch.isnan(out[9]).all() and torch.isfinite(out[8]).all()
+
+
+def test_refusals():
+    from spark_b200._lib import SparkError
+    y, x, a, b, ids, scale = make(6, 12, 64, 32, 8, 3, BF)
+    f = ops().lora_add
+    for args, kw, error in [
+        ((y.cpu(), x, a, b, ids), {}, RuntimeError), ((y, x.cpu(), a, b, ids), {}, RuntimeError), ((y, x, a, b, ids.cpu()), {}, RuntimeError),
+        ((y, x.half(), a, b, ids), {}, TypeError), ((y.half(), x, a, b, ids), {}, TypeError), ((y, x.float(), a.float(), b.float(), ids), {}, TypeError),
+        ((y, x, a, b, ids.long()), {}, TypeError), ((y, x, a, b, ids[:5]), {}, ValueError), ((y, x, a, b, ids[:0]), {}, ValueError),
+        ((y[:5], x, a, b, ids), {}, ValueError), ((y, x, a[:, :, :32], b, ids), {}, ValueError), ((y, x, a[:2], b, ids), {}, ValueError),
+        ((y, x, a[:, :4], b, ids), {}, ValueError), ((y, x, a[0], b, ids), {}, ValueError), ((y, x, a[:, :0], b[:, :, :0], ids), {}, ValueError),
+        ((y, x, a, b, ids), dict(scale=scale.double()), TypeError), ((y, x, a, b, ids), dict(scale=scale[:2]), TypeError),
+        ((y, x, a, b, ids), dict(out=y.float()), ValueError), ((y, x, a, b, ids), dict(out=y[:5]), ValueError),
+        ((y, x, a, b, ids), dict(out=torch.empty(32, 12, dtype=BF, device="cuda").t()), ValueError),
+        ((y, x, a, b, ids), dict(out=y[:1].expand(12, 32)), SparkError),
+    ]:
+        with pytest.raises(error):
+            f(*args, **kw)
+    big = torch.zeros(1, 257, 64, dtype=BF, device="cuda"), torch.zeros(1, 32, 257, dtype=BF, device="cuda")
+    with pytest.raises(SparkError, match="256"):
+        f(y, x, *big, ids)
+
+
+def test_captured_and_on_another_stream():
+    y, x, a, b, ids, scale = make(7, 48, 512, 384, 16, 8, BF)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops().lora_add(y, x, a, b, ids, scale=scale)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(other, ops().lora_add(y, x, a, b, ids, scale=scale))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    for seed in (1, 2):
+        x.copy_(randn(gen(seed), 48, 512))
+        ids.copy_(torch.randint(-1, 8, (48,), generator=gen(seed), device="cuda"))
+        scale.mul_(0.7)
+        graph.replay()
+        check(y, x, a, b, ids, scale, out)
