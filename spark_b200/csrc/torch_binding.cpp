@@ -524,9 +524,9 @@ std::tuple<Tensor, Tensor, Tensor, int> tree_verify(const Tensor& logits, Tensor
 }
 
 // ------------------------------------------------------------------ sampling
-// One setting of all sequences, or a tensor [batch].
+// One setting of all sequences, or a tensor [batch] (which comes first: one of a single value converts to a number, on the host).
 template <typename N>
-using Setting = std::variant<N, Tensor>;
+using Setting = std::variant<Tensor, N>;
 template <typename T, typename N>
 const T* setting(const char* what, const char* name, Setting<N>& s, N& all, at::ScalarType type, int64_t batch, const Tensor& like) {
     if (const N* one = std::get_if<N>(&s)) {

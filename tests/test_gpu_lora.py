@@ -194,3 +194,13 @@ def test_captured_and_on_another_stream():
         scale.mul_(0.7)
         graph.replay()
         check(y, x, a, b, ids, scale, out)
+
+
+def test_a_pool_of_one_captured():
+    y, x, a, b, ids, scale = make(8, 5, 64, 48, 8, 1, BF)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    scale.fill_(1.75)
+    graph.replay()
+    check(y, x, a, b, ids, scale, out)

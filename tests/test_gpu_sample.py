@@ -289,3 +289,20 @@ def test_captured_and_on_another_stream():
         graph.replay()
         check_filter(x, cut, s)
         check_sample(x, noise, token, logprob, s)
+
+
+def test_settings_of_one_sequence_stay_on_the_device():
+    """Tensors of one value each, in a graph: replays follow them."""
+    g = gen(9)
+    x, noise = randn(g, 1, 5000) * 3, noise_of(g, 1, 5000)
+    s = {"temperature": torch.tensor([0.7], device="cuda"), "top_k": torch.tensor([20], dtype=torch.int32, device="cuda"),
+         "top_p": torch.tensor([0.9], device="cuda"), "min_p": torch.tensor([0.01], device="cuda")}
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cut = ops().filter_logits(x, **s)
+        token, logprob = ops().sample(x, noise, **s, return_logprob=True)
+    for k in (20, 3, 1000):
+        s["top_k"].fill_(k)
+        graph.replay()
+        check_filter(x, cut, s)
+        check_sample(x, noise, token, logprob, s)
