@@ -9,9 +9,10 @@
 //
 // No sort.  Entries are told apart by their distance from M in bins (512 over 32 T,
 // below which e is under 2^-45).
-//  1. A histogram of the largest entries of 16-byte vectors gives a bin with at least k
-//     entries at or before it (without a count: about a thirtieth of the row); what
-//     lies there is listed, usually all that can stay.
+//  1. A thread has the largest entries of four groups of its 16-byte vectors.  A
+//     histogram of those gives a bin with at least k entries at or before it (without a
+//     count: about a thirtieth of the row); what lies there is listed, usually all that
+//     can stay.
 //  2. A list of at most kPairs entries is compared with itself.  A longer one is
 //     divided by a histogram with counts and sums of e, whose scan gives the bin that
 //     the cut is in, and that bin again, by the integers in the order of the floats,
@@ -23,12 +24,14 @@
 // of atomics: e in 64 bits, added as multiples of 2^-44 in integers (409,600 entries of
 // at most 1 fit 64 bits).
 //
-// One thread-block cluster of 8 CTAs (fewer where there are many rows) per row, each
-// CTA a slice of the vocabulary that it keeps in shared memory, so that a row is read
-// once; noise is read where an entry stays.  Bins and lists are exchanged through
-// distributed shared memory; all CTAs take the same decisions.
+// A row is kept in shared memory, so that it is read once; noise is read where an entry
+// stays.  A CTA takes a row that fits (up to 200 KB).  A longer one is cut into the
+// slices of a thread-block cluster, which exchange bins and lists through distributed
+// shared memory and all take the same decisions; a step costs a cluster barrier
+// then (2000 cycles or more each, against some hundred).
 #include <float.h>
 #include <math.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
@@ -41,8 +44,8 @@ int sm_count_cached(int dev);
 
 namespace sm {
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxThreads = 1024;       // of a CTA: 1024, or 512 where two CTAs fit an SM
+constexpr int kWarps = kMaxThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 512;              // the last one: all that is further away
 constexpr int kPairs = 256;             // entries that are compared with one another
@@ -50,8 +53,7 @@ constexpr int kList = 4096;             // entries that a CTA lists
 constexpr int kRowBytes = 200 * 1024;   // of a CTA's slice
 constexpr int kMaxVocab = kMaxCluster * kRowBytes / 4;
 constexpr int kSmemSm = 228 * 1024;     // shared memory of an SM
-constexpr int kBatch = 4;               // vectors of a thread on the way together
-static_assert(kBins == kThreads, "a thread has a bin");
+constexpr int kGroups = 4;              // of a thread's vectors, which are on the way together
 
 struct Params {
     SparkSample a;
@@ -95,29 +97,35 @@ struct Shared {
     };
     unsigned long long mass[kBins];                           // of the row
     unsigned counts[kBins];
-    uint16_t list[kList];
+    uint16_t list[kList];                                     // indices in the slice; those from 65536 on from the end back
     Note note[2][kMaxCluster];
-    Note red[kWarps];
+    Note red[2][kWarps];
     Rest rest[kMaxCluster];
     double red_sum[kWarps], red_slope[kWarps];
     unsigned long long scan_mass[kWarps];
     unsigned scan_count[kWarps];
-    unsigned listed, pairs, base;
+    unsigned listed[2], pairs, base;
+    double per_temp, reach;                                   // 1 / T; how far below M min_p reaches
+    float bins;
     Found found;
     Cut cut;
 };
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-}
 __device__ __forceinline__ uint32_t cluster_size() {
     uint32_t n;
     asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
     return n;
+}
+__device__ __forceinline__ void cluster_sync() {
+    if (cluster_size() == 1) {
+        __syncthreads();
+        return;
+    }
+    __syncwarp();
+    cluster_arrive();
+    cluster_wait();
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -136,6 +144,12 @@ __device__ __forceinline__ void to_l2(const void* p, int64_t n) {
     const uintptr_t a = (reinterpret_cast<uintptr_t>(p) + 15) & ~uintptr_t(15);
     const int64_t m = (reinterpret_cast<intptr_t>(p) + n - (intptr_t)a) & ~int64_t(15);
     if (m > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(a), "r"((uint32_t)m) : "memory");
+}
+
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Integers that rise where the floats fall (no NaN; both zeros are one value), and back.
@@ -182,30 +196,36 @@ __device__ __forceinline__ float Vec<__nv_bfloat16>::largest() const {
     return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
 }
 
-// How notes are joined: the largest a with its lowest index i (-1: none), b summed.
 __device__ __forceinline__ Note none() { return Note{-INFINITY, 0.f, -1, 0}; }
 __device__ __forceinline__ void add(Note& v, float a, int i) {
     if (v.i < 0 || a > v.a || (a == v.a && i < v.i)) v.a = a, v.i = i;
 }
+// Integers in the order of the floats (no NaN), and back.
+__device__ __forceinline__ int ordered(float x) {
+    const int i = __float_as_int(x);
+    return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+// How notes are joined: the largest a with its lowest index i (-1: none), b summed.
 __device__ __forceinline__ Note join_warp(Note v) {
+    const float top = unordered(__reduce_max_sync(0xffffffffu, ordered(v.i < 0 ? -INFINITY : v.a)));
+    const unsigned first = __reduce_min_sync(0xffffffffu, v.i >= 0 && v.a == top ? (unsigned)v.i : 0xffffffffu);
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const float a = __shfl_xor_sync(0xffffffffu, v.a, o);
-        const int i = __shfl_xor_sync(0xffffffffu, v.i, o);
-        v.b += __shfl_xor_sync(0xffffffffu, v.b, o);
-        if (i >= 0) add(v, a, i);
-    }
-    return v;
+    for (int o = 1; o < 32; o <<= 1) v.b += __shfl_xor_sync(0xffffffffu, v.b, o);
+    return Note{top, v.b, (int)first, 0};
 }
 // Of all threads of the cluster, for every thread, in a fixed order.
+template <int TH>
 __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (int)cluster_size();
     v = join_warp(v);
-    if (lane == 0) s.red[warp] = v;
+    Note* red = s.red[step & 1];
+    if (lane == 0) red[warp] = v;
     __syncthreads();
     Note* slot = s.note[step++ & 1];
+    if (n == 1) return join_warp(lane < TH / 32 ? red[lane] : none());
     if (warp == 0) {
-        v = join_warp(lane < kWarps ? s.red[lane] : none());
+        v = join_warp(lane < TH / 32 ? red[lane] : none());
         if (lane < n) *of_rank(&slot[cluster_rank()], lane) = v;
     }
     cluster_sync();
@@ -226,19 +246,24 @@ __device__ __forceinline__ unsigned long long mass_of(const Row& r, float x) {
 }
 
 // A CTA's part of a row, in shared memory, and the entries of it that are looked at: those listed, or all.
-template <typename L>
+template <typename L, int TH>
 struct Slice {
     const L* v;
     int v0, n;               // index of the first, how many
     const uint16_t* list;    // NULL: all
-    int listed;
+    int listed, low;         // of them below 65536
+
+    __device__ __forceinline__ int at(int i) const { return i < low ? list[i] : 65536 + list[kList - 1 - (i - low)]; }
 
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         if (list) {
-            for (int i = threadIdx.x; i < listed; i += kThreads) f((float)v[list[i]], v0 + list[i]);
+            for (int i = threadIdx.x; i < listed; i += TH) {
+                const int j = at(i);
+                f((float)v[j], v0 + j);
+            }
         } else {
-            for (int i = threadIdx.x; i < n; i += kThreads) f((float)v[i], v0 + i);
+            for (int i = threadIdx.x; i < n; i += TH) f((float)v[i], v0 + i);
         }
     }
 };
@@ -269,10 +294,28 @@ __device__ __forceinline__ void count_one(Shared& s, int bin, unsigned long long
     if (high) atomicAdd(&s.high[bin], high);
 }
 
+// Adds the bins of the CTAs into s.counts and, if asked, s.mass: each CTA its share, which it gives to all.
+__device__ __forceinline__ void add_bins(Shared& s, bool masses) {
+    cluster_sync();
+    const int n = (int)cluster_size(), share = kBins / n, b = (int)cluster_rank() * share + threadIdx.x;
+    if (threadIdx.x < share) {
+        unsigned count = 0;
+        unsigned long long mass = 0;
+        for (int k = 0; k < n; ++k) {
+            count += *of_rank(&s.count[b], k);
+            if (masses) mass += ((unsigned long long)*of_rank(&s.high[b], k) << 32) + *of_rank(&s.low[b], k);
+        }
+        for (int k = 0; k < n; ++k) {
+            *of_rank(&s.counts[b], k) = count;
+            if (masses) *of_rank(&s.mass[b], k) = mass;
+        }
+    }
+    cluster_sync();
+}
 // Fills s.counts and s.mass with the row's bins: mode 0: all entries but those of the last bin; else those of the range.
-template <typename L>
-__device__ __noinline__ void histogram(Shared& s, const Slice<L>& x, const Row& r, const Range& g, bool masses) {
-    s.count[threadIdx.x] = s.low[threadIdx.x] = s.high[threadIdx.x] = 0;
+template <typename L, int TH>
+__device__ __noinline__ void histogram(Shared& s, const Slice<L, TH>& x, const Row& r, const Range& g, bool masses) {
+    for (int i = threadIdx.x; i < kBins; i += TH) s.count[i] = s.low[i] = s.high[i] = 0;
     __syncthreads();
     x.each([&](float v, int index) {
         int bin;
@@ -285,77 +328,89 @@ __device__ __noinline__ void histogram(Shared& s, const Slice<L>& x, const Row& 
         }
         count_one(s, bin, masses ? mass_of(r, v) : 0ull);
     });
-    cluster_sync();
-    // each CTA adds its share of the bins and gives the sums to all
-    const int n = (int)cluster_size(), share = kBins / n, b = (int)cluster_rank() * share + threadIdx.x;
-    if (threadIdx.x < share) {
-        unsigned count = 0;
-        unsigned long long mass = 0;
-        for (int k = 0; k < n; ++k) {
-            count += *of_rank(&s.count[b], k);
-            mass += ((unsigned long long)*of_rank(&s.high[b], k) << 32) + *of_rank(&s.low[b], k);
-        }
-        for (int k = 0; k < n; ++k) *of_rank(&s.counts[b], k) = count, *of_rank(&s.mass[b], k) = mass;
+    add_bins(s, true);
+}
+
+// The bin in which the count reaches k, from s.counts; bin -1 where none does.
+__device__ __forceinline__ void find_count(Shared& s, unsigned k) {
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
+    const unsigned own = t < kBins ? s.counts[t] : 0;
+    unsigned c = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned pc = __shfl_up_sync(0xffffffffu, c, o);
+        if (lane >= o) c += pc;
     }
-    cluster_sync();
+    if (lane == 31) s.scan_count[warp] = c;
+    if (t == 0) s.found = Found{-1, 0, 0, 0};
+    __syncthreads();
+    const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s.scan_count[lane] : 0) + c - own;
+    if (before < k && k <= before + own) s.found = Found{t, (int)before, (int)own, 0};
+    __syncthreads();
 }
 
 // The bin in which a cut lies: where the count reaches `k` (k > 0), else where the mass reaches `target`; bin -1 where none does.
 // Behind count0 entries of mass0.  Returns the mass of all bins.
 __device__ __noinline__ unsigned long long find(Shared& s, unsigned k, double target, unsigned count0, unsigned long long mass0) {
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const unsigned own = s.counts[t];
-    const unsigned long long own_mass = s.mass[t];
-    unsigned c = own;
-    unsigned long long m = own_mass;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const unsigned pc = __shfl_up_sync(0xffffffffu, c, o);
-        const unsigned long long pm = __shfl_up_sync(0xffffffffu, m, o);
-        if (lane >= o) c += pc, m += pm;
-    }
-    if (lane == 31) s.scan_count[warp] = c, s.scan_mass[warp] = m;
+    unsigned own = 0, c = 0;
+    unsigned long long own_mass = 0, m = 0;
     if (t == 0) s.found = Found{-1, 0, 0, 0};
-    __syncthreads();
-    unsigned before = count0;
-    unsigned long long mass = mass0, all = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s.scan_count[w], mass += s.scan_mass[w];
-        all += s.scan_mass[w];
+    if (t < kBins) {
+        c = own = s.counts[t], m = own_mass = s.mass[t];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned pc = __shfl_up_sync(0xffffffffu, c, o);
+            const unsigned long long pm = __shfl_up_sync(0xffffffffu, m, o);
+            if (lane >= o) c += pc, m += pm;
+        }
+        if (lane == 31) s.scan_count[warp] = c, s.scan_mass[warp] = m;
     }
-    before += c - own, mass += m - own_mass;
-    const bool here = k ? before < k && k <= before + own
-                        : (double)mass < target && target <= (double)(mass + own_mass) && own_mass > 0;
-    if (here) s.found = Found{t, (int)before, (int)own, mass};
     __syncthreads();
+    if (t < kBins) {
+        unsigned before = count0;
+        unsigned long long mass = mass0;
+        for (int w = 0; w < warp; ++w) before += s.scan_count[w], mass += s.scan_mass[w];
+        before += c - own, mass += m - own_mass;
+        const bool here = k ? before < k && k <= before + own
+                            : own_mass > 0 && (double)mass < target && target <= (double)(mass + own_mass);
+        if (here) s.found = Found{t, (int)before, (int)own, mass};
+    }
+    __syncthreads();
+    unsigned long long all = 0;
+#pragma unroll
+    for (int w = 0; w < kBins / 32; ++w) all += s.scan_mass[w];
     return all;
 }
 
 // Rank 0 compares its s.pairs entries with one another and tells all CTAs the cut: by count (k > 0), by mass (target > 0), or by
 // top_p of the mass of the first k or, without k, of all and `rest`.  Behind count0 entries of mass0.  Where the cut is behind
 // them all its mass is 0.
+template <int TH>
 __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, double target, double top_p, double rest, unsigned count0,
                                    unsigned long long mass0) {
     if (cluster_rank() == 0) {
         const int n = min((int)s.pairs, kPairs), t = threadIdx.x;
         if (t < n) s.pair_mass[t] = mass_of(r, value_of(s.pair[t].key));
         if (t == 0) s.cut.mass = 0;
-        // as many threads an entry as there are
-        int a_time = 32;
-        while (a_time > kThreads / kPairs && a_time * n > kThreads) a_time >>= 1;
-        const int e = t / a_time, sub = t & (a_time - 1);
+        // a few threads an entry, so that each compares about 16
+        int part = TH / kPairs == 4 ? 2 : 1;
+        while (part < 4 && (n >> part) > 16 && (n << (part + 1)) <= TH) ++part;
+        const int e = t >> part, sub = t & ((1 << part) - 1);
         __syncthreads();
         Entry mine{0xffffffffu, 0x7fffffff};
         unsigned before = 0;
         unsigned long long sum = 0, mass = 0;
         if (e < n) {
             mine = s.pair[e], mass = s.pair_mass[e];
-            for (int j = sub; j < n; j += a_time) {
+            const uint64_t place = (uint64_t)mine.key << 32 | (uint32_t)mine.index;
+            for (int j = sub; j < n; j += 1 << part) {
                 const Entry other = s.pair[j];
-                if (other.key < mine.key || (other.key == mine.key && other.index < mine.index)) ++before, sum += s.pair_mass[j];
+                const bool first = ((uint64_t)other.key << 32 | (uint32_t)other.index) < place;
+                before += first, sum += first ? s.pair_mass[j] : 0;
             }
         }
-        for (int o = 1; o < a_time; o <<= 1) {
+        for (int o = 1; o < 1 << part; o <<= 1) {
             before += __shfl_xor_sync(0xffffffffu, before, o);
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
@@ -379,8 +434,8 @@ __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, double t
 
 // The cut by count (k > 0: behind the first k entries) or by mass (behind the shortest prefix with `target`) of x's entries, from
 // their bins by distance, which are in s if `fresh`.  s.cut afterwards.  Returns whether the bins are still there.
-template <typename L>
-__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L>& x, const Row& r, bool fresh, unsigned k, double target, int entries,
+template <typename L, int TH>
+__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, bool fresh, unsigned k, double target, int entries,
                                     int vocab, bool masses) {
     Range g{0, 0, 0, 0, 0, 0};
     if (!fresh) histogram(s, x, r, g, masses);
@@ -389,7 +444,7 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L>& x, con
     if (f.bin < 0) {
         // behind all bins: the last one has the rest (and no mass)
         f = Found{kBins - 1, 0, 0, 0};
-        for (int w = 0; w < kWarps; ++w) f.count += (int)s.scan_count[w], f.mass += s.scan_mass[w];
+        for (int w = 0; w < kBins / 32; ++w) f.count += (int)s.scan_count[w], f.mass += s.scan_mass[w];
         f.in = entries - f.count;
     }
     g.bin = f.bin;
@@ -402,7 +457,7 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L>& x, con
             x.each([&](float v, int index) {
                 if (bin_of(r, v) == g.bin) add(hi, v, index), add(lo, -v, index);
             });
-            const float top = join_all(s, step, hi).a, bottom = -join_all(s, step, lo).a;
+            const float top = join_all<TH>(s, step, hi).a, bottom = -join_all<TH>(s, step, lo).a;
             g.mode = 1, g.lo = key_of(top), g.span = key_of(bottom) - g.lo;
         }
         if (g.mode == 1 && g.span == 0) g.mode = 2, g.from = 0, g.span = (uint32_t)vocab - 1;
@@ -426,13 +481,13 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L>& x, con
         if (at < kPairs) pair[at] = Entry{key_of(v), index};
     });
     cluster_sync();
-    solve(s, r, k, target, 1.0, 0.0, (unsigned)f.count, f.mass);
+    solve<TH>(s, r, k, target, 1.0, 0.0, (unsigned)f.count, f.mass);
     return fresh;
 }
 
 // The cut of x's entries, which have all that stays: by count, and by top_p of those; or by mass.
-template <typename L>
-__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L>& x, const Row& r, unsigned k, double top_p, double target,
+template <typename L, int TH>
+__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, unsigned k, double top_p, double target,
                                         bool fresh, int entries, int vocab) {
     if (k) {
         fresh = cut_at(s, step, x, r, false, k, 0.0, entries, vocab, top_p < 1);
@@ -444,8 +499,8 @@ __device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L>& x,
     cut_at(s, step, x, r, fresh, 0, target, entries, vocab, true);
 }
 
-template <typename L>
-__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ Params p) {
+template <typename L, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant__ Params p) {
     using V = Vec<L>;
     constexpr int N = V::N;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -457,10 +512,19 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const L* logits = reinterpret_cast<const L*>(a.logits) + b * a.logits_stride[0] + node * a.logits_stride[1] + v0;
     cluster_arrive();
     grid_wait();
+    // (what is computed in 64 bits is computed by one thread: the unit for it is slow)
     const double temp = a.temperature ? (double)a.temperature[b] : a.temperature_all;
     const int64_t top_k = a.top_k ? (int64_t)a.top_k[b] : a.top_k_all;
     const double top_p = a.top_p ? (double)a.top_p[b] : a.top_p_all, min_p = a.min_p ? (double)a.min_p[b] : a.min_p_all;
     bool by_k = top_k > 0 && top_k < vocab, by_p = top_p < 1;
+    if (tid == 0) {
+        const double t = fmin(fmax(temp, 1e-30), 1e30);
+        s.per_temp = 1.0 / t;
+        // (a cut by count has nothing to do with the temperature)
+        s.bins = (float)((kBins - 1) / (by_k ? fmax(32 * t, 32.0) : 32 * t));
+        // e >= min_p, where exp's argument is (l - M) / T
+        s.reach = min_p > 0 ? -fmin(log(min_p), 0.0) * t : INFINITY;
+    }
     const float* noise = a.token ? a.noise + b * a.noise_stride + v0 : nullptr;
     if (noise && !by_k && !by_p && !(min_p > 0) && temp > 0 && tid == 0) to_l2(noise, (int64_t)n * 4);
 
@@ -468,12 +532,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     const int head = (int)((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(L)), vectors = n ? (head + n + N - 1) / N : 0;
     uint4* const vec = reinterpret_cast<uint4*>(raw);
     const uint4* const from = reinterpret_cast<const uint4*>(logits - head);
-    float most = -INFINITY;
-    for (int i0 = tid; i0 < vectors; i0 += kBatch * kThreads) {
-        V x[kBatch];
+    float most[kGroups];      // the largest of this thread's vectors, every fourth of them
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int i = i0 + k * kThreads;
+    for (int k = 0; k < kGroups; ++k) most[k] = -INFINITY;
+    for (int i0 = tid; i0 < vectors; i0 += kGroups * TH) {
+        V x[kGroups];
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+            const int i = i0 + k * TH;
             if (i >= vectors) continue;
             if (i * N >= head && (i + 1) * N <= head + n) {
                 x[k].raw = from[i];
@@ -486,29 +552,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
             }
         }
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const int i = i0 + k * kThreads;
+        for (int k = 0; k < kGroups; ++k) {
+            const int i = i0 + k * TH;
             if (i >= vectors) continue;
             vec[i] = x[k].raw;
             const float m = x[k].largest();
-            asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(m));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(most[k]) : "f"(m));
         }
     }
-    Slice<L> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0};
+    Slice<L, TH> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0};
     cluster_wait();      // every CTA of the cluster has started: its shared memory may be written
     int step = 0;
-    Note best{most == most ? most : -INFINITY, most == most ? 0.f : 1.f, 0, 0};
-    best = join_all(s, step, best);
+    Note best{-INFINITY, 0.f, 0, 0};
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) best.a = fmaxf(best.a, most[k]), best.b += most[k] == most[k] ? 0.f : 1.f;
+    best = join_all<TH>(s, step, best);
     Row r;
     r.top = best.a;
     const bool none_here = best.b != 0.f || !(best.a > -INFINITY && best.a < INFINITY) || !(temp >= 0);
     const bool greedy = !none_here && temp == 0;
-    const double t = fmin(fmax(temp, 1e-30), 1e30);
-    r.per_temp = 1.0 / t;
+    r.per_temp = s.per_temp, r.bins = s.bins;
+    const float per2 = (float)(r.per_temp * 1.4426950408889634);   // (exponents of 2)
     by_k = by_k && !none_here && !greedy, by_p = by_p && !none_here && !greedy;
-    // (a cut by count has nothing to do with the temperature)
-    r.bins = (float)((kBins - 1) / (by_k ? fmax(32 * t, 32.0) : 32 * t));
-    const float per = (float)r.per_temp;
     float limit = -INFINITY;      // what stays: above this, or equal with an index up to `last`
     int last = 0x7fffffff;
     if (greedy) {
@@ -516,65 +581,79 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
         x.each([&](float f, int index) {
             if (f == r.top) add(first, f, index);
         });
-        limit = r.top, last = join_all(s, step, first).i;
+        limit = r.top, last = join_all<TH>(s, step, first).i;
     } else if (by_k || by_p) {
-        // the bin by which there are enough entries, from the vectors' largest
-        s.count[tid] = 0;
-        if (tid == 0) s.listed = s.pairs = 0;
+        // the bin by which there are enough entries, from the groups' largest
+        for (int i = tid; i < kBins; i += TH) s.count[i] = 0;
+        if (tid == 0) s.listed[0] = s.listed[1] = s.pairs = 0;
         __syncthreads();
-        for (int i = tid; i < vectors; i += kThreads) {
-            const int bin = bin_of(r, V(vec[i]).largest());
+#pragma unroll
+        for (int k = 0; k < kGroups; ++k) {
+            const int bin = bin_of(r, most[k]);
             if (bin < kBins - 1) atomicAdd(&s.count[bin], 1u);
         }
-        cluster_sync();
-        {
-            unsigned count = 0;
-            for (int k = 0; k < cs; ++k) count += *of_rank(&s.count[tid], k);
-            s.counts[tid] = count, s.mass[tid] = 0;
+        add_bins(s, false);
+        unsigned enough = (unsigned)top_k;
+        if (!by_k) {
+            // groups of m entries each, of which a share of 1 - (1 - 1 / 30)^m has one of the largest thirtieth
+            const float groups = fminf((float)(cs * kGroups * TH), (float)vocab / N), m = (float)vocab / groups;
+            enough = max(64u, (unsigned)(groups * (1.f - __expf(-0.0339f * m))));
         }
-        __syncthreads();
-        find(s, by_k ? (unsigned)top_k : (unsigned)max(64, vocab / 32), 0.0, 0, 0);
-        const int bound = s.found.bin >= 0 ? s.found.bin : kBins - 2;
+        find_count(s, enough);
         const bool reached = !by_k || s.found.bin >= 0;
-        // what is not further away; of the rest the sum, where that is asked for
+        // what has a bin up to that one (and, by the rounding of the edge, perhaps some more); of the rest the sum, where that
+        // is asked for
+        const float edge = __fsub_rd(r.top, __fmul_ru(__fdiv_ru((float)((s.found.bin >= 0 ? s.found.bin : kBins - 2) + 1), r.bins), 1.00001f));
         double sum = 0, slope = 0;
-        for (int i = tid; i < vectors && reached; i += kThreads) {
-            const V u(vec[i]);
-            if (bin_of(r, u.largest()) <= bound) {
 #pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (bin_of(r, (float)u.v[j]) <= bound) {
-                        const unsigned at = atomicAdd(&s.listed, 1u);
-                        if (at < kList) s.list[at] = (uint16_t)(i * N + j - head);
+        for (int k = 0; k < kGroups; ++k) {
+            if (!reached || (by_k && most[k] < edge)) continue;
+            for (int i = tid + k * TH; i < vectors; i += kGroups * TH) {
+                const V u(vec[i]);
+                if (u.largest() >= edge) {
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        if ((float)u.v[j] < edge) continue;
+                        const int index = i * N + j - head, far = index >> 16;
+                        const unsigned at = atomicAdd(&s.listed[far], 1u);
+                        if (at < kList) s.list[far ? kList - 1 - at : at] = (uint16_t)index;
                     }
-            }
-            if (by_k) continue;
-            float e = 0.f, f = 0.f;
+                }
+                if (by_k) continue;
+                float e = 0.f, f = 0.f;
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float d = (float)u.v[j] - r.top;
-                if (bin_of(r, (float)u.v[j]) <= bound || !(d > -INFINITY)) continue;
-                const float z = d * per, q = expf(z);
-                e += q, f = fmaf(-z, q, f);
+                for (int j = 0; j < N; ++j) {
+                    const float v = (float)u.v[j], z = fmaxf((v - r.top) * per2, -200.f);   // (2^-200 is 0)
+                    const float q = v < edge ? exp2_of(z) : 0.f;
+                    e += q, f = fmaf(z, q, f);
+                }
+                sum += e, slope -= f;
             }
-            sum += e, slope += f;
         }
+        if (!by_k) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
-        if (lane == 0) s.red_sum[warp] = sum, s.red_slope[warp] = slope;
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
+            if (lane == 0) s.red_sum[warp] = sum, s.red_slope[warp] = slope;
+        }
         __syncthreads();
-        const int listed = (int)s.listed;
-        if (tid < cs) {
-            Rest mine{listed, 0, 0, 0};
-            for (int w = 0; w < kWarps; ++w) mine.sum += s.red_sum[w], mine.slope += s.red_slope[w];
-            *of_rank(&s.rest[rank], tid) = mine;
+        const int listed = (int)(s.listed[0] + s.listed[1]);
+        x.listed = listed, x.low = (int)s.listed[0];
+        if (warp == 0) {
+            sum = slope = 0;
+            if (!by_k) {
+                if (lane < TH / 32) sum = s.red_sum[lane], slope = s.red_slope[lane];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
+            }
+            if (lane < cs) *of_rank(&s.rest[rank], lane) = Rest{listed, 0, sum, slope};
         }
+        x.list = s.list;
         if (listed <= kPairs) {
             // perhaps all are few: rank 0 has them then
             if (tid == 0) s.base = atomicAdd(of_rank(&s.pairs, 0), (unsigned)listed);
             __syncthreads();
             Entry* pair = of_rank(&s.pair[0], 0);
-            if (tid < listed && s.base + tid < kPairs) pair[s.base + tid] = Entry{key_of((float)x.v[s.list[tid]]), v0 + s.list[tid]};
+            if (tid < listed && s.base + tid < kPairs) pair[s.base + tid] = Entry{key_of((float)x.v[x.at(tid)]), v0 + x.at(tid)};
         }
         cluster_sync();
         int total = 0;
@@ -584,17 +663,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
             const Rest& c = s.rest[k];
             total += c.listed, fits = fits && c.listed <= kList, sum += c.sum, slope += c.slope;
         }
-        x.list = s.list, x.listed = listed;
         bool done = false;
         const double scale = 0x1p44, rest = sum * scale;
         const unsigned k = by_k ? (unsigned)top_k : 0;
         if (fits && by_k) {
-            if (total <= kPairs) solve(s, r, k, 0.0, top_p, 0.0, 0, 0);
+            if (total <= kPairs) solve<TH>(s, r, k, 0.0, top_p, 0.0, 0, 0);
             else cut_all(s, step, x, r, k, top_p, 0.0, false, total, vocab);
             done = true;
         } else if (fits) {
             if (total <= kPairs) {
-                solve(s, r, 0, 0.0, top_p, rest, 0, 0);
+                solve<TH>(s, r, 0, 0.0, top_p, rest, 0, 0);
                 done = s.cut.mass > 0;
             } else {
                 histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
@@ -604,8 +682,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
                 if (done) cut_all(s, step, x, r, 0, 1.0, target, true, total, vocab);
             }
             if (done) {
-                // The terms of the rest are off by 2^-23 (expf) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z| (a
-                // difference, a factor and a product); the cut is certain where that does not reach the next entry.
+                // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
+                // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
                 const double off = top_p * (sum * 0x1p-20 + slope * 0x1p-22) * scale;
                 done = (double)s.cut.before < s.cut.target - off && s.cut.target + off <= (double)s.cut.mass;
             }
@@ -623,16 +701,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
         }
         limit = value_of(s.cut.key), last = s.cut.index;
     }
-    // e >= min_p, where exp's argument is (l - M) / T
     if (min_p > 0 && !none_here && !greedy) {
-        const float least = fminf(__double2float_ru((double)r.top + fmin(log(min_p), 0.0) * t), r.top);
+        const float least = fminf(__double2float_ru((double)r.top - s.reach), r.top);
         if (least > limit) limit = least, last = 0x7fffffff;
     }
     auto stays = [&](float f, int index) { return f > limit || (f == limit && index <= last); };
     if (a.out) {
         L* out = reinterpret_cast<L*>(a.out) + b * a.out_stride[0] + node * a.out_stride[1] + v0;
         const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0;
-        for (int i = tid; i < vectors; i += kThreads) {
+        for (int i = tid; i < vectors; i += TH) {
             V u(vec[i]);
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -651,39 +728,42 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
     if (!a.token) return;
     Note got = none();
     if (!none_here && !greedy) {
-        auto draw = [&](float f, int index, float e) {
-            const float q = expf((f - r.top) * per);
-            got.b += q;
-            if (q > 0.f) add(got, __fdividef(q, e), index);
-        };
+        // (e to 2^-22 and 3 2^-24 |z|, the quotient to 2 units more)
+        got.a = 0.f;
         if (x.list) {
             x.each([&](float f, int index) {
-                if (stays(f, index)) draw(f, index, noise[index - v0]);
+                if (!stays(f, index)) return;
+                const float q = exp2_of((f - r.top) * per2), chance = __fdividef(q, noise[index - v0]);
+                got.b += q;
+                if (chance > got.a || (chance == got.a && index < got.i)) got.a = chance, got.i = index;
             });
         } else {
             constexpr int kAhead = 8;
-            for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
+            const bool all = limit == -INFINITY;
+            for (int i0 = tid; i0 < n; i0 += kAhead * TH) {
                 float f[kAhead], e[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int i = i0 + k * kThreads;
+                    const int i = i0 + k * TH;
                     f[k] = i < n ? (float)x.v[i] : -INFINITY;
-                    e[k] = i < n && stays(f[k], v0 + i) ? noise[i] : 0.f;
+                    if (!all && !stays(f[k], v0 + i)) f[k] = -INFINITY;
+                    e[k] = f[k] > -INFINITY ? noise[i] : 1.f;
                 }
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int i = i0 + k * kThreads;
-                    if (i < n && stays(f[k], v0 + i)) draw(f[k], v0 + i, e[k]);
+                    const float q = exp2_of((f[k] - r.top) * per2), chance = __fdividef(q, e[k]);
+                    got.b += q;
+                    if (chance > got.a) got.a = chance, got.i = v0 + i0 + k * TH;
                 }
             }
         }
-        got = join_all(s, step, got);
+        got = join_all<TH>(s, step, got);
     } else if (greedy) {
         got.i = last;
     }
     // the owner of the token knows its logit
     if (a.logprob && !none_here && !greedy && got.i >= v0 && got.i < v0 + n && tid == 0)
-        a.logprob[b] = ((float)x.v[got.i - v0] - r.top) * per - logf(got.b);
+        a.logprob[b] = (float)(((double)(float)x.v[got.i - v0] - (double)r.top) * r.per_temp) - logf(got.b);
     if (rank == 0 && tid == 0) {
         a.token[b] = got.i;
         if (a.logprob && (got.i < 0 || greedy)) a.logprob[b] = got.i < 0 ? NAN : 0.f;
@@ -693,28 +773,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
 
 inline int64_t slice_of(int64_t vocab, int cs) { return ((vocab + cs - 1) / cs + 15) / 16 * 16; }
 
-// CTAs of a cluster: as in tree_verify.cu, where there are more rows than fit at once smaller clusters wait less.
-int cluster_ctas(int64_t rows, int64_t vocab, int item, int sms) {
-    int best = kMaxCluster;
-    double least = 0;
-    for (int cs = kMaxCluster; cs >= 1; cs /= 2) {
-        const int64_t slice = slice_of(vocab, cs);
-        if (slice * item > kRowBytes) break;
-        const size_t bytes = sizeof(Shared) + slice * item + 1024;
-        const double at_once = (double)sms * std::min<size_t>(4, kSmemSm / bytes) / cs;
-        const double time = std::max(1.0, rows / at_once) * (16 * kThreads + slice);
-        if (cs == kMaxCluster || time < least) best = cs, least = time;
-    }
-    return best;
-}
-
-template <typename L>
+template <typename L, int TH>
 int launch(const Params& p, int64_t rows, int cs, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(k_sample<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
+    cudaError_t e = cudaFuncSetAttribute(k_sample<L, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * cs));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(TH);
     cfg.dynamicSmemBytes = (size_t)p.slice * sizeof(L) + 16;   // (a vector more where the slice does not begin with one)
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -724,9 +789,22 @@ int launch(const Params& p, int64_t rows, int cs, cudaStream_t s) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, k_sample<L>, p);
+    e = cudaLaunchKernelEx(&cfg, k_sample<L, TH>, p);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: launch failed: %s", cudaGetErrorString(e));
     return check_launch("spark_sample");
+}
+template <typename L>
+int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
+    // one CTA a row where that fits, else as large a cluster as leaves all rows at work at once
+    int cs = 1;
+    while (slice_of(p.a.vocab, cs) * sizeof(L) > kRowBytes) cs *= 2;
+    while (cs > 1 && cs < kMaxCluster && 2 * cs * rows <= sms) cs *= 2;
+    if (const char* e = getenv("SAMPLE_CS")) cs = std::max(cs, atoi(e));
+    p.slice = (int)slice_of(p.a.vocab, cs);
+    // two CTAs an SM where there are more than one for each and both fit
+    const size_t bytes = sizeof(Shared) + p.slice * sizeof(L) + 16 + 1024;
+    if (rows * cs > sms && 2 * bytes <= kSmemSm) return launch<L, 512>(p, rows, cs, s);
+    return launch<L, 1024>(p, rows, cs, s);
 }
 
 }  // namespace sm
@@ -763,14 +841,11 @@ int spark_sample(const SparkSample* a, void* stream) {
     const cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: %s", cudaGetErrorString(e));
     const int64_t rows = a->batch * a->nodes;
-    const int item = a->dtype == SPARK_DTYPE_F32 ? 4 : 2;
-    const int cs = cluster_ctas(rows, a->vocab, item, tc::sm_count_cached(dev));
-    SPARK_REQUIRE(slice_of(a->vocab, cs) * item <= kRowBytes, SPARK_ERR_UNSUPPORTED, "spark_sample: vocabulary");
-    p.slice = (int)slice_of(a->vocab, cs);
+    const int sms = tc::sm_count_cached(dev);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (a->dtype == SPARK_DTYPE_BF16) return launch<__nv_bfloat16>(p, rows, cs, st);
-    if (a->dtype == SPARK_DTYPE_F16) return launch<__half>(p, rows, cs, st);
-    return launch<float>(p, rows, cs, st);
+    if (a->dtype == SPARK_DTYPE_BF16) return launch<__nv_bfloat16>(p, rows, sms, st);
+    if (a->dtype == SPARK_DTYPE_F16) return launch<__half>(p, rows, sms, st);
+    return launch<float>(p, rows, sms, st);
 }
 
 }  // extern "C"

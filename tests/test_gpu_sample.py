@@ -6,10 +6,11 @@ A sum of n exponentials in multiples of 2^-44 of the largest is off by at most n
 where the mass before an entry is within 2 n 2^-45 of top_p times the whole, either side is
 right.  min_p's border, an exponent in 64 bits that is rounded up to a logit of 32 bits, is
 never closer than that in the cases here.
-The token is argmax e / noise in fp32: the exponent is off by 2^-23 |z| (a difference and a product), the
-exponential and the quotient by 2 units each: equal, unless the two largest quotients are
-within 1e-5 (|z| < 64).  logprob: z - log(sum), with |z| 2^-23 + 2^-24 (z, log) and sums of at most
-100003 terms in chains of 100 and trees, 2^-24 (120 + 4): within 1e-5 + 2^-22 |logprob|.
+The token is argmax e / noise in fp32: the exponent is off by 3 2^-24 |z| (a difference, a factor and a
+product), the exponential by 2^-22 and the quotient by 2^-23; a token that wins has |z| < 25 here: 4.9e-6
+each.  Equal, unless the two largest quotients are within 1e-5.  logprob: z in 64 bits less the log of a sum of
+such terms, most of the mass at |z| < 10: 2^-22 + 30 2^-24, and chains of at most 100 terms with trees of 10,
+110 2^-24: within 1e-5 + 2^-22 |logprob|.
 """
 from __future__ import annotations
 
