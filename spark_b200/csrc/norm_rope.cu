@@ -28,6 +28,12 @@ int sm_count_cached(int dev);
 }
 
 namespace nr {
+#ifndef FH
+#define FH 4
+#define FB 2
+#define BH 2
+#define BB 2
+#endif
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
@@ -37,7 +43,7 @@ struct Part {
     const void *x, *g;   // g: the gradient of y
     void* y;             // y, or the gradient of x
     const void* w;       // NULL: ones
-    int heads, w_dtype;
+    int heads, w_dtype, w_wide;   // w_wide: vectors of w lie as those of x do; fp32 on 16 bytes
     int64_t xs[3], gs[3], ys[3];
 };
 struct Params {
@@ -173,8 +179,23 @@ __device__ __forceinline__ void turn_both(float* a, float* b, const Place& at, c
     }
 }
 
-template <int N>
+template <typename T, int N>
 __device__ __forceinline__ void load_weight(const Part& part, int at, float* w) {
+    if (part.w_wide && at >= 0) {
+        if (part.w_dtype == SPARK_DTYPE_F32) {
+            if constexpr (N % 4 == 0) {
+#pragma unroll
+                for (int k = 0; k < N; k += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(part.w) + at + k);
+                    w[k] = x.x, w[k + 1] = x.y, w[k + 2] = x.z, w[k + 3] = x.w;
+                }
+                return;
+            }
+        } else {
+            Vec<T, N>::get(*reinterpret_cast<const typename Vec<T, N>::type*>(reinterpret_cast<const T*>(part.w) + at), w);
+            return;
+        }
+    }
 #pragma unroll
     for (int k = 0; k < N; ++k) w[k] = at >= 0 && part.w ? load_as_float(part.w, part.w_dtype, at + k) : 1.f;
 }
@@ -194,10 +215,10 @@ constexpr int kUnits = N >= 4 ? 1 : 4 / N;   // of a lane: kMaxDim / 2 / N over 
 
 // A group of `lanes` lanes takes HEADS heads of one token, of q or of k.
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ Params p, int lanes) {
+__global__ void __launch_bounds__(kThreads, FB) k_norm_rope(const __grid_constant__ Params p, int lanes) {
     using V = Vec<T, N>;
     using R = typename V::type;
-    constexpr int U = kUnits<N>, HEADS = 4 / (U > 2 ? 2 : U);
+    constexpr int U = kUnits<N>, HEADS = (FH / (U > 2 ? 2 : U) > 0 ? FH / (U > 2 ? 2 : U) : 1);
     grid_wait();
     const int groups_q = (p.part[0].heads + HEADS - 1) / HEADS, groups = groups_q + (p.part[1].heads + HEADS - 1) / HEADS;
     const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / lanes;
@@ -228,8 +249,8 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         load_turn<N, INTER>(p, at[u], good ? pos : 0, c[u], s[u]);
-        load_weight<N>(part, at[u].a, wa[u]);
-        load_weight<N>(part, at[u].b, wb[u]);
+        load_weight<T, N>(part, at[u].a, wa[u]);
+        load_weight<T, N>(part, at[u].b, wb[u]);
     }
     float rstd[HEADS];
 #pragma unroll
@@ -269,10 +290,10 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const __grid_constant__ 
 // side, of q or of k at once, so that a lane's sums of the weights' gradients are of one part and are put away when the
 // other begins.  The order of the additions depends on the sizes alone.
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(kThreads) k_norm_rope_backward(const __grid_constant__ Params p, int lanes) {
+__global__ void __launch_bounds__(kThreads, BB) k_norm_rope_backward(const __grid_constant__ Params p, int lanes) {
     using V = Vec<T, N>;
     using R = typename V::type;
-    constexpr int U = kUnits<N>, HEADS = U > 2 ? 1 : 2;
+    constexpr int U = kUnits<N>, HEADS = U > 2 ? 1 : BH;
     extern __shared__ float sums[];   // [2, kWarps, dim]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) / lanes, a_warp = 32 / lanes;
     for (int k = threadIdx.x; p.partial && k < 2 * kWarps * p.dim; k += kThreads) sums[k] = 0.f;
@@ -291,8 +312,8 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope_backward(const __grid_co
         if (w < warps) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                load_weight<N>(part, at[u].a, wa[u]);
-                load_weight<N>(part, at[u].b, wb[u]);
+                load_weight<T, N>(part, at[u].a, wa[u]);
+                load_weight<T, N>(part, at[u].b, wb[u]);
 #pragma unroll
                 for (int k = 0; k < N; ++k) da[u][k] = db[u][k] = 0.f;
             }
@@ -434,7 +455,7 @@ cudaError_t launch(const Params& p, int vec, int lanes, bool inter, bool backwar
 int backward_blocks() {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    return 2 * tc::sm_count_cached(dev);
+    return BB * tc::sm_count_cached(dev);
 }
 
 int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace_bytes, int* err, cudaStream_t s, const char* name) {
@@ -504,18 +525,21 @@ int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace
         if (ok) break;
     }
     SPARK_REQUIRE(vec > 1 || !inter, SPARK_ERR_ALIGNMENT, "%s: interleaved pairs lie on %d bytes, with even strides", name, 2 * es);
+    for (Part& t : p.part)
+        t.w_wide = t.w && (t.w_dtype == SPARK_DTYPE_F32 ? vec % 4 == 0 && aligned(t.w, 16)
+                                                        : t.w_dtype == (int)a->dtype && aligned(t.w, (size_t)vec * es));
     const int units = units_of(p.dim, p.rot, vec, inter);
     int lanes = 1;
     while (lanes < units && lanes < 32) lanes *= 2;
     int64_t grid;
     const int u = vec >= 4 ? 1 : 4 / vec;   // kUnits
     if (!backward) {
-        const int a_group = 4 / (u > 2 ? 2 : u);
+        const int a_group = (FH / (u > 2 ? 2 : u) > 0 ? FH / (u > 2 ? 2 : u) : 1);
         const int64_t groups = (p.part[0].heads + a_group - 1) / a_group + (p.part[1].heads + a_group - 1) / a_group;
         const int64_t a_block = kThreads / lanes;
         grid = (p.n_tokens * groups + a_block - 1) / a_block;
     } else {
-        const int a_group = u > 2 ? 1 : 2;
+        const int a_group = u > 2 ? 1 : BH;
         const int64_t most = std::max((p.part[0].heads + a_group - 1) / a_group, (p.part[1].heads + a_group - 1) / a_group);
         const int64_t a_block = kThreads / lanes;
         const int blocks = backward_blocks();

@@ -31,7 +31,6 @@
 // then (2000 cycles or more each, against some hundred).
 #include <float.h>
 #include <math.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -78,7 +77,7 @@ struct Cut {
     uint32_t key;                       // what stays: smaller keys, of equal ones the indices up to this
     int index;
     unsigned long long before, mass;    // sums of e of what stays, without and with the last entry
-    double target;                      // what they were compared with
+    unsigned long long target;          // what they were compared with
 };
 // What a CTA tells the others with its list: entries in it (more than kList: too many), sum of e of the others, of |z| e.
 struct Rest {
@@ -97,7 +96,7 @@ struct Shared {
     };
     unsigned long long mass[kBins];                           // of the row
     unsigned counts[kBins];
-    uint16_t list[kList];                                     // indices in the slice; those from 65536 on from the end back
+    uint16_t list[kList];                                     // places among the vectors; those from 65536 on from the end back
     Note note[2][kMaxCluster];
     Note red[2][kWarps];
     Rest rest[kMaxCluster];
@@ -252,8 +251,9 @@ struct Slice {
     int v0, n;               // index of the first, how many
     const uint16_t* list;    // NULL: all
     int listed, low;         // of them below 65536
+    int head;                // places before v
 
-    __device__ __forceinline__ int at(int i) const { return i < low ? list[i] : 65536 + list[kList - 1 - (i - low)]; }
+    __device__ __forceinline__ int at(int i) const { return (i < low ? list[i] : 65536 + list[kList - 1 - (i - low)]) - head; }
 
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
@@ -296,6 +296,16 @@ __device__ __forceinline__ void count_one(Shared& s, int bin, unsigned long long
 
 // Adds the bins of the CTAs into s.counts and, if asked, s.mass: each CTA its share, which it gives to all.
 __device__ __forceinline__ void add_bins(Shared& s, bool masses) {
+    if (cluster_size() == 1) {
+        const int b = threadIdx.x;
+        __syncthreads();
+        if (b < kBins) {
+            s.counts[b] = s.count[b];
+            if (masses) s.mass[b] = ((unsigned long long)s.high[b] << 32) + s.low[b];
+        }
+        __syncthreads();
+        return;
+    }
     cluster_sync();
     const int n = (int)cluster_size(), share = kBins / n, b = (int)cluster_rank() * share + threadIdx.x;
     if (threadIdx.x < share) {
@@ -349,13 +359,44 @@ __device__ __forceinline__ void find_count(Shared& s, unsigned k) {
     __syncthreads();
 }
 
-// The bin in which a cut lies: where the count reaches `k` (k > 0), else where the mass reaches `target`; bin -1 where none does.
-// Behind count0 entries of mass0.  Returns the mass of all bins.
-__device__ __noinline__ unsigned long long find(Shared& s, unsigned k, double target, unsigned count0, unsigned long long mass0) {
+// The sum over a warp.
+__device__ __forceinline__ unsigned long long sum_of_warp(unsigned long long x) {
+    const unsigned a = __reduce_add_sync(0xffffffffu, (unsigned)x & 0x7ffffff), b = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 27) & 0x7ffffff),
+                   c = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 54));
+    return ((unsigned long long)c << 54) + ((unsigned long long)b << 27) + a;
+}
+// The mass of all bins, for every thread.
+__device__ __noinline__ unsigned long long mass_of_bins(Shared& s) {
+    const int t = threadIdx.x, lane = t & 31;
+    if (t < kBins) {
+        const unsigned long long m = sum_of_warp(s.mass[t]);
+        if (lane == 0) s.scan_mass[t >> 5] = m;
+    }
+    __syncthreads();
+    const unsigned long long all = sum_of_warp(lane < kBins / 32 ? s.scan_mass[lane] : 0);
+    __syncthreads();
+    return all;
+}
+// The sum over the cluster, for every thread.
+template <int TH>
+__device__ __noinline__ unsigned long long sum_of_all(Shared& s, unsigned long long x) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (int)cluster_size();
+    x = sum_of_warp(x);
+    __syncthreads();
+    if (lane == 0) s.scan_mass[warp] = x;
+    __syncthreads();
+    x = sum_of_warp(lane < TH / 32 ? s.scan_mass[lane] : 0);
+    if (n == 1) return x;
+    if (threadIdx.x < n) *of_rank(&s.mass[cluster_rank()], threadIdx.x) = x;
+    cluster_sync();
+    return sum_of_warp(lane < n ? s.mass[lane] : 0);
+}
+// The bin in which a cut lies: where the count reaches `k` (k > 0), else where the mass reaches `target`.  Behind count0 entries of
+// mass0.  Where none does, bin -1, with the count and the mass of all.
+__device__ __noinline__ void find(Shared& s, unsigned k, unsigned long long target, unsigned count0, unsigned long long mass0) {
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     unsigned own = 0, c = 0;
     unsigned long long own_mass = 0, m = 0;
-    if (t == 0) s.found = Found{-1, 0, 0, 0};
     if (t < kBins) {
         c = own = s.counts[t], m = own_mass = s.mass[t];
 #pragma unroll
@@ -368,26 +409,22 @@ __device__ __noinline__ unsigned long long find(Shared& s, unsigned k, double ta
     }
     __syncthreads();
     if (t < kBins) {
-        unsigned before = count0;
-        unsigned long long mass = mass0;
-        for (int w = 0; w < warp; ++w) before += s.scan_count[w], mass += s.scan_mass[w];
-        before += c - own, mass += m - own_mass;
-        const bool here = k ? before < k && k <= before + own
-                            : own_mass > 0 && (double)mass < target && target <= (double)(mass + own_mass);
+        const unsigned before = count0 + c - own + __reduce_add_sync(0xffffffffu, lane < warp ? s.scan_count[lane] : 0);
+        const unsigned long long mass = mass0 + m - own_mass + sum_of_warp(lane < warp ? s.scan_mass[lane] : 0);
+        const bool here = k ? before < k && k <= before + own : mass < target && target <= mass + own_mass;
         if (here) s.found = Found{t, (int)before, (int)own, mass};
+        if (t == kBins - 1 && (k ? before + own < k : mass + own_mass < target)) s.found = Found{-1, (int)(before + own), 0, mass + own_mass};
     }
     __syncthreads();
-    unsigned long long all = 0;
-#pragma unroll
-    for (int w = 0; w < kBins / 32; ++w) all += s.scan_mass[w];
-    return all;
 }
+// The share top_p of a mass (at least one multiple: the largest entry stays).
+__device__ __forceinline__ unsigned long long share_of(double top_p, double mass) { return (unsigned long long)fmax(ceil(top_p * mass), 1.0); }
 
 // Rank 0 compares its s.pairs entries with one another and tells all CTAs the cut: by count (k > 0), by mass (target > 0), or by
 // top_p of the mass of the first k or, without k, of all and `rest`.  Behind count0 entries of mass0.  Where the cut is behind
 // them all its mass is 0.
 template <int TH>
-__device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, double target, double top_p, double rest, unsigned count0,
+__device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, unsigned long long target, double top_p, double rest, unsigned count0,
                                    unsigned long long mass0) {
     if (cluster_rank() == 0) {
         const int n = min((int)s.pairs, kPairs), t = threadIdx.x;
@@ -414,16 +451,15 @@ __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, double t
             before += __shfl_xor_sync(0xffffffffu, before, o);
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        if (!(target > 0) && top_p < 1) {
+        if (target == 0 && top_p < 1) {
             // the last of the entries that count has the mass of them all
             if (e < n && sub == 0 && before + 1 == (k ? k : (unsigned)n)) s.scan_mass[0] = sum + mass;
             __syncthreads();
-            // (at least half a multiple: the largest entry stays)
-            target = fmax(top_p * ((double)s.scan_mass[0] + rest), 0.5);
+            target = share_of(top_p, (double)s.scan_mass[0] + rest);
         }
         before += count0, sum += mass0;
         if (e < n && sub == 0) {
-            const bool last = target > 0 ? (double)sum < target && target <= (double)(sum + mass) && mass > 0 : before + 1 == k;
+            const bool last = target ? sum < target && target <= sum + mass : before + 1 == k;
             if (last) s.cut = Cut{mine.key, mine.index, sum, sum + mass, target};
         }
         __syncthreads();
@@ -435,18 +471,14 @@ __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, double t
 // The cut by count (k > 0: behind the first k entries) or by mass (behind the shortest prefix with `target`) of x's entries, from
 // their bins by distance, which are in s if `fresh`.  s.cut afterwards.  Returns whether the bins are still there.
 template <typename L, int TH>
-__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, bool fresh, unsigned k, double target, int entries,
+__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, bool fresh, unsigned k, unsigned long long target, int entries,
                                     int vocab, bool masses) {
     Range g{0, 0, 0, 0, 0, 0};
     if (!fresh) histogram(s, x, r, g, masses);
     find(s, k, target, 0, 0);
     Found f = s.found;
-    if (f.bin < 0) {
-        // behind all bins: the last one has the rest (and no mass)
-        f = Found{kBins - 1, 0, 0, 0};
-        for (int w = 0; w < kBins / 32; ++w) f.count += (int)s.scan_count[w], f.mass += s.scan_mass[w];
-        f.in = entries - f.count;
-    }
+    // behind all bins: the last one has the rest (and no mass)
+    if (f.bin < 0) f.bin = kBins - 1, f.in = entries - f.count;
     g.bin = f.bin;
     fresh = true;
     while (f.in > kPairs) {
@@ -487,13 +519,12 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x,
 
 // The cut of x's entries, which have all that stays: by count, and by top_p of those; or by mass.
 template <typename L, int TH>
-__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, unsigned k, double top_p, double target,
+__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, unsigned k, double top_p, unsigned long long target,
                                         bool fresh, int entries, int vocab) {
     if (k) {
-        fresh = cut_at(s, step, x, r, false, k, 0.0, entries, vocab, top_p < 1);
+        fresh = cut_at(s, step, x, r, false, k, 0ull, entries, vocab, top_p < 1);
         if (!(top_p < 1)) return;
-        // (at least half a multiple: the largest entry stays)
-        target = fmax(top_p * (double)s.cut.mass, 0.5);
+        target = share_of(top_p, (double)s.cut.mass);
         __syncthreads();
     }
     cut_at(s, step, x, r, fresh, 0, target, entries, vocab, true);
@@ -560,7 +591,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
             asm("max.NaN.f32 %0, %0, %1;" : "+f"(most[k]) : "f"(m));
         }
     }
-    Slice<L, TH> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0};
+    Slice<L, TH> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0, head};
     cluster_wait();      // every CTA of the cluster has started: its shared memory may be written
     int step = 0;
     Note best{-INFINITY, 0.f, 0, 0};
@@ -611,13 +642,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
             for (int i = tid + k * TH; i < vectors; i += kGroups * TH) {
                 const V u(vec[i]);
                 if (u.largest() >= edge) {
+                    unsigned which = 0;
 #pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        if ((float)u.v[j] < edge) continue;
-                        const int index = i * N + j - head, far = index >> 16;
-                        const unsigned at = atomicAdd(&s.listed[far], 1u);
-                        if (at < kList) s.list[far ? kList - 1 - at : at] = (uint16_t)index;
-                    }
+                    for (int j = 0; j < N; ++j) which |= (float)u.v[j] >= edge ? 1u << j : 0u;
+                    const int place = i * N, far = place >> 16;
+                    unsigned at = atomicAdd(&s.listed[far], (unsigned)__popc(which));
+                    for (; which && at < kList; which &= which - 1, ++at)
+                        s.list[far ? kList - 1 - at : at] = (uint16_t)(place + __ffs(which) - 1);
                 }
                 if (by_k) continue;
                 float e = 0.f, f = 0.f;
@@ -667,35 +698,40 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         const double scale = 0x1p44, rest = sum * scale;
         const unsigned k = by_k ? (unsigned)top_k : 0;
         if (fits && by_k) {
-            if (total <= kPairs) solve<TH>(s, r, k, 0.0, top_p, 0.0, 0, 0);
-            else cut_all(s, step, x, r, k, top_p, 0.0, false, total, vocab);
+            if (total <= kPairs) solve<TH>(s, r, k, 0ull, top_p, 0.0, 0, 0);
+            else cut_all(s, step, x, r, k, top_p, 0ull, false, total, vocab);
             done = true;
         } else if (fits) {
-            if (total <= kPairs) {
-                solve<TH>(s, r, 0, 0.0, top_p, rest, 0, 0);
-                done = s.cut.mass > 0;
-            } else {
+            // (a mass of all that the list does not reach is found out about below)
+            auto cut = [&](double more) {
+                if (total <= kPairs) {
+                    solve<TH>(s, r, 0, 0ull, top_p, more, 0, 0);
+                    return s.cut.mass > 0;
+                }
                 histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
-                const double whole = (double)find(s, 1, 0.0, 0, 0), target = fmax(top_p * (whole + rest), 0.5);
-                __syncthreads();
-                done = target <= whole;
-                if (done) cut_all(s, step, x, r, 0, 1.0, target, true, total, vocab);
-            }
-            if (done) {
-                // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
-                // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
-                const double off = top_p * (sum * 0x1p-20 + slope * 0x1p-22) * scale;
-                done = (double)s.cut.before < s.cut.target - off && s.cut.target + off <= (double)s.cut.mass;
+                const unsigned long long whole = mass_of_bins(s), target = share_of(top_p, (double)whole + more);
+                if (target <= whole) cut_all(s, step, x, r, 0, 1.0, target, true, total, vocab);
+                return target <= whole;
+            };
+            done = cut(rest);
+            // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
+            // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
+            const double off = top_p * (sum * 0x1p-20 + slope * 0x1p-22) * scale;
+            if (done && !((double)s.cut.before < (double)s.cut.target - off && (double)s.cut.target + off <= (double)s.cut.mass)) {
+                // it is not: the rest as the list's entries are summed
+                unsigned long long exact = 0;
+                for (int i = tid; i < n; i += TH)
+                    if ((float)x.v[i] < edge) exact += mass_of(r, (float)x.v[i]);
+                done = cut((double)sum_of_all<TH>(s, exact));
             }
         }
         if (!done) {
             x.list = nullptr;
-            double target = 0;
+            unsigned long long target = 0;
             __syncthreads();
             if (!by_k) {
                 histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
-                target = fmax(top_p * (double)find(s, 1, 0.0, 0, 0), 0.5);
-                __syncthreads();
+                target = share_of(top_p, (double)mass_of_bins(s));
             }
             cut_all(s, step, x, r, k, top_p, target, !by_k, vocab, vocab);
         }
@@ -799,7 +835,6 @@ int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
     int cs = 1;
     while (slice_of(p.a.vocab, cs) * sizeof(L) > kRowBytes) cs *= 2;
     while (cs > 1 && cs < kMaxCluster && 2 * cs * rows <= sms) cs *= 2;
-    if (const char* e = getenv("SAMPLE_CS")) cs = std::max(cs, atoi(e));
     p.slice = (int)slice_of(p.a.vocab, cs);
     // two CTAs an SM where there are more than one for each and both fit
     const size_t bytes = sizeof(Shared) + p.slice * sizeof(L) + 16 + 1024;

@@ -307,3 +307,17 @@ def test_settings_of_one_sequence_stay_on_the_device():
         graph.replay()
         check_filter(x, cut, s)
         check_sample(x, noise, token, logprob, s)
+
+
+@pytest.mark.parametrize("vocab,dtype", [(3000, FP), (32000, FP), (32000, BF), (120000, FP)])
+def test_borders_that_only_good_sums_tell(vocab, dtype):
+    """top_p within 1e-8 of the mass before an entry, on either side: sums in 32 bits of what is far below would not do."""
+    x = (randn(gen(vocab), 1, vocab) * 4).to(dtype)
+    row = x[0].double().cpu()
+    e = (row.sort(descending=True).values - row.max()).exp()
+    before = (e.cumsum(0) - e) / e.sum()
+    for share in (0.5, 0.8, 0.93):
+        i = int((before < share).sum())
+        for p in (float(before[i]) * (1 + 1e-8), float(before[i]) * (1 - 1e-8)):
+            assert cut64(row, 1.0, 0, p, 0.0)[2] == [] and len(cut64(row, 1.0, 0, p, 0.0)[0]) == (i + 1 if p > before[i] else i)
+            check_filter(x, ops().filter_logits(x, top_p=p), dict(top_p=p))
