@@ -10,12 +10,17 @@
 // s is computed anew in the backward pass, which costs less than reading it.  All in
 // fp32, rounded once to the tensors' type.
 //
-// Its bound is HBM.  A head belongs to a group of lanes (a power of two), a lane has
-// one vector of its turned part and the partners half a rotation away, so that sums
-// go over a few shuffles and the rotation needs none.  What is not turned comes in
-// pairs of vectors too.  A thread has four heads of a token (two in the backward
-// pass, which holds dy too): cosines, sines and weights are loaded once for them,
-// and eight loads are on the way together.
+// Its bound is HBM: 2 accesses a value forward, 3 backward, where 8 and 13 instructions a
+// value take half to two thirds of that time.  A head belongs to a group of lanes (a
+// power of two); a lane has one vector of its turned part and the partners half a
+// rotation away, so that sums go over a few shuffles and the rotation needs none.  What
+// is not turned comes in pairs of vectors too.  A group walks along the heads of a
+// token, whose angles (with the weights in them, forward) stay in registers; vectors
+// come three steps ahead by asynchronous copies.  Measured: 8 x 4096 tokens of 32 + 8
+// heads of 128 in bf16, forward 126 us (5.3 TB/s), forward and backward 298 us (5.6
+// TB/s); without the copies ahead 372 us, with one head's products in scalar
+// instructions 454 us.  2048 tokens 13.4 us, of which half is the launch and the way
+// from a position to its angles.
 #include <string.h>
 
 #include <algorithm>
@@ -28,16 +33,12 @@ int sm_count_cached(int dev);
 }
 
 namespace nr {
-#ifndef FH
-#define FH 4
-#define FB 2
-#define BH 2
-#define BB 2
-#endif
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxDim = 256;
+constexpr int kBlocks = 2;     // of an SM (128 registers a thread; 3 spill, and take 10 to 60% longer)
+constexpr int kStages = 3;     // steps on their way (4 are no faster)
 
 struct Part {
     const void *x, *g;   // g: the gradient of y
@@ -322,24 +323,74 @@ __device__ __forceinline__ void sum_of_group(float (&x)[N], int lanes) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
 }
-// What a group of lanes does of an item.
-struct Work {
-    int token, head;    // the first head
-    bool in;
-    int64_t b, t;
+// The steps of a warp, in order: HEADS heads of a token at a time for each of its groups of lanes; the items of q first, then those
+// of k.
+template <typename T, int HEADS>
+struct Steps {
+    int which, item, k, left, token;    // left: heads from this step on (0 or fewer: none for this group)
+    const T *x, *g;
+    T* y;
+
+    __device__ __forceinline__ bool done() const { return which == 2; }
+    __device__ __forceinline__ void begin(const Params& p, int group, int a_warp) {
+        which = 0, item = blockIdx.x * kWarps + (threadIdx.x >> 5);
+        enter(p, group, a_warp);
+    }
+    __device__ __forceinline__ void enter(const Params& p, int group, int a_warp) {
+        while (which < 2 && item >= p.part[which].items) item -= p.part[which++].items;
+        if (which == 2) return;
+        const Part& part = p.part[which];
+        const int tile = part.chunks == 1 ? item : item / part.chunks, chunk = item - tile * part.chunks;
+        const int head = ((chunk * part.span << part.across) + (group & ((1 << part.across) - 1))) * HEADS;
+        token = tile * (a_warp >> part.across) + (group >> part.across);
+        left = token < p.n_tokens ? part.heads - head : 0;
+        if (token >= p.n_tokens) token = 0;
+        const int b = token / p.tokens, t = token - b * p.tokens;
+        k = 0;
+        x = reinterpret_cast<const T*>(part.x) + b * part.xs[0] + t * part.xs[1] + head * part.xs[2];
+        g = reinterpret_cast<const T*>(part.g) + b * part.gs[0] + t * part.gs[1] + head * part.gs[2];
+        y = reinterpret_cast<T*>(part.y) + b * part.ys[0] + t * part.ys[1] + head * part.ys[2];
+    }
+    __device__ __forceinline__ void next(const Params& p, int group, int a_warp) {
+        const Part& part = p.part[which];
+        if (++k < part.span) {
+            const int on = HEADS << part.across;
+            x += on * part.xs[2], g += on * part.gs[2], y += on * part.ys[2], left -= on;
+        } else {
+            item += gridDim.x * kWarps;
+            enter(p, group, a_warp);
+        }
+    }
 };
-template <int HEADS>
-__device__ __forceinline__ Work work_of(const Params& p, const Part& part, int item, int group, int a_warp) {
-    Work w;
-    const int tile = part.chunks == 1 ? item : item / part.chunks, chunk = item - tile * part.chunks;
-    w.token = tile * (a_warp >> part.across) + (group >> part.across);
-    w.head = ((chunk * part.span << part.across) + (group & ((1 << part.across) - 1))) * HEADS;
-    w.in = w.token < p.n_tokens;
-    if (!w.in) w.token = 0;
-    const int b = w.token / p.tokens;
-    w.b = b, w.t = w.token - b * p.tokens;
-    return w;
-}
+
+// What a thread reads, kStages steps ahead: its vectors, in places of its own in shared memory, so that registers hold none on
+// their way and no thread waits for another.  (Vectors of 2 bytes are below what can be copied so: they are loaded when needed.)
+template <typename T, int N, int VECTORS>
+struct Ring {
+    using V = Vec<T, N>;
+    using R = typename V::type;
+    static constexpr int kBytes = sizeof(R);
+    static constexpr bool kAsync = kBytes >= 4;
+    R* mine;      // [kStages, VECTORS], kThreads apart
+
+    __device__ __forceinline__ R* place(int stage, int v) const { return mine + (stage * VECTORS + v) * kThreads; }
+    __device__ __forceinline__ void fetch(int stage, int v, const T* from, bool is) const {
+        if constexpr (kAsync) {
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(place(stage, v));
+            if constexpr (kBytes == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(is ? 16 : 0) : "memory");
+            else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(kBytes), "r"(is ? kBytes : 0) : "memory");
+        }
+    }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+    __device__ __forceinline__ R get(int stage, int v, const T* from, bool is) const {
+        if constexpr (kAsync) return *place(stage, v);
+        return is ? *reinterpret_cast<const R*>(from) : V::zero();
+    }
+};
+
 __device__ __forceinline__ int64_t position(const Params& p, int64_t token) {
     return p.pos_bytes == 8 ? reinterpret_cast<const int64_t*>(p.positions)[token]
                             : (int64_t)reinterpret_cast<const int*>(p.positions)[token];
@@ -352,204 +403,219 @@ __device__ __forceinline__ float rstd_of(float squares, const Params& p) {
 
 template <int N>
 constexpr int kUnits = N >= 4 ? 1 : 4 / N;   // of a lane: kMaxDim / 2 / N over 32 lanes
-template <int N>
-constexpr int kHeads = N >= 4 ? FH : 2;      // of a step, forward
-template <int N>
-constexpr int kHeadsBack = N >= 2 ? BH : 1;  // backward
+constexpr int kHeads = 2;                    // of a step, forward (backward 1; more spill, or take as long)
 
 // A group of `lanes` lanes takes HEADS heads of one token at a step.
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(kThreads, FB) k_norm_rope(const __grid_constant__ Params p, int lanes) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rope(const __grid_constant__ Params p, int lanes) {
     using V = Vec<T, N>;
     using R = typename V::type;
-    constexpr int U = kUnits<N>, HEADS = kHeads<N>;
+    constexpr int U = kUnits<N>, HEADS = kHeads;
+    extern __shared__ __align__(16) unsigned char raw[];
+    const Ring<T, N, 2 * U * HEADS> ring{reinterpret_cast<R*>(raw) + threadIdx.x};
     const int lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) / lanes, a_warp = 32 / lanes;
-    grid_wait();
     Place at[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) at[u] = place<N, INTER>(lane + u * lanes, p.dim, p.rot);
-    int item = blockIdx.x * kWarps + (threadIdx.x >> 5);
-    for (int which = 0; which < 2; item -= p.part[which++].items) {
-        const Part& part = p.part[which];
-        if (item >= part.items) continue;
-        for (; item < part.items; item += gridDim.x * kWarps) {
-            const Work w = work_of<HEADS>(p, part, item, group, a_warp);
-            const int64_t pos = position(p, w.token);
-            const bool good = pos >= 0 && pos < p.table_rows;
-            if (w.in && !good && lane == 0) report_device_error(p.err, 8);
-            const T* x = reinterpret_cast<const T*>(part.x) + w.b * part.xs[0] + w.t * part.xs[1] + w.head * part.xs[2];
-            T* y = reinterpret_cast<T*>(part.y) + w.b * part.ys[0] + w.t * part.ys[1] + w.head * part.ys[2];
-            Turn<N, INTER> turn[U];
-            for (int k = 0, left = w.in ? part.heads - w.head : 0; k < part.span; ++k) {
-                R va[U][HEADS], vb[U][HEADS];
-                // (lanes without a head take part in the shuffles)
+    Steps<T, HEADS> ahead, now;
+    ahead.begin(p, group, a_warp);
+    now = ahead;
+    grid_wait();
+    auto fetch = [&](int stage) {
+        if (!ahead.done()) {
+            const int64_t apart = p.part[ahead.which].xs[2];
 #pragma unroll
-                for (int h = 0; h < HEADS; ++h)
+            for (int h = 0; h < HEADS; ++h)
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        va[u][h] = h < left && at[u].a >= 0 ? *reinterpret_cast<const R*>(x + h * part.xs[2] + at[u].a) : V::zero();
-                        vb[u][h] = h < left && at[u].b >= 0 ? *reinterpret_cast<const R*>(x + h * part.xs[2] + at[u].b) : V::zero();
-                    }
-                if (k == 0) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        float wa[N], wb[N];
-                        turn[u].load(p, at[u], good ? pos : 0, false);
-                        load_weight<T, N>(part, at[u].a, wa);
-                        load_weight<T, N>(part, at[u].b, wb);
-                        turn[u].weigh(at[u], wa, wb);
-                    }
+                for (int u = 0; u < U; ++u) {
+                    const bool is = h < ahead.left, ha = is && at[u].a >= 0, hb = is && at[u].b >= 0;
+                    const T* x = ahead.x + (is ? h * apart : 0);
+                    ring.fetch(stage, (h * U + u) * 2, ha ? x + at[u].a : ahead.x, ha);
+                    ring.fetch(stage, (h * U + u) * 2 + 1, hb ? x + at[u].b : ahead.x, hb);
                 }
-                float squares[HEADS];
+            ahead.next(p, group, a_warp);
+        }
+        ring.commit();
+    };
 #pragma unroll
-                for (int h = 0; h < HEADS; ++h) {
-                    float both[2] = {0.f, 0.f};
+    for (int i = 0; i < kStages; ++i) fetch(i);
+    Turn<N, INTER> turn[U];
+    bool good = true;
+    for (int stage = 0; !now.done(); stage = stage + 1 == kStages ? 0 : stage + 1) {
+        const Part& part = p.part[now.which];
+        if (now.k == 0) {
+            const int64_t pos = position(p, now.token);
+            good = pos >= 0 && pos < p.table_rows;
+            if (now.left > 0 && !good && lane == 0) report_device_error(p.err, 8);
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        float f[N];
-                        V::get(va[u][h], f);
-                        dot(both, f, f);
-                        V::get(vb[u][h], f);
-                        dot(both, f, f);
-                    }
-                    squares[h] = both[0] + both[1];
-                }
-                sum_of_group(squares, lanes);
-#pragma unroll
-                for (int h = 0; h < HEADS; ++h) {
-                    if (h >= left) break;
-                    const float rstd = rstd_of(squares[h], p);
-                    T* yh = y + h * part.ys[2];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        float fa[N], fb[N];
-                        V::get(va[u][h], fa);
-                        V::get(vb[u][h], fb);
-                        mul(fa, fa, rstd);
-                        mul(fb, fb, rstd);
-                        turn[u].template apply<false>(at[u], fa, fb);
-                        va[u][h] = V::put(fa), vb[u][h] = V::put(fb);
-                        if (!good) va[u][h] = vb[u][h] = V::zero();
-                        if (at[u].a >= 0) *reinterpret_cast<R*>(yh + at[u].a) = va[u][h];
-                        if (at[u].b >= 0) *reinterpret_cast<R*>(yh + at[u].b) = vb[u][h];
-                    }
-                }
-                const int on = HEADS << part.across;
-                x += on * part.xs[2], y += on * part.ys[2], left -= on;
+            for (int u = 0; u < U; ++u) {
+                float wa[N], wb[N];
+                turn[u].load(p, at[u], good ? pos : 0, false);
+                load_weight<T, N>(part, at[u].a, wa);
+                load_weight<T, N>(part, at[u].b, wb);
+                turn[u].weigh(at[u], wa, wb);
             }
         }
+        ring.wait();
+        R va[U][HEADS], vb[U][HEADS];
+        float squares[HEADS];
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            float both[2] = {0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool is = h < now.left;
+                const T* x = now.x + h * part.xs[2];
+                va[u][h] = ring.get(stage, (h * U + u) * 2, x + at[u].a, is && at[u].a >= 0);
+                vb[u][h] = ring.get(stage, (h * U + u) * 2 + 1, x + at[u].b, is && at[u].b >= 0);
+                float f[N];
+                V::get(va[u][h], f);
+                dot(both, f, f);
+                V::get(vb[u][h], f);
+                dot(both, f, f);
+            }
+            squares[h] = both[0] + both[1];
+        }
+        sum_of_group(squares, lanes);    // (lanes without a head take part)
+#pragma unroll
+        for (int h = 0; h < HEADS; ++h) {
+            if (h >= now.left) break;
+            const float rstd = rstd_of(squares[h], p);
+            T* yh = now.y + h * part.ys[2];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float fa[N], fb[N];
+                V::get(va[u][h], fa);
+                V::get(vb[u][h], fb);
+                mul(fa, fa, rstd);
+                mul(fb, fb, rstd);
+                turn[u].template apply<false>(at[u], fa, fb);
+                va[u][h] = V::put(fa), vb[u][h] = V::put(fb);
+                if (!good) va[u][h] = vb[u][h] = V::zero();
+                if (at[u].a >= 0) *reinterpret_cast<R*>(yh + at[u].a) = va[u][h];
+                if (at[u].b >= 0) *reinterpret_cast<R*>(yh + at[u].b) = vb[u][h];
+            }
+        }
+        fetch(stage);
+        now.next(p, group, a_warp);
     }
 }
 
-// Backward.  The items of q come first, then those of k, so that a lane's sums of the weights' gradients are of one part and are
-// put away when the other begins.  The order of the additions depends on the sizes alone.
+// Backward.  A lane's sums of the weights' gradients are of one part, and are put away when the other begins.  The order of the
+// additions depends on the sizes alone.
 template <typename T, int N, bool INTER>
-__global__ void __launch_bounds__(kThreads, BB) k_norm_rope_backward(const __grid_constant__ Params p, int lanes) {
+__global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rope_backward(const __grid_constant__ Params p, int lanes) {
     using V = Vec<T, N>;
     using R = typename V::type;
-    constexpr int U = kUnits<N>, HEADS = kHeadsBack<N>;
-    extern __shared__ float sums[];   // [2, kWarps, dim]
+    constexpr int U = kUnits<N>;
+    extern __shared__ __align__(16) unsigned char raw[];
+    float* sums = reinterpret_cast<float*>(raw);   // [2, kWarps, dim], when there are weights
+    const Ring<T, N, 4 * U> ring{reinterpret_cast<R*>(raw + (p.partial ? 2 * kWarps * kMaxDim * sizeof(float) : 0)) + threadIdx.x};
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) / lanes, a_warp = 32 / lanes;
     for (int k = threadIdx.x; p.partial && k < 2 * kWarps * p.dim; k += kThreads) sums[k] = 0.f;
     __syncthreads();
-    grid_wait();
     Place at[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) at[u] = place<N, INTER>(lane + u * lanes, p.dim, p.rot);
-    int item = blockIdx.x * kWarps + warp;
-    for (int which = 0; which < 2; item -= p.part[which++].items) {
-        const Part& part = p.part[which];
-        if (item >= part.items) continue;
-        float wa[U][N], wb[U][N], da[U][N], db[U][N];
+    Steps<T, 1> ahead, now;
+    ahead.begin(p, group, a_warp);
+    now = ahead;
+    grid_wait();
+    auto fetch = [&](int stage) {
+        if (!ahead.done()) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool ha = ahead.left > 0 && at[u].a >= 0, hb = ahead.left > 0 && at[u].b >= 0;
+                ring.fetch(stage, u * 4, ha ? ahead.x + at[u].a : ahead.x, ha);
+                ring.fetch(stage, u * 4 + 1, hb ? ahead.x + at[u].b : ahead.x, hb);
+                ring.fetch(stage, u * 4 + 2, ha ? ahead.g + at[u].a : ahead.g, ha);
+                ring.fetch(stage, u * 4 + 3, hb ? ahead.g + at[u].b : ahead.g, hb);
+            }
+            ahead.next(p, group, a_warp);
+        }
+        ring.commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kStages; ++i) fetch(i);
+    Turn<N, INTER> turn[U];
+    bool good = true;
+    float wa[U][N], wb[U][N], da[U][N], db[U][N];
+    for (int stage = 0, which = -1; ; stage = stage + 1 == kStages ? 0 : stage + 1) {
+        if (now.which != which) {
+            if (which >= 0 && p.partial) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        for (int o = lanes; o < 32; o <<= 1) {
+                            da[u][j] += __shfl_xor_sync(0xffffffffu, da[u][j], o);
+                            db[u][j] += __shfl_xor_sync(0xffffffffu, db[u][j], o);
+                        }
+                        float* to = sums + (which * kWarps + warp) * p.dim;
+                        if (group == 0 && at[u].a >= 0) to[at[u].a + j] = da[u][j];
+                        if (group == 0 && at[u].b >= 0) to[at[u].b + j] = db[u][j];
+                    }
+            }
+            if (now.done()) break;
+            which = now.which;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                load_weight<T, N>(p.part[which], at[u].a, wa[u]);
+                load_weight<T, N>(p.part[which], at[u].b, wb[u]);
+#pragma unroll
+                for (int j = 0; j < N; ++j) da[u][j] = db[u][j] = 0.f;
+            }
+        }
+        if (now.k == 0) {
+            const int64_t pos = position(p, now.token);
+            good = pos >= 0 && pos < p.table_rows;
+            if (now.left > 0 && !good && lane == 0) report_device_error(p.err, 8);
+#pragma unroll
+            for (int u = 0; u < U; ++u) turn[u].load(p, at[u], good ? pos : 0, true);
+        }
+        ring.wait();
+        R xa[U], xb[U];
+        float squares[2] = {0.f, 0.f}, dots[2] = {0.f, 0.f};     // sums of squares and of w d x
+        float ea[U][N], eb[U][N];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            load_weight<T, N>(part, at[u].a, wa[u]);
-            load_weight<T, N>(part, at[u].b, wb[u]);
-#pragma unroll
-            for (int j = 0; j < N; ++j) da[u][j] = db[u][j] = 0.f;
+            const bool ha = now.left > 0 && at[u].a >= 0, hb = now.left > 0 && at[u].b >= 0;
+            float f[N], wd[N];
+            xa[u] = ring.get(stage, u * 4, now.x + at[u].a, ha), xb[u] = ring.get(stage, u * 4 + 1, now.x + at[u].b, hb);
+            V::get(ring.get(stage, u * 4 + 2, now.g + at[u].a, ha), ea[u]);
+            V::get(ring.get(stage, u * 4 + 3, now.g + at[u].b, hb), eb[u]);
+            turn[u].template apply<true>(at[u], ea[u], eb[u]);
+            V::get(xa[u], f);
+            dot(squares, f, f);
+            mul(wd, ea[u], wa[u]);
+            dot(dots, wd, f);
+            V::get(xb[u], f);
+            dot(squares, f, f);
+            mul(wd, eb[u], wb[u]);
+            dot(dots, wd, f);
         }
-        for (; item < part.items; item += gridDim.x * kWarps) {
-            const Work w = work_of<HEADS>(p, part, item, group, a_warp);
-            const int64_t pos = position(p, w.token);
-            const bool good = pos >= 0 && pos < p.table_rows;
-            if (w.in && !good && lane == 0) report_device_error(p.err, 8);
-            const T* x = reinterpret_cast<const T*>(part.x) + w.b * part.xs[0] + w.t * part.xs[1] + w.head * part.xs[2];
-            const T* gy = reinterpret_cast<const T*>(part.g) + w.b * part.gs[0] + w.t * part.gs[1] + w.head * part.gs[2];
-            T* dx = reinterpret_cast<T*>(part.y) + w.b * part.ys[0] + w.t * part.ys[1] + w.head * part.ys[2];
-            Turn<N, INTER> turn[U];
-            for (int k = 0, left = w.in ? part.heads - w.head : 0; k < part.span; ++k) {
-                R xa[U][HEADS], xb[U][HEADS], ga[U][HEADS], gb[U][HEADS];
+        float sum[2] = {squares[0] + squares[1], dots[0] + dots[1]};
+        sum_of_group(sum, lanes);
+        if (now.left > 0) {
+            const float r = rstd_of(sum[0], p), mean = -(sum[1] * r) * p.per_dim;   // of w d times the unit row, negative
+            auto half = [&](const R& v, float (&e)[N], const float (&w)[N], float (&d)[N], int to) {
+                float n[N];
+                V::get(v, n);
+                mul(n, n, r);
+                if (good) fma(d, e, n, d);
+                mul(e, e, w);
+                fma(e, n, mean, e);
+                mul(e, e, r);
+                if (to >= 0) *reinterpret_cast<R*>(now.y + to) = good ? V::put(e) : V::zero();
+            };
 #pragma unroll
-                for (int h = 0; h < HEADS; ++h)
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const bool ha = h < left && at[u].a >= 0, hb = h < left && at[u].b >= 0;
-                        xa[u][h] = ha ? *reinterpret_cast<const R*>(x + h * part.xs[2] + at[u].a) : V::zero();
-                        xb[u][h] = hb ? *reinterpret_cast<const R*>(x + h * part.xs[2] + at[u].b) : V::zero();
-                        ga[u][h] = ha ? *reinterpret_cast<const R*>(gy + h * part.gs[2] + at[u].a) : V::zero();
-                        gb[u][h] = hb ? *reinterpret_cast<const R*>(gy + h * part.gs[2] + at[u].b) : V::zero();
-                    }
-                if (k == 0) {
-#pragma unroll
-                    for (int u = 0; u < U; ++u) turn[u].load(p, at[u], good ? pos : 0, true);
-                }
-#pragma unroll
-                for (int h = 0; h < HEADS; ++h) {
-                    float squares[2] = {0.f, 0.f}, dots[2] = {0.f, 0.f};     // sums of squares and of w d x
-                    float ea[U][N], eb[U][N];
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        float f[N], wd[N];
-                        V::get(ga[u][h], ea[u]);
-                        V::get(gb[u][h], eb[u]);
-                        turn[u].template apply<true>(at[u], ea[u], eb[u]);
-                        V::get(xa[u][h], f);
-                        dot(squares, f, f);
-                        mul(wd, ea[u], wa[u]);
-                        dot(dots, wd, f);
-                        V::get(xb[u][h], f);
-                        dot(squares, f, f);
-                        mul(wd, eb[u], wb[u]);
-                        dot(dots, wd, f);
-                    }
-                    float sum[2] = {squares[0] + squares[1], dots[0] + dots[1]};
-                    sum_of_group(sum, lanes);
-                    if (h >= left) continue;   // (not further on: the others' shuffles take all lanes)
-                    const float r = rstd_of(sum[0], p), mean = -(sum[1] * r) * p.per_dim;   // of w d times the unit row, negative
-                    T* dh = dx + h * part.ys[2];
-                    auto half = [&](const R& v, float (&e)[N], const float (&w)[N], float (&d)[N], int to) {
-                        float n[N];
-                        V::get(v, n);
-                        mul(n, n, r);
-                        if (good) fma(d, e, n, d);
-                        mul(e, e, w);
-                        fma(e, n, mean, e);
-                        mul(e, e, r);
-                        if (to >= 0) *reinterpret_cast<R*>(dh + to) = good ? V::put(e) : V::zero();
-                    };
-#pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        half(xa[u][h], ea[u], wa[u], da[u], at[u].a);
-                        half(xb[u][h], eb[u], wb[u], db[u], at[u].b);
-                    }
-                }
-                const int on = HEADS << part.across;
-                x += on * part.xs[2], gy += on * part.gs[2], dx += on * part.ys[2], left -= on;
+            for (int u = 0; u < U; ++u) {
+                half(xa[u], ea[u], wa[u], da[u], at[u].a);
+                half(xb[u], eb[u], wb[u], db[u], at[u].b);
             }
         }
-        if (!p.partial) continue;
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < N; ++j) {
-                for (int o = lanes; o < 32; o <<= 1) {
-                    da[u][j] += __shfl_xor_sync(0xffffffffu, da[u][j], o);
-                    db[u][j] += __shfl_xor_sync(0xffffffffu, db[u][j], o);
-                }
-                float* to = sums + (which * kWarps + warp) * p.dim;
-                if (group == 0 && at[u].a >= 0) to[at[u].a + j] = da[u][j];
-                if (group == 0 && at[u].b >= 0) to[at[u].b + j] = db[u][j];
-            }
+        fetch(stage);
+        now.next(p, group, a_warp);
     }
     if (!p.partial) return;
     __syncthreads();
@@ -587,9 +653,13 @@ __global__ void __launch_bounds__(256) k_norm_weights(const float* partial, int 
 
 template <typename T, int N, bool INTER>
 cudaError_t launch(const Params& p, int lanes, bool backward, int grid, cudaStream_t s) {
-    if (!backward) return launch_overlapped(k_norm_rope<T, N, INTER>, grid, kThreads, 0, s, p, lanes);
-    return launch_overlapped(k_norm_rope_backward<T, N, INTER>, grid, kThreads, p.partial ? 2 * kWarps * p.dim * sizeof(float) : 0, s,
-                             p, lanes);
+    auto go = [&](void (*kernel)(const Params, int), int vectors, size_t more) {
+        const size_t smem = (N * sizeof(T) >= 4 ? (size_t)kStages * vectors * kThreads * N * sizeof(T) : 0) + more;
+        const cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+        return e != cudaSuccess ? e : launch_overlapped(kernel, dim3(grid), dim3(kThreads), smem, s, p, lanes);
+    };
+    if (!backward) return go(k_norm_rope<T, N, INTER>, 2 * kUnits<N> * kHeads, 0);
+    return go(k_norm_rope_backward<T, N, INTER>, 4 * kUnits<N>, p.partial ? 2 * kWarps * kMaxDim * sizeof(float) : 0);
 }
 template <typename T, int N>
 cudaError_t launch(const Params& p, int lanes, bool inter, bool backward, int grid, cudaStream_t s) {
@@ -609,6 +679,37 @@ cudaError_t launch(const Params& p, int vec, int lanes, bool inter, bool backwar
 int sm_count() {
     int dev = 0;
     return cudaGetDevice(&dev) == cudaSuccess ? tc::sm_count_cached(dev) : 0;
+}
+
+// Divides the tokens and their heads into items of at most `most` steps each, for groups of lanes that take `step` heads a step;
+// most is what costs least: a warp's share of all steps, each item's angles counting as one more, and at the end half an item that
+// some warps have and others have not.  (Measured with 1 / 4 / 16 steps at most: 8 x 4096
+// tokens 561 / 342 / 325 us, 2048 tokens 16.4 / 13.5 / 21.7 us, 16 tokens 3.9 / 5.9 / 13.7 us.)  Returns the number
+// of items.
+int64_t split(Params& p, int groups, int step, int64_t warps) {
+    double least = 0;
+    int64_t items = 0;
+    Params best = p;
+    for (int most = 1; most <= 32; most *= 2) {
+        double work = 0, longest = 0;
+        int64_t all = 0;
+        for (Part& t : p.part) {
+            if (t.heads == 0) continue;
+            const int steps = (t.heads + step - 1) / step;
+            t.across = 0;
+            while ((1 << t.across) < groups && (steps + (1 << t.across) - 1) >> t.across > most) ++t.across;
+            const int each = (steps + (1 << t.across) - 1) >> t.across, side = groups >> t.across;
+            t.chunks = (each + most - 1) / most;
+            t.span = (each + t.chunks - 1) / t.chunks;
+            const int64_t n = (int64_t)((p.n_tokens + side - 1) / side) * t.chunks;
+            t.items = (int)std::min<int64_t>(n, 1 << 30);
+            all += n, work += (double)n * (t.span + 1), longest = std::max(longest, t.span + 1.0);
+        }
+        const double time = all <= warps ? longest : work / warps + longest / 2;
+        if (most == 1 || time < least) least = time, best = p, items = all;
+    }
+    p = best;
+    return items;
 }
 
 int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace_bytes, int* err, cudaStream_t s, const char* name) {
@@ -685,23 +786,11 @@ int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace
     const int units = units_of(p.dim, p.rot, vec, inter);
     int lanes = 1;
     while (lanes < units && lanes < 32) lanes *= 2;
-    const int blocks = (backward ? BB : FB) * sm_count();
+    const int blocks = kBlocks * sm_count();
     SPARK_REQUIRE(blocks > 0, SPARK_ERR_DEVICE, "%s: no device", name);
-    const int step = backward ? (vec >= 2 ? BH : 1) : (vec >= 4 ? FH : 2);
-    int64_t items = 0;
-    for (Part& t : p.part) {
-        if (t.heads == 0) continue;
-        const int steps = (t.heads + step - 1) / step;     // of one group of lanes for a token's heads
-        while ((1 << t.across) < 32 / lanes && (1 << t.across) < steps) ++t.across;
-        const int64_t tiles = (p.n_tokens + (32 / lanes >> t.across) - 1) / (32 / lanes >> t.across);
-        const int all = (steps + (1 << t.across) - 1) >> t.across;
-        // as few items for a token as keep all warps at work, twice
-        t.chunks = (int)std::min<int64_t>(all, std::max<int64_t>(1, 2 * (int64_t)blocks * kWarps / tiles));
-        t.span = (all + t.chunks - 1) / t.chunks;
-        SPARK_REQUIRE(tiles * t.chunks < (1ll << 30), SPARK_ERR_UNSUPPORTED, "%s: too many values for one call", name);
-        t.items = (int)(tiles * t.chunks);
-        items += t.items;
-    }
+    const int step = backward ? 1 : kHeads;
+    const int64_t items = split(p, 32 / lanes, step, (int64_t)blocks * kWarps);
+    SPARK_REQUIRE(items < (1ll << 30), SPARK_ERR_UNSUPPORTED, "%s: too many values for one call", name);
     const int64_t grid = std::min<int64_t>((items + kWarps - 1) / kWarps, blocks);
     if (backward && weights) {
         const size_t need = (size_t)blocks * 2 * p.dim * sizeof(float);
@@ -732,7 +821,7 @@ int spark_qk_norm_rope(const SparkNormRope* a, int* err, void* stream) {
 }
 
 size_t spark_qk_norm_rope_backward_workspace_size(int64_t head_dim) {
-    return head_dim > 0 ? (size_t)BB * spark::nr::sm_count() * 2 * head_dim * sizeof(float) : 0;
+    return head_dim > 0 ? (size_t)spark::nr::kBlocks * spark::nr::sm_count() * 2 * head_dim * sizeof(float) : 0;
 }
 
 int spark_qk_norm_rope_backward(const SparkNormRope* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
