@@ -47,7 +47,6 @@ struct Params {
     int rank, repeat;            // tokens of an entry of `adapter`
     int splits, slots;           // of the input's columns; of a tile's items, worked on side by side
     int rank_blocks, columns;    // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y
-    int a_time;                  // second product: column blocks of a CTA
     int wide_y;                  // rows of y and out on 16 bytes
     float* h;                    // [splits, tokens, rank]
     int* err;
@@ -63,6 +62,7 @@ struct Mma<__nv_bfloat16> {
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ void round2(__nv_bfloat16* to, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b); }
 };
 template <>
 struct Mma<__half> {
@@ -72,25 +72,53 @@ struct Mma<__half> {
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ void round2(__half* to, float a, float b) { *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b); }
 };
 
-// Values k..k + 7 of a row of n, zeros behind its end; VEC: rows on 16 bytes, n a multiple of 8.
+// A matrix's first value and what comes behind its last.
+template <typename T>
+struct Span {
+    const T *begin, *end;
+};
+// Values k..k + 7 of a row of n, zeros behind its end; VEC: rows on 16 bytes, n a multiple of 8.  Else out of the two 16-byte
+// vectors that they are in, where these are within the matrix.
 template <typename T, bool VEC>
-__device__ __forceinline__ uint4 load8(const T* row, int64_t k, int64_t n) {
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if constexpr (VEC) {
-        if (k < n) v = *reinterpret_cast<const uint4*>(row + k);
+__device__ __forceinline__ uint4 load8(const T* row, int64_t k, int64_t n, const Span<T>& all) {
+    if (k >= n) return make_uint4(0, 0, 0, 0);
+    if constexpr (VEC) return *reinterpret_cast<const uint4*>(row + k);
+    uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + k), from = at & ~uintptr_t(15);
+    const int off = (int)(at - from) / 2;
+    if (from >= reinterpret_cast<uintptr_t>(all.begin) && from + (off ? 32 : 16) <= reinterpret_cast<uintptr_t>(all.end)) {
+        const uint4 a = *reinterpret_cast<const uint4*>(from);
+        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        if (off) {
+            const uint4 b = *reinterpret_cast<const uint4*>(from + 16);
+            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        }
+        if (off & 4) {
+#pragma unroll
+            for (int j = 0; j < 6; ++j) w[j] = w[j + 2];
+        }
+        if (off & 2) {
+#pragma unroll
+            for (int j = 0; j < 5; ++j) w[j] = w[j + 1];
+        }
+        if (off & 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] &= k + 2 * j >= n ? 0u : k + 2 * j + 1 >= n ? 0xffffu : 0xffffffffu;
     } else {
         const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
-        uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t lo = k + 2 * j < n ? p[k + 2 * j] : 0, hi = k + 2 * j + 1 < n ? p[k + 2 * j + 1] : 0;
             w[j] = lo | hi << 16;
         }
-        v = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    return v;
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // A tile's adapters: ids[row] (-1: none, or no such token), and the distinct ones in order of their first rows.
@@ -99,40 +127,31 @@ struct Tile {
     int ids[ROWS];
     int distinct[ROWS];
     int count;
-    unsigned first[2];
 };
 template <int ROWS>
 __device__ __forceinline__ void load_tile(Tile<ROWS>& s, const Params& p, int64_t t0, bool report) {
+    static_assert(ROWS <= 32, "a lane has a row");
     const int i = threadIdx.x;
-    if (i < ROWS) {
-        int id = t0 + i < p.tokens ? p.adapter[(t0 + i) / p.repeat] : -1;
+    if (i < 32) {
+        const bool is = i < ROWS && t0 + i < p.tokens;
+        int id = is ? p.adapter[p.repeat == 1 ? t0 + i : (t0 + i) / p.repeat] : -1;
         if (id >= p.adapters) {
             if (report) report_device_error(p.err, 12);
             id = -1;
         }
-        s.ids[i] = id < 0 ? -1 : id;
-    }
-    if (i == 0) s.count = 0;
-    __syncthreads();
-    if (i < (ROWS + 31) / 32 * 32) {
-        bool lead = i < ROWS && t0 + i < p.tokens;
-        for (int j = 0; j < i && lead; ++j) lead = s.ids[j] != s.ids[i];
-        const unsigned leads = __ballot_sync(0xffffffffu, lead);
-        if ((i & 31) == 0) s.first[i >> 5] = leads;
-    }
-    __syncthreads();
-    if (i < ROWS) {
-        const unsigned mine = s.first[i >> 5];
-        const int before = (i >= 32 ? __popc(s.first[0]) : 0) + __popc(mine & ((1u << (i & 31)) - 1));
-        if (mine >> (i & 31) & 1) s.distinct[before] = s.ids[i];
-        if (i == ROWS - 1) s.count = before + (int)(mine >> (i & 31) & 1);
+        if (id < 0) id = -1;
+        const unsigned same = __match_any_sync(0xffffffffu, is ? id : -2);
+        const unsigned leads = __ballot_sync(0xffffffffu, is && __ffs(same) - 1 == i);
+        if (i < ROWS) s.ids[i] = id;
+        if (leads >> i & 1) s.distinct[__popc(leads & ((1u << i) - 1))] = id;
+        if (i == 0) s.count = __popc(leads);
     }
     __syncthreads();
 }
 
 // h[split, t, :] = A[a] x[t] over the split's columns.  The warps of a CTA take chunks of 32 columns in turn.
 template <typename T, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_lora_down(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(const __grid_constant__ Params p) {
     constexpr int ROWS = 16 * MT, RANKS = 8 * NT;
     __shared__ Tile<ROWS> s;
     extern __shared__ float part[];   // [kWarps, ROWS, RANKS]
@@ -155,28 +174,53 @@ __global__ void __launch_bounds__(kThreads) k_lora_down(const __grid_constant__ 
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
-#pragma unroll 2
-        for (int64_t k = ((int64_t)split * kWarps + warp) * 32 + 8 * t; k - 8 * t < p.ic; k += (int64_t)p.splits * kWarps * 32) {
+        const Span<T> ax{reinterpret_cast<const T*>(p.a), reinterpret_cast<const T*>(p.a) + p.adapters * p.rank * p.ic};
+        const Span<T> xx{x, x + (p.tokens - 1) * p.ldx + p.ic};
+        struct Part {
             uint4 u[MT][2], w[NT];
+        };
+        auto load = [&](Part& q, int64_t k) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int64_t row = t0 + m * 16 + e * 8 + g;
-                    u[m][e] = load8<T, VEC>(x + (row < p.tokens ? row : 0) * p.ldx, k, row < p.tokens ? p.ic : 0);
+                    q.u[m][e] = load8<T, VEC>(x + (row < p.tokens ? row : 0) * p.ldx, k, row < p.tokens ? p.ic : 0, xx);
                 }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int r = r0 + n * 8 + g;
-                w[n] = load8<T, VEC>(a + (int64_t)(r < p.rank ? r : 0) * p.ic, k, r < p.rank ? p.ic : 0);
+                q.w[n] = load8<T, VEC>(a + (int64_t)(r < p.rank ? r : 0) * p.ic, k, r < p.rank ? p.ic : 0, ax);
             }
+        };
+        auto products = [&](const Part& q) {
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    Mma<T>::run(acc[m][n], u[m][0].x, u[m][1].x, u[m][0].y, u[m][1].y, w[n].x, w[n].y);
-                    Mma<T>::run(acc[m][n], u[m][0].z, u[m][1].z, u[m][0].w, u[m][1].w, w[n].z, w[n].w);
+                    Mma<T>::run(acc[m][n], q.u[m][0].x, q.u[m][1].x, q.u[m][0].y, q.u[m][1].y, q.w[n].x, q.w[n].y);
+                    Mma<T>::run(acc[m][n], q.u[m][0].z, q.u[m][1].z, q.u[m][0].w, q.u[m][1].w, q.w[n].z, q.w[n].w);
                 }
+        };
+        // (zeros behind the end: the loop may run one part further)
+        const int64_t step = (int64_t)p.splits * kWarps * 32;
+        int64_t k = ((int64_t)split * kWarps + warp) * 32 + 8 * t;
+        if constexpr (MT * NT <= 4) {
+            Part q0, q1;
+            load(q0, k);
+            for (; k - 8 * t < p.ic; k += 2 * step) {
+                load(q1, k + step);
+                products(q0);
+                load(q0, k + 2 * step);
+                products(q1);
+            }
+        } else {
+            Part q;
+#pragma unroll 2
+            for (; k - 8 * t < p.ic; k += step) {
+                load(q, k);
+                products(q);
+            }
         }
         float* mine = part + warp * ROWS * RANKS;
 #pragma unroll
@@ -228,7 +272,7 @@ struct Eight {
     static __device__ __forceinline__ void store(Y* p, const float* f) {
         Eight e;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e.v[j] = Mma<Y>::round(f[j]);
+        for (int j = 0; j < 8; j += 2) Mma<Y>::round2(e.v + j, f[j], f[j + 1]);
         *reinterpret_cast<uint4*>(p) = e.raw;
     }
 };
@@ -236,80 +280,139 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 template <typename Y>
 __device__ __forceinline__ void put(Y* p, float v) { *p = Mma<Y>::round(v); }
 
-// out[t, :] = y[t, :] + scale B[a] h[t].  A warp has kColumns columns at a time.
+// out[t, :] = y[t, :] + scale B[a] h[t].  A CTA has a run of column blocks (kColumns for each warp), most often of one tile, and of the
+// tile every slots-th adapter with its rows.  Where these are more than one, a product has zeros in place of the others' rows, and
+// y is read and written once for all.
 template <typename T, typename Y, int MT, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_lora_up(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__ Params p) {
     constexpr int ROWS = 16 * MT, TERMS = sizeof(Y) == 4 ? 3 : 2;
+    constexpr bool kScaled = std::is_same<T, __half>::value;
     __shared__ Tile<ROWS> s;
     __shared__ float row_scale[ROWS];
+    __shared__ int mine_ids[ROWS];
     extern __shared__ __align__(16) unsigned char raw[];
-    T* terms = reinterpret_cast<T*>(raw);   // [TERMS, ROWS, width]
     asm volatile("griddepcontrol.launch_dependents;");
-    const int chunks = (p.rank + 31) / 32, width = chunks * 32 + 8;
+    const int chunks = (p.rank + 31) / 32, ranks = chunks * 32, width = ranks + 8;
+    T* terms = reinterpret_cast<T*>(raw);                                             // [TERMS, ROWS, width]
+    float* sums = reinterpret_cast<float*>(raw + (size_t)TERMS * ROWS * width * sizeof(T));   // [ROWS, ranks], where rows are scaled
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int per_tile = (p.columns + p.a_time - 1) / p.a_time;
-    const int64_t t0 = (int64_t)(blockIdx.x / per_tile) * ROWS;
-    const int c0 = (int)(blockIdx.x % per_tile) * p.a_time, c1 = min(c0 + p.a_time, p.columns), slot = blockIdx.y;
-    // (what was ready before the first product may be read before it ends)
-    load_tile(s, p, t0, false);
-    if (slot >= s.count) return;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (int row = warp; row < ROWS; row += kWarps) {
-        const bool is = s.ids[row] >= 0;
-        float v[kMaxRank / 32], most = 0.f;
-#pragma unroll
-        for (int c = 0; c < kMaxRank / 32; ++c) {
-            const int r = c * 32 + lane;
-            v[c] = 0.f;
-            if (c < chunks && is && r < p.rank)
-                for (int k = 0; k < p.splits; ++k) v[c] += p.h[((int64_t)k * p.tokens + t0 + row) * p.rank + r];
-            most = fmaxf(most, fabsf(v[c]));
-        }
-        float up = 1.f, down = 1.f;
-        if constexpr (std::is_same<T, __half>::value) {
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            // (zeros and infinities stay what they are)
-            if (most > 0.f && most < INFINITY) {
-                const int e = min(max(14 - ilogbf(most), -100), 100);
-                up = ldexpf(1.f, e), down = ldexpf(1.f, -e);
-            }
-        }
-        const float scale = is ? (p.scale ? p.scale[s.ids[row]] : p.scale_all) : 0.f;
-        if (lane == 0) row_scale[row] = down * scale;
-#pragma unroll
-        for (int c = 0; c < kMaxRank / 32; ++c) {
-            if (c >= chunks) break;
-            float rest = v[c] * up;
-#pragma unroll
-            for (int k = 0; k < TERMS; ++k) {
-                const T q = Mma<T>::round(rest);
-                terms[(k * ROWS + row) * width + c * 32 + lane] = q;
-                const float f = (float)q;
-                rest = fabsf(f) < INFINITY ? rest - f : 0.f;
-            }
-        }
-    }
-    __syncthreads();
     const Y* y = reinterpret_cast<const Y*>(p.y);
     Y* out = reinterpret_cast<Y*>(p.out);
-    for (int d = slot; d < s.count; d += p.slots) {
-        const int id = s.distinct[d];
-        if (id < 0 && p.y == p.out) continue;
-        const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)max(id, 0) * p.oc * p.rank;
-        for (int c = c0; c < c1; ++c) {
-            const int64_t o0 = ((int64_t)c * kWarps + warp) * kColumns;
-            if (o0 >= p.oc) break;
-            const int64_t mine = o0 + 8 * t;                 // this lane's columns
-            const bool whole = p.wide_y && mine + 8 <= p.oc;
-            Eight<Y> old[MT][2];
+    const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
+    const int64_t blocks = (p.tokens + ROWS - 1) / ROWS * p.columns;
+    const int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
+    bool waited = false;
+    for (int64_t at = lo; at < hi;) {
+        const int64_t tile = at / p.columns, t0 = tile * ROWS;
+        const int c0 = (int)(at - tile * p.columns), n_c = (int)min((int64_t)(p.columns - c0), hi - at);
+        at += n_c;
+        __syncthreads();      // (the last tile is done with)
+        load_tile(s, p, t0, false);
+        // this slot's adapters, and a lane's rows (g, g + 8, ...) with one of them (or none, which is copied)
+        const int slot = blockIdx.y;
+        unsigned rows = 0;
+        int n_ids = 0;
+        for (int d = slot; d < s.count; d += p.slots) {
+            const int id = s.distinct[d];
+            if (id < 0 && p.y == p.out) continue;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int i = 0; i < 2 * MT; ++i) rows |= t0 + i * 8 + g < p.tokens && s.ids[i * 8 + g] == id ? 1u << i : 0u;
+            if (id < 0) continue;
+            if (threadIdx.x == 0) mine_ids[n_ids] = id;
+            ++n_ids;
+        }
+        const bool any = __syncthreads_or(rows != 0);
+        const int steps = n_ids * chunks;       // of a column block: an adapter's 32 ranks each
+        const Y* y_row = y + (t0 + g) * p.ldy + 8 * t;
+        Y* out_row = out + (t0 + g) * p.ldo + 8 * t;
+        auto load_old = [&](Eight<Y> (&old)[MT][2], int c) {
+            const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
+            if (c >= n_c || !p.wide_y || o0 + 8 * t + 8 > p.oc) return;
+            const Y* from = y_row + o0;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = m * 16 + e * 8 + g;
-                    if (whole && t0 + row < p.tokens && s.ids[row] == id) old[m][e].load(y + (t0 + row) * p.ldy + mine);
+            for (int i = 0; i < 2 * MT; ++i, from += 8 * p.ldy)
+                if (rows >> i & 1) old[i / 2][i % 2].load(from);
+        };
+        // step j of block c; behind the last step comes the next block's first
+        auto load_weights = [&](uint4 (&w)[4], int c, int j) {
+            if (j >= steps) ++c, j = 0;
+            if (c >= n_c || steps == 0) return;
+            const int id = mine_ids[chunks == 1 ? j : j / chunks], k = chunks == 1 ? 0 : j % chunks;
+            const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
+            // column n of a step is one of lane g / 2's eight
+            const int64_t o = o0 + 8 * (g >> 1) + (g & 1);
+            const T* from = bb.begin + ((int64_t)id * p.oc + o) * p.rank;
+            if (o0 + kColumns <= p.oc) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n, from += 2 * p.rank) w[n] = load8<T, VEC>(from, k * 32 + 8 * t, p.rank, bb);
+            } else {
+#pragma unroll
+                for (int n = 0; n < 4; ++n, from += 2 * p.rank)
+                    w[n] = o + 2 * n < p.oc ? load8<T, VEC>(from, k * 32 + 8 * t, p.rank, bb) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        Eight<Y> old_a[MT][2], old_b[MT][2];
+        uint4 w[4], w2[4];
+        load_old(old_a, 0);
+        load_weights(w, 0, 0);
+        if (!waited) {
+            // (what was ready before the first product could be read before it ends)
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+        }
+        if (!any) continue;
+        // h of the rows, summed over the splits
+        for (int i = threadIdx.x; i < ROWS * ranks; i += kThreads) {
+            const int row = i / ranks, r = i - row * ranks;
+            float v = 0.f;
+            if (s.ids[row] >= 0 && r < p.rank) {
+                const float* h = p.h + (t0 + row) * p.rank + r;
+                const int64_t apart = p.tokens * p.rank;
+#pragma unroll 4
+                for (int k = 0; k < p.splits; ++k) v += h[k * apart];
+            }
+            if constexpr (kScaled) {
+                sums[i] = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < TERMS; ++k) {
+                    const T q = Mma<T>::round(v);
+                    terms[(k * ROWS + row) * width + r] = q;
+                    const float f = (float)q;
+                    v = fabsf(f) < INFINITY ? v - f : 0.f;
                 }
+            }
+        }
+        if (threadIdx.x < ROWS) {
+            const int id = s.ids[threadIdx.x];
+            row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
+        }
+        __syncthreads();
+        if constexpr (kScaled) {
+            for (int row = warp; row < ROWS; row += kWarps) {
+                float most = 0.f;
+                for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(sums[row * ranks + r]));
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                // (zeros and infinities stay what they are)
+                const int e = most > 0.f && most < INFINITY ? min(max(14 - ilogbf(most), -100), 100) : 0;
+                const float up = ldexpf(1.f, e);
+                if (lane == 0) row_scale[row] *= ldexpf(1.f, -e);
+                for (int r = lane; r < ranks; r += 32) {
+                    float v = sums[row * ranks + r] * up;
+#pragma unroll
+                    for (int k = 0; k < TERMS; ++k) {
+                        const T q = Mma<T>::round(v);
+                        terms[(k * ROWS + row) * width + r] = q;
+                        const float f = (float)q;
+                        v = fabsf(f) < INFINITY ? v - f : 0.f;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        auto work = [&](int c, Eight<Y> (&old)[MT][2], Eight<Y> (&coming)[MT][2]) {
+            load_old(coming, c + 1);
             float acc[MT][4][4];
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -317,49 +420,69 @@ __global__ void __launch_bounds__(kThreads) k_lora_up(const __grid_constant__ Pa
                 for (int n = 0; n < 4; ++n)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
-            if (id >= 0) {
-                for (int k = 0; k < chunks; ++k) {
-                    uint4 w[4];
+            auto products = [&](const uint4 (&w)[4], int j) {
+                const T* a = terms + g * width + (chunks == 1 ? 0 : j % chunks) * 32 + 8 * t;
+                const int id = mine_ids[chunks == 1 ? j : j / chunks];
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        // column n of a step is one of lane g / 2's eight
-                        const int64_t o = o0 + 8 * (g >> 1) + 2 * n + (g & 1);
-                        w[n] = load8<T, VEC>(b + (o < p.oc ? o : 0) * p.rank, k * 32 + 8 * t, o < p.oc ? p.rank : 0);
-                    }
+                for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-                    for (int q = 0; q < TERMS; ++q)
-#pragma unroll
-                        for (int m = 0; m < MT; ++m) {
-                            const T* at = terms + (q * ROWS + m * 16 + g) * width + k * 32 + 8 * t;
-                            const uint4 lo = *reinterpret_cast<const uint4*>(at), hi = *reinterpret_cast<const uint4*>(at + 8 * width);
-#pragma unroll
-                            for (int n = 0; n < 4; ++n) {
-                                Mma<T>::run(acc[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
-                                Mma<T>::run(acc[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
-                            }
+                    for (int m = 0; m < MT; ++m, a += 16 * width) {
+                        uint4 lo = *reinterpret_cast<const uint4*>(a), hi = *reinterpret_cast<const uint4*>(a + 8 * width);
+                        if (n_ids > 1) {
+                            if (s.ids[m * 16 + g] != id) lo = make_uint4(0, 0, 0, 0);
+                            if (s.ids[m * 16 + 8 + g] != id) hi = make_uint4(0, 0, 0, 0);
                         }
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            Mma<T>::run(acc[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
+                            Mma<T>::run(acc[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
+                        }
+                    }
+            };
+            // the next step's weights come during this one's products (MT = 2 has no registers for that: during what follows them)
+            if constexpr (MT == 1) {
+                for (int j = 0; j < steps; j += 2) {
+                    load_weights(w2, c, j + 1);
+                    products(w, j);
+                    if (j + 1 == steps) {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) w[n] = w2[n];
+                        break;
+                    }
+                    load_weights(w, c, j + 2);
+                    products(w2, j + 1);
+                }
+            } else {
+                for (int j = 0; j < steps; ++j) {
+                    products(w, j);
+                    load_weights(w, c, j + 1);
                 }
             }
+            const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
+            const bool whole = p.wide_y && o0 + 8 * t + 8 <= p.oc;
+            Y* to = out_row + o0;
+            const Y* from = y_row + o0;
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int i = 0; i < 2 * MT; ++i, to += 8 * p.ldo, from += 8 * p.ldy) {
+                if (!(rows >> i & 1)) continue;
+                const float f = row_scale[i * 8 + g];
+                const float(&v)[4][4] = acc[i / 2];
+                const int e = i % 2;
+                if (whole) {
+                    float x[8];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = m * 16 + e * 8 + g;
-                    if (t0 + row >= p.tokens || s.ids[row] != id) continue;
-                    const float f = row_scale[row];
-                    if (whole) {
-                        float v[8];
+                    for (int j = 0; j < 8; ++j) x[j] = fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
+                    Eight<Y>::store(to, x);
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) v[j] = fmaf(acc[m][j >> 1][2 * e + (j & 1)], f, old[m][e].get(j));
-                        Eight<Y>::store(out + (t0 + row) * p.ldo + mine, v);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (mine + j < p.oc)
-                                put(out + (t0 + row) * p.ldo + mine + j,
-                                    fmaf(acc[m][j >> 1][2 * e + (j & 1)], f, (float)y[(t0 + row) * p.ldy + mine + j]));
-                    }
+                    for (int j = 0; j < 8; ++j)
+                        if (o0 + 8 * t + j < p.oc) put(to + j, fmaf(v[j >> 1][2 * e + (j & 1)], f, (float)from[j]));
                 }
+            }
+        };
+        for (int c = 0; c < n_c; c += 2) {
+            work(c, old_a, old_b);
+            if (c + 1 < n_c) work(c + 1, old_b, old_a);
         }
     }
 }
@@ -393,7 +516,8 @@ cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
 }
 template <typename T, typename Y, int MT>
 cudaError_t up(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
-    const size_t smem = (size_t)(sizeof(Y) == 4 ? 3 : 2) * 16 * MT * ((p.rank + 31) / 32 * 32 + 8) * sizeof(T);
+    const size_t ranks = (p.rank + 31) / 32 * 32, rows = 16 * MT;
+    const size_t smem = (sizeof(Y) == 4 ? 3 : 2) * rows * (ranks + 8) * sizeof(T) + (std::is_same<T, __half>::value ? rows * ranks * 4 : 0);
     return vec ? start(k_lora_up<T, Y, MT, true>, grid, smem, s, p) : start(k_lora_up<T, Y, MT, false>, grid, smem, s, p);
 }
 template <typename T>
@@ -410,9 +534,9 @@ cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaS
     }
     const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
     p.columns = (int)((p.oc + kWarps * kColumns - 1) / (kWarps * kColumns));
+    // two CTAs an SM; few tiles are divided by their adapters too
     p.slots = (int)std::min<int64_t>(std::min<int64_t>(rows, p.tokens), std::max<int64_t>(1, 4 * sms / (tiles * p.columns)));
-    p.a_time = (int)std::min<int64_t>(p.columns, std::max<int64_t>(1, tiles * p.columns / (8 * sms)));
-    const dim3 grid((unsigned)(tiles * ((p.columns + p.a_time - 1) / p.a_time)), (unsigned)p.slots);
+    const dim3 grid((unsigned)std::min<int64_t>(tiles * p.columns, p.slots > 1 ? tiles * p.columns : 2 * sms), (unsigned)p.slots);
     if (few) return wide ? up<T, float, 1>(p, vec_up, grid, s) : up<T, T, 1>(p, vec_up, grid, s);
     return wide ? up<T, float, 2>(p, vec_up, grid, s) : up<T, T, 2>(p, vec_up, grid, s);
 }
