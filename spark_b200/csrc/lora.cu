@@ -18,6 +18,7 @@
 // (fp32) terms of B's type, which together are good to 2^-17 or 2^-23 of it; for f16,
 // whose exponents are few, a row is brought to 2^14 by a power of 2 first.
 #include <math.h>
+#include <string.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -35,6 +36,8 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
 constexpr int kColumns = 32;   // of y, by one warp at a time
+constexpr int kFew = 64;       // tokens up to which tiles have 16 rows, and B h is computed without tensor cores
+constexpr int kFewThreads = 128;
 
 struct Params {
     const void *x, *a, *b, *y;
@@ -46,7 +49,7 @@ struct Params {
     int64_t adapters;
     int rank, repeat;            // tokens of an entry of `adapter`
     int splits, slots;           // of the input's columns; of a tile's items, worked on side by side
-    int rank_blocks, columns;    // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y
+    int rank_blocks, columns, run;   // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y, of an item
     int wide_y;                  // rows of y and out on 16 bytes
     float* h;                    // [splits, tokens, rank]
     int* err;
@@ -244,6 +247,47 @@ __global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(co
     }
 }
 
+// f(row, rank, value) for the rows' h, summed over the splits; zeros behind the rank and where the row has no adapter (or is not in
+// `rows`).  Four ranks a thread where they lie on 16 bytes; the loads of four splits are on the way together.
+template <int ROWS, int THREADS, typename F>
+__device__ __forceinline__ void sum_h(const Params& p, const Tile<ROWS>& s, int64_t t0, unsigned rows, int chunks, F f) {
+    const int64_t apart = p.tokens * p.rank;
+    if (p.rank % 4 == 0) {
+        for (int i = threadIdx.x; i < ROWS * chunks * 8; i += THREADS) {
+            const int row = i / (chunks * 8), r = (i - row * chunks * 8) * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (s.ids[row] >= 0 && (rows >> row & 1) && r < p.rank) {
+                const float* from = p.h + (t0 + row) * p.rank + r;
+                for (int k0 = 0; k0 < p.splits; k0 += 4) {
+                    float4 u[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        u[k] = k0 + k < p.splits ? *reinterpret_cast<const float4*>(from + (k0 + k) * apart) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v.x += u[k].x, v.y += u[k].y, v.z += u[k].z, v.w += u[k].w;
+                }
+            }
+            f(row, r, v.x), f(row, r + 1, v.y), f(row, r + 2, v.z), f(row, r + 3, v.w);
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < ROWS * chunks * 32; i += THREADS) {
+        const int row = i / (chunks * 32), r = i - row * chunks * 32;
+        float v = 0.f;
+        if (s.ids[row] >= 0 && (rows >> row & 1) && r < p.rank) {
+            const float* from = p.h + (t0 + row) * p.rank + r;
+            for (int k0 = 0; k0 < p.splits; k0 += 4) {
+                float u[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[k] = k0 + k < p.splits ? from[(k0 + k) * apart] : 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v += u[k];
+            }
+        }
+        f(row, r, v);
+    }
+}
+
 // 8 values of a row of y as floats, and back.
 template <typename Y>
 struct Eight;
@@ -280,12 +324,12 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 template <typename Y>
 __device__ __forceinline__ void put(Y* p, float v) { *p = Mma<Y>::round(v); }
 
-// out[t, :] = y[t, :] + scale B[a] h[t].  A CTA has a run of column blocks (kColumns for each warp), most often of one tile, and of the
-// tile every slots-th adapter with its rows.  Where these are more than one, a product has zeros in place of the others' rows, and
-// y is read and written once for all.
-template <typename T, typename Y, int MT, bool VEC>
+// out[t, :] = y[t, :] + scale B[a] h[t], for many tokens.  An item is a run of column blocks (kColumns for each warp) of a tile, with
+// every slots-th adapter and its rows.  Where these are more than one, a product has zeros in place of the others' rows, and y is
+// read and written once for all.  Tiles with several adapters take longer: their runs go to different CTAs.
+template <typename T, typename Y, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__ Params p) {
-    constexpr int ROWS = 16 * MT, TERMS = sizeof(Y) == 4 ? 3 : 2;
+    constexpr int MT = 2, ROWS = 16 * MT, TERMS = sizeof(Y) == 4 ? 3 : 2;
     constexpr bool kScaled = std::is_same<T, __half>::value;
     __shared__ Tile<ROWS> s;
     __shared__ float row_scale[ROWS];
@@ -299,13 +343,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
     const Y* y = reinterpret_cast<const Y*>(p.y);
     Y* out = reinterpret_cast<Y*>(p.out);
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
-    const int64_t blocks = (p.tokens + ROWS - 1) / ROWS * p.columns;
-    const int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
+    const int runs = (p.columns + p.run - 1) / p.run;
+    const int64_t items = (p.tokens + ROWS - 1) / ROWS * runs;
     bool waited = false;
-    for (int64_t at = lo; at < hi;) {
-        const int64_t tile = at / p.columns, t0 = tile * ROWS;
-        const int c0 = (int)(at - tile * p.columns), n_c = (int)min((int64_t)(p.columns - c0), hi - at);
-        at += n_c;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t tile = item / runs, t0 = tile * ROWS;
+        const int c0 = (int)(item - tile * runs) * p.run, n_c = min(p.run, p.columns - c0);
         __syncthreads();      // (the last tile is done with)
         load_tile(s, p, t0, false);
         // this slot's adapters, and a lane's rows (g, g + 8, ...) with one of them (or none, which is copied)
@@ -327,8 +370,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
         Y* out_row = out + (t0 + g) * p.ldo + 8 * t;
         auto load_old = [&](Eight<Y> (&old)[MT][2], int c) {
             const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
-            if (c >= n_c || !p.wide_y || o0 + 8 * t + 8 > p.oc) return;
+            if (c >= n_c) return;
             const Y* from = y_row + o0;
+            if (!p.wide_y || o0 + 8 * t + 8 > p.oc) {
+#pragma unroll
+                for (int i = 0; i < 2 * MT; ++i, from += 8 * p.ldy)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if ((rows >> i & 1) && o0 + 8 * t + j < p.oc) old[i / 2][i % 2].v[j] = from[j];
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i, from += 8 * p.ldy)
                 if (rows >> i & 1) old[i / 2][i % 2].load(from);
@@ -352,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
             }
         };
         Eight<Y> old_a[MT][2], old_b[MT][2];
-        uint4 w[4], w2[4];
+        uint4 w[4];
         load_old(old_a, 0);
         load_weights(w, 0, 0);
         if (!waited) {
@@ -362,17 +413,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
         }
         if (!any) continue;
         // h of the rows, summed over the splits
-        for (int i = threadIdx.x; i < ROWS * ranks; i += kThreads) {
-            const int row = i / ranks, r = i - row * ranks;
-            float v = 0.f;
-            if (s.ids[row] >= 0 && r < p.rank) {
-                const float* h = p.h + (t0 + row) * p.rank + r;
-                const int64_t apart = p.tokens * p.rank;
-#pragma unroll 4
-                for (int k = 0; k < p.splits; ++k) v += h[k * apart];
-            }
+        sum_h<ROWS, kThreads>(p, s, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
             if constexpr (kScaled) {
-                sums[i] = v;
+                sums[row * ranks + r] = v;
             } else {
 #pragma unroll
                 for (int k = 0; k < TERMS; ++k) {
@@ -382,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
                     v = fabsf(f) < INFINITY ? v - f : 0.f;
                 }
             }
-        }
+        });
         if (threadIdx.x < ROWS) {
             const int id = s.ids[threadIdx.x];
             row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
@@ -439,44 +482,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
                         }
                     }
             };
-            // the next step's weights come during this one's products (MT = 2 has no registers for that: during what follows them)
-            if constexpr (MT == 1) {
-                for (int j = 0; j < steps; j += 2) {
-                    load_weights(w2, c, j + 1);
-                    products(w, j);
-                    if (j + 1 == steps) {
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) w[n] = w2[n];
-                        break;
-                    }
-                    load_weights(w, c, j + 2);
-                    products(w2, j + 1);
-                }
-            } else {
-                for (int j = 0; j < steps; ++j) {
-                    products(w, j);
-                    load_weights(w, c, j + 1);
-                }
+            for (int j = 0; j < steps; ++j) {
+                products(w, j);
+                load_weights(w, c, j + 1);
             }
             const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
             const bool whole = p.wide_y && o0 + 8 * t + 8 <= p.oc;
             Y* to = out_row + o0;
-            const Y* from = y_row + o0;
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i, to += 8 * p.ldo, from += 8 * p.ldy) {
+            for (int i = 0; i < 2 * MT; ++i, to += 8 * p.ldo) {
                 if (!(rows >> i & 1)) continue;
                 const float f = row_scale[i * 8 + g];
                 const float(&v)[4][4] = acc[i / 2];
                 const int e = i % 2;
-                if (whole) {
-                    float x[8];
+                float x[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
+                for (int j = 0; j < 8; ++j) x[j] = fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
+                if (whole) {
                     Eight<Y>::store(to, x);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (o0 + 8 * t + j < p.oc) put(to + j, fmaf(v[j >> 1][2 * e + (j & 1)], f, (float)from[j]));
+                        if (o0 + 8 * t + j < p.oc) put(to + j, x[j]);
                 }
             }
         };
@@ -487,11 +514,92 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
     }
 }
 
-constexpr int kFew = 64;        // tokens up to which tiles have 16 rows
-// Splits of the input's columns: as many as give two CTAs an SM work, each at least two chunks of 32 columns a warp.
+// The same for few tokens, most with an adapter of their own: a tensor core's 16 rows would be one row's work and 15 others'.  A lane
+// has a column of y, a warp 32, and of a tile of 16 rows every slots-th adapter: of B 32 ranks at a time in registers, for as many
+// rows as have that adapter; the next adapter's are on the way meanwhile.  fp32 throughout.
+template <typename T, typename Y, bool VEC>
+__global__ void __launch_bounds__(kFewThreads, 5) k_lora_up_few(const __grid_constant__ Params p) {
+    constexpr int ROWS = 16;
+    __shared__ Tile<ROWS> s;
+    __shared__ float row_scale[ROWS];
+    extern __shared__ __align__(16) float h[];   // [ROWS, chunks * 32]
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int chunks = (p.rank + 31) / 32, ranks = chunks * 32, lane = threadIdx.x & 31, slot = blockIdx.z;
+    const int64_t t0 = (int64_t)blockIdx.y * ROWS, o = (int64_t)blockIdx.x * kFewThreads + threadIdx.x;
+    const bool in_place = p.y == p.out;
+    const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
+    load_tile(s, p, t0, false);
+    if (slot >= s.count) return;
+    unsigned rows = 0;      // those of this slot
+    for (int d = slot; d < s.count; d += p.slots)
+        rows |= __ballot_sync(0xffffffffu, lane < ROWS && t0 + lane < p.tokens && s.ids[lane & (ROWS - 1)] == s.distinct[d]);
+    auto load = [&](uint4 (&w)[4], int d, int k) {
+        if (d >= s.count) return;
+        const int id = s.distinct[d];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            w[j] = id >= 0 && o < p.oc ? load8<T, VEC>(bb.begin + ((int64_t)id * p.oc + o) * p.rank, k * 32 + 8 * j, p.rank, bb)
+                                       : make_uint4(0, 0, 0, 0);
+    };
+    uint4 now[4], coming[4];
+    load(now, slot, 0);
+    const Y* y = reinterpret_cast<const Y*>(p.y) + t0 * p.ldy + o;
+    Y* out = reinterpret_cast<Y*>(p.out) + t0 * p.ldo + o;
+    Y old[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+        if ((rows >> r & 1) && o < p.oc) old[r] = y[r * p.ldy];
+    // (what was ready before the first product could be read before it ends)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    sum_h<ROWS, kFewThreads>(p, s, t0, rows, chunks, [&](int row, int r, float v) { h[row * ranks + r] = v; });
+    if (threadIdx.x < ROWS) {
+        const int id = s.ids[threadIdx.x];
+        row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
+    }
+    __syncthreads();
+    for (int d = slot; d < s.count; d += p.slots) {
+        const int id = s.distinct[d];
+        const unsigned mine = __ballot_sync(0xffffffffu, lane < ROWS && t0 + lane < p.tokens && s.ids[lane & (ROWS - 1)] == id);
+        float acc[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) acc[r] = 0.f;
+        for (int k = 0; k < chunks; ++k) {
+            if (k + 1 < chunks) load(coming, d, k + 1);
+            else load(coming, d + p.slots, 0);
+            if (id >= 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (k * 32 + 8 * j >= p.rank) break;
+                    T v[8];
+                    memcpy(v, &now[j], 16);
+                    float b[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[i] = (float)v[i];
+#pragma unroll
+                    for (int r = 0; r < ROWS; ++r) {
+                        if (!(mine >> r & 1)) continue;
+                        const float4* hr = reinterpret_cast<const float4*>(h + r * ranks + k * 32 + 8 * j);
+                        const float4 c = hr[0], e = hr[1];
+                        acc[r] = fmaf(c.x, b[0], acc[r]), acc[r] = fmaf(c.y, b[1], acc[r]), acc[r] = fmaf(c.z, b[2], acc[r]);
+                        acc[r] = fmaf(c.w, b[3], acc[r]), acc[r] = fmaf(e.x, b[4], acc[r]), acc[r] = fmaf(e.y, b[5], acc[r]);
+                        acc[r] = fmaf(e.z, b[6], acc[r]), acc[r] = fmaf(e.w, b[7], acc[r]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) now[j] = coming[j];
+        }
+        if (o >= p.oc || (id < 0 && in_place)) continue;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+            if (mine >> r & 1) put(out + r * p.ldo, fmaf(acc[r], row_scale[r], (float)old[r]));
+    }
+}
+
+// Splits of the input's columns: as many as give two CTAs an SM work, each at least a chunk of 32 columns a warp.
 int splits_of(int64_t tokens, int64_t ic, int64_t rank, int sms) {
     const int64_t rows = tokens <= kFew ? 16 : 32, tiles = (tokens + rows - 1) / rows * ((rank + 63) / 64);
-    const int64_t most = std::max<int64_t>(1, ic / (2 * 32 * kWarps));
+    const int64_t most = std::max<int64_t>(1, ic / (32 * kWarps));
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 16), 2 * sms / tiles));
 }
 
@@ -514,11 +622,16 @@ cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
     if (p.rank <= 32) return down<T, MT, 4>(p, vec, grid, s);
     return down<T, MT, 8>(p, vec, grid, s);
 }
-template <typename T, typename Y, int MT>
-cudaError_t up(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
-    const size_t ranks = (p.rank + 31) / 32 * 32, rows = 16 * MT;
-    const size_t smem = (sizeof(Y) == 4 ? 3 : 2) * rows * (ranks + 8) * sizeof(T) + (std::is_same<T, __half>::value ? rows * ranks * 4 : 0);
-    return vec ? start(k_lora_up<T, Y, MT, true>, grid, smem, s, p) : start(k_lora_up<T, Y, MT, false>, grid, smem, s, p);
+template <typename T, typename Y>
+cudaError_t up(const Params& p, bool vec, dim3 grid, bool few, cudaStream_t s) {
+    const size_t ranks = (p.rank + 31) / 32 * 32;
+    if (few) {
+        const size_t smem = 16 * ranks * sizeof(float);
+        return vec ? launch_overlapped(k_lora_up_few<T, Y, true>, grid, dim3(kFewThreads), smem, s, p)
+                   : launch_overlapped(k_lora_up_few<T, Y, false>, grid, dim3(kFewThreads), smem, s, p);
+    }
+    const size_t smem = (sizeof(Y) == 4 ? 3 : 2) * 32 * (ranks + 8) * sizeof(T) + (std::is_same<T, __half>::value ? 32 * ranks * 4 : 0);
+    return vec ? start(k_lora_up<T, Y, true>, grid, smem, s, p) : start(k_lora_up<T, Y, false>, grid, smem, s, p);
 }
 template <typename T>
 cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t s) {
@@ -532,13 +645,21 @@ cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaS
         const cudaError_t e = few ? down<T, 1>(p, vec_down, grid, s) : down<T, 2>(p, vec_down, grid, s);
         if (e != cudaSuccess) return e;
     }
+    // few tiles are divided by their adapters too
     const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
-    p.columns = (int)((p.oc + kWarps * kColumns - 1) / (kWarps * kColumns));
-    // two CTAs an SM; few tiles are divided by their adapters too
-    p.slots = (int)std::min<int64_t>(std::min<int64_t>(rows, p.tokens), std::max<int64_t>(1, 4 * sms / (tiles * p.columns)));
-    const dim3 grid((unsigned)std::min<int64_t>(tiles * p.columns, p.slots > 1 ? tiles * p.columns : 2 * sms), (unsigned)p.slots);
-    if (few) return wide ? up<T, float, 1>(p, vec_up, grid, s) : up<T, T, 1>(p, vec_up, grid, s);
-    return wide ? up<T, float, 2>(p, vec_up, grid, s) : up<T, T, 2>(p, vec_up, grid, s);
+    dim3 grid;
+    if (few) {
+        const int64_t columns = (p.oc + kFewThreads - 1) / kFewThreads;
+        p.slots = (int)std::min<int64_t>(std::min<int64_t>(rows, p.tokens), std::max<int64_t>(1, 5 * sms / (tiles * columns)));
+        grid = dim3((unsigned)columns, (unsigned)tiles, (unsigned)p.slots);
+    } else {
+        p.columns = (int)((p.oc + kWarps * kColumns - 1) / (kWarps * kColumns));
+        p.run = (int)std::min<int64_t>(4, std::max<int64_t>(1, tiles * p.columns / (8 * sms)));
+        const int64_t items = tiles * ((p.columns + p.run - 1) / p.run);
+        p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2 * sms / items));
+        grid = dim3((unsigned)std::min<int64_t>(items, std::max(1, 2 * sms / p.slots)), (unsigned)p.slots);
+    }
+    return wide ? up<T, float>(p, vec_up, grid, few, s) : up<T, T>(p, vec_up, grid, few, s);
 }
 
 }  // namespace lora
