@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "tc_common.cuh"
 
 namespace spark {
 namespace tc {
@@ -38,6 +39,11 @@ constexpr int kMaxRank = 256;
 constexpr int kColumns = 32;   // of y, by one warp at a time
 constexpr int kFew = 64;       // tokens up to which tiles have 16 rows, and B h is computed without tensor cores
 constexpr int kFewThreads = 128;
+// B h on the tensor memory, for tiles of 128 tokens that are not crowded
+constexpr int kMany = 256;     // tokens from which on
+constexpr int kTcRows = 128, kTcCols = 128;
+constexpr int kTcRank = 64;    // ranks up to which one 128-byte row of B holds them
+constexpr int kTcIds = 4;      // adapters of a tile; more: the other kernel's
 
 struct Params {
     const void *x, *a, *b, *y;
@@ -51,6 +57,7 @@ struct Params {
     int splits, slots;           // of the input's columns; of a tile's items, worked on side by side
     int rank_blocks, columns, run;   // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y, of an item
     int wide_y;                  // rows of y and out on 16 bytes
+    int crowded;                 // only the tiles that the tensor memory's kernel leaves
     float* h;                    // [splits, tokens, rank]
     int* err;
 };
@@ -148,6 +155,44 @@ __device__ __forceinline__ void load_tile(Tile<ROWS>& s, const Params& p, int64_
         if (i < ROWS) s.ids[i] = id;
         if (leads >> i & 1) s.distinct[__popc(leads & ((1u << i) - 1))] = id;
         if (i == 0) s.count = __popc(leads);
+    }
+    __syncthreads();
+}
+
+// The same for 128 rows: of the distinct ones the first kTcIds and their number.
+struct WideTile {
+    int ids[kTcRows];
+    int distinct[kTcIds];
+    int count;
+    unsigned leads[kTcRows / 32];
+};
+__device__ __forceinline__ void load_wide_tile(WideTile& s, const Params& p, int64_t t0) {
+    const int i = threadIdx.x, warp = i >> 5, lane = i & 31;
+    const bool is = i < kTcRows && t0 + i < p.tokens;
+    int id = -1;
+    if (is) id = p.adapter[p.repeat == 1 ? t0 + i : (t0 + i) / p.repeat];
+    if (id < 0 || id >= p.adapters) id = -1;
+    if (i < kTcRows) s.ids[i] = id;
+    __syncthreads();
+    if (__syncthreads_and(!is || id == s.ids[0])) {
+        if (i == 0) s.count = id >= 0, s.distinct[0] = id;
+    } else {
+        if (i < kTcRows) {
+            const unsigned same = __match_any_sync(0xffffffffu, id);
+            bool lead = id >= 0 && __ffs(same) - 1 == lane;
+            for (int j = 0; j < warp * 32; ++j) lead = lead && s.ids[j] != id;
+            const unsigned leads = __ballot_sync(0xffffffffu, lead);
+            if (lane == 0) s.leads[warp] = leads;
+        }
+        __syncthreads();
+        if (i < kTcRows) {
+            int before = 0;
+            for (int w = 0; w < warp; ++w) before += __popc(s.leads[w]);
+            const unsigned mine = s.leads[warp];
+            before += __popc(mine & ((1u << lane) - 1));
+            if ((mine >> lane & 1) && before < kTcIds) s.distinct[before] = id;
+            if (i == kTcRows - 1) s.count = before + (int)(mine >> 31);
+        }
     }
     __syncthreads();
 }
@@ -250,13 +295,13 @@ __global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(co
 // f(row, rank, value) for the rows' h, summed over the splits; zeros behind the rank and where the row has no adapter (or is not in
 // `rows`).  Four ranks a thread where they lie on 16 bytes; the loads of four splits are on the way together.
 template <int ROWS, int THREADS, typename F>
-__device__ __forceinline__ void sum_h(const Params& p, const Tile<ROWS>& s, int64_t t0, unsigned rows, int chunks, F f) {
+__device__ __forceinline__ void sum_h(const Params& p, const int* ids, int64_t t0, unsigned rows, int chunks, F f) {
     const int64_t apart = p.tokens * p.rank;
     if (p.rank % 4 == 0) {
         for (int i = threadIdx.x; i < ROWS * chunks * 8; i += THREADS) {
             const int row = i / (chunks * 8), r = (i - row * chunks * 8) * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (s.ids[row] >= 0 && (rows >> row & 1) && r < p.rank) {
+            if (ids[row] >= 0 && (rows >> (row & 31) & 1) && r < p.rank) {
                 const float* from = p.h + (t0 + row) * p.rank + r;
                 for (int k0 = 0; k0 < p.splits; k0 += 4) {
                     float4 u[4];
@@ -274,7 +319,7 @@ __device__ __forceinline__ void sum_h(const Params& p, const Tile<ROWS>& s, int6
     for (int i = threadIdx.x; i < ROWS * chunks * 32; i += THREADS) {
         const int row = i / (chunks * 32), r = i - row * chunks * 32;
         float v = 0.f;
-        if (s.ids[row] >= 0 && (rows >> row & 1) && r < p.rank) {
+        if (ids[row] >= 0 && (rows >> (row & 31) & 1) && r < p.rank) {
             const float* from = p.h + (t0 + row) * p.rank + r;
             for (int k0 = 0; k0 < p.splits; k0 += 4) {
                 float u[4];
@@ -345,11 +390,17 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
     const int runs = (p.columns + p.run - 1) / p.run;
     const int64_t items = (p.tokens + ROWS - 1) / ROWS * runs;
+    __shared__ WideTile around;
+    int64_t checked = -1;
     bool waited = false;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
         const int64_t tile = item / runs, t0 = tile * ROWS;
         const int c0 = (int)(item - tile * runs) * p.run, n_c = min(p.run, p.columns - c0);
         __syncthreads();      // (the last tile is done with)
+        if (p.crowded) {
+            if (t0 / kTcRows != checked) load_wide_tile(around, p, t0 / kTcRows * kTcRows), checked = t0 / kTcRows;
+            if (around.count <= kTcIds) continue;
+        }
         load_tile(s, p, t0, false);
         // this slot's adapters, and a lane's rows (g, g + 8, ...) with one of them (or none, which is copied)
         const int slot = blockIdx.y;
@@ -413,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
         }
         if (!any) continue;
         // h of the rows, summed over the splits
-        sum_h<ROWS, kThreads>(p, s, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
+        sum_h<ROWS, kThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
             if constexpr (kScaled) {
                 sums[row * ranks + r] = v;
             } else {
@@ -512,6 +563,233 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
             if (c + 1 < n_c) work(c + 1, old_b, old_a);
         }
     }
+    // (the end of this launch is to be the end of those before it)
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// The same on the tensor memory, for many tokens of few adapters a tile.  D [128 tokens, 128 columns] = A B^T with the rows of h in A
+// (its terms side by side along K, split as above) and 128 rows of B[a], both in shared memory in 128-byte rows, swizzled.  While a
+// block's D is read back and added to y, the next one's B arrives and is multiplied into the other half of the tensor memory.
+// Read back, a lane has a row; through shared memory it becomes 8 columns of a row, so that y is read and written in 64-byte
+// pieces.  Bound by memory: the products take a tenth of the time.
+template <typename T, typename Y, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) k_lora_up_tc(const __grid_constant__ Params p) {
+    using namespace tcx;
+    constexpr int TERMS = sizeof(Y) == 4 ? 3 : 2;
+    constexpr bool kScaled = std::is_same<T, __half>::value;
+    constexpr uint32_t kTypes = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+    constexpr uint32_t kIdesc = (1u << 4) | kTypes | ((uint32_t)(kTcCols >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
+    constexpr int kPitch = 36;     // floats of a row on its way from the tensor memory to y
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ WideTile s;
+    __shared__ float row_scale[kTcRows];
+    __shared__ __align__(8) uint64_t bars[2];
+    __shared__ uint32_t s_tmem;
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const int padded = (p.rank + 15) / 16 * 16, parts_a = (TERMS * padded + 63) / 64;
+    uint8_t* const a_smem = smem;
+    uint8_t* const b_smem = smem + parts_a * kTcRows * 128;                      // two
+    float* const way = reinterpret_cast<float*>(b_smem + 2 * kTcCols * 128);     // [kThreads / 32, 32, kPitch]; sums of h before
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t bar = smem_u32(&bars[0]);
+    asm volatile("griddepcontrol.launch_dependents;");
+    if (threadIdx.x == 0) {
+        mbar_init(bar, 1), mbar_init(bar + 8, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(2 * kTcCols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
+    const int runs = (p.columns + p.run - 1) / p.run;
+    const int64_t items = (p.tokens + kTcRows - 1) / kTcRows * runs;
+    bool waited = false, ok = true;
+    uint32_t done = 0;      // units whose products were waited for: their parity
+    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
+        const int64_t tile = item / runs, t0 = tile * kTcRows;
+        const int c0 = (int)(item - tile * runs) * p.run, n_c = min(p.run, p.columns - c0);
+        __syncthreads();      // (the last item is done with)
+        load_wide_tile(s, p, t0);
+        const int n_ids = s.count;
+        if (!waited) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+        }
+        if (n_ids > kTcIds || (n_ids == 0 && p.y == p.out)) continue;
+        // A: value (row, k) of the terms, 16 bytes of a row exchanged by its number
+        auto put_terms = [&](int row, int r, float v) {
+#pragma unroll
+            for (int q = 0; q < TERMS; ++q) {
+                const T x = Mma<T>::round(v);
+                const int k = q * padded + r, in = k & 63;
+                *reinterpret_cast<T*>(a_smem + (k >> 6) * kTcRows * 128 + row * 128 + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
+                const float f = (float)x;
+                v = fabsf(f) < INFINITY ? v - f : 0.f;
+            }
+        };
+        const int chunks = (p.rank + 31) / 32, ranks = chunks * 32;
+        sum_h<kTcRows, kThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
+            if (kScaled) way[row * ranks + r] = v;
+            else if (r < padded) put_terms(row, r, v);
+        });
+        if (threadIdx.x < kTcRows) {
+            const int id = s.ids[threadIdx.x];
+            row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
+        }
+        if constexpr (kScaled) {
+            __syncthreads();
+            for (int row = warp; row < kTcRows; row += kWarps) {
+                float most = 0.f;
+                for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(way[row * ranks + r]));
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int e = most > 0.f && most < INFINITY ? min(max(14 - ilogbf(most), -100), 100) : 0;
+                const float up = ldexpf(1.f, e);
+                if (lane == 0) row_scale[row] *= ldexpf(1.f, -e);
+                for (int r = lane; r < padded; r += 32) put_terms(row, r, way[row * ranks + r] * up);
+            }
+        }
+        // units: the adapters of a column block, then those of the next
+        const int units = n_c * max(n_ids, 1);
+        uint4 w[kTcCols * kTcRank * 2 / 16 / kThreads];     // this thread's part of a block's B: 16 bytes of a column
+        auto load_b = [&](int unit) {
+            const int c = n_ids > 1 ? unit / n_ids : unit, id = s.distinct[n_ids > 1 ? unit - c * n_ids : 0];
+            const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
+#pragma unroll
+            for (int j = 0; j < kTcCols * kTcRank * 2 / 16 / kThreads; ++j) {
+                const int i = j * kThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
+                w[j] = o0 + col < p.oc ? load8<T, VEC>(bb.begin + ((int64_t)id * p.oc + o0 + col) * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
+            }
+        };
+        auto put_b = [&](int unit) {
+            uint8_t* to = b_smem + (unit & 1) * kTcCols * 128;
+#pragma unroll
+            for (int j = 0; j < kTcCols * kTcRank * 2 / 16 / kThreads; ++j) {
+                const int i = j * kThreads + threadIdx.x, col = i >> 3, k = i & 7;
+                if (k * 8 < padded) *reinterpret_cast<uint4*>(to + col * 128 + ((k ^ (col & 7)) << 4)) = w[j];
+            }
+        };
+        auto multiply = [&](int unit) {
+            const uint32_t d = tmem + (unit & 1) * kTcCols, b = smem_u32(b_smem) + (unit & 1) * kTcCols * 128;
+            tc_fence_after();
+            for (int q = 0; q < TERMS; ++q)
+                for (int k = 0; k < padded; k += 16) {
+                    const int ka = q * padded + k;
+                    const uint64_t da = sdesc_sw128(smem_u32(a_smem) + (ka >> 6) * kTcRows * 128 + (ka & 63) * 2), db = sdesc_sw128(b + k * 2);
+                    asm volatile(
+                        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+                        "l"(da), "l"(db), "r"(kIdesc), "r"((uint32_t)(q + k > 0))
+                        : "memory");
+                }
+            mma_commit(bar + 8 * (unit & 1));
+        };
+        // the unit's rows and columns of a warp: 32 rows of its quarter of the tensor memory, half of the columns
+        const int quarter = warp & 3, half = warp >> 2;
+        const Y* y_row = reinterpret_cast<const Y*>(p.y) + (t0 + quarter * 32 + g) * p.ldy + half * 64 + 8 * t;
+        Y* out_row = reinterpret_cast<Y*>(p.out) + (t0 + quarter * 32 + g) * p.ldo + half * 64 + 8 * t;
+        if (n_ids > 0) {
+            load_b(0);
+            put_b(0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0 && n_ids > 0) multiply(0);
+        for (int unit = 0; unit < units; ++unit) {
+            const int c = n_ids > 1 ? unit / n_ids : unit, d = n_ids > 1 ? unit - c * n_ids : 0, id = n_ids > 0 ? s.distinct[d] : -1;
+            const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
+            const bool more = unit + 1 < units && n_ids > 0;
+            if (more) load_b(unit + 1);
+            unsigned rows = 0;     // this lane's, with the unit's adapter (the first unit of a block has those without any, too)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = quarter * 32 + g + 8 * i;
+                rows |= t0 + row < p.tokens && (s.ids[row] == id || (s.ids[row] < 0 && d == 0 && p.y != p.out)) ? 1u << i : 0u;
+            }
+            Eight<Y> old[2][4];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t o = o0 + half * 64 + h * 32 + 8 * t;
+                    const Y* from = y_row + o0 + h * 32 + i * 8 * p.ldy;
+                    if (!(rows >> i & 1)) continue;
+                    if (p.wide_y && o + 8 <= p.oc) {
+                        old[h][i].load(from);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (o + j < p.oc) old[h][i].v[j] = from[j];
+                    }
+                }
+            if (more) {
+                put_b(unit + 1);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            }
+            tc_fence_before();
+            if (!__syncthreads_and(ok)) {
+                ok = false;
+                break;
+            }
+            if (threadIdx.x == 0 && more) multiply(unit + 1);
+            if (n_ids > 0) {
+                ok = mbar_wait(bar + 8 * (unit & 1), done >> (unit & 1) & 1);
+                done ^= 1u << (unit & 1);
+                tc_fence_after();
+            }
+            float* mine = way + warp * 32 * kPitch;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float v[16];
+                    if (n_ids > 0) {
+                        tmem_ld16(tmem + (unit & 1) * kTcCols + half * 64 + h * 32 + 16 * j + ((uint32_t)(quarter * 32) << 16), v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<float4*>(mine + lane * kPitch + 16 * j + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                }
+                __syncwarp();
+                const int64_t o = o0 + half * 64 + h * 32 + 8 * t;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (!(rows >> i & 1)) continue;
+                    const float f = row_scale[quarter * 32 + g + 8 * i];
+                    const float4 u0 = *reinterpret_cast<const float4*>(mine + (g + 8 * i) * kPitch + 8 * t);
+                    const float4 u1 = *reinterpret_cast<const float4*>(mine + (g + 8 * i) * kPitch + 8 * t + 4);
+                    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = fmaf(u[j], f, old[h][i].get(j));
+                    Y* to = out_row + o0 + h * 32 + i * 8 * p.ldo;
+                    if (p.wide_y && o + 8 <= p.oc) {
+                        Eight<Y>::store(to, x);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (o + j < p.oc) put(to + j, x[j]);
+                    }
+                }
+            }
+        }
+        ok = __syncthreads_and(ok);
+    }
+    if (!ok) report_device_error(p.err, 10);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTcCols) : "memory");
+    }
 }
 
 // The same for few tokens, most with an adapter of their own: a tensor core's 16 rows would be one row's work and 15 others'.  A lane
@@ -529,7 +807,10 @@ __global__ void __launch_bounds__(kFewThreads, 5) k_lora_up_few(const __grid_con
     const bool in_place = p.y == p.out;
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
     load_tile(s, p, t0, false);
-    if (slot >= s.count) return;
+    if (slot >= s.count) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     unsigned rows = 0;      // those of this slot
     for (int d = slot; d < s.count; d += p.slots)
         rows |= __ballot_sync(0xffffffffu, lane < ROWS && t0 + lane < p.tokens && s.ids[lane & (ROWS - 1)] == s.distinct[d]);
@@ -551,7 +832,7 @@ __global__ void __launch_bounds__(kFewThreads, 5) k_lora_up_few(const __grid_con
         if ((rows >> r & 1) && o < p.oc) old[r] = y[r * p.ldy];
     // (what was ready before the first product could be read before it ends)
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    sum_h<ROWS, kFewThreads>(p, s, t0, rows, chunks, [&](int row, int r, float v) { h[row * ranks + r] = v; });
+    sum_h<ROWS, kFewThreads>(p, s.ids, t0, rows, chunks, [&](int row, int r, float v) { h[row * ranks + r] = v; });
     if (threadIdx.x < ROWS) {
         const int id = s.ids[threadIdx.x];
         row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
@@ -633,6 +914,12 @@ cudaError_t up(const Params& p, bool vec, dim3 grid, bool few, cudaStream_t s) {
     const size_t smem = (sizeof(Y) == 4 ? 3 : 2) * 32 * (ranks + 8) * sizeof(T) + (std::is_same<T, __half>::value ? 32 * ranks * 4 : 0);
     return vec ? start(k_lora_up<T, Y, true>, grid, smem, s, p) : start(k_lora_up<T, Y, false>, grid, smem, s, p);
 }
+template <typename T, typename Y>
+cudaError_t up_tc(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
+    const int padded = (p.rank + 15) / 16 * 16, parts = ((sizeof(Y) == 4 ? 3 : 2) * padded + 63) / 64;
+    const size_t smem = 1024 + parts * kTcRows * 128 + 2 * kTcCols * 128 + kWarps * 32 * 36 * sizeof(float);
+    return vec ? start(k_lora_up_tc<T, Y, true>, grid, smem, s, p) : start(k_lora_up_tc<T, Y, false>, grid, smem, s, p);
+}
 template <typename T>
 cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t s) {
     const bool few = p.tokens <= kFew;
@@ -648,6 +935,22 @@ cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaS
     // few tiles are divided by their adapters too
     const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
     dim3 grid;
+    if (p.tokens >= kMany && p.rank <= kTcRank) {
+        const int64_t wide_tiles = (p.tokens + kTcRows - 1) / kTcRows;
+        p.columns = (int)((p.oc + kTcCols - 1) / kTcCols);
+        // runs that leave the CTAs the least to do, a tile's beginning counting as a block
+        int64_t least = 0;
+        for (int run = 1, r = 1; r <= 16 && r <= p.columns; ++r) {
+            const int64_t items = wide_tiles * ((p.columns + r - 1) / r), time = (items + 2 * sms - 1) / (2 * sms) * (r + 1);
+            if (r == 1 || time < least) least = time, run = r;
+            p.run = run;
+        }
+        const int64_t items = wide_tiles * ((p.columns + p.run - 1) / p.run);
+        grid = dim3((unsigned)std::min<int64_t>(items, 2 * sms));
+        const cudaError_t e = wide ? up_tc<T, float>(p, vec_up, grid, s) : up_tc<T, T>(p, vec_up, grid, s);
+        if (e != cudaSuccess) return e;
+        p.crowded = 1;
+    }
     if (few) {
         const int64_t columns = (p.oc + kFewThreads - 1) / kFewThreads;
         p.slots = (int)std::min<int64_t>(std::min<int64_t>(rows, p.tokens), std::max<int64_t>(1, 5 * sms / (tiles * columns)));

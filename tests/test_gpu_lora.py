@@ -78,7 +78,7 @@ def test_mixed_adapters(size, dtype, y_dtype):
 
 @pytest.mark.parametrize("tokens,per", [(1, 1), (64, 4), (96, 16), (4096, 512), (777, 7), (2048, 2048)])
 def test_runs_of_tokens(tokens, per):
-    """One adapter for each run; a row's result does not depend on its neighbours."""
+    """One adapter for each run, in any of the ways that tiles are worked on."""
     y, x, a, b, _, scale = make(tokens, tokens, 264, 272, 16, 5, BF)
     ids = (torch.arange(tokens // per, device="cuda") * 3 % 6 - 1).to(torch.int32)
     out = ops().lora_add(y, x, a, b, ids, scale=scale)
@@ -88,9 +88,32 @@ def test_runs_of_tokens(tokens, per):
         assert torch.equal(ops().lora_add(y3, x3, a, b, ids, scale=scale).view(-1, 272), out)
     mixed = ids.repeat_interleave(per)
     mixed[1::2] = (mixed[1::2] + 3) % 5
-    other = ops().lora_add(y, x, a, b, mixed, scale=scale)
-    same = mixed == ids.repeat_interleave(per)
-    assert torch.equal(other[same], out[same])
+    check(y, x, a, b, mixed, scale, ops().lora_add(y, x, a, b, mixed, scale=scale))
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [(BF, BF), (HF, HF), (BF, FP), (HF, FP)])
+@pytest.mark.parametrize("rank,ic,oc", [(1, 40, 130), (12, 72, 128), (16, 256, 513), (24, 96, 1000), (40, 64, 136), (64, 128, 392)])
+def test_many_tokens(rank, ic, oc, dtype, y_dtype):
+    """Tiles of 128 tokens with one adapter, two, four, none, some without, and more than four, in one call and its last tile short."""
+    y, x, a, b, _, scale = make(rank, 900, ic, oc, rank, 12, dtype, y_dtype)
+    ids = torch.zeros(900, dtype=torch.int32, device="cuda")
+    ids[128:200], ids[200:256] = 3, 5
+    ids[256:384] = torch.arange(128, device="cuda") // 32 + 6
+    ids[384:512] = -1
+    ids[512:600], ids[600:640] = 2, -1
+    ids[640:768] = torch.arange(128, device="cuda") * 5 % 12
+    ids[768:900] = torch.arange(132, device="cuda") % 3 - 1
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    check(y, x, a, b, ids, scale, out)
+    assert torch.equal(out[384:512], y[384:512])
+    assert torch.equal(out, ops().lora_add(y, x, a, b, ids, scale=scale))
+    wide = torch.cat([y, y[:, :3]], 1)
+    part = wide[:, 3:]
+    before = part.clone()
+    ops().lora_add(part, x, a, b, ids, scale=scale, out=part)
+    check(before, x, a, b, ids, scale, part)
+    assert torch.equal(wide[:, :3], y[:, :3])
+    ops().check_device_errors()
 
 
 def test_no_adapter_and_every_token_its_own():
