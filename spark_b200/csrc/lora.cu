@@ -29,6 +29,9 @@
 namespace spark {
 namespace tc {
 int sm_count_cached(int dev);
+int get_encoder();
+int encode_2d(CUtensorMap* map, CUtensorMapDataType dt, const void* base, uint64_t inner, uint64_t outer,
+              uint64_t row_stride_bytes, uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle sw);
 }
 
 namespace lora {
@@ -44,6 +47,7 @@ constexpr int kMany = 256;     // tokens from which on
 constexpr int kTcRows = 128, kTcCols = 128;
 constexpr int kTcRank = 64;    // ranks up to which one 128-byte row of B holds them
 constexpr int kTcIds = 4;      // adapters of a tile; more: the other kernel's
+constexpr int kTcStages = 3;   // blocks of y
 
 struct Params {
     const void *x, *a, *b, *y;
@@ -568,33 +572,35 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
 }
 
 // The same on the tensor memory, for many tokens of few adapters a tile.  D [128 tokens, 128 columns] = A B^T with the rows of h in A
-// (its terms side by side along K, split as above) and 128 rows of B[a], both in shared memory in 128-byte rows, swizzled.  While a
-// block's D is read back and added to y, the next one's B arrives and is multiplied into the other half of the tensor memory.
-// Read back, a lane has a row; through shared memory it becomes 8 columns of a row, so that y is read and written in 64-byte
-// pieces.  Bound by memory: the products take a tenth of the time.
-template <typename T, typename Y, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) k_lora_up_tc(const __grid_constant__ Params p) {
+// (its two terms side by side along K) and 128 rows of B[a], both in shared memory in 128-byte rows, swizzled.  Blocks of y come two
+// ahead by TMA, in the same layout; a lane, which has a row of D, adds to its row of the block, and the block leaves by TMA.  While
+// that is done for one adapter of a block, the next one's B arrives and is multiplied into the other half of the tensor memory.
+// Rows without an adapter go out as they came in.  Bound by memory: the products take a tenth of the time.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__ CUtensorMap y_map, const __grid_constant__ CUtensorMap out_map,
+                                                         const __grid_constant__ Params p) {
     using namespace tcx;
-    constexpr int TERMS = sizeof(Y) == 4 ? 3 : 2;
+    constexpr int TERMS = 2;
     constexpr bool kScaled = std::is_same<T, __half>::value;
     constexpr uint32_t kTypes = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t kIdesc = (1u << 4) | kTypes | ((uint32_t)(kTcCols >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
-    constexpr int kPitch = 36;     // floats of a row on its way from the tensor memory to y
+    constexpr int kPart = kTcRows * 128, kBlock = 2 * kPart;      // bytes of 128 rows of 64 values, of a block of y
+    constexpr int kWeights = kTcCols * kTcRank * 2 / 16 / kThreads;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WideTile s;
     __shared__ float row_scale[kTcRows];
-    __shared__ __align__(8) uint64_t bars[2];
+    __shared__ __align__(8) uint64_t bars[2 + kTcStages];
     __shared__ uint32_t s_tmem;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int padded = (p.rank + 15) / 16 * 16, parts_a = (TERMS * padded + 63) / 64;
-    uint8_t* const a_smem = smem;
-    uint8_t* const b_smem = smem + parts_a * kTcRows * 128;                      // two
-    float* const way = reinterpret_cast<float*>(b_smem + 2 * kTcCols * 128);     // [kThreads / 32, 32, kPitch]; sums of h before
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t bar = smem_u32(&bars[0]);
+    uint8_t* const y_smem = smem;                                // [kTcStages]
+    uint8_t* const b_smem = y_smem + kTcStages * kBlock;         // [2]
+    uint8_t* const a_smem = b_smem + 2 * kPart;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t product = smem_u32(&bars[0]), arrived = smem_u32(&bars[2]);
     asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) {
-        mbar_init(bar, 1), mbar_init(bar + 8, 1);
+        for (int i = 0; i < 2 + kTcStages; ++i) mbar_init(product + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
@@ -606,183 +612,171 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up_tc(const __grid_constan
     tc_fence_after();
     const uint32_t tmem = s_tmem;
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
-    const int runs = (p.columns + p.run - 1) / p.run;
-    const int64_t items = (p.tokens + kTcRows - 1) / kTcRows * runs;
+    const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
+    const int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
     bool waited = false, ok = true;
-    uint32_t done = 0;      // units whose products were waited for: their parity
-    for (int64_t item = blockIdx.x; item < items && ok; item += gridDim.x) {
-        const int64_t tile = item / runs, t0 = tile * kTcRows;
-        const int c0 = (int)(item - tile * runs) * p.run, n_c = min(p.run, p.columns - c0);
-        __syncthreads();      // (the last item is done with)
+    uint32_t block = 0, unit = 0;      // so far: blocks, and products (one for each adapter of a block)
+    for (int64_t at = lo; at < hi && ok;) {
+        const int64_t tile = at / p.columns, t0 = tile * kTcRows;
+        const int c0 = (int)(at - tile * p.columns), n_c = (int)min((int64_t)(p.columns - c0), hi - at);
+        at += n_c;
+        __syncthreads();      // (the last tile is done with)
         load_wide_tile(s, p, t0);
         const int n_ids = s.count;
+        if (n_ids > kTcIds || (n_ids == 0 && p.y == p.out)) continue;
+        // block c of this tile into the next stage; what left that stage has to have been read
+        auto fetch = [&](int c) {
+            const uint32_t stage = (block + c) % kTcStages, to = smem_u32(y_smem) + stage * kBlock;
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            mbar_expect_tx(arrived + 8 * stage, kBlock);
+            tma_load_2d(to, &y_map, (c0 + c) * kTcCols, (int)t0, arrived + 8 * stage);
+            tma_load_2d(to + kPart, &y_map, (c0 + c) * kTcCols + 64, (int)t0, arrived + 8 * stage);
+        };
+        if (threadIdx.x == 0)
+            for (int c = 0; c < kTcStages - 1 && c < n_c; ++c) fetch(c);
         if (!waited) {
+            // (y was ready before the first product, and could be read before that ends)
             asm volatile("griddepcontrol.wait;" ::: "memory");
             waited = true;
         }
-        if (n_ids > kTcIds || (n_ids == 0 && p.y == p.out)) continue;
         // A: value (row, k) of the terms, 16 bytes of a row exchanged by its number
         auto put_terms = [&](int row, int r, float v) {
 #pragma unroll
             for (int q = 0; q < TERMS; ++q) {
                 const T x = Mma<T>::round(v);
                 const int k = q * padded + r, in = k & 63;
-                *reinterpret_cast<T*>(a_smem + (k >> 6) * kTcRows * 128 + row * 128 + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
+                *reinterpret_cast<T*>(a_smem + (k >> 6) * kPart + row * 128 + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
                 const float f = (float)x;
                 v = fabsf(f) < INFINITY ? v - f : 0.f;
             }
         };
         const int chunks = (p.rank + 31) / 32, ranks = chunks * 32;
-        sum_h<kTcRows, kThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
-            if (kScaled) way[row * ranks + r] = v;
-            else if (r < padded) put_terms(row, r, v);
-        });
+        // (the stage that no block is on its way to holds the sums before they are scaled)
+        float* const sums = reinterpret_cast<float*>(y_smem + (block + kTcStages - 1) % kTcStages * kBlock);
+        if (kScaled) __syncthreads();
+        if (n_ids > 0)
+            sum_h<kTcRows, kThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
+                if (kScaled) sums[row * ranks + r] = v;
+                else if (r < padded) put_terms(row, r, v);
+            });
         if (threadIdx.x < kTcRows) {
             const int id = s.ids[threadIdx.x];
             row_scale[threadIdx.x] = id < 0 ? 0.f : p.scale ? p.scale[id] : p.scale_all;
         }
-        if constexpr (kScaled) {
+        if (kScaled && n_ids > 0) {
             __syncthreads();
             for (int row = warp; row < kTcRows; row += kWarps) {
                 float most = 0.f;
-                for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(way[row * ranks + r]));
+                for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(sums[row * ranks + r]));
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const int e = most > 0.f && most < INFINITY ? min(max(14 - ilogbf(most), -100), 100) : 0;
                 const float up = ldexpf(1.f, e);
                 if (lane == 0) row_scale[row] *= ldexpf(1.f, -e);
-                for (int r = lane; r < padded; r += 32) put_terms(row, r, way[row * ranks + r] * up);
+                for (int r = lane; r < padded; r += 32) put_terms(row, r, sums[row * ranks + r] * up);
             }
         }
-        // units: the adapters of a column block, then those of the next
-        const int units = n_c * max(n_ids, 1);
-        uint4 w[kTcCols * kTcRank * 2 / 16 / kThreads];     // this thread's part of a block's B: 16 bytes of a column
-        auto load_b = [&](int unit) {
-            const int c = n_ids > 1 ? unit / n_ids : unit, id = s.distinct[n_ids > 1 ? unit - c * n_ids : 0];
+        uint4 w[kWeights];     // this thread's part of a block's B: 16 bytes of a column
+        auto load_b = [&](int c, int d) {
             const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
+            const T* b = bb.begin + ((int64_t)s.distinct[d] * p.oc + o0) * p.rank;
 #pragma unroll
-            for (int j = 0; j < kTcCols * kTcRank * 2 / 16 / kThreads; ++j) {
+            for (int j = 0; j < kWeights; ++j) {
                 const int i = j * kThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
-                w[j] = o0 + col < p.oc ? load8<T, VEC>(bb.begin + ((int64_t)id * p.oc + o0 + col) * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
+                w[j] = o0 + col < p.oc ? load8<T, VEC>(b + col * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
             }
         };
-        auto put_b = [&](int unit) {
-            uint8_t* to = b_smem + (unit & 1) * kTcCols * 128;
+        auto put_b = [&](uint32_t u) {
+            uint8_t* to = b_smem + (u & 1) * kPart;
 #pragma unroll
-            for (int j = 0; j < kTcCols * kTcRank * 2 / 16 / kThreads; ++j) {
+            for (int j = 0; j < kWeights; ++j) {
                 const int i = j * kThreads + threadIdx.x, col = i >> 3, k = i & 7;
                 if (k * 8 < padded) *reinterpret_cast<uint4*>(to + col * 128 + ((k ^ (col & 7)) << 4)) = w[j];
             }
         };
-        auto multiply = [&](int unit) {
-            const uint32_t d = tmem + (unit & 1) * kTcCols, b = smem_u32(b_smem) + (unit & 1) * kTcCols * 128;
+        auto multiply = [&](uint32_t u) {
+            const uint32_t d = tmem + (u & 1) * kTcCols, b = smem_u32(b_smem) + (u & 1) * kPart;
             tc_fence_after();
             for (int q = 0; q < TERMS; ++q)
                 for (int k = 0; k < padded; k += 16) {
                     const int ka = q * padded + k;
-                    const uint64_t da = sdesc_sw128(smem_u32(a_smem) + (ka >> 6) * kTcRows * 128 + (ka & 63) * 2), db = sdesc_sw128(b + k * 2);
+                    const uint64_t da = sdesc_sw128(smem_u32(a_smem) + (ka >> 6) * kPart + (ka & 63) * 2), db = sdesc_sw128(b + k * 2);
                     asm volatile(
                         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
                         "l"(da), "l"(db), "r"(kIdesc), "r"((uint32_t)(q + k > 0))
                         : "memory");
                 }
-            mma_commit(bar + 8 * (unit & 1));
+            mma_commit(product + 8 * (u & 1));
         };
-        // the unit's rows and columns of a warp: 32 rows of its quarter of the tensor memory, half of the columns
-        const int quarter = warp & 3, half = warp >> 2;
-        const Y* y_row = reinterpret_cast<const Y*>(p.y) + (t0 + quarter * 32 + g) * p.ldy + half * 64 + 8 * t;
-        Y* out_row = reinterpret_cast<Y*>(p.out) + (t0 + quarter * 32 + g) * p.ldo + half * 64 + 8 * t;
         if (n_ids > 0) {
-            load_b(0);
-            put_b(0);
+            load_b(0, 0);
+            put_b(unit);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0 && n_ids > 0) multiply(0);
-        for (int unit = 0; unit < units; ++unit) {
-            const int c = n_ids > 1 ? unit / n_ids : unit, d = n_ids > 1 ? unit - c * n_ids : 0, id = n_ids > 0 ? s.distinct[d] : -1;
-            const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
-            const bool more = unit + 1 < units && n_ids > 0;
-            if (more) load_b(unit + 1);
-            unsigned rows = 0;     // this lane's, with the unit's adapter (the first unit of a block has those without any, too)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = quarter * 32 + g + 8 * i;
-                rows |= t0 + row < p.tokens && (s.ids[row] == id || (s.ids[row] < 0 && d == 0 && p.y != p.out)) ? 1u << i : 0u;
+        if (threadIdx.x == 0 && n_ids > 0) multiply(unit);
+        // a lane's row: one of the 32 of its warp's quarter of the tensor memory; half of a block's columns
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane, mine = s.ids[row];
+        const float f = row_scale[row];
+        for (int c = 0; c < n_c && ok; ++c, ++block) {
+            const uint32_t stage = block % kTcStages;
+            uint8_t* const here = y_smem + stage * kBlock + half * kPart + row * 128;
+            if (threadIdx.x == 0 && c + kTcStages - 1 < n_c) {
+                // (block counts from this one on: c blocks of the tile are behind)
+                const uint32_t next = (block + kTcStages - 1) % kTcStages, to = smem_u32(y_smem) + next * kBlock;
+                const int x = (c0 + c + kTcStages - 1) * kTcCols;
+                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                mbar_expect_tx(arrived + 8 * next, kBlock);
+                tma_load_2d(to, &y_map, x, (int)t0, arrived + 8 * next);
+                tma_load_2d(to + kPart, &y_map, x + 64, (int)t0, arrived + 8 * next);
             }
-            Eight<Y> old[2][4];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int64_t o = o0 + half * 64 + h * 32 + 8 * t;
-                    const Y* from = y_row + o0 + h * 32 + i * 8 * p.ldy;
-                    if (!(rows >> i & 1)) continue;
-                    if (p.wide_y && o + 8 <= p.oc) {
-                        old[h][i].load(from);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (o + j < p.oc) old[h][i].v[j] = from[j];
-                    }
+            ok = mbar_wait(arrived + 8 * stage, block / kTcStages & 1);
+            for (int d = 0; d < n_ids; ++d, ++unit) {
+                const bool more = d + 1 < n_ids || c + 1 < n_c;
+                if (more) {
+                    load_b(d + 1 < n_ids ? c : c + 1, d + 1 < n_ids ? d + 1 : 0);
+                    put_b(unit + 1);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-            if (more) {
-                put_b(unit + 1);
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            }
-            tc_fence_before();
-            if (!__syncthreads_and(ok)) {
-                ok = false;
-                break;
-            }
-            if (threadIdx.x == 0 && more) multiply(unit + 1);
-            if (n_ids > 0) {
-                ok = mbar_wait(bar + 8 * (unit & 1), done >> (unit & 1) & 1);
-                done ^= 1u << (unit & 1);
+                tc_fence_before();
+                ok = __syncthreads_and(ok);
+                if (!ok) break;
+                if (threadIdx.x == 0 && more) multiply(unit + 1);
+                ok = mbar_wait(product + 8 * (unit & 1), unit >> 1 & 1);
                 tc_fence_after();
-            }
-            float* mine = way + warp * 32 * kPitch;
+                const bool takes = mine == s.distinct[d];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                __syncwarp();
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     float v[16];
-                    if (n_ids > 0) {
-                        tmem_ld16(tmem + (unit & 1) * kTcCols + half * 64 + h * 32 + 16 * j + ((uint32_t)(quarter * 32) << 16), v);
-                    } else {
+                    tmem_ld16(tmem + (unit & 1) * kTcCols + half * 64 + 16 * j + ((uint32_t)((warp & 3) * 32) << 16), v);
+                    if (!takes) continue;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                    }
+                    for (int h = 0; h < 2; ++h) {
+                        uint4* const place = reinterpret_cast<uint4*>(here + (((2 * j + h) ^ (row & 7)) << 4));
+                        Eight<T> old;
+                        old.raw = *place;
+                        float x[8];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<float4*>(mine + lane * kPitch + 16 * j + 4 * i) = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-                }
-                __syncwarp();
-                const int64_t o = o0 + half * 64 + h * 32 + 8 * t;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (!(rows >> i & 1)) continue;
-                    const float f = row_scale[quarter * 32 + g + 8 * i];
-                    const float4 u0 = *reinterpret_cast<const float4*>(mine + (g + 8 * i) * kPitch + 8 * t);
-                    const float4 u1 = *reinterpret_cast<const float4*>(mine + (g + 8 * i) * kPitch + 8 * t + 4);
-                    const float u[8] = {u0.x, u0.y, u0.z, u0.w, u1.x, u1.y, u1.z, u1.w};
-                    float x[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = fmaf(u[j], f, old[h][i].get(j));
-                    Y* to = out_row + o0 + h * 32 + i * 8 * p.ldo;
-                    if (p.wide_y && o + 8 <= p.oc) {
-                        Eight<Y>::store(to, x);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            if (o + j < p.oc) put(to + j, x[j]);
+                        for (int i = 0; i < 8; ++i) x[i] = fmaf(v[8 * h + i], f, old.get(i));
+                        Eight<T>::store(reinterpret_cast<T*>(place), x);
                     }
                 }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            ok = __syncthreads_and(ok);
+            if (threadIdx.x == 0 && ok) {
+                const uint32_t from = smem_u32(y_smem) + stage * kBlock;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(&out_map),
+                                 "r"((c0 + c) * kTcCols + 64 * h), "r"((int)t0), "r"(from + h * kPart)
+                                 : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
         }
-        ok = __syncthreads_and(ok);
     }
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (threadIdx.x == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if (!ok) report_device_error(p.err, 10);
     tc_fence_before();
     __syncthreads();
@@ -914,14 +908,26 @@ cudaError_t up(const Params& p, bool vec, dim3 grid, bool few, cudaStream_t s) {
     const size_t smem = (sizeof(Y) == 4 ? 3 : 2) * 32 * (ranks + 8) * sizeof(T) + (std::is_same<T, __half>::value ? 32 * ranks * 4 : 0);
     return vec ? start(k_lora_up<T, Y, true>, grid, smem, s, p) : start(k_lora_up<T, Y, false>, grid, smem, s, p);
 }
-template <typename T, typename Y>
-cudaError_t up_tc(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
-    const int padded = (p.rank + 15) / 16 * 16, parts = ((sizeof(Y) == 4 ? 3 : 2) * padded + 63) / 64;
-    const size_t smem = 1024 + parts * kTcRows * 128 + 2 * kTcCols * 128 + kWarps * 32 * 36 * sizeof(float);
-    return vec ? start(k_lora_up_tc<T, Y, true>, grid, smem, s, p) : start(k_lora_up_tc<T, Y, false>, grid, smem, s, p);
+template <typename T>
+int up_tc(const Params& p, bool vec, int grid, cudaStream_t s, const char* name) {
+    const int rc = tc::get_encoder();
+    if (rc) return rc;
+    CUtensorMap maps[2];
+    for (int i = 0; i < 2; ++i) {
+        const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        const int e = tc::encode_2d(&maps[i], type, i ? p.out : p.y, (uint64_t)p.oc, (uint64_t)p.tokens, (uint64_t)(i ? p.ldo : p.ldy) * 2, 64,
+                                    kTcRows, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (e) return e;
+    }
+    const int padded = (p.rank + 15) / 16 * 16, parts = (2 * padded + 63) / 64;
+    const size_t smem = 1024 + (2 * kTcStages + 2 + parts) * (size_t)kTcRows * 128;
+    auto kernel = vec ? k_lora_up_tc<T, true> : k_lora_up_tc<T, false>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) e = launch_overlapped(kernel, dim3((unsigned)grid), dim3(kThreads), smem, s, maps[0], maps[1], p);
+    return e == cudaSuccess ? SPARK_OK : set_error((int)e, "%s: %s", name, cudaGetErrorString(e));
 }
 template <typename T>
-cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t s) {
+int run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t s, const char* name) {
     const bool few = p.tokens <= kFew;
     {
         const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
@@ -930,25 +936,17 @@ cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaS
         p.slots = (int)std::min<int64_t>(p.slots, p.tokens);
         const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)(p.slots * p.rank_blocks));
         const cudaError_t e = few ? down<T, 1>(p, vec_down, grid, s) : down<T, 2>(p, vec_down, grid, s);
-        if (e != cudaSuccess) return e;
+        if (e != cudaSuccess) return set_error((int)e, "%s: launch failed: %s", name, cudaGetErrorString(e));
     }
     // few tiles are divided by their adapters too
     const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
     dim3 grid;
-    if (p.tokens >= kMany && p.rank <= kTcRank) {
-        const int64_t wide_tiles = (p.tokens + kTcRows - 1) / kTcRows;
+    // (the tensor maps' rows are on 16 bytes, apart)
+    if (p.tokens >= kMany && p.rank <= kTcRank && !wide && p.wide_y && p.ldy >= p.oc) {
         p.columns = (int)((p.oc + kTcCols - 1) / kTcCols);
-        // runs that leave the CTAs the least to do, a tile's beginning counting as a block
-        int64_t least = 0;
-        for (int run = 1, r = 1; r <= 16 && r <= p.columns; ++r) {
-            const int64_t items = wide_tiles * ((p.columns + r - 1) / r), time = (items + 2 * sms - 1) / (2 * sms) * (r + 1);
-            if (r == 1 || time < least) least = time, run = r;
-            p.run = run;
-        }
-        const int64_t items = wide_tiles * ((p.columns + p.run - 1) / p.run);
-        grid = dim3((unsigned)std::min<int64_t>(items, 2 * sms));
-        const cudaError_t e = wide ? up_tc<T, float>(p, vec_up, grid, s) : up_tc<T, T>(p, vec_up, grid, s);
-        if (e != cudaSuccess) return e;
+        const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
+        const int rc = up_tc<T>(p, vec_up, (int)std::min<int64_t>(blocks, sms), s, name);
+        if (rc) return rc;
         p.crowded = 1;
     }
     if (few) {
@@ -962,7 +960,8 @@ cudaError_t run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaS
         p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2 * sms / items));
         grid = dim3((unsigned)std::min<int64_t>(items, std::max(1, 2 * sms / p.slots)), (unsigned)p.slots);
     }
-    return wide ? up<T, float>(p, vec_up, grid, few, s) : up<T, T>(p, vec_up, grid, few, s);
+    const cudaError_t e = wide ? up<T, float>(p, vec_up, grid, few, s) : up<T, T>(p, vec_up, grid, few, s);
+    return e == cudaSuccess ? SPARK_OK : set_error((int)e, "%s: launch failed: %s", name, cudaGetErrorString(e));
 }
 
 }  // namespace lora
@@ -1015,9 +1014,9 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     const bool vec_down = p.ic % 8 == 0 && p.ldx % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16);
     const bool vec_up = p.rank % 8 == 0 && aligned(p.b, 16), wide = a->y_dtype == SPARK_DTYPE_F32;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    e = a->dtype == SPARK_DTYPE_BF16 ? run<__nv_bfloat16>(p, vec_down, vec_up, wide, sms, st)
-                                     : run<__half>(p, vec_down, vec_up, wide, sms, st);
-    if (e != cudaSuccess) return set_error((int)e, "%s: launch failed: %s", name, cudaGetErrorString(e));
+    const int rc = a->dtype == SPARK_DTYPE_BF16 ? run<__nv_bfloat16>(p, vec_down, vec_up, wide, sms, st, name)
+                                                : run<__half>(p, vec_down, vec_up, wide, sms, st, name);
+    if (rc) return rc;
     return check_launch(name);
 }
 
