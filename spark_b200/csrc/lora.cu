@@ -46,8 +46,9 @@ constexpr int kFewThreads = 128;
 constexpr int kMany = 256;     // tokens from which on
 constexpr int kTcRows = 128, kTcCols = 128;
 constexpr int kTcRank = 64;    // ranks up to which one 128-byte row of B holds them
-constexpr int kTcIds = 4;      // adapters of a tile; more: the other kernel's
-constexpr int kTcStages = 3;   // blocks of y
+constexpr int kTcIds = 2;      // adapters of a tile; more: the other kernel's
+constexpr int kTcStages = 4;   // blocks of y: one worked on, two on their way in, one on its way in or out
+constexpr int kTcThreads = 512;
 
 struct Params {
     const void *x, *a, *b, *y;
@@ -61,7 +62,7 @@ struct Params {
     int splits, slots;           // of the input's columns; of a tile's items, worked on side by side
     int rank_blocks, columns, run;   // first product: blocks of ranks; second: column blocks of kWarps * kColumns in y, of an item
     int wide_y;                  // rows of y and out on 16 bytes
-    int crowded;                 // only the tiles that the tensor memory's kernel leaves
+    int* crowded;                // their number, and the tiles that the tensor memory's kernel leaves; NULL: all are the other's
     float* h;                    // [splits, tokens, rank]
     int* err;
 };
@@ -212,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(co
     asm volatile("griddepcontrol.launch_dependents;");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int64_t t0 = (int64_t)blockIdx.x * ROWS;
+    if (p.crowded && blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *p.crowded = 0;
     const int split = blockIdx.y, r0 = (int)(blockIdx.z % p.rank_blocks) * RANKS, slot = blockIdx.z / p.rank_blocks;
     load_tile(s, p, t0, split == 0 && r0 == 0 && slot == 0);
     const T* x = reinterpret_cast<const T*>(p.x);
@@ -297,44 +299,48 @@ __global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(co
 }
 
 // f(row, rank, value) for the rows' h, summed over the splits; zeros behind the rank and where the row has no adapter (or is not in
-// `rows`).  Four ranks a thread where they lie on 16 bytes; the loads of four splits are on the way together.
+// `rows`).  Four ranks a thread where they lie on 16 bytes; four such loads are on the way together.
 template <int ROWS, int THREADS, typename F>
 __device__ __forceinline__ void sum_h(const Params& p, const int* ids, int64_t t0, unsigned rows, int chunks, F f) {
     const int64_t apart = p.tokens * p.rank;
-    if (p.rank % 4 == 0) {
-        for (int i = threadIdx.x; i < ROWS * chunks * 8; i += THREADS) {
-            const int row = i / (chunks * 8), r = (i - row * chunks * 8) * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (ids[row] >= 0 && (rows >> (row & 31) & 1) && r < p.rank) {
-                const float* from = p.h + (t0 + row) * p.rank + r;
-                for (int k0 = 0; k0 < p.splits; k0 += 4) {
-                    float4 u[4];
+    auto sum = [&](auto one, int n, int wide) {
+        using V = decltype(one);
+        constexpr int W = sizeof(V) / 4;
+        // four values of a thread at a time, or, where there are not that many, four splits of each
+        const int across = n > THREADS ? 4 : 1, along = 4 / across;
+        for (int i0 = threadIdx.x; i0 < n; i0 += across * THREADS) {
+            float v[4][W];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        u[k] = k0 + k < p.splits ? *reinterpret_cast<const float4*>(from + (k0 + k) * apart) : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v.x += u[k].x, v.y += u[k].y, v.z += u[k].z, v.w += u[k].w;
+                for (int e = 0; e < W; ++e) v[j][e] = 0.f;
+            for (int k0 = 0; k0 < p.splits; k0 += along) {
+                V u[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int i = i0 + (across > 1 ? j * THREADS : 0), k = k0 + (across > 1 ? 0 : j), row = i / wide, r = (i - row * wide) * W;
+                    const bool is = i < n && k < p.splits && ids[i < n ? row : 0] >= 0 && (rows >> (row & 31) & 1) && r < p.rank;
+                    u[j] = is ? *reinterpret_cast<const V*>(p.h + k * apart + (t0 + row) * p.rank + r) : V{};
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float e[W];
+                    memcpy(e, &u[j], sizeof(V));
+#pragma unroll
+                    for (int w = 0; w < W; ++w) (across > 1 ? v[j][w] : v[0][w]) += e[w];
                 }
             }
-            f(row, r, v.x), f(row, r + 1, v.y), f(row, r + 2, v.z), f(row, r + 3, v.w);
-        }
-        return;
-    }
-    for (int i = threadIdx.x; i < ROWS * chunks * 32; i += THREADS) {
-        const int row = i / (chunks * 32), r = i - row * chunks * 32;
-        float v = 0.f;
-        if (ids[row] >= 0 && (rows >> (row & 31) & 1) && r < p.rank) {
-            const float* from = p.h + (t0 + row) * p.rank + r;
-            for (int k0 = 0; k0 < p.splits; k0 += 4) {
-                float u[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) u[k] = k0 + k < p.splits ? from[(k0 + k) * apart] : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                const int i = i0 + j * THREADS, row = i / wide, r = (i - row * wide) * W;
+                if (j >= across || i >= n) break;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v += u[k];
+                for (int w = 0; w < W; ++w) f(row, r + w, v[j][w]);
             }
         }
-        f(row, r, v);
-    }
+    };
+    if (p.rank % 4 == 0) sum(float4{}, ROWS * chunks * 8, chunks * 8);
+    else sum(float{}, ROWS * chunks * 32, chunks * 32);
 }
 
 // 8 values of a row of y as floats, and back.
@@ -374,8 +380,8 @@ template <typename Y>
 __device__ __forceinline__ void put(Y* p, float v) { *p = Mma<Y>::round(v); }
 
 // out[t, :] = y[t, :] + scale B[a] h[t], for many tokens.  An item is a run of column blocks (kColumns for each warp) of a tile, with
-// every slots-th adapter and its rows.  Where these are more than one, a product has zeros in place of the others' rows, and y is
-// read and written once for all.  Tiles with several adapters take longer: their runs go to different CTAs.
+// every slots-th adapter and its rows: y is read for all of them at once, and written for each adapter's.  Tiles with several
+// adapters take longer: their runs go to different CTAs.
 template <typename T, typename Y, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__ Params p) {
     constexpr int MT = 2, ROWS = 16 * MT, TERMS = sizeof(Y) == 4 ? 3 : 2;
@@ -392,19 +398,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
     const Y* y = reinterpret_cast<const Y*>(p.y);
     Y* out = reinterpret_cast<Y*>(p.out);
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
+    constexpr int kInWide = kTcRows / ROWS;
     const int runs = (p.columns + p.run - 1) / p.run;
-    const int64_t items = (p.tokens + ROWS - 1) / ROWS * runs;
-    __shared__ WideTile around;
-    int64_t checked = -1;
     bool waited = false;
+    if (p.crowded) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        waited = true;
+    }
+    const int64_t items = (p.crowded ? (int64_t)*p.crowded * kInWide : (p.tokens + ROWS - 1) / ROWS) * runs;
     for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-        const int64_t tile = item / runs, t0 = tile * ROWS;
-        const int c0 = (int)(item - tile * runs) * p.run, n_c = min(p.run, p.columns - c0);
+        int64_t tile = item / runs;
+        if (p.crowded) tile = (int64_t)p.crowded[1 + tile / kInWide] * kInWide + tile % kInWide;
+        const int64_t t0 = tile * ROWS;
+        const int c0 = (int)(item % runs) * p.run, n_c = min(p.run, p.columns - c0);
         __syncthreads();      // (the last tile is done with)
-        if (p.crowded) {
-            if (t0 / kTcRows != checked) load_wide_tile(around, p, t0 / kTcRows * kTcRows), checked = t0 / kTcRows;
-            if (around.count <= kTcIds) continue;
-        }
+        if (t0 >= p.tokens) continue;
         load_tile(s, p, t0, false);
         // this slot's adapters, and a lane's rows (g, g + 8, ...) with one of them (or none, which is copied)
         const int slot = blockIdx.y;
@@ -511,54 +519,50 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
         }
         auto work = [&](int c, Eight<Y> (&old)[MT][2], Eight<Y> (&coming)[MT][2]) {
             load_old(coming, c + 1);
-            float acc[MT][4][4];
-#pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
-            auto products = [&](const uint4 (&w)[4], int j) {
-                const T* a = terms + g * width + (chunks == 1 ? 0 : j % chunks) * 32 + 8 * t;
-                const int id = mine_ids[chunks == 1 ? j : j / chunks];
-#pragma unroll
-                for (int q = 0; q < TERMS; ++q)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m, a += 16 * width) {
-                        uint4 lo = *reinterpret_cast<const uint4*>(a), hi = *reinterpret_cast<const uint4*>(a + 8 * width);
-                        if (n_ids > 1) {
-                            if (s.ids[m * 16 + g] != id) lo = make_uint4(0, 0, 0, 0);
-                            if (s.ids[m * 16 + 8 + g] != id) hi = make_uint4(0, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            Mma<T>::run(acc[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
-                            Mma<T>::run(acc[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
-                        }
-                    }
-            };
-            for (int j = 0; j < steps; ++j) {
-                products(w, j);
-                load_weights(w, c, j + 1);
-            }
             const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
             const bool whole = p.wide_y && o0 + 8 * t + 8 <= p.oc;
-            Y* to = out_row + o0;
+            for (int d = 0; d < max(n_ids, 1); ++d) {
+                const int id = n_ids > 0 ? mine_ids[d] : -1;
+                float acc[MT][4][4];
 #pragma unroll
-            for (int i = 0; i < 2 * MT; ++i, to += 8 * p.ldo) {
-                if (!(rows >> i & 1)) continue;
-                const float f = row_scale[i * 8 + g];
-                const float(&v)[4][4] = acc[i / 2];
-                const int e = i % 2;
-                float x[8];
+                for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
-                if (whole) {
-                    Eight<Y>::store(to, x);
-                } else {
+                    for (int n = 0; n < 4; ++n)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (o0 + 8 * t + j < p.oc) put(to + j, x[j]);
+                        for (int j = 0; j < 4; ++j) acc[m][n][j] = 0.f;
+                for (int k = 0; k < chunks && n_ids > 0; ++k) {
+                    const T* a = terms + g * width + k * 32 + 8 * t;
+#pragma unroll
+                    for (int q = 0; q < TERMS; ++q)
+#pragma unroll
+                        for (int m = 0; m < MT; ++m, a += 16 * width) {
+                            const uint4 lo = *reinterpret_cast<const uint4*>(a), hi = *reinterpret_cast<const uint4*>(a + 8 * width);
+#pragma unroll
+                            for (int n = 0; n < 4; ++n) {
+                                Mma<T>::run(acc[m][n], lo.x, hi.x, lo.y, hi.y, w[n].x, w[n].y);
+                                Mma<T>::run(acc[m][n], lo.z, hi.z, lo.w, hi.w, w[n].z, w[n].w);
+                            }
+                        }
+                    load_weights(w, c, d * chunks + k + 1);
+                }
+                Y* to = out_row + o0;
+#pragma unroll
+                for (int i = 0; i < 2 * MT; ++i, to += 8 * p.ldo) {
+                    const int its = s.ids[i * 8 + g];
+                    if (!(rows >> i & 1) || (its != id && (its >= 0 || d > 0))) continue;
+                    const float f = row_scale[i * 8 + g];
+                    const float(&v)[4][4] = acc[i / 2];
+                    const int e = i % 2;
+                    float x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = its < 0 ? old[i / 2][e].get(j) : fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
+                    if (whole) {
+                        Eight<Y>::store(to, x);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            if (o0 + 8 * t + j < p.oc) put(to + j, x[j]);
+                    }
                 }
             }
         };
@@ -573,11 +577,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
 
 // The same on the tensor memory, for many tokens of few adapters a tile.  D [128 tokens, 128 columns] = A B^T with the rows of h in A
 // (its two terms side by side along K) and 128 rows of B[a], both in shared memory in 128-byte rows, swizzled.  Blocks of y come two
-// ahead by TMA, in the same layout; a lane, which has a row of D, adds to its row of the block, and the block leaves by TMA.  While
-// that is done for one adapter of a block, the next one's B arrives and is multiplied into the other half of the tensor memory.
-// Rows without an adapter go out as they came in.  Bound by memory: the products take a tenth of the time.
+// ahead by TMA, in the same layout; a lane, which has a row of D, adds to its row of the block, and the block leaves by TMA.
+// Meanwhile the next step's B arrives and is multiplied, into another part of the tensor memory.  Of a tile's two adapters each has a
+// D of all rows, from which a lane takes its own: an infinity in one adapter is nothing to the other's rows.  Rows without an adapter
+// go out as they came in.  Bound by memory: the products take a tenth of the time.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__ CUtensorMap y_map, const __grid_constant__ CUtensorMap out_map,
+__global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant__ CUtensorMap y_map, const __grid_constant__ CUtensorMap out_map,
                                                          const __grid_constant__ Params p) {
     using namespace tcx;
     constexpr int TERMS = 2;
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
     constexpr uint32_t kTypes = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
     constexpr uint32_t kIdesc = (1u << 4) | kTypes | ((uint32_t)(kTcCols >> 3) << 17) | ((uint32_t)(kTcRows >> 4) << 24);
     constexpr int kPart = kTcRows * 128, kBlock = 2 * kPart;      // bytes of 128 rows of 64 values, of a block of y
-    constexpr int kWeights = kTcCols * kTcRank * 2 / 16 / kThreads;
+    constexpr int kWeights = kTcCols * kTcRank * 2 / 16 / kTcThreads;
     extern __shared__ uint8_t smem_raw[];
     __shared__ WideTile s;
     __shared__ float row_scale[kTcRows];
@@ -594,8 +599,8 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int padded = (p.rank + 15) / 16 * 16, parts_a = (TERMS * padded + 63) / 64;
     uint8_t* const y_smem = smem;                                // [kTcStages]
-    uint8_t* const b_smem = y_smem + kTcStages * kBlock;         // [2]
-    uint8_t* const a_smem = b_smem + 2 * kPart;
+    uint8_t* const b_smem = y_smem + kTcStages * kBlock;         // [2, kTcIds]
+    uint8_t* const a_smem = b_smem + 2 * kTcIds * kPart;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t product = smem_u32(&bars[0]), arrived = smem_u32(&bars[2]);
     asm volatile("griddepcontrol.launch_dependents;");
@@ -604,7 +609,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(2 * kTcCols) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(2 * kTcIds * kTcCols) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
@@ -615,7 +620,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
     const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
     const int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
     bool waited = false, ok = true;
-    uint32_t block = 0, unit = 0;      // so far: blocks, and products (one for each adapter of a block)
+    uint32_t block = 0, products = 0;      // blocks so far; parities of the products waited for
     for (int64_t at = lo; at < hi && ok;) {
         const int64_t tile = at / p.columns, t0 = tile * kTcRows;
         const int c0 = (int)(at - tile * p.columns), n_c = (int)min((int64_t)(p.columns - c0), hi - at);
@@ -623,17 +628,24 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
         __syncthreads();      // (the last tile is done with)
         load_wide_tile(s, p, t0);
         const int n_ids = s.count;
+        if (!waited && n_ids > kTcIds) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+        }
+        if (n_ids > kTcIds && c0 == 0 && threadIdx.x == 0) p.crowded[1 + atomicAdd(p.crowded, 1)] = (int)tile;
         if (n_ids > kTcIds || (n_ids == 0 && p.y == p.out)) continue;
-        // block c of this tile into the next stage; what left that stage has to have been read
-        auto fetch = [&](int c) {
-            const uint32_t stage = (block + c) % kTcStages, to = smem_u32(y_smem) + stage * kBlock;
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        // block c of the tile, number `to`, into its stage; what left that stage has been read: all copies out but the last one have
+        auto fetch = [&](int c, uint32_t to) {
+            const uint32_t stage = to % kTcStages, at_smem = smem_u32(y_smem) + stage * kBlock;
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             mbar_expect_tx(arrived + 8 * stage, kBlock);
-            tma_load_2d(to, &y_map, (c0 + c) * kTcCols, (int)t0, arrived + 8 * stage);
-            tma_load_2d(to + kPart, &y_map, (c0 + c) * kTcCols + 64, (int)t0, arrived + 8 * stage);
+            tma_load_2d(at_smem, &y_map, (c0 + c) * kTcCols, (int)t0, arrived + 8 * stage);
+            tma_load_2d(at_smem + kPart, &y_map, (c0 + c) * kTcCols + 64, (int)t0, arrived + 8 * stage);
         };
-        if (threadIdx.x == 0)
-            for (int c = 0; c < kTcStages - 1 && c < n_c; ++c) fetch(c);
+        if (threadIdx.x == 0) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            for (int c = 0; c < kTcStages - 1 && c < n_c; ++c) fetch(c, block + c);
+        }
         if (!waited) {
             // (y was ready before the first product, and could be read before that ends)
             asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -641,11 +653,12 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
         }
         // A: value (row, k) of the terms, 16 bytes of a row exchanged by its number
         auto put_terms = [&](int row, int r, float v) {
+            uint8_t* const to = a_smem + row * 128;
 #pragma unroll
             for (int q = 0; q < TERMS; ++q) {
                 const T x = Mma<T>::round(v);
                 const int k = q * padded + r, in = k & 63;
-                *reinterpret_cast<T*>(a_smem + (k >> 6) * kPart + row * 128 + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
+                *reinterpret_cast<T*>(to + (k >> 6) * kPart + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
                 const float f = (float)x;
                 v = fabsf(f) < INFINITY ? v - f : 0.f;
             }
@@ -655,7 +668,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
         float* const sums = reinterpret_cast<float*>(y_smem + (block + kTcStages - 1) % kTcStages * kBlock);
         if (kScaled) __syncthreads();
         if (n_ids > 0)
-            sum_h<kTcRows, kThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
+            sum_h<kTcRows, kTcThreads>(p, s.ids, t0, 0xffffffffu, chunks, [&](int row, int r, float v) {
                 if (kScaled) sums[row * ranks + r] = v;
                 else if (r < padded) put_terms(row, r, v);
             });
@@ -665,7 +678,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
         }
         if (kScaled && n_ids > 0) {
             __syncthreads();
-            for (int row = warp; row < kTcRows; row += kWarps) {
+            for (int row = warp; row < kTcRows; row += kTcThreads / 32) {
                 float most = 0.f;
                 for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(sums[row * ranks + r]));
 #pragma unroll
@@ -676,83 +689,90 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
                 for (int r = lane; r < padded; r += 32) put_terms(row, r, sums[row * ranks + r] * up);
             }
         }
-        uint4 w[kWeights];     // this thread's part of a block's B: 16 bytes of a column
-        auto load_b = [&](int c, int d) {
+        uint4 w[kTcIds][kWeights];     // this thread's part of a block's B: 16 bytes of a column
+        auto load_b = [&](int c) {
             const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
-            const T* b = bb.begin + ((int64_t)s.distinct[d] * p.oc + o0) * p.rank;
 #pragma unroll
-            for (int j = 0; j < kWeights; ++j) {
-                const int i = j * kThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
-                w[j] = o0 + col < p.oc ? load8<T, VEC>(b + col * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
-            }
-        };
-        auto put_b = [&](uint32_t u) {
-            uint8_t* to = b_smem + (u & 1) * kPart;
+            for (int d = 0; d < kTcIds; ++d) {
+                if (d >= n_ids || c >= n_c) break;
+                const T* b = bb.begin + ((int64_t)s.distinct[d] * p.oc + o0) * p.rank;
 #pragma unroll
-            for (int j = 0; j < kWeights; ++j) {
-                const int i = j * kThreads + threadIdx.x, col = i >> 3, k = i & 7;
-                if (k * 8 < padded) *reinterpret_cast<uint4*>(to + col * 128 + ((k ^ (col & 7)) << 4)) = w[j];
-            }
-        };
-        auto multiply = [&](uint32_t u) {
-            const uint32_t d = tmem + (u & 1) * kTcCols, b = smem_u32(b_smem) + (u & 1) * kPart;
-            tc_fence_after();
-            for (int q = 0; q < TERMS; ++q)
-                for (int k = 0; k < padded; k += 16) {
-                    const int ka = q * padded + k;
-                    const uint64_t da = sdesc_sw128(smem_u32(a_smem) + (ka >> 6) * kPart + (ka & 63) * 2), db = sdesc_sw128(b + k * 2);
-                    asm volatile(
-                        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-                        "l"(da), "l"(db), "r"(kIdesc), "r"((uint32_t)(q + k > 0))
-                        : "memory");
+                for (int j = 0; j < kWeights; ++j) {
+                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
+                    w[d][j] = o0 + col < p.oc ? load8<T, VEC>(b + col * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
                 }
-            mma_commit(product + 8 * (u & 1));
+            }
         };
-        if (n_ids > 0) {
-            load_b(0, 0);
-            put_b(unit);
-        }
+        auto put_b = [&](uint32_t to) {
+#pragma unroll
+            for (int d = 0; d < kTcIds; ++d) {
+                if (d >= n_ids) break;
+                uint8_t* const at_smem = b_smem + ((to & 1) * kTcIds + d) * kPart;
+#pragma unroll
+                for (int j = 0; j < kWeights; ++j) {
+                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = i & 7;
+                    if (k * 8 < padded) *reinterpret_cast<uint4*>(at_smem + col * 128 + ((k ^ (col & 7)) << 4)) = w[d][j];
+                }
+            }
+        };
+        // block number `to`
+        auto multiply = [&](uint32_t to) {
+            tc_fence_after();
+            for (int d = 0; d < n_ids; ++d) {
+                const uint32_t part = (to & 1) * kTcIds + d, a = smem_u32(a_smem), b = smem_u32(b_smem) + part * kPart;
+                for (int q = 0; q < TERMS; ++q)
+                    for (int k = 0; k < padded; k += 16) {
+                        const int ka = q * padded + k;
+                        const uint64_t da = sdesc_sw128(a + (ka >> 6) * kPart + (ka & 63) * 2), db = sdesc_sw128(b + k * 2);
+                        asm volatile(
+                            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + part * kTcCols),
+                            "l"(da), "l"(db), "r"(kIdesc), "r"((uint32_t)(q + k > 0))
+                            : "memory");
+                    }
+            }
+            mma_commit(product + 8 * (to & 1));
+        };
+        // a block's product begins two blocks before it is read back, and its B comes through registers one more before
+        load_b(0);
+        put_b(block);
+        load_b(1);
+        put_b(block + 1);
+        load_b(2);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
-        if (threadIdx.x == 0 && n_ids > 0) multiply(unit);
-        // a lane's row: one of the 32 of its warp's quarter of the tensor memory; half of a block's columns
-        const int half = warp >> 2, row = (warp & 3) * 32 + lane, mine = s.ids[row];
+        if (threadIdx.x == 0 && n_ids > 0) {
+            multiply(block);
+            if (n_c > 1) multiply(block + 1);
+        }
+        // a lane's row: one of the 32 of its warp's quarter of the tensor memory; a quarter of a block's columns
+        const int across = warp >> 2, row = (warp & 3) * 32 + lane, mine = s.ids[row];
+        const bool second = n_ids > 1 && mine == s.distinct[1];
         const float f = row_scale[row];
-        for (int c = 0; c < n_c && ok; ++c, ++block) {
+        for (int c = 0; c < n_c; ++c, ++block) {
             const uint32_t stage = block % kTcStages;
-            uint8_t* const here = y_smem + stage * kBlock + half * kPart + row * 128;
-            if (threadIdx.x == 0 && c + kTcStages - 1 < n_c) {
-                // (block counts from this one on: c blocks of the tile are behind)
-                const uint32_t next = (block + kTcStages - 1) % kTcStages, to = smem_u32(y_smem) + next * kBlock;
-                const int x = (c0 + c + kTcStages - 1) * kTcCols;
-                asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                mbar_expect_tx(arrived + 8 * next, kBlock);
-                tma_load_2d(to, &y_map, x, (int)t0, arrived + 8 * next);
-                tma_load_2d(to + kPart, &y_map, x + 64, (int)t0, arrived + 8 * next);
-            }
+            uint8_t* const here = y_smem + stage * kBlock + (across >> 1) * kPart + row * 128;
             ok = mbar_wait(arrived + 8 * stage, block / kTcStages & 1);
-            for (int d = 0; d < n_ids; ++d, ++unit) {
-                const bool more = d + 1 < n_ids || c + 1 < n_c;
-                if (more) {
-                    load_b(d + 1 < n_ids ? c : c + 1, d + 1 < n_ids ? d + 1 : 0);
-                    put_b(unit + 1);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                }
-                tc_fence_before();
-                ok = __syncthreads_and(ok);
-                if (!ok) break;
-                if (threadIdx.x == 0 && more) multiply(unit + 1);
-                ok = mbar_wait(product + 8 * (unit & 1), unit >> 1 & 1);
+            if (n_ids > 0) {
+                ok = mbar_wait(product + 8 * (block & 1), products >> (block & 1) & 1) && ok;
+                products ^= 1u << (block & 1);
                 tc_fence_after();
-                const bool takes = mine == s.distinct[d];
+            }
+            if (n_ids > 0 && __all_sync(0xffffffffu, ok)) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t from = tmem + (block & 1) * kTcIds * kTcCols + across * 32 + 16 * j + ((uint32_t)((warp & 3) * 32) << 16);
                     float v[16];
-                    tmem_ld16(tmem + (unit & 1) * kTcCols + half * 64 + 16 * j + ((uint32_t)((warp & 3) * 32) << 16), v);
-                    if (!takes) continue;
+                    tmem_ld16(from, v);
+                    if (n_ids > 1) {
+                        float u[16];
+                        tmem_ld16(from + kTcCols, u);
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i] = second ? u[i] : v[i];
+                    }
+                    if (mine < 0) continue;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        uint4* const place = reinterpret_cast<uint4*>(here + (((2 * j + h) ^ (row & 7)) << 4));
+                        uint4* const place = reinterpret_cast<uint4*>(here + ((((across & 1) * 4 + 2 * j + h) ^ (row & 7)) << 4));
                         Eight<T> old;
                         old.raw = *place;
                         float x[8];
@@ -761,10 +781,13 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
                         Eight<T>::store(reinterpret_cast<T*>(place), x);
                     }
                 }
+                tc_fence_before();
             }
+            if (c + 2 < n_c) put_b(block + 2);     // (this block's product is done with its B)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             ok = __syncthreads_and(ok);
-            if (threadIdx.x == 0 && ok) {
+            if (!ok) break;
+            if (threadIdx.x == 0) {
                 const uint32_t from = smem_u32(y_smem) + stage * kBlock;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -772,7 +795,10 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
                                  "r"((c0 + c) * kTcCols + 64 * h), "r"((int)t0), "r"(from + h * kPart)
                                  : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                if (n_ids > 0 && c + 2 < n_c) multiply(block + 2);
+                if (c + kTcStages - 1 < n_c) fetch(c + kTcStages - 1, block + kTcStages - 1);
             }
+            load_b(c + 3);
         }
     }
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -782,7 +808,7 @@ __global__ void __launch_bounds__(kThreads) k_lora_up_tc(const __grid_constant__
     __syncthreads();
     if (warp == 0) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTcCols) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * kTcIds * kTcCols) : "memory");
     }
 }
 
@@ -867,7 +893,7 @@ __global__ void __launch_bounds__(kFewThreads, 5) k_lora_up_few(const __grid_con
         if (o >= p.oc || (id < 0 && in_place)) continue;
 #pragma unroll
         for (int r = 0; r < ROWS; ++r)
-            if (mine >> r & 1) put(out + r * p.ldo, fmaf(acc[r], row_scale[r], (float)old[r]));
+            if (mine >> r & 1) put(out + r * p.ldo, id < 0 ? (float)old[r] : fmaf(acc[r], row_scale[r], (float)old[r]));
     }
 }
 
@@ -876,6 +902,12 @@ int splits_of(int64_t tokens, int64_t ic, int64_t rank, int sms) {
     const int64_t rows = tokens <= kFew ? 16 : 32, tiles = (tokens + rows - 1) / rows * ((rank + 63) / 64);
     const int64_t most = std::max<int64_t>(1, ic / (32 * kWarps));
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 16), 2 * sms / tiles));
+}
+
+// The workspace: h, then the crowded tiles.
+size_t h_bytes(int64_t tokens, int64_t rank, int splits) { return ((size_t)splits * tokens * rank * sizeof(float) + 15) / 16 * 16; }
+size_t workspace_bytes_of(int64_t tokens, int64_t rank, int splits) {
+    return h_bytes(tokens, rank, splits) + (tokens >= kMany ? (1 + (tokens + kTcRows - 1) / kTcRows) * sizeof(int) : 0);
 }
 
 template <typename F>
@@ -920,10 +952,10 @@ int up_tc(const Params& p, bool vec, int grid, cudaStream_t s, const char* name)
         if (e) return e;
     }
     const int padded = (p.rank + 15) / 16 * 16, parts = (2 * padded + 63) / 64;
-    const size_t smem = 1024 + (2 * kTcStages + 2 + parts) * (size_t)kTcRows * 128;
+    const size_t smem = 1024 + (2 * kTcStages + 2 * kTcIds + parts) * (size_t)kTcRows * 128;
     auto kernel = vec ? k_lora_up_tc<T, true> : k_lora_up_tc<T, false>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = launch_overlapped(kernel, dim3((unsigned)grid), dim3(kThreads), smem, s, maps[0], maps[1], p);
+    if (e == cudaSuccess) e = launch_overlapped(kernel, dim3((unsigned)grid), dim3(kTcThreads), smem, s, maps[0], maps[1], p);
     return e == cudaSuccess ? SPARK_OK : set_error((int)e, "%s: %s", name, cudaGetErrorString(e));
 }
 template <typename T>
@@ -941,13 +973,11 @@ int run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t 
     // few tiles are divided by their adapters too
     const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
     dim3 grid;
-    // (the tensor maps' rows are on 16 bytes, apart)
-    if (p.tokens >= kMany && p.rank <= kTcRank && !wide && p.wide_y && p.ldy >= p.oc) {
+    if (p.crowded) {
         p.columns = (int)((p.oc + kTcCols - 1) / kTcCols);
         const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
         const int rc = up_tc<T>(p, vec_up, (int)std::min<int64_t>(blocks, sms), s, name);
         if (rc) return rc;
-        p.crowded = 1;
     }
     if (few) {
         const int64_t columns = (p.oc + kFewThreads - 1) / kFewThreads;
@@ -973,7 +1003,7 @@ size_t spark_lora_workspace_size(int64_t tokens, int64_t ic, int64_t rank) {
     using namespace spark;
     int dev = 0;
     if (tokens <= 0 || ic <= 0 || rank <= 0 || cudaGetDevice(&dev) != cudaSuccess) return 0;
-    return (size_t)lora::splits_of(tokens, ic, rank, tc::sm_count_cached(dev)) * tokens * rank * sizeof(float);
+    return lora::workspace_bytes_of(tokens, rank, lora::splits_of(tokens, ic, rank, tc::sm_count_cached(dev)));
 }
 
 int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int* err, void* stream) {
@@ -999,7 +1029,7 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     const int sms = tc::sm_count_cached(dev);
     Params p{};
     p.splits = splits_of(a->tokens, a->ic, a->rank, sms);
-    const size_t need = (size_t)p.splits * a->tokens * a->rank * sizeof(float);
+    const size_t need = workspace_bytes_of(a->tokens, a->rank, p.splits);
     SPARK_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), SPARK_ERR_WORKSPACE,
                   "%s: workspace of %zu bytes on 16, %zu needed", name, workspace_bytes, need);
     p.x = a->x, p.a = a->a, p.b = a->b, p.y = a->y, p.out = a->out, p.adapter = a->adapter, p.scale = a->scale;
@@ -1013,6 +1043,9 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     p.wide_y = aligned(p.y, 16) && aligned(p.out, 16) && p.ldy % items == 0 && p.ldo % items == 0;
     const bool vec_down = p.ic % 8 == 0 && p.ldx % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16);
     const bool vec_up = p.rank % 8 == 0 && aligned(p.b, 16), wide = a->y_dtype == SPARK_DTYPE_F32;
+    // (the tensor maps' rows are on 16 bytes, apart)
+    if (p.tokens >= kMany && p.rank <= kTcRank && !wide && p.wide_y && p.ldy >= p.oc)
+        p.crowded = reinterpret_cast<int*>(reinterpret_cast<char*>(workspace) + h_bytes(p.tokens, p.rank, p.splits));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int rc = a->dtype == SPARK_DTYPE_BF16 ? run<__nv_bfloat16>(p, vec_down, vec_up, wide, sms, st, name)
                                                 : run<__half>(p, vec_down, vec_up, wide, sms, st, name);

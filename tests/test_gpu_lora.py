@@ -178,6 +178,25 @@ def test_scales_of_activations(dtype):
     assert not torch.isfinite(out[7]).any() and torch.isnan(out[9]).all() and torch.isfinite(out[8]).all()
 
 
+@pytest.mark.parametrize("tokens", [1, 40, 100, 700])
+def test_infinities_stay_with_their_adapter(tokens):
+    """An adapter whose weights hold infinities and NaN beside others in the same tiles; so does a token's x, and y without an adapter."""
+    y, x, a, b, _, scale = make(9, tokens, 128, 136, 16, 3, BF)
+    ids = (torch.arange(tokens, device="cuda") * 2 // 64 % 4 - 1).to(torch.int32)
+    ids[::7] = 2
+    a[1, 3, 5], b[1, 20], b[1, :, 2] = float("inf"), float("nan"), float("-inf")
+    x[tokens // 2, 0] = float("nan")
+    bad = ids == 1
+    bad[tokens // 2] = ids[tokens // 2] >= 0
+    y[ids < 0, 0] = float("inf")
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    good = ~bad & (ids >= 0)
+    assert torch.equal(out[ids < 0], y[ids < 0])
+    if good.any():
+        check(y[good], x[good], a, b, ids[good], scale, out[good])
+    assert torch.isnan(out[bad][:, 20]).all()
+
+
 def test_refusals():
     from spark_b200._lib import SparkError
     y, x, a, b, ids, scale = make(6, 12, 64, 32, 8, 3, BF)
