@@ -1,21 +1,32 @@
 // lora.cu -- low-rank adapters of many requests beside a shared projection:
 //     out[t] = y[t] + scale[a] B[a] (A[a] x[t]),   a = the adapter of token t.
 //
-// Two launches: h = A x (fp32, split over the input's columns), then B h on top of y.
-// Tokens are taken in tiles of consecutive rows; a tile's items are its distinct
-// adapters: mma.sync of all its rows with that adapter's weights, of which the rows
-// that have the adapter are kept.  Tokens of a request lie together, so that a
-// prompt's tile has one or two of them, and a decoding batch's sixteen cost no more
-// than reading each adapter once: no sorting, and what a row gets does not depend on
-// its neighbours.  The work is bound by memory (r <= 128 needs at most 2 r flop a byte of y), which
-// mma.sync can feed; tcgen05 would want 128 rows of one adapter.
+// Two launches: h = A x (fp32, split over the input's columns where there are few
+// tokens), then B h on top of y.  Tokens are taken in tiles of consecutive rows; a
+// tile's items are its distinct adapters: the product of all its rows with that
+// adapter's weights, of which the rows that have the adapter are kept.  Tokens of a
+// request lie together, so that a prompt's tile has one or two of them, and a decoding
+// batch's sixteen cost no more than reading each adapter once: nothing is sorted, and
+// nothing of an adapter reaches another one's rows.
+//
+// Bound by memory: x, y in and out, and the weights of the adapters once.  The second product
+// has three forms:
+//   k_lora_up_tc   many tokens: tcgen05, 128 tokens and columns a block, y by TMA in and
+//                  out.  4096 tokens, rank 32, 2560 to 9728: 57 us in all (27 us more for 4096 more: 6
+//                  TB/s; 11 us are the first product, 15 the beginning), five requests 66 us.
+//   k_lora_up      the tiles that have more adapters than that takes, fp32 y, rows off 16
+//                  bytes: mma.sync from registers.  All tiles so: 79 and 93 us.
+//   k_lora_up_few  few tokens, most with an adapter of their own: no tensor cores, where 15 of 16 rows
+//                  would be computed for nothing.  48 requests 15 us, one token 6.7 us.
+// The first product is mma.sync throughout: rank rows are too few for tcgen05's tiles,
+// and at up to 2 x 256 flop a value of x the tensor cores are not what it waits for.
 //
 // Fragments come straight from memory: the order of a contraction's terms is free, so
 // that a lane takes 8 consecutive values of a row (16 bytes) as its share of two
-// steps, and in the second product the columns of a lane are 8 consecutive ones of y.
+// steps, and in k_lora_up the columns of a lane are 8 consecutive ones of y.
 //
-// h is in fp32 and meets B in 16 bits: it is split into two (y in 16 bits) or three
-// (fp32) terms of B's type, which together are good to 2^-17 or 2^-23 of it; for f16,
+// h is in fp32 and meets B in 16 bits on the tensor cores: it is split into two (y in 16 bits) or
+// three (fp32) terms of B's type, which together are good to 2^-17 or 2^-23 of it; for f16,
 // whose exponents are few, a row is brought to 2^14 by a power of 2 first.
 #include <math.h>
 #include <string.h>
@@ -39,11 +50,13 @@ namespace lora {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
+constexpr int kRanks = 32;     // of a CTA of the first product (64 leave an SM one CTA: 512 tokens of rank 128 28.6 us instead of 21.6)
 constexpr int kColumns = 32;   // of y, by one warp at a time
 constexpr int kFew = 64;       // tokens up to which tiles have 16 rows, and B h is computed without tensor cores
 constexpr int kFewThreads = 128;
 // B h on the tensor memory, for tiles of 128 tokens that are not crowded
-constexpr int kMany = 256;     // tokens from which on
+constexpr int kMany = 256;     // tokens from which on, and values of y: below, its beginning takes longer than it saves (measured, us
+constexpr int64_t kManyValues = 1 << 23;   // without / with: 1024 x 1024 11 / 20, 512 x 9728 22.6 / 23.5, 1024 x 9728 39 / 30, 4096 x 9728 79 / 57)
 constexpr int kTcRows = 128, kTcCols = 128;
 constexpr int kTcRank = 64;    // ranks up to which one 128-byte row of B holds them
 constexpr int kTcIds = 2;      // adapters of a tile; more: the other kernel's
@@ -204,7 +217,7 @@ __device__ __forceinline__ void load_wide_tile(WideTile& s, const Params& p, int
 
 // h[split, t, :] = A[a] x[t] over the split's columns.  The warps of a CTA take chunks of 32 columns in turn.
 template <typename T, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) k_lora_down(const __grid_constant__ Params p) {
     constexpr int ROWS = 16 * MT, RANKS = 8 * NT;
     __shared__ Tile<ROWS> s;
     extern __shared__ float part[];   // [kWarps, ROWS, RANKS]
@@ -256,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, MT * NT < 16 ? 2 : 1) k_lora_down(co
                     Mma<T>::run(acc[m][n], q.u[m][0].z, q.u[m][1].z, q.u[m][0].w, q.u[m][1].w, q.w[n].z, q.w[n].w);
                 }
         };
-        // (zeros behind the end: the loop may run one part further)
+        // (zeros behind the end: the loop may run one part further; two parts at once take the registers of a second CTA with more)
         const int64_t step = (int64_t)p.splits * kWarps * 32;
         int64_t k = ((int64_t)split * kWarps + warp) * 32 + 8 * t;
         if constexpr (MT * NT <= 4) {
@@ -597,7 +610,7 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
     __shared__ __align__(8) uint64_t bars[2 + kTcStages];
     __shared__ uint32_t s_tmem;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const int padded = (p.rank + 15) / 16 * 16, parts_a = (TERMS * padded + 63) / 64;
+    const int padded = (p.rank + 15) / 16 * 16;
     uint8_t* const y_smem = smem;                                // [kTcStages]
     uint8_t* const b_smem = y_smem + kTcStages * kBlock;         // [2, kTcIds]
     uint8_t* const a_smem = b_smem + 2 * kTcIds * kPart;
@@ -618,7 +631,12 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
     const uint32_t tmem = s_tmem;
     const Span<T> bb{reinterpret_cast<const T*>(p.b), reinterpret_cast<const T*>(p.b) + p.adapters * p.oc * p.rank};
     const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
-    const int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
+    // a CTA's blocks: an equal share of them all, or of one of its tile's `run` shares
+    int64_t lo = blocks * blockIdx.x / gridDim.x, hi = blocks * (blockIdx.x + 1) / gridDim.x;
+    if (p.run > 0) {
+        const int64_t tile = blockIdx.x / p.run, part = blockIdx.x % p.run;
+        lo = tile * p.columns + p.columns * part / p.run, hi = tile * p.columns + p.columns * (part + 1) / p.run;
+    }
     bool waited = false, ok = true;
     uint32_t block = 0, products = 0;      // blocks so far; parities of the products waited for
     for (int64_t at = lo; at < hi && ok;) {
@@ -646,6 +664,36 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             for (int c = 0; c < kTcStages - 1 && c < n_c; ++c) fetch(c, block + c);
         }
+        // this thread's part of a block's B: 16 bytes of a column
+        using Weights = uint4[kTcIds][kWeights];
+        auto load_b = [&](Weights& w, int c) {
+            const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
+#pragma unroll
+            for (int d = 0; d < kTcIds; ++d) {
+                if (d >= n_ids || c >= n_c) break;
+                const T* b = bb.begin + ((int64_t)s.distinct[d] * p.oc + o0) * p.rank;
+#pragma unroll
+                for (int j = 0; j < kWeights; ++j) {
+                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
+                    w[d][j] = o0 + col < p.oc ? load8<T, VEC>(b + col * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
+                }
+            }
+        };
+        auto put_b = [&](const Weights& w, uint32_t to) {
+#pragma unroll
+            for (int d = 0; d < kTcIds; ++d) {
+                if (d >= n_ids) break;
+                uint8_t* const at_smem = b_smem + ((to & 1) * kTcIds + d) * kPart;
+#pragma unroll
+                for (int j = 0; j < kWeights; ++j) {
+                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = i & 7;
+                    if (k * 8 < padded) *reinterpret_cast<uint4*>(at_smem + col * 128 + ((k ^ (col & 7)) << 4)) = w[d][j];
+                }
+            }
+        };
+        Weights w, first;
+        load_b(first, 0);
+        load_b(w, 1);
         if (!waited) {
             // (y was ready before the first product, and could be read before that ends)
             asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -689,32 +737,6 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
                 for (int r = lane; r < padded; r += 32) put_terms(row, r, sums[row * ranks + r] * up);
             }
         }
-        uint4 w[kTcIds][kWeights];     // this thread's part of a block's B: 16 bytes of a column
-        auto load_b = [&](int c) {
-            const int64_t o0 = (int64_t)(c0 + c) * kTcCols;
-#pragma unroll
-            for (int d = 0; d < kTcIds; ++d) {
-                if (d >= n_ids || c >= n_c) break;
-                const T* b = bb.begin + ((int64_t)s.distinct[d] * p.oc + o0) * p.rank;
-#pragma unroll
-                for (int j = 0; j < kWeights; ++j) {
-                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = (i & 7) * 8;
-                    w[d][j] = o0 + col < p.oc ? load8<T, VEC>(b + col * p.rank, k, p.rank, bb) : make_uint4(0, 0, 0, 0);
-                }
-            }
-        };
-        auto put_b = [&](uint32_t to) {
-#pragma unroll
-            for (int d = 0; d < kTcIds; ++d) {
-                if (d >= n_ids) break;
-                uint8_t* const at_smem = b_smem + ((to & 1) * kTcIds + d) * kPart;
-#pragma unroll
-                for (int j = 0; j < kWeights; ++j) {
-                    const int i = j * kTcThreads + threadIdx.x, col = i >> 3, k = i & 7;
-                    if (k * 8 < padded) *reinterpret_cast<uint4*>(at_smem + col * 128 + ((k ^ (col & 7)) << 4)) = w[d][j];
-                }
-            }
-        };
         // block number `to`
         auto multiply = [&](uint32_t to) {
             tc_fence_after();
@@ -733,11 +755,9 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
             mma_commit(product + 8 * (to & 1));
         };
         // a block's product begins two blocks before it is read back, and its B comes through registers one more before
-        load_b(0);
-        put_b(block);
-        load_b(1);
-        put_b(block + 1);
-        load_b(2);
+        put_b(first, block);
+        put_b(w, block + 1);
+        load_b(w, 2);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncthreads();
         if (threadIdx.x == 0 && n_ids > 0) {
@@ -783,7 +803,7 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
                 }
                 tc_fence_before();
             }
-            if (c + 2 < n_c) put_b(block + 2);     // (this block's product is done with its B)
+            if (c + 2 < n_c) put_b(w, block + 2);     // (this block's product is done with its B)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             ok = __syncthreads_and(ok);
             if (!ok) break;
@@ -798,7 +818,7 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
                 if (n_ids > 0 && c + 2 < n_c) multiply(block + 2);
                 if (c + kTcStages - 1 < n_c) fetch(c + kTcStages - 1, block + kTcStages - 1);
             }
-            load_b(c + 3);
+            load_b(w, c + 3);
         }
     }
     if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -899,7 +919,7 @@ __global__ void __launch_bounds__(kFewThreads, 5) k_lora_up_few(const __grid_con
 
 // Splits of the input's columns: as many as give two CTAs an SM work, each at least a chunk of 32 columns a warp.
 int splits_of(int64_t tokens, int64_t ic, int64_t rank, int sms) {
-    const int64_t rows = tokens <= kFew ? 16 : 32, tiles = (tokens + rows - 1) / rows * ((rank + 63) / 64);
+    const int64_t rows = tokens <= kFew ? 16 : 32, tiles = (tokens + rows - 1) / rows * ((rank + kRanks - 1) / kRanks);
     const int64_t most = std::max<int64_t>(1, ic / (32 * kWarps));
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 16), 2 * sms / tiles));
 }
@@ -926,8 +946,7 @@ cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
 template <typename T, int MT>
 cudaError_t down(const Params& p, bool vec, dim3 grid, cudaStream_t s) {
     if (p.rank <= 16) return down<T, MT, 2>(p, vec, grid, s);
-    if (p.rank <= 32) return down<T, MT, 4>(p, vec, grid, s);
-    return down<T, MT, 8>(p, vec, grid, s);
+    return down<T, MT, 4>(p, vec, grid, s);
 }
 template <typename T, typename Y>
 cudaError_t up(const Params& p, bool vec, dim3 grid, bool few, cudaStream_t s) {
@@ -963,7 +982,7 @@ int run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t 
     const bool few = p.tokens <= kFew;
     {
         const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
-        p.rank_blocks = (p.rank + 63) / 64;
+        p.rank_blocks = (p.rank + kRanks - 1) / kRanks;
         p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2 * sms / (tiles * p.splits * p.rank_blocks)));
         p.slots = (int)std::min<int64_t>(p.slots, p.tokens);
         const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)(p.slots * p.rank_blocks));
@@ -975,8 +994,11 @@ int run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t 
     dim3 grid;
     if (p.crowded) {
         p.columns = (int)((p.oc + kTcCols - 1) / kTcCols);
-        const int64_t blocks = (p.tokens + kTcRows - 1) / kTcRows * p.columns;
-        const int rc = up_tc<T>(p, vec_up, (int)std::min<int64_t>(blocks, sms), s, name);
+        // Shares of the CTAs: equal ones go over a tile's end, whose new beginning takes as long as four blocks.
+        const int64_t wide_tiles = (p.tokens + kTcRows - 1) / kTcRows, blocks = wide_tiles * p.columns, parts = std::min<int64_t>(sms / wide_tiles, p.columns);
+        const bool whole = parts > 0 && (p.columns + parts - 1) / parts <= (blocks + sms - 1) / sms + 4;
+        p.run = whole ? (int)parts : 0;
+        const int rc = up_tc<T>(p, vec_up, (int)(whole ? wide_tiles * parts : std::min<int64_t>(blocks, sms)), s, name);
         if (rc) return rc;
     }
     if (few) {
@@ -1044,7 +1066,7 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     const bool vec_down = p.ic % 8 == 0 && p.ldx % 8 == 0 && aligned(p.x, 16) && aligned(p.a, 16);
     const bool vec_up = p.rank % 8 == 0 && aligned(p.b, 16), wide = a->y_dtype == SPARK_DTYPE_F32;
     // (the tensor maps' rows are on 16 bytes, apart)
-    if (p.tokens >= kMany && p.rank <= kTcRank && !wide && p.wide_y && p.ldy >= p.oc)
+    if (p.tokens >= kMany && p.tokens * p.oc >= kManyValues && p.rank <= kTcRank && !wide && p.wide_y && p.ldy >= p.oc)
         p.crowded = reinterpret_cast<int*>(reinterpret_cast<char*>(workspace) + h_bytes(p.tokens, p.rank, p.splits));
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const int rc = a->dtype == SPARK_DTYPE_BF16 ? run<__nv_bfloat16>(p, vec_down, vec_up, wide, sms, st, name)
