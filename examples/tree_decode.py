@@ -2,7 +2,7 @@
 (NVFP4 embedding and head, FP3 attention, SPFP2 MLP), drafts by its first layer
 alone, the tree verified against the whole model's logits.
 
-    python examples/tree_decode.py [--tokens 64] [--temperature 0.0]
+    python examples/tree_decode.py [--tokens 64] [--temperature 0.0] [--top-k 0] [--top-p 1.0]
 
 Prints the steps that the tokens took: with one token a step there would be as many
 steps as tokens."""
@@ -62,7 +62,7 @@ def draft(first_layer: TreeDecoder, cache: PagedKVCache, last: torch.Tensor, par
 
 
 def generate(model: TreeDecoder, prompts: torch.Tensor, n_tokens: int, parents: list[int], temperature=0.0, seed=0,
-             vocab=2048):
+             vocab=2048, top_k=0, top_p=1.0):
     """([batch] lists of new tokens, steps)."""
     batch, dev = prompts.shape[0], prompts.device
     attention = model.blocks[0][0]
@@ -79,7 +79,8 @@ def generate(model: TreeDecoder, prompts: torch.Tensor, n_tokens: int, parents: 
         tokens = draft(first_layer, cache, torch.tensor([t[-1] for t in text], device=dev), parents)
         u = torch.rand(batch, len(parents), generator=gen, device=dev)
         noise = torch.empty(batch, vocab, device=dev).exponential_(generator=gen)
-        path, accepted, last = model.step(tokens, tree, depths, cache, u, noise, temperature=temperature)
+        path, accepted, last = model.step(tokens, tree, depths, cache, u, noise, temperature=temperature, top_k=top_k,
+                                          top_p=top_p)
         steps += 1
         for i, (nodes, n, token) in enumerate(zip(path.tolist(), accepted.tolist(), last.tolist())):
             text[i] += [int(tokens[i, k]) for k in nodes[1:n]] + [token]
@@ -96,11 +97,14 @@ def main() -> None:
     ap.add_argument("--tokens", type=int, default=64)
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--temperature", type=float, default=0.0)
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
     a = ap.parse_args()
     model = build()
     prompts = torch.randint(0, 2048, (a.batch, 40), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
-    _, plain = generate(model, prompts, a.tokens, [-1], a.temperature)
-    _, steps = generate(model, prompts, a.tokens, PARENTS, a.temperature)
+    how = {"temperature": a.temperature, "top_k": a.top_k, "top_p": a.top_p}
+    _, plain = generate(model, prompts, a.tokens, [-1], **how)
+    _, steps = generate(model, prompts, a.tokens, PARENTS, **how)
     print(f"{a.tokens} tokens a sequence: {plain} steps with one token a step, {steps} steps with a tree of {len(PARENTS)} nodes")
 
 

@@ -166,6 +166,59 @@ class V3MergedLinear(nn.Module):
         return f"fmt={self.merged.fmt}, in_features={self.in_features}, splits={self.splits}"
 
 
+class V3LoRALinear(nn.Module):
+    """A packed layer with low-rank adapters of many requests on top of its output
+    (ops.lora_add).  base: a V3PackedLinear with a [adapters, rank, in_features] and b
+    [adapters, out_features, rank], or a V3MergedLinear with a list of (a, b) or None for
+    each of its parts; scale: a number or fp32 [adapters].  use(adapter) says which
+    adapter each token has from then on: int32, one for each token or for each run of as
+    many (one for each sequence of a batch), negative for none; None takes all off.
+    A V3GateUpSiLU has its activation in the projection's launch, and takes none."""
+
+    def __init__(self, base: V3PackedLinear | V3MergedLinear, a, b=None, scale: torch.Tensor | float = 1.0):
+        super().__init__()
+        if not isinstance(base, (V3PackedLinear, V3MergedLinear)):
+            raise TypeError(f"V3LoRALinear: the base must be a V3PackedLinear or a V3MergedLinear, got {type(base).__name__}")
+        merged = isinstance(base, V3MergedLinear)
+        parts = list(a) if merged else [(a, b)]
+        widths = base.splits if merged else [base.out_features]
+        if len(parts) != len(widths):
+            raise ValueError(f"V3LoRALinear: {len(widths)} parts, {len(parts)} pairs of adapters")
+        for i, (pair, width) in enumerate(zip(parts, widths)):
+            if pair is None:
+                continue
+            pa, pb = pair
+            if (pa.dim() != 3 or pb.dim() != 3 or pa.shape[0] != pb.shape[0] or pa.shape[1] != pb.shape[2]
+                    or pa.shape[2] != base.in_features or pb.shape[1] != width):
+                raise ValueError(f"V3LoRALinear: part {i} has {base.in_features} inputs and {width} outputs, its adapters are "
+                                 f"{tuple(pa.shape)} and {tuple(pb.shape)}")
+            self.register_buffer(f"a{i}", pa.contiguous())
+            self.register_buffer(f"b{i}", pb.contiguous())
+        self.base, self._parts = base, [i for i, pair in enumerate(parts) if pair is not None]
+        if isinstance(scale, torch.Tensor):
+            self.register_buffer("scale", scale)
+        else:
+            self.scale = float(scale)
+        self.adapter: torch.Tensor | None = None
+        self.in_features = base.in_features
+        if merged:
+            self.splits = base.splits
+        else:
+            self.out_features = base.out_features
+
+    def use(self, adapter: torch.Tensor | None) -> None:
+        self.adapter = adapter
+
+    def forward(self, x: torch.Tensor, out: torch.Tensor | None = None):
+        y = self.base(x, out=out)
+        if self.adapter is None:
+            return y
+        for i in self._parts:
+            part = y[i] if isinstance(y, tuple) else y
+            ops.lora_add(part, x, getattr(self, f"a{i}"), getattr(self, f"b{i}"), self.adapter, scale=self.scale, out=part)
+        return y
+
+
 class V3GateUpSiLU(nn.Module):
     """SiLU(gate(x)) * up(x) of an MLP as one launch: gate and up are kept as
     one packed weight whose rows come in 16-row groups -- 8 gate rows, then the

@@ -1,6 +1,7 @@
 """Decoding with a tree of drafted tokens: the paged K/V cache, one attention
-block and a small decoder around the tree operators of ops (rope,
-tree_attention, tree_verify, kv_append) and the packed linears.
+block and a small decoder around the operators of ops (rope or qk_norm_rope,
+tree_attention, filter_logits, tree_verify, sample, kv_append) and the packed
+linears, with or without adapters (inference_v3.V3LoRALinear).
 
 A step takes T tokens a sequence (node 0 the last accepted token, the others
 drafted, `parents` says on which node each hangs), runs the layers on all of
@@ -16,6 +17,7 @@ import torch
 from torch import nn
 
 from . import ops
+from .inference_v3 import V3LoRALinear
 from .rotary import rope_table
 
 
@@ -89,12 +91,18 @@ def tree_depths(parents) -> torch.Tensor:
 
 
 class TreeAttention(nn.Module):
-    """Attention block: q|k|v (an inference_v3.V3MergedLinear), rotary positions, tree
+    """Attention block: q|k|v (an inference_v3.V3MergedLinear, or one with adapters), rotary
+    positions, with q_norm and k_norm [head_dim] after RMS norms of each head, tree
     attention, output projection."""
 
-    def __init__(self, qkv, out_proj, head_dim: int, interleaved: bool = False):
+    def __init__(self, qkv, out_proj, head_dim: int, interleaved: bool = False, q_norm: torch.Tensor | None = None,
+                 k_norm: torch.Tensor | None = None, eps: float = 1e-6):
         super().__init__()
-        self.qkv, self.out_proj = qkv, out_proj
+        if (q_norm is None) != (k_norm is None):
+            raise ValueError("TreeAttention: q_norm and k_norm come together")
+        self.qkv, self.out_proj, self.eps = qkv, out_proj, eps
+        self.register_buffer("q_norm", q_norm)
+        self.register_buffer("k_norm", k_norm)
         self.head_dim, self.interleaved = head_dim, interleaved
         self.kv_heads = qkv.splits[1] // head_dim
 
@@ -104,7 +112,11 @@ class TreeAttention(nn.Module):
         b, t, _ = x.shape
         q, k, v = (u.unflatten(-1, (-1, self.head_dim)).unflatten(0, (b, t)) for u in self.qkv(x.reshape(b * t, -1)))
         # in place: q and k are parts of the projection's output
-        q, k = ops.rope(q, k, positions, table, interleaved=self.interleaved, out=(q, k))
+        if self.q_norm is None:
+            q, k = ops.rope(q, k, positions, table, interleaved=self.interleaved, out=(q, k))
+        else:
+            q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, positions, table, eps=self.eps,
+                                    interleaved=self.interleaved, out=(q, k))
         y = cache.attend(layer, q, k, v, parents)
         return self.out_proj(y.reshape(b * t, -1)).reshape(b, t, -1), (k, v)
 
@@ -119,10 +131,19 @@ class TreeDecoder(nn.Module):
         self.embed, self.head = embed, head
         self.blocks = nn.ModuleList(nn.ModuleList(b) for b in blocks)
         self.register_buffer("table", rope_table(max_positions, rot_dim, base, **scaling), persistent=False)
+        # the tree of one node, which hangs on the context
+        self.register_buffer("root", torch.full((1,), -1, dtype=torch.int32, device=self.table.device), persistent=False)
 
     @staticmethod
     def norm(x: torch.Tensor) -> torch.Tensor:
         return nn.functional.rms_norm(x, x.shape[-1:])
+
+    def use_adapters(self, adapter: torch.Tensor | None) -> None:
+        """The adapter of each sequence of the batch (int32 [batch], negative for none) in all
+        layers that have some; None takes them off."""
+        for m in self.modules():
+            if isinstance(m, V3LoRALinear):
+                m.use(adapter)
 
     def forward(self, tokens: torch.Tensor, parents: torch.Tensor, depths: torch.Tensor, cache: PagedKVCache):
         """tokens [batch, nodes] -> (logits [batch, nodes, vocab], every layer's (k, v)).
@@ -147,12 +168,25 @@ class TreeDecoder(nn.Module):
             cache.append(new)
 
     def step(self, tokens: torch.Tensor, parents: torch.Tensor, depths: torch.Tensor, cache: PagedKVCache,
-             uniforms: torch.Tensor, noise: torch.Tensor, draft_probs: torch.Tensor | None = None, temperature=1.0):
+             uniforms: torch.Tensor, noise: torch.Tensor, draft_probs: torch.Tensor | None = None, temperature=1.0,
+             top_k=0, top_p=1.0, min_p=0.0):
         """One step: forward, verification, append of the accepted nodes.  Returns
         ops.tree_verify's (path, accepted, next); those of a row whose sequence has no
-        pages mean nothing."""
+        pages mean nothing.  top_k, top_p and min_p (numbers, or tensors [batch], as in ops.sample)
+        cut the distributions that the tokens are samples of."""
         logits, new = self(tokens, parents, depths, cache)
+        if any(isinstance(s, torch.Tensor) or s != off for s, off in ((top_k, 0), (top_p, 1.0), (min_p, 0.0))):
+            logits = ops.filter_logits(logits, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p, out=logits)
         path, accepted, last = ops.tree_verify(logits, tokens, parents, uniforms, noise, draft_probs=draft_probs,
                                                temperature=temperature)
         cache.append(new, index=path, counts=accepted)
         return path, accepted, last
+
+    def decode(self, last: torch.Tensor, cache: PagedKVCache, noise: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
+               min_p=0.0, return_logprob: bool = False):
+        """One token a sequence: forward of the last ones [batch], whose K/V rows go into the
+        cache, and the next ones, drawn by ops.sample with its settings."""
+        logits, new = self(last[:, None], self.root, self.root + 1, cache)
+        cache.append(new)
+        return ops.sample(logits[:, 0], noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                          return_logprob=return_logprob)
