@@ -581,7 +581,8 @@ SPARK_API int spark_sample(const SparkSample* a, void* stream);
  * fp32 [adapters], or NULL: scale_all.  adapter int32 [tokens / repeat, rounded up].
  * Products and sums are fp32, A x to 2^-17 of it (fp32 y: 2^-22), the result is rounded
  * once.  rank <= 256.  workspace: spark_lora_workspace_size bytes on the current device,
- * 16-byte aligned; what is in it does not matter. */
+ * 16-byte aligned; what is in it does not matter.  A wait in the kernel that runs out sets
+ * error 10, and leaves columns of out as they were. */
 typedef struct {
     int64_t tokens, ic, oc, rank, adapters, repeat, dtype, y_dtype;
     const void *x, *a, *b, *y;

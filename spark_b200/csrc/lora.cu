@@ -806,7 +806,14 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
             if (c + 2 < n_c) put_b(w, block + 2);     // (this block's product is done with its B)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             ok = __syncthreads_and(ok);
-            if (!ok) break;
+            if (!ok) {
+                // (given up: what is still on its way into this memory ends first, or gets as long again)
+                for (int i = 0; threadIdx.x == 0 && i < kTcStages - 1 && c + i < n_c; ++i) {
+                    mbar_wait(arrived + 8 * ((block + i) % kTcStages), (block + i) / kTcStages & 1);
+                    if (n_ids > 0 && i < 2) mbar_wait(product + 8 * ((block + i) & 1), (products >> ((block + i) & 1) & 1) ^ (i == 0));
+                }
+                break;
+            }
             if (threadIdx.x == 0) {
                 const uint32_t from = smem_u32(y_smem) + stage * kBlock;
 #pragma unroll

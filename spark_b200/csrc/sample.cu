@@ -592,6 +592,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         }
     }
     Slice<L, TH> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0, head};
+    __syncwarp();
     cluster_wait();      // every CTA of the cluster has started: its shared memory may be written
     int step = 0;
     Note best{-INFINITY, 0.f, 0, 0};
@@ -634,7 +635,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         const bool reached = !by_k || s.found.bin >= 0;
         // what has a bin up to that one (and, by the rounding of the edge, perhaps some more); of the rest the sum, where that
         // is asked for
-        const float edge = __fsub_rd(r.top, __fmul_ru(__fdiv_ru((float)((s.found.bin >= 0 ? s.found.bin : kBins - 2) + 1), r.bins), 1.00001f));
+        // (-inf, which fills the vectors' ends too, is never among them: below the lowest number there is no edge)
+        const float edge = fmaxf(__fsub_rd(r.top, __fmul_ru(__fdiv_ru((float)((s.found.bin >= 0 ? s.found.bin : kBins - 2) + 1), r.bins), 1.00001f)), -FLT_MAX);
         double sum = 0, slope = 0;
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {

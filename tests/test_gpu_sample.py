@@ -321,3 +321,19 @@ def test_borders_that_only_good_sums_tell(vocab, dtype):
         for p in (float(before[i]) * (1 + 1e-8), float(before[i]) * (1 - 1e-8)):
             assert cut64(row, 1.0, 0, p, 0.0)[2] == [] and len(cut64(row, 1.0, 0, p, 0.0)[0]) == (i + 1 if p > before[i] else i)
             check_filter(x, ops().filter_logits(x, top_p=p), dict(top_p=p))
+
+
+@pytest.mark.parametrize("dtype", [FP, BF, HF])
+@pytest.mark.parametrize("vocab", [1001, 70003])
+def test_rows_of_the_lowest_value(vocab, dtype):
+    """Masks of the type's lowest value beside -inf, in rows that begin inside a vector: fewer entries than top_k."""
+    low = torch.finfo(dtype).min
+    logits = torch.full((5, vocab), -math.inf, dtype=dtype, device="cuda")
+    for i in range(4):
+        logits[i, [0, vocab - 1, vocab // 2, 7][i]] = low
+    logits[4] = low
+    noise = noise_of(gen(5), 5, vocab)
+    for s in (dict(top_k=5), dict(top_k=900), dict(top_p=0.9), dict(top_k=40, top_p=0.5, temperature=3.0), dict(top_k=5, temperature=1e30), dict()):
+        check_filter(logits, ops().filter_logits(logits, **s), s)
+        token, logprob = ops().sample(logits, noise, **s, return_logprob=True)
+        check_sample(logits, noise, token, logprob, s)
