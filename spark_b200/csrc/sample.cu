@@ -29,6 +29,13 @@
 // slices of a thread-block cluster, which exchange bins and lists through distributed
 // shared memory and all take the same decisions; a step costs a cluster barrier
 // then (2000 cycles or more each, against some hundred).
+//
+// Few rows are bound by that chain of steps: one of 151,936 in fp32 takes 8.6 us without
+// a cut, 12.5 with top_k 50, 12.7 with top_p 0.9 of those, 23 with top_p 0.95 of all.
+// Many are bound by the instructions a value (a few to find the largest, some 10 more where
+// top_p sums a row): 1024 rows of 32,000 in bf16 with top_k 50 45 us (1.4 TB/s).  A
+// flat distribution, of which more stays than a list holds, is divided by histograms of all
+// its entries: 60 to 160 us for 64 rows of 100,003.
 #include <float.h>
 #include <math.h>
 
@@ -43,15 +50,15 @@ int sm_count_cached(int dev);
 
 namespace sm {
 
-constexpr int kMaxThreads = 1024;       // of a CTA: 1024, or 512 where two CTAs fit an SM
-constexpr int kWarps = kMaxThreads / 32;
+constexpr int kThreads = 512;           // two CTAs an SM, where their slices fit (one of 1024: 1 to 70% longer, 200 rows of 32,000 19.8 us for 12.2)
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 512;              // the last one: all that is further away
 constexpr int kPairs = 256;             // entries that are compared with one another
 constexpr int kList = 4096;             // entries that a CTA lists
 constexpr int kRowBytes = 200 * 1024;   // of a CTA's slice
+constexpr int kLongBytes = 96 * 1024;   // of a row that a cluster may be faster for
 constexpr int kMaxVocab = kMaxCluster * kRowBytes / 4;
-constexpr int kSmemSm = 228 * 1024;     // shared memory of an SM
 constexpr int kGroups = 4;              // of a thread's vectors, which are on the way together
 
 struct Params {
@@ -214,7 +221,6 @@ __device__ __forceinline__ Note join_warp(Note v) {
     return Note{top, v.b, (int)first, 0};
 }
 // Of all threads of the cluster, for every thread, in a fixed order.
-template <int TH>
 __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (int)cluster_size();
     v = join_warp(v);
@@ -222,9 +228,9 @@ __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
     if (lane == 0) red[warp] = v;
     __syncthreads();
     Note* slot = s.note[step++ & 1];
-    if (n == 1) return join_warp(lane < TH / 32 ? red[lane] : none());
+    if (n == 1) return join_warp(lane < kWarps ? red[lane] : none());
     if (warp == 0) {
-        v = join_warp(lane < TH / 32 ? red[lane] : none());
+        v = join_warp(lane < kWarps ? red[lane] : none());
         if (lane < n) *of_rank(&slot[cluster_rank()], lane) = v;
     }
     cluster_sync();
@@ -245,7 +251,7 @@ __device__ __forceinline__ unsigned long long mass_of(const Row& r, float x) {
 }
 
 // A CTA's part of a row, in shared memory, and the entries of it that are looked at: those listed, or all.
-template <typename L, int TH>
+template <typename L>
 struct Slice {
     const L* v;
     int v0, n;               // index of the first, how many
@@ -258,12 +264,12 @@ struct Slice {
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
         if (list) {
-            for (int i = threadIdx.x; i < listed; i += TH) {
+            for (int i = threadIdx.x; i < listed; i += kThreads) {
                 const int j = at(i);
                 f((float)v[j], v0 + j);
             }
         } else {
-            for (int i = threadIdx.x; i < n; i += TH) f((float)v[i], v0 + i);
+            for (int i = threadIdx.x; i < n; i += kThreads) f((float)v[i], v0 + i);
         }
     }
 };
@@ -323,9 +329,9 @@ __device__ __forceinline__ void add_bins(Shared& s, bool masses) {
     cluster_sync();
 }
 // Fills s.counts and s.mass with the row's bins: mode 0: all entries but those of the last bin; else those of the range.
-template <typename L, int TH>
-__device__ __noinline__ void histogram(Shared& s, const Slice<L, TH>& x, const Row& r, const Range& g, bool masses) {
-    for (int i = threadIdx.x; i < kBins; i += TH) s.count[i] = s.low[i] = s.high[i] = 0;
+template <typename L>
+__device__ __noinline__ void histogram(Shared& s, const Slice<L>& x, const Row& r, const Range& g, bool masses) {
+    for (int i = threadIdx.x; i < kBins; i += kThreads) s.count[i] = s.low[i] = s.high[i] = 0;
     __syncthreads();
     x.each([&](float v, int index) {
         int bin;
@@ -378,14 +384,13 @@ __device__ __noinline__ unsigned long long mass_of_bins(Shared& s) {
     return all;
 }
 // The sum over the cluster, for every thread.
-template <int TH>
 __device__ __noinline__ unsigned long long sum_of_all(Shared& s, unsigned long long x) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = (int)cluster_size();
     x = sum_of_warp(x);
     __syncthreads();
     if (lane == 0) s.scan_mass[warp] = x;
     __syncthreads();
-    x = sum_of_warp(lane < TH / 32 ? s.scan_mass[lane] : 0);
+    x = sum_of_warp(lane < kWarps ? s.scan_mass[lane] : 0);
     if (n == 1) return x;
     if (threadIdx.x < n) *of_rank(&s.mass[cluster_rank()], threadIdx.x) = x;
     cluster_sync();
@@ -423,7 +428,6 @@ __device__ __forceinline__ unsigned long long share_of(double top_p, double mass
 // Rank 0 compares its s.pairs entries with one another and tells all CTAs the cut: by count (k > 0), by mass (target > 0), or by
 // top_p of the mass of the first k or, without k, of all and `rest`.  Behind count0 entries of mass0.  Where the cut is behind
 // them all its mass is 0.
-template <int TH>
 __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, unsigned long long target, double top_p, double rest, unsigned count0,
                                    unsigned long long mass0) {
     if (cluster_rank() == 0) {
@@ -431,8 +435,8 @@ __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, unsigned
         if (t < n) s.pair_mass[t] = mass_of(r, value_of(s.pair[t].key));
         if (t == 0) s.cut.mass = 0;
         // a few threads an entry, so that each compares about 16
-        int part = TH / kPairs == 4 ? 2 : 1;
-        while (part < 4 && (n >> part) > 16 && (n << (part + 1)) <= TH) ++part;
+        int part = 1;
+        while (part < 4 && (n >> part) > 16 && (n << (part + 1)) <= kThreads) ++part;
         const int e = t >> part, sub = t & ((1 << part) - 1);
         __syncthreads();
         Entry mine{0xffffffffu, 0x7fffffff};
@@ -470,8 +474,8 @@ __device__ __noinline__ void solve(Shared& s, const Row& r, unsigned k, unsigned
 
 // The cut by count (k > 0: behind the first k entries) or by mass (behind the shortest prefix with `target`) of x's entries, from
 // their bins by distance, which are in s if `fresh`.  s.cut afterwards.  Returns whether the bins are still there.
-template <typename L, int TH>
-__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, bool fresh, unsigned k, unsigned long long target, int entries,
+template <typename L>
+__device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L>& x, const Row& r, bool fresh, unsigned k, unsigned long long target, int entries,
                                     int vocab, bool masses) {
     Range g{0, 0, 0, 0, 0, 0};
     if (!fresh) histogram(s, x, r, g, masses);
@@ -489,7 +493,7 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x,
             x.each([&](float v, int index) {
                 if (bin_of(r, v) == g.bin) add(hi, v, index), add(lo, -v, index);
             });
-            const float top = join_all<TH>(s, step, hi).a, bottom = -join_all<TH>(s, step, lo).a;
+            const float top = join_all(s, step, hi).a, bottom = -join_all(s, step, lo).a;
             g.mode = 1, g.lo = key_of(top), g.span = key_of(bottom) - g.lo;
         }
         if (g.mode == 1 && g.span == 0) g.mode = 2, g.from = 0, g.span = (uint32_t)vocab - 1;
@@ -513,13 +517,13 @@ __device__ __noinline__ bool cut_at(Shared& s, int& step, const Slice<L, TH>& x,
         if (at < kPairs) pair[at] = Entry{key_of(v), index};
     });
     cluster_sync();
-    solve<TH>(s, r, k, target, 1.0, 0.0, (unsigned)f.count, f.mass);
+    solve(s, r, k, target, 1.0, 0.0, (unsigned)f.count, f.mass);
     return fresh;
 }
 
 // The cut of x's entries, which have all that stays: by count, and by top_p of those; or by mass.
-template <typename L, int TH>
-__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L, TH>& x, const Row& r, unsigned k, double top_p, unsigned long long target,
+template <typename L>
+__device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L>& x, const Row& r, unsigned k, double top_p, unsigned long long target,
                                         bool fresh, int entries, int vocab) {
     if (k) {
         fresh = cut_at(s, step, x, r, false, k, 0ull, entries, vocab, top_p < 1);
@@ -530,8 +534,8 @@ __device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L, TH>
     cut_at(s, step, x, r, fresh, 0, target, entries, vocab, true);
 }
 
-template <typename L, int TH>
-__global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant__ Params p) {
+template <typename L>
+__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ Params p) {
     using V = Vec<L>;
     constexpr int N = V::N;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -566,11 +570,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
     float most[kGroups];      // the largest of this thread's vectors, every fourth of them
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) most[k] = -INFINITY;
-    for (int i0 = tid; i0 < vectors; i0 += kGroups * TH) {
+    for (int i0 = tid; i0 < vectors; i0 += kGroups * kThreads) {
         V x[kGroups];
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
-            const int i = i0 + k * TH;
+            const int i = i0 + k * kThreads;
             if (i >= vectors) continue;
             if (i * N >= head && (i + 1) * N <= head + n) {
                 x[k].raw = from[i];
@@ -584,21 +588,21 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         }
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
-            const int i = i0 + k * TH;
+            const int i = i0 + k * kThreads;
             if (i >= vectors) continue;
             vec[i] = x[k].raw;
             const float m = x[k].largest();
             asm("max.NaN.f32 %0, %0, %1;" : "+f"(most[k]) : "f"(m));
         }
     }
-    Slice<L, TH> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0, head};
+    Slice<L> x{reinterpret_cast<const L*>(raw) + head, v0, n, nullptr, 0, 0, head};
     __syncwarp();
     cluster_wait();      // every CTA of the cluster has started: its shared memory may be written
     int step = 0;
     Note best{-INFINITY, 0.f, 0, 0};
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) best.a = fmaxf(best.a, most[k]), best.b += most[k] == most[k] ? 0.f : 1.f;
-    best = join_all<TH>(s, step, best);
+    best = join_all(s, step, best);
     Row r;
     r.top = best.a;
     const bool none_here = best.b != 0.f || !(best.a > -INFINITY && best.a < INFINITY) || !(temp >= 0);
@@ -613,10 +617,10 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         x.each([&](float f, int index) {
             if (f == r.top) add(first, f, index);
         });
-        limit = r.top, last = join_all<TH>(s, step, first).i;
+        limit = r.top, last = join_all(s, step, first).i;
     } else if (by_k || by_p) {
         // the bin by which there are enough entries, from the groups' largest
-        for (int i = tid; i < kBins; i += TH) s.count[i] = 0;
+        for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
         if (tid == 0) s.listed[0] = s.listed[1] = s.pairs = 0;
         __syncthreads();
 #pragma unroll
@@ -628,7 +632,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         unsigned enough = (unsigned)top_k;
         if (!by_k) {
             // groups of m entries each, of which a share of 1 - (1 - 1 / 30)^m has one of the largest thirtieth
-            const float groups = fminf((float)(cs * kGroups * TH), (float)vocab / N), m = (float)vocab / groups;
+            const float groups = fminf((float)(cs * kGroups * kThreads), (float)vocab / N), m = (float)vocab / groups;
             enough = max(64u, (unsigned)(groups * (1.f - __expf(-0.0339f * m))));
         }
         find_count(s, enough);
@@ -641,7 +645,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
 #pragma unroll
         for (int k = 0; k < kGroups; ++k) {
             if (!reached || (by_k && most[k] < edge)) continue;
-            for (int i = tid + k * TH; i < vectors; i += kGroups * TH) {
+            for (int i = tid + k * kThreads; i < vectors; i += kGroups * kThreads) {
                 const V u(vec[i]);
                 if (u.largest() >= edge) {
                     unsigned which = 0;
@@ -674,7 +678,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         if (warp == 0) {
             sum = slope = 0;
             if (!by_k) {
-                if (lane < TH / 32) sum = s.red_sum[lane], slope = s.red_slope[lane];
+                if (lane < kWarps) sum = s.red_sum[lane], slope = s.red_slope[lane];
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
             }
@@ -700,14 +704,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         const double scale = 0x1p44, rest = sum * scale;
         const unsigned k = by_k ? (unsigned)top_k : 0;
         if (fits && by_k) {
-            if (total <= kPairs) solve<TH>(s, r, k, 0ull, top_p, 0.0, 0, 0);
+            if (total <= kPairs) solve(s, r, k, 0ull, top_p, 0.0, 0, 0);
             else cut_all(s, step, x, r, k, top_p, 0ull, false, total, vocab);
             done = true;
         } else if (fits) {
             // (a mass of all that the list does not reach is found out about below)
             auto cut = [&](double more) {
                 if (total <= kPairs) {
-                    solve<TH>(s, r, 0, 0ull, top_p, more, 0, 0);
+                    solve(s, r, 0, 0ull, top_p, more, 0, 0);
                     return s.cut.mass > 0;
                 }
                 histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
@@ -722,9 +726,9 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
             if (done && !((double)s.cut.before < (double)s.cut.target - off && (double)s.cut.target + off <= (double)s.cut.mass)) {
                 // it is not: the rest as the list's entries are summed
                 unsigned long long exact = 0;
-                for (int i = tid; i < n; i += TH)
+                for (int i = tid; i < n; i += kThreads)
                     if ((float)x.v[i] < edge) exact += mass_of(r, (float)x.v[i]);
-                done = cut((double)sum_of_all<TH>(s, exact));
+                done = cut((double)sum_of_all(s, exact));
             }
         }
         if (!done) {
@@ -747,7 +751,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
     if (a.out) {
         L* out = reinterpret_cast<L*>(a.out) + b * a.out_stride[0] + node * a.out_stride[1] + v0;
         const bool alike = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(logits)) & 15) == 0;
-        for (int i = tid; i < vectors; i += TH) {
+        for (int i = tid; i < vectors; i += kThreads) {
             V u(vec[i]);
 #pragma unroll
             for (int j = 0; j < N; ++j)
@@ -778,11 +782,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
         } else {
             constexpr int kAhead = 8;
             const bool all = limit == -INFINITY;
-            for (int i0 = tid; i0 < n; i0 += kAhead * TH) {
+            for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
                 float f[kAhead], e[kAhead];
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
-                    const int i = i0 + k * TH;
+                    const int i = i0 + k * kThreads;
                     f[k] = i < n ? (float)x.v[i] : -INFINITY;
                     if (!all && !stays(f[k], v0 + i)) f[k] = -INFINITY;
                     e[k] = f[k] > -INFINITY ? noise[i] : 1.f;
@@ -791,11 +795,11 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
                 for (int k = 0; k < kAhead; ++k) {
                     const float q = exp2_of((f[k] - r.top) * per2), chance = __fdividef(q, e[k]);
                     got.b += q;
-                    if (chance > got.a) got.a = chance, got.i = v0 + i0 + k * TH;
+                    if (chance > got.a) got.a = chance, got.i = v0 + i0 + k * kThreads;
                 }
             }
         }
-        got = join_all<TH>(s, step, got);
+        got = join_all(s, step, got);
     } else if (greedy) {
         got.i = last;
     }
@@ -811,13 +815,21 @@ __global__ void __launch_bounds__(TH, 1024 / TH) k_sample(const __grid_constant_
 
 inline int64_t slice_of(int64_t vocab, int cs) { return ((vocab + cs - 1) / cs + 15) / 16 * 16; }
 
-template <typename L, int TH>
-int launch(const Params& p, int64_t rows, int cs, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(k_sample<L, TH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
+template <typename L>
+int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
+    // A CTA takes a row, a cluster one that does not fit, or a long one where SMs are left over.  Measured, us a call of sample without
+    // a cut / with top_k 50 / with top_p 0.95:
+    //   one row of 90,000 in bf16, by 1 / 4 / 8 CTAs: 18.6, 14.0, 30; 8.5, 11.8, 20; 6.3, 11.2, 18.  Of 32,000 by 1 / 8: 8.6, 9.4, 17;
+    //   4.9, 10.8, 17.  36 of 50,000 in fp32 by 1 / 4 / 8 (more CTAs than SMs): 14.1, 14.5, 27; 10.4, 13.5, 25; 12.8, 23.7, 41.
+    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.
+    int cs = slice_of(p.a.vocab, 1) * sizeof(L) <= kRowBytes ? 1 : slice_of(p.a.vocab, 4) * sizeof(L) <= kRowBytes ? 4 : 8;
+    if (p.a.vocab * (int64_t)sizeof(L) >= kLongBytes) cs = 16 * rows <= sms ? 8 : 4 * rows <= sms ? std::max(cs, 4) : cs;
+    p.slice = (int)slice_of(p.a.vocab, cs);
+    cudaError_t e = cudaFuncSetAttribute(k_sample<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * cs));
-    cfg.blockDim = dim3(TH);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = (size_t)p.slice * sizeof(L) + 16;   // (a vector more where the slice does not begin with one)
     cfg.stream = s;
     cudaLaunchAttribute at[2];
@@ -827,21 +839,9 @@ int launch(const Params& p, int64_t rows, int cs, cudaStream_t s) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, k_sample<L, TH>, p);
+    e = cudaLaunchKernelEx(&cfg, k_sample<L>, p);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: launch failed: %s", cudaGetErrorString(e));
     return check_launch("spark_sample");
-}
-template <typename L>
-int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
-    // one CTA a row where that fits, else as large a cluster as leaves all rows at work at once
-    int cs = 1;
-    while (slice_of(p.a.vocab, cs) * sizeof(L) > kRowBytes) cs *= 2;
-    while (cs > 1 && cs < kMaxCluster && 2 * cs * rows <= sms) cs *= 2;
-    p.slice = (int)slice_of(p.a.vocab, cs);
-    // two CTAs an SM where there are more than one for each and both fit
-    const size_t bytes = sizeof(Shared) + p.slice * sizeof(L) + 16 + 1024;
-    if (rows * cs > sms && 2 * bytes <= kSmemSm) return launch<L, 512>(p, rows, cs, s);
-    return launch<L, 1024>(p, rows, cs, s);
 }
 
 }  // namespace sm
