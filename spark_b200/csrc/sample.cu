@@ -50,13 +50,14 @@ int sm_count_cached(int dev);
 
 namespace sm {
 
-constexpr int kThreads = 512;           // two CTAs an SM, where their slices fit (one of 1024: 1 to 70% longer, 200 rows of 32,000 19.8 us for 12.2)
+constexpr int kThreads = 512;           // (1024: 1 to 70% longer, 200 rows of 32,000 19.8 us for 12.2)
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kBins = 512;              // the last one: all that is further away
 constexpr int kPairs = 256;             // entries that are compared with one another
-constexpr int kList = 4096;             // entries that a CTA lists
+constexpr int kList = 6144;             // entries that a CTA lists
 constexpr int kRowBytes = 200 * 1024;   // of a CTA's slice
+constexpr int kSmemSm = 228 * 1024;     // shared memory of an SM
 constexpr int kLongBytes = 96 * 1024;   // of a row that a cluster may be faster for
 constexpr int kMaxVocab = kMaxCluster * kRowBytes / 4;
 constexpr int kGroups = 4;              // of a thread's vectors, which are on the way together
@@ -114,6 +115,7 @@ struct Shared {
     double per_temp, reach;                                   // 1 / T; how far below M min_p reaches
     float bins;
     Found found;
+    int further;
     Cut cut;
 };
 
@@ -347,8 +349,8 @@ __device__ __noinline__ void histogram(Shared& s, const Slice<L>& x, const Row& 
     add_bins(s, true);
 }
 
-// The bin in which the count reaches k, from s.counts; bin -1 where none does.
-__device__ __forceinline__ void find_count(Shared& s, unsigned k) {
+// The bin in which the count reaches k, from s.counts; bin -1 where none does.  And that for `more`, in s.further.
+__device__ __forceinline__ void find_count(Shared& s, unsigned k, unsigned more) {
     const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
     const unsigned own = t < kBins ? s.counts[t] : 0;
     unsigned c = own;
@@ -358,10 +360,11 @@ __device__ __forceinline__ void find_count(Shared& s, unsigned k) {
         if (lane >= o) c += pc;
     }
     if (lane == 31) s.scan_count[warp] = c;
-    if (t == 0) s.found = Found{-1, 0, 0, 0};
+    if (t == 0) s.found = Found{-1, 0, 0, 0}, s.further = -1;
     __syncthreads();
     const unsigned before = __reduce_add_sync(0xffffffffu, lane < warp ? s.scan_count[lane] : 0) + c - own;
     if (before < k && k <= before + own) s.found = Found{t, (int)before, (int)own, 0};
+    if (before < more && more <= before + own) s.further = t;
     __syncthreads();
 }
 
@@ -534,8 +537,107 @@ __device__ __forceinline__ void cut_all(Shared& s, int& step, const Slice<L>& x,
     cut_at(s, step, x, r, fresh, 0, target, entries, vocab, true);
 }
 
+// Lists x's entries from `edge` on, of the groups of vectors that have some, and gives rank 0 all of them where they are few; with
+// `sums`, those of what is not listed.
+struct Listed {
+    int total;      // of the cluster
+    bool fits;
+    double sum, slope;
+};
 template <typename L>
-__global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ Params p) {
+__device__ __forceinline__ Listed list_from(Shared& s, Slice<L>& x, const Row& r, const uint4* vec, int vectors, unsigned groups, bool sums, float per2,
+                                         float edge) {
+    using V = Vec<L>;
+    constexpr int N = V::N;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cs = (int)cluster_size();
+    double sum = 0, slope = 0;
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+        if (!(groups >> k & 1)) continue;
+        for (int i = tid + k * kThreads; i < vectors; i += kGroups * kThreads) {
+            const V u(vec[i]);
+            if (u.largest() >= edge) {
+                unsigned which = 0;
+#pragma unroll
+                for (int j = 0; j < N; ++j) which |= (float)u.v[j] >= edge ? 1u << j : 0u;
+                const int place = i * N, far = place >> 16;
+                unsigned at = atomicAdd(&s.listed[far], (unsigned)__popc(which));
+                for (; which && at < kList; which &= which - 1, ++at)
+                    s.list[far ? kList - 1 - at : at] = (uint16_t)(place + __ffs(which) - 1);
+            }
+            if (!sums) continue;
+            float e = 0.f, f = 0.f;
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const float v = (float)u.v[j], z = fmaxf((v - r.top) * per2, -200.f);   // (2^-200 is 0)
+                const float q = v < edge ? exp2_of(z) : 0.f;
+                e += q, f = fmaf(z, q, f);
+            }
+            sum += e, slope -= f;
+        }
+    }
+    if (sums) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
+        if (lane == 0) s.red_sum[warp] = sum, s.red_slope[warp] = slope;
+    }
+    __syncthreads();
+    const int listed = (int)(s.listed[0] + s.listed[1]);
+    x.list = s.list, x.listed = listed, x.low = (int)s.listed[0];
+    if (warp == 0) {
+        sum = slope = 0;
+        if (sums) {
+            if (lane < kWarps) sum = s.red_sum[lane], slope = s.red_slope[lane];
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
+        }
+        if (lane < cs) *of_rank(&s.rest[cluster_rank()], lane) = Rest{listed, 0, sum, slope};
+    }
+    if (listed <= kPairs) {
+        // perhaps all are few: rank 0 has them then
+        if (tid == 0) s.base = atomicAdd(of_rank(&s.pairs, 0), (unsigned)listed);
+        __syncthreads();
+        Entry* pair = of_rank(&s.pair[0], 0);
+        if (tid < listed && s.base + tid < kPairs) pair[s.base + tid] = Entry{key_of((float)x.v[x.at(tid)]), x.v0 + x.at(tid)};
+    }
+    cluster_sync();
+    Listed all{0, true, 0, 0};
+    for (int k = 0; k < cs; ++k) {
+        const Rest& c = s.rest[k];
+        all.total += c.listed, all.fits = all.fits && c.listed <= kList, all.sum += c.sum, all.slope += c.slope;
+    }
+    return all;
+}
+
+// The cut by top_p of a row of which x's entries are listed, from `edge` on, if it is among them.
+template <typename L>
+__device__ __forceinline__ bool cut_by_mass(Shared& s, int& step, const Slice<L>& x, const Row& r, const Listed& l, double top_p, int vocab, float edge) {
+    // (a mass of all that the list does not reach is found out about by the caller)
+    auto cut = [&](double more) {
+        if (l.total <= kPairs) {
+            solve(s, r, 0, 0ull, top_p, more, 0, 0);
+            return s.cut.mass > 0;
+        }
+        histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
+        const unsigned long long whole = mass_of_bins(s), target = share_of(top_p, (double)whole + more);
+        if (target <= whole) cut_all(s, step, x, r, 0, 1.0, target, true, l.total, vocab);
+        return target <= whole;
+    };
+    constexpr double scale = 0x1p44;
+    if (!cut(l.sum * scale)) return false;
+    // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
+    // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
+    const double off = top_p * (l.sum * 0x1p-20 + l.slope * 0x1p-22) * scale;
+    if ((double)s.cut.before < (double)s.cut.target - off && (double)s.cut.target + off <= (double)s.cut.mass) return true;
+    // it is not: the rest as the list's entries are summed
+    unsigned long long exact = 0;
+    for (int i = threadIdx.x; i < x.n; i += kThreads)
+        if ((float)x.v[i] < edge) exact += mass_of(r, (float)x.v[i]);
+    return cut((double)sum_of_all(s, exact));
+}
+
+template <typename L, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant__ Params p) {
     using V = Vec<L>;
     constexpr int N = V::N;
     extern __shared__ __align__(16) unsigned char raw[];
@@ -629,106 +731,41 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
             if (bin < kBins - 1) atomicAdd(&s.count[bin], 1u);
         }
         add_bins(s, false);
-        unsigned enough = (unsigned)top_k;
+        unsigned enough = (unsigned)top_k, more = 0;
         if (!by_k) {
-            // groups of m entries each, of which a share of 1 - (1 - 1 / 30)^m has one of the largest thirtieth
+            // Groups of m entries each, of which a share of 1 - (1 - q)^m has one of the largest q.  A thirtieth, and if that has less mass
+            // than stays as many as the lists hold (some rows in 64 of 32,000, whose call took 53 us without, 19 otherwise).
             const float groups = fminf((float)(cs * kGroups * kThreads), (float)vocab / N), m = (float)vocab / groups;
+            const float most_listed = fminf(0.75f * kList * cs / (float)vocab, 0.25f);
             enough = max(64u, (unsigned)(groups * (1.f - __expf(-0.0339f * m))));
+            more = max(enough, (unsigned)(groups * (1.f - __expf(m * __logf(1.f - most_listed)))));
         }
-        find_count(s, enough);
+        find_count(s, enough, more);
         const bool reached = !by_k || s.found.bin >= 0;
-        // what has a bin up to that one (and, by the rounding of the edge, perhaps some more); of the rest the sum, where that
-        // is asked for
+        // what has a bin up to that one (and, by the rounding of the edge, perhaps some more)
         // (-inf, which fills the vectors' ends too, is never among them: below the lowest number there is no edge)
-        const float edge = fmaxf(__fsub_rd(r.top, __fmul_ru(__fdiv_ru((float)((s.found.bin >= 0 ? s.found.bin : kBins - 2) + 1), r.bins), 1.00001f)), -FLT_MAX);
-        double sum = 0, slope = 0;
+        auto edge_of = [&](int bin) {
+            return fmaxf(__fsub_rd(r.top, __fmul_ru(__fdiv_ru((float)((bin >= 0 ? bin : kBins - 2) + 1), r.bins), 1.00001f)), -FLT_MAX);
+        };
+        const float edge = edge_of(s.found.bin), further = edge_of(s.further);
+        unsigned groups = 0;
 #pragma unroll
-        for (int k = 0; k < kGroups; ++k) {
-            if (!reached || (by_k && most[k] < edge)) continue;
-            for (int i = tid + k * kThreads; i < vectors; i += kGroups * kThreads) {
-                const V u(vec[i]);
-                if (u.largest() >= edge) {
-                    unsigned which = 0;
-#pragma unroll
-                    for (int j = 0; j < N; ++j) which |= (float)u.v[j] >= edge ? 1u << j : 0u;
-                    const int place = i * N, far = place >> 16;
-                    unsigned at = atomicAdd(&s.listed[far], (unsigned)__popc(which));
-                    for (; which && at < kList; which &= which - 1, ++at)
-                        s.list[far ? kList - 1 - at : at] = (uint16_t)(place + __ffs(which) - 1);
-                }
-                if (by_k) continue;
-                float e = 0.f, f = 0.f;
-#pragma unroll
-                for (int j = 0; j < N; ++j) {
-                    const float v = (float)u.v[j], z = fmaxf((v - r.top) * per2, -200.f);   // (2^-200 is 0)
-                    const float q = v < edge ? exp2_of(z) : 0.f;
-                    e += q, f = fmaf(z, q, f);
-                }
-                sum += e, slope -= f;
-            }
-        }
-        if (!by_k) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
-            if (lane == 0) s.red_sum[warp] = sum, s.red_slope[warp] = slope;
-        }
-        __syncthreads();
-        const int listed = (int)(s.listed[0] + s.listed[1]);
-        x.listed = listed, x.low = (int)s.listed[0];
-        if (warp == 0) {
-            sum = slope = 0;
-            if (!by_k) {
-                if (lane < kWarps) sum = s.red_sum[lane], slope = s.red_slope[lane];
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o), slope += __shfl_xor_sync(0xffffffffu, slope, o);
-            }
-            if (lane < cs) *of_rank(&s.rest[rank], lane) = Rest{listed, 0, sum, slope};
-        }
-        x.list = s.list;
-        if (listed <= kPairs) {
-            // perhaps all are few: rank 0 has them then
-            if (tid == 0) s.base = atomicAdd(of_rank(&s.pairs, 0), (unsigned)listed);
-            __syncthreads();
-            Entry* pair = of_rank(&s.pair[0], 0);
-            if (tid < listed && s.base + tid < kPairs) pair[s.base + tid] = Entry{key_of((float)x.v[x.at(tid)]), v0 + x.at(tid)};
-        }
-        cluster_sync();
-        int total = 0;
-        bool fits = reached;
-        sum = slope = 0;
-        for (int k = 0; k < cs; ++k) {
-            const Rest& c = s.rest[k];
-            total += c.listed, fits = fits && c.listed <= kList, sum += c.sum, slope += c.slope;
-        }
+        for (int k = 0; k < kGroups; ++k) groups |= reached && !(by_k && most[k] < edge) ? 1u << k : 0u;
+        const Listed l = list_from(s, x, r, vec, vectors, groups, !by_k, per2, edge);
         bool done = false;
-        const double scale = 0x1p44, rest = sum * scale;
         const unsigned k = by_k ? (unsigned)top_k : 0;
-        if (fits && by_k) {
-            if (total <= kPairs) solve(s, r, k, 0ull, top_p, 0.0, 0, 0);
-            else cut_all(s, step, x, r, k, top_p, 0ull, false, total, vocab);
-            done = true;
-        } else if (fits) {
-            // (a mass of all that the list does not reach is found out about below)
-            auto cut = [&](double more) {
-                if (total <= kPairs) {
-                    solve(s, r, 0, 0ull, top_p, more, 0, 0);
-                    return s.cut.mass > 0;
-                }
-                histogram(s, x, r, Range{0, 0, 0, 0, 0, 0}, true);
-                const unsigned long long whole = mass_of_bins(s), target = share_of(top_p, (double)whole + more);
-                if (target <= whole) cut_all(s, step, x, r, 0, 1.0, target, true, total, vocab);
-                return target <= whole;
-            };
-            done = cut(rest);
-            // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
-            // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
-            const double off = top_p * (sum * 0x1p-20 + slope * 0x1p-22) * scale;
-            if (done && !((double)s.cut.before < (double)s.cut.target - off && (double)s.cut.target + off <= (double)s.cut.mass)) {
-                // it is not: the rest as the list's entries are summed
-                unsigned long long exact = 0;
-                for (int i = tid; i < n; i += kThreads)
-                    if ((float)x.v[i] < edge) exact += mass_of(r, (float)x.v[i]);
-                done = cut((double)sum_of_all(s, exact));
+        if (by_k) {
+            done = reached && l.fits;
+            if (done && l.total <= kPairs) solve(s, r, k, 0ull, top_p, 0.0, 0, 0);
+            else if (done) cut_all(s, step, x, r, k, top_p, 0ull, false, l.total, vocab);
+        } else if (l.fits) {
+            done = cut_by_mass(s, step, x, r, l, top_p, vocab, edge);
+            if (!done && further < edge) {
+                __syncthreads();
+                if (tid == 0) s.listed[0] = s.listed[1] = s.pairs = 0;
+                cluster_sync();
+                const Listed all = list_from(s, x, r, vec, vectors, (1u << kGroups) - 1, true, per2, further);
+                done = all.fits && cut_by_mass(s, step, x, r, all, top_p, vocab, further);
             }
         }
         if (!done) {
@@ -815,17 +852,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_sample(const __grid_constant__ 
 
 inline int64_t slice_of(int64_t vocab, int cs) { return ((vocab + cs - 1) / cs + 15) / 16 * 16; }
 
-template <typename L>
-int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
-    // A CTA takes a row, a cluster one that does not fit, or a long one where SMs are left over.  Measured, us a call of sample without
-    // a cut / with top_k 50 / with top_p 0.95:
-    //   one row of 90,000 in bf16, by 1 / 4 / 8 CTAs: 18.6, 14.0, 30; 8.5, 11.8, 20; 6.3, 11.2, 18.  Of 32,000 by 1 / 8: 8.6, 9.4, 17;
-    //   4.9, 10.8, 17.  36 of 50,000 in fp32 by 1 / 4 / 8 (more CTAs than SMs): 14.1, 14.5, 27; 10.4, 13.5, 25; 12.8, 23.7, 41.
-    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.
-    int cs = slice_of(p.a.vocab, 1) * sizeof(L) <= kRowBytes ? 1 : slice_of(p.a.vocab, 4) * sizeof(L) <= kRowBytes ? 4 : 8;
-    if (p.a.vocab * (int64_t)sizeof(L) >= kLongBytes) cs = 16 * rows <= sms ? 8 : 4 * rows <= sms ? std::max(cs, 4) : cs;
-    p.slice = (int)slice_of(p.a.vocab, cs);
-    cudaError_t e = cudaFuncSetAttribute(k_sample<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
+template <typename L, int CTAS>
+int launch(const Params& p, int64_t rows, int cs, cudaStream_t s) {
+    cudaError_t e = cudaFuncSetAttribute(k_sample<L, CTAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowBytes + 16);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(rows * cs));
@@ -839,9 +868,24 @@ int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, k_sample<L>, p);
+    e = cudaLaunchKernelEx(&cfg, k_sample<L, CTAS>, p);
     if (e != cudaSuccess) return set_error((int)e, "spark_sample: launch failed: %s", cudaGetErrorString(e));
     return check_launch("spark_sample");
+}
+template <typename L>
+int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
+    // A CTA takes a row, a cluster one that does not fit, or a long one where SMs are left over.  Measured, us a call of sample without
+    // a cut / with top_k 50 / with top_p 0.95:
+    //   one row of 90,000 in bf16, by 1 / 4 / 8 CTAs: 18.6, 14.0, 30; 8.5, 11.8, 20; 6.3, 11.2, 18.  Of 32,000 by 1 / 8: 8.6, 9.4, 17;
+    //   4.9, 10.8, 17.  36 of 50,000 in fp32 by 1 / 4 / 8 (more CTAs than SMs): 14.1, 14.5, 27; 10.4, 13.5, 25; 12.8, 23.7, 41.
+    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.
+    int cs = slice_of(p.a.vocab, 1) * sizeof(L) <= kRowBytes ? 1 : slice_of(p.a.vocab, 4) * sizeof(L) <= kRowBytes ? 4 : 8;
+    if (p.a.vocab * (int64_t)sizeof(L) >= kLongBytes) cs = 16 * rows <= sms ? 8 : 4 * rows <= sms ? std::max(cs, 4) : cs;
+    p.slice = (int)slice_of(p.a.vocab, cs);
+    // Two CTAs share an SM (64 registers a thread) where there are more than SMs and both fit, else one has it alone (128): 256 rows of
+    // 32,000 in bf16 27.4 / 29.0 us, 8 of them in fp32 17.2 / 15.7, 64 of 100,003 34.8 / 33.4.
+    const size_t bytes = sizeof(Shared) + p.slice * sizeof(L) + 16 + 1024;
+    return rows * cs > sms && 2 * bytes <= kSmemSm ? launch<L, 2>(p, rows, cs, s) : launch<L, 1>(p, rows, cs, s);
 }
 
 }  // namespace sm
