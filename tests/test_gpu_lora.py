@@ -246,3 +246,53 @@ def test_a_pool_of_one_captured():
     scale.fill_(1.75)
     graph.replay()
     check(y, x, a, b, ids, scale, out)
+
+
+@pytest.mark.parametrize("tokens,oc", [(1, 512), (40, 2048), (200, 1000), (4096, 2304)])
+def test_a_chain_of_calls_without_a_pause(tokens, oc):
+    """What a call reads (y, x, the numbers of the adapters) is written by the launch before it, and what it writes is read by the
+    next: one graph of twelve steps gives what the steps give one by one."""
+    y, x, a, b, ids, scale = make(tokens, tokens, 256, oc, 16, 6, BF)
+    ys, xs = (torch.stack([v * (i + 1) for i in range(12)]) for v in (y, x))
+    ids = torch.stack([(ids + i).remainder(7) - 1 for i in range(12)]).to(torch.int32)
+    if tokens > 1000:
+        ids = ids[:, ::tokens // 8].contiguous()
+    now = [torch.empty_like(v[0]) for v in (ys, xs, ids)]
+    out = torch.empty(12, tokens, oc, dtype=BF, device="cuda")
+
+    def step(i, wait):
+        for to, v in zip(now, (ys, xs, ids)):
+            to.copy_(v[i])
+            if wait:
+                torch.cuda.synchronize()
+        ops().lora_add(now[0], now[1], a, b, now[2], scale=scale, out=now[0])
+        if wait:
+            torch.cuda.synchronize()
+        ops().lora_add(now[0], now[1] * 0.5, a, b, now[2], scale=scale, out=out[i])
+
+    for i in range(12):
+        step(i, True)
+    torch.cuda.synchronize()
+    want, graph = out.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(12):
+            step(i, False)
+    for _ in range(5):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_two_streams_at_once():
+    """Calls on two streams have workspaces of their own."""
+    sets = [make(s, 512, 512, 4096, 16, 4, BF) for s in (1, 2)]
+    want = [ops().lora_add(*v[:5], scale=v[5]) for v in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(10):
+        for i, (s, v) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(s):
+                got[i].append(ops().lora_add(*v[:5], scale=v[5]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])

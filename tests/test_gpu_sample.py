@@ -337,3 +337,14 @@ def test_rows_of_the_lowest_value(vocab, dtype):
         check_filter(logits, ops().filter_logits(logits, **s), s)
         token, logprob = ops().sample(logits, noise, **s, return_logprob=True)
         check_sample(logits, noise, token, logprob, s)
+
+
+@pytest.mark.parametrize("dtype", [FP, BF])
+def test_many_rows_of_wide_distributions(dtype):
+    """Rows whose top_p takes more entries than the first list has, whole rows, and borders that sums in fp32 leave open."""
+    g = gen(17)
+    logits = (randn(g, 160, 20011) * torch.tensor([0.5, 2.0, 3.0, 4.0], device="cuda").repeat(40)[:, None]).to(dtype)
+    p = torch.rand(160, generator=g, device="cuda") * 0.2 + 0.79
+    s = dict(top_p=p)
+    check_filter(logits, ops().filter_logits(logits, **s), s)
+    check_filter(logits[:8], ops().filter_logits(logits[:8], top_p=p[:8]), dict(top_p=p[:8]))
