@@ -38,7 +38,7 @@
 // TB/s), 47 with top_k 50, 93 with top_p 0.95.  A flat distribution, of which more stays
 // than lists hold, is divided by histograms of all its entries, whose exponentials in 64
 // bits bound it (four at a time take no less): 130 to 220 us for 64 rows of 100,003; and a
-// row in some hundred whose border the sums in fp32 leave open takes 40 us more.
+// row in some hundred whose border the sums in fp32 leave open takes 20 to 50 us more.
 #include <float.h>
 #include <math.h>
 
@@ -553,6 +553,7 @@ __device__ __forceinline__ Listed list_from(Shared& s, Slice<L>& x, const Row& r
     using V = Vec<L>;
     constexpr int N = V::N;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, cs = (int)cluster_size();
+    const float per2_low = (float)(r.per_temp * 1.4426950408889634 - (double)per2), lowest = fmaxf(-200.f / per2, -FLT_MAX);
     double sum = 0, slope = 0;
 #pragma unroll
     for (int k = 0; k < kGroups; ++k) {
@@ -569,14 +570,19 @@ __device__ __forceinline__ Listed list_from(Shared& s, Slice<L>& x, const Row& r
                     s.list[far ? kList - 1 - at : at] = (uint16_t)(place + __ffs(which) - 1);
             }
             if (!sums) continue;
-            float e = 0.f, f = 0.f;
+            float e[N], f = 0.f;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float v = (float)u.v[j], z = fmaxf((v - r.top) * per2, -200.f);   // (2^-200 is 0)
-                const float q = v < edge ? exp2_of(z) : 0.f;
-                e += q, f = fmaf(z, q, f);
+                // 2^z, z in two terms: a difference and 1 / T in two
+                const float v = (float)u.v[j], d = fmaxf(v - r.top, lowest), z = d * per2;   // (2^-200 is 0)
+                const float q = v < edge ? exp2_of(z) : 0.f, low = fmaf(d, per2_low, fmaf(d, per2, -z)) * 0.69314718f;
+                e[j] = fmaf(q, low, q), f = fmaf(z, q, f);
             }
-            sum += e, slope -= f;
+#pragma unroll
+            for (int o = N / 2; o > 0; o >>= 1)
+#pragma unroll
+                for (int j = 0; j < o; ++j) e[j] += e[j + o];
+            sum += e[0], slope -= f;
         }
     }
     if (sums) {
@@ -628,9 +634,9 @@ __device__ __forceinline__ bool cut_by_mass(Shared& s, int& step, const Slice<L>
     };
     constexpr double scale = 0x1p44;
     if (!cut(l.sum * scale)) return false;
-    // The terms of the rest are off by 2^-22 (the exponential) and 7 2^-24 (sums of 8) of themselves, and by 3 2^-24 |z|
-    // (a difference, a factor and a product); the cut is certain where that does not reach the next entry.
-    const double off = top_p * (l.sum * 0x1p-20 + l.slope * 0x1p-22) * scale;
+    // The terms of the rest are off by 2^-22 (the exponential), 2^-24 (its second factor) and 3 2^-24 (sums of 8) of themselves, and by
+    // 2^-24 |z| (a difference); the cut is certain where that does not reach the next entry.
+    const double off = top_p * (l.sum * 0x1.4p-21 + l.slope * 0x1p-24) * scale;
     if ((double)s.cut.before < (double)s.cut.target - off && (double)s.cut.target + off <= (double)s.cut.mass) return true;
     // it is not: the rest as the list's entries are summed
     unsigned long long exact = 0;
@@ -879,16 +885,21 @@ template <typename L>
 int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
     // A CTA takes a row, a cluster one that does not fit, or a long one where SMs are left over.  Measured, us a call of sample without
     // a cut / with top_k 50 / with top_p 0.95:
+    // (seven eighths of the SMs, of an SM's two places where rows are long)
     //   one row of 90,000 in bf16, by 1 / 4 / 8 CTAs: 18.6, 14.0, 30; 8.5, 11.8, 20; 6.3, 11.2, 18.  Of 32,000 by 1 / 8: 8.6, 9.4, 17;
     //   4.9, 10.8, 17.  36 of 50,000 in fp32 by 1 / 4 / 8 (more CTAs than SMs): 14.1, 14.5, 27; 10.4, 13.5, 25; 12.8, 23.7, 41.
-    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.
+    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.  64 of 100,003 by 1 / 4: 22.2, 15.6,
+    //   36 (85 with a border left open); 15.8, 15.9, 33 (48).  64 of 65,000 by 1 / 4: 14.7, 12.4, 24; 10.8, 13.3, 39.
     int cs = slice_of(p.a.vocab, 1) * sizeof(L) <= kRowBytes ? 1 : slice_of(p.a.vocab, 4) * sizeof(L) <= kRowBytes ? 4 : 8;
-    if (p.a.vocab * (int64_t)sizeof(L) >= kLongBytes) cs = 16 * rows <= sms ? 8 : 4 * rows <= sms ? std::max(cs, 4) : cs;
+    const int64_t bytes_row = p.a.vocab * (int64_t)sizeof(L);
+    if (bytes_row >= kLongBytes) cs = 16 * rows <= sms ? 8 : (bytes_row >= 160 * 1024 ? 16 : 32) * rows <= 7 * sms ? std::max(cs, 4) : cs;
     p.slice = (int)slice_of(p.a.vocab, cs);
     // Two CTAs share an SM (64 registers a thread) where there are more than SMs and both fit, else one has it alone (128): 256 rows of
-    // 32,000 in bf16 27.4 / 29.0 us, 8 of them in fp32 17.2 / 15.7, 64 of 100,003 34.8 / 33.4.
+    // 32,000 in bf16 27.4 / 29.0 us, 8 of them in fp32 17.2 / 15.7, 64 of 100,003 34.8 / 33.4.  Clusters do not find all SMs: 36 rows
+    // of 90,000 by 4 with an SM each 39.9 us, sharing SMs 30.0; 30 of 151,936 27.2 and 36.7.
     const size_t bytes = sizeof(Shared) + p.slice * sizeof(L) + 16 + 1024;
-    return rows * cs > sms && 2 * bytes <= kSmemSm ? launch<L, 2>(p, rows, cs, s) : launch<L, 1>(p, rows, cs, s);
+    const bool more = cs > 1 ? 8 * rows * cs > 7 * sms : rows > sms;
+    return more && 2 * bytes <= kSmemSm ? launch<L, 2>(p, rows, cs, s) : launch<L, 1>(p, rows, cs, s);
 }
 
 }  // namespace sm
