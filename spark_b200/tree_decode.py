@@ -133,6 +133,7 @@ class TreeDecoder(nn.Module):
         self.register_buffer("table", rope_table(max_positions, rot_dim, base, **scaling), persistent=False)
         # the tree of one node, which hangs on the context
         self.register_buffer("root", torch.full((1,), -1, dtype=torch.int32, device=self.table.device), persistent=False)
+        self.register_buffer("root_depth", torch.zeros(1, dtype=torch.int32, device=self.table.device), persistent=False)
 
     @staticmethod
     def norm(x: torch.Tensor) -> torch.Tensor:
@@ -185,8 +186,10 @@ class TreeDecoder(nn.Module):
     def decode(self, last: torch.Tensor, cache: PagedKVCache, noise: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0,
                min_p=0.0, return_logprob: bool = False):
         """One token a sequence: forward of the last ones [batch], whose K/V rows go into the
-        cache, and the next ones, drawn by ops.sample with its settings."""
-        logits, new = self(last[:, None], self.root, self.root + 1, cache)
+        cache, and the next ones, drawn by ops.sample with its settings.  A negative one (a
+        row that had no distribution gives -1) stands for token 0, and what follows it means
+        nothing, as in a row whose sequence has no pages."""
+        logits, new = self(last.clamp(min=0)[:, None], self.root, self.root_depth, cache)
         cache.append(new)
         return ops.sample(logits[:, 0], noise, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
                           return_logprob=return_logprob)

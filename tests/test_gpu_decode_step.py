@@ -183,3 +183,64 @@ def test_adapters_of_layers():
     layer.use(torch.zeros(4, dtype=torch.int32, device="cuda"))
     with pytest.raises(ValueError):
         layer(x)
+
+
+def test_rows_that_have_ended():
+    """A batch's sequence without pages, and one whose last draw gave nothing, leave the others' tokens as they are."""
+    from spark_b200 import ops
+    _, model = build(5)
+    prompts = torch.randint(0, VOCAB, (3, 40), generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    model.use_adapters(torch.tensor(ADAPTERS, dtype=torch.int32, device="cuda"))
+    noise, got = torch.ones(3, VOCAB, device="cuda"), []
+    for ended in (False, True):
+        cache = cache_of(model, prompts, 60)
+        last, tokens = prompts[:, -1].clone(), []
+        if ended:
+            cache.release(1)
+            last[1] = -1
+        for _ in range(8):
+            last = model.decode(last, cache, noise, temperature=0.0)
+            if ended:
+                last[1] = -1
+            tokens.append(last)
+        got.append(torch.stack(tokens, 1))
+    ops.check_device_errors()
+    assert torch.equal(got[0][::2], got[1][::2]) and int(cache.lens[1]) == 0
+
+
+def test_a_captured_step_takes_new_numbers():
+    """One graph of a step: other adapters, settings, tokens and noise at each replay, and what the same calls give one by one."""
+    from spark_b200 import ops
+    _, model = build(6)
+    g = torch.Generator("cuda").manual_seed(3)
+    prompts = torch.randint(0, VOCAB, (4, 50), generator=g, device="cuda")
+    ids = torch.zeros(4, dtype=torch.int32, device="cuda")
+    model.use_adapters(ids)
+    cache = cache_of(model, prompts, 64)
+    last, noise = torch.zeros(4, dtype=torch.long, device="cuda"), torch.ones(4, VOCAB, device="cuda")
+    heat, p = torch.ones(4, device="cuda"), torch.ones(4, device="cuda")
+    k = torch.zeros(4, dtype=torch.int32, device="cuda")
+
+    def step():
+        logits, _ = model(last[:, None], model.root, model.root_depth, cache)
+        return ops.sample(logits[:, 0], noise, temperature=heat, top_k=k, top_p=p, return_logprob=True)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(6):
+        ids.copy_(torch.randint(-1, POOL, (4,), generator=g, device="cuda"))
+        last.copy_(torch.randint(0, VOCAB, (4,), generator=g, device="cuda"))
+        noise.exponential_(generator=g)
+        heat.copy_(torch.tensor([0.0, 0.5, 1.0, 2.0], device="cuda").roll(i))
+        p.copy_(torch.tensor([1.0, 0.9, 0.3, 0.99], device="cuda").roll(-i))
+        k.copy_(torch.tensor([0, 3, 100, VOCAB], device="cuda").roll(i // 2))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [u.clone() for u in out]
+        assert all(torch.equal(u, v) for u, v in zip(got, step()))
