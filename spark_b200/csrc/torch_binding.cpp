@@ -340,7 +340,7 @@ struct NormRope : torch::autograd::Function<NormRope> {
 
 std::tuple<Tensor, OptTensor, int> apply_qk_norm_rope(const Tensor& q, const OptTensor& k, const OptTensor& q_weight, const OptTensor& k_weight,
                                                       const Tensor& positions, const Tensor& table, double eps, bool interleaved,
-                                                      uint64_t ws, uint64_t stream) {
+                                                      bool capturing, uint64_t ws, uint64_t stream) {
     bool grad = q.requires_grad();
     TORCH_CHECK_NOT_IMPLEMENTED(!q._fw_grad(0).defined() && !table._fw_grad(0).defined(), "apply_qk_norm_rope: no forward-mode differentiation");
     for (const OptTensor* t : {&k, &q_weight, &k_weight}) {
@@ -350,6 +350,16 @@ std::tuple<Tensor, OptTensor, int> apply_qk_norm_rope(const Tensor& q, const Opt
     }
     if (!grad || !at::GradMode::is_enabled())
         return qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, std::nullopt, std::nullopt, ws, stream);
+    // An eager graph of a leaf keeps the node that its gradient goes to, with its stream: the default stream's would draw that into the
+    // capture when the backward pass is captured, which ends the process.
+    for (const Tensor* t : {&q, k ? &*k : nullptr, q_weight ? &*q_weight : nullptr, k_weight ? &*k_weight : nullptr}) {
+        if (!capturing || !t || !t->requires_grad() || t->grad_fn()) continue;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto on = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!on || on->native_handle() != nullptr,
+                    "apply_qk_norm_rope: under capture no graph of the same leaves on the default stream may live (drop its outputs, or make "
+                    "it on another stream)");
+    }
     int rc = SPARK_OK;
     const auto out = NormRope::apply(q, k, q_weight, k_weight, positions, table, eps, interleaved, ws, stream, &rc);
     return {out[0], k ? OptTensor(out[1]) : std::nullopt, rc};

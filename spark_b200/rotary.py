@@ -71,9 +71,11 @@ def apply_qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.
                        interleaved: bool = False):
     """Differentiable ops.qk_norm_rope: (q', k'), with gradients for q, k and the weights.
     Those of positions and table are not computed; gradients of gradients and forward-mode
-    differentiation are refused."""
+    differentiation are refused, and so are leaves, under stream capture, of which an eager
+    graph on the default stream lives."""
     _, ws, stream = ops._place("qk_norm_rope", q)
-    y, z, rc = ops._native().apply_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, ws, stream)
+    y, z, rc = ops._native().apply_qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved,
+                                                torch.cuda.is_current_stream_capturing(), ws, stream)
     if rc:
         ops._check("spark_qk_norm_rope", rc)
     return y, z

@@ -349,3 +349,27 @@ def test_captured_and_on_another_stream():
     check_forward(now, qw, out[0], positions, table, False, 1e-6)
     check_backward(now, qw, gy, grads[0], grads[2], positions, table, False, 1e-6)
     ops().check_device_errors()
+
+
+def test_capture_beside_a_living_graph():
+    """Leaves of which an eager graph lives: refused under capture if it is the default stream's, and taken once it is gone."""
+    g, q, k, qw, kw, positions, table = make(23, 1, 24, 4, 2, 64, 64, BF, FP)
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, qw, kw)]
+    gy, gz = randn(g, *q.shape, dtype=BF), randn(g, *k.shape, dtype=BF)
+    out = rotary().apply_qk_norm_rope(*leaves, positions, table)
+    want = torch.autograd.grad(out, leaves, (gy, gz), retain_graph=True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="default stream"):
+            rotary().apply_qk_norm_rope(*leaves, positions, table)
+        with torch.no_grad():
+            plain = rotary().apply_qk_norm_rope(*leaves, positions, table)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(plain, out))
+    del out
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = rotary().apply_qk_norm_rope(*leaves, positions, table)
+        got = torch.autograd.grad(out, leaves, (gy, gz))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
