@@ -284,9 +284,10 @@ def test_a_chain_of_calls_without_a_pause(tokens, oc):
         assert torch.equal(out, want)
 
 
-def test_two_streams_at_once():
+@pytest.mark.parametrize("tokens", [512, 2048])
+def test_two_streams_at_once(tokens):
     """Calls on two streams have workspaces of their own."""
-    sets = [make(s, 512, 512, 4096, 16, 4, BF) for s in (1, 2)]
+    sets = [make(s, tokens, 512, 4096, 16, 4, BF, ids=torch.randint(-1, 4, (tokens // 64,), device="cuda").repeat_interleave(64)) for s in (1, 2)]
     want = [ops().lora_add(*v[:5], scale=v[5]) for v in sets]
     torch.cuda.synchronize()
     streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
@@ -296,3 +297,33 @@ def test_two_streams_at_once():
                 got[i].append(ops().lora_add(*v[:5], scale=v[5]))
     torch.cuda.synchronize()
     assert all(torch.equal(g, want[i]) for i in (0, 1) for g in got[i])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("tokens,rank,ic,oc", [(8400, 24, 96, 1000), (8389, 64, 40, 1000), (61700, 40, 64, 136), (21411, 12, 72, 392), (1050000, 4, 16, 8)])
+def test_as_many_values_as_tensor_memory_takes(tokens, rank, ic, oc, dtype):
+    """The tiles of test_many_tokens, again and again at other offsets, where y has 2^23 values or more; rows with a gap; an adapter
+    of infinities."""
+    y, x, a, b, _, scale = make(rank, tokens, ic, oc, rank, 12, dtype)
+    ids = torch.zeros(900, dtype=torch.int32, device="cuda")
+    ids[128:200], ids[200:256] = 3, 5
+    ids[256:384] = torch.arange(128, device="cuda") // 32 + 6
+    ids[384:512] = -1
+    ids[512:600], ids[600:640] = 2, -1
+    ids[640:768] = torch.arange(128, device="cuda") * 5 % 12
+    ids[768:900] = torch.arange(132, device="cuda") % 3 - 1
+    ids = ids.repeat(tokens // 900 + 1)[:tokens].contiguous()
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    check(y, x, a, b, ids, scale, out)
+    none = ids < 0
+    assert torch.equal(out[none], y[none])
+    wide = torch.cat([y[:, :8], y, y[:, :8]], 1)
+    part = wide[:, 8:8 + oc]
+    ops().lora_add(part, x, a, b, ids, scale=scale, out=part)
+    assert torch.equal(part, out) and torch.equal(wide[:, :8], y[:, :8]) and torch.equal(wide[:, -8:], y[:, :8])
+    a[3, rank - 1] = float("inf")
+    b[5, oc // 2] = float("nan")
+    bad = ops().lora_add(y, x, a, b, ids, scale=scale)
+    others = (ids != 3) & (ids != 5)
+    assert torch.equal(bad[others], out[others]) and not bad[ids == 3].isfinite().all() and bad[ids == 5][:, oc // 2].isnan().all()
+    ops().check_device_errors()

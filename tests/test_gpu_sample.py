@@ -348,3 +348,20 @@ def test_many_rows_of_wide_distributions(dtype):
     s = dict(top_p=p)
     check_filter(logits, ops().filter_logits(logits, **s), s)
     check_filter(logits[:8], ops().filter_logits(logits[:8], top_p=p[:8]), dict(top_p=p[:8]))
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 50021, BF), (10, 50021, HF), (30, 30011, FP), (40, 90001, BF), (64, 100003, HF), (70, 90001, BF),
+                                              (150, 30011, FP), (300, 20011, BF), (20, 110003, FP), (40, 110003, FP), (2, 210011, FP)])
+def test_rows_by_ctas_and_clusters(rows, vocab, dtype):
+    """Numbers and lengths of rows that one CTA takes, and clusters of 4 and 8, alone on an SM and two of them."""
+    g = gen(rows)
+    logits, noise = (randn(g, rows, vocab) * 4).to(dtype), noise_of(g, rows, vocab)
+    kinds = [(1.0, 0, 0.95, 0.0), (0.7, 50, 0.9, 0.0), (1.2, 900, 0.99, 0.01), (2.0, 0, 0.9, 0.0), (0.9, 0, 1.0, 0.0)]
+    values = list(zip(*(kinds[i % 5] for i in range(rows))))
+    s = {n: torch.tensor(v, dtype=torch.int32 if n == "top_k" else FP, device="cuda") for n, v in zip(("temperature", "top_k", "top_p", "min_p"), values)}
+    out = ops().filter_logits(logits, **s)
+    token, logprob = ops().sample(logits, noise, **s, return_logprob=True)
+    some = torch.randperm(rows, generator=torch.Generator().manual_seed(rows))[:8].cuda()
+    cut = {n: v[some] for n, v in s.items()}
+    check_filter(logits[some], out[some], cut)
+    check_sample(logits[some], noise[some], token[some], logprob[some], cut)
