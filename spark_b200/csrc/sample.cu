@@ -71,8 +71,9 @@ struct Params {
 };
 
 struct Note {
-    float a, b;
-    int i, pad;
+    float a;
+    int i;
+    unsigned long long b;
 };
 // An entry's place in the falling order is (key, index), rising.
 struct Entry {
@@ -207,7 +208,7 @@ __device__ __forceinline__ float Vec<__nv_bfloat16>::largest() const {
     return __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
 }
 
-__device__ __forceinline__ Note none() { return Note{-INFINITY, 0.f, -1, 0}; }
+__device__ __forceinline__ Note none() { return Note{-INFINITY, -1, 0}; }
 __device__ __forceinline__ void add(Note& v, float a, int i) {
     if (v.i < 0 || a > v.a || (a == v.a && i < v.i)) v.a = a, v.i = i;
 }
@@ -217,13 +218,17 @@ __device__ __forceinline__ int ordered(float x) {
     return i ^ ((i >> 31) & 0x7fffffff);
 }
 __device__ __forceinline__ float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+// The sum over a warp.
+__device__ __forceinline__ unsigned long long sum_of_warp(unsigned long long x) {
+    const unsigned a = __reduce_add_sync(0xffffffffu, (unsigned)x & 0x7ffffff), b = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 27) & 0x7ffffff),
+                   c = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 54));
+    return ((unsigned long long)c << 54) + ((unsigned long long)b << 27) + a;
+}
 // How notes are joined: the largest a with its lowest index i (-1: none), b summed.
 __device__ __forceinline__ Note join_warp(Note v) {
     const float top = unordered(__reduce_max_sync(0xffffffffu, ordered(v.i < 0 ? -INFINITY : v.a)));
     const unsigned first = __reduce_min_sync(0xffffffffu, v.i >= 0 && v.a == top ? (unsigned)v.i : 0xffffffffu);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) v.b += __shfl_xor_sync(0xffffffffu, v.b, o);
-    return Note{top, v.b, (int)first, 0};
+    return Note{top, (int)first, sum_of_warp(v.b)};
 }
 // Of all threads of the cluster, for every thread, in a fixed order.
 __device__ __forceinline__ Note join_all(Shared& s, int& step, Note v) {
@@ -371,12 +376,6 @@ __device__ __forceinline__ void find_count(Shared& s, unsigned k, unsigned more)
     __syncthreads();
 }
 
-// The sum over a warp.
-__device__ __forceinline__ unsigned long long sum_of_warp(unsigned long long x) {
-    const unsigned a = __reduce_add_sync(0xffffffffu, (unsigned)x & 0x7ffffff), b = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 27) & 0x7ffffff),
-                   c = __reduce_add_sync(0xffffffffu, (unsigned)(x >> 54));
-    return ((unsigned long long)c << 54) + ((unsigned long long)b << 27) + a;
-}
 // The mass of all bins, for every thread.
 __device__ __noinline__ unsigned long long mass_of_bins(Shared& s) {
     const int t = threadIdx.x, lane = t & 31;
@@ -710,13 +709,13 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
     __syncwarp();
     cluster_wait();      // every CTA of the cluster has started: its shared memory may be written
     int step = 0;
-    Note best{-INFINITY, 0.f, 0, 0};
+    Note best{-INFINITY, 0, 0};
 #pragma unroll
-    for (int k = 0; k < kGroups; ++k) best.a = fmaxf(best.a, most[k]), best.b += most[k] == most[k] ? 0.f : 1.f;
+    for (int k = 0; k < kGroups; ++k) best.a = fmaxf(best.a, most[k]), best.b += most[k] == most[k] ? 0 : 1;
     best = join_all(s, step, best);
     Row r;
     r.top = best.a;
-    const bool none_here = best.b != 0.f || !(best.a > -INFINITY && best.a < INFINITY) || !(temp >= 0);
+    const bool none_here = best.b != 0 || !(best.a > -INFINITY && best.a < INFINITY) || !(temp >= 0);
     const bool greedy = !none_here && temp == 0;
     r.per_temp = s.per_temp, r.bins = s.bins;
     const float per2 = (float)(r.per_temp * 1.4426950408889634);   // (exponents of 2)
@@ -816,18 +815,19 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
     if (!a.token) return;
     Note got = none();
     if (!none_here && !greedy) {
-        // (e to 2^-22 and 3 2^-24 |z|, the quotient to 2 units more)
+        // (e to 2^-22 and 3 2^-24 |z|, the quotient to 2 units more; a list's order is the atomics', so its sum is in integers)
         got.a = 0.f;
         if (x.list) {
             x.each([&](float f, int index) {
                 if (!stays(f, index)) return;
                 const float q = exp2_of((f - r.top) * per2), chance = __fdividef(q, noise[index - v0]);
-                got.b += q;
+                got.b += __float2ull_rn(q * 0x1p44f);
                 if (chance > got.a || (chance == got.a && index < got.i)) got.a = chance, got.i = index;
             });
         } else {
             constexpr int kAhead = 8;
             const bool all = limit == -INFINITY;
+            float sum = 0.f;
             for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
                 float f[kAhead], e[kAhead];
 #pragma unroll
@@ -840,10 +840,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
                     const float q = exp2_of((f[k] - r.top) * per2), chance = __fdividef(q, e[k]);
-                    got.b += q;
+                    sum += q;
                     if (chance > got.a) got.a = chance, got.i = v0 + i0 + k * kThreads;
                 }
             }
+            got.b = __double2ull_rn((double)sum * 0x1p44);
         }
         got = join_all(s, step, got);
     } else if (greedy) {
@@ -851,7 +852,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
     }
     // the owner of the token knows its logit
     if (a.logprob && !none_here && !greedy && got.i >= v0 && got.i < v0 + n && tid == 0)
-        a.logprob[b] = (float)(((double)(float)x.v[got.i - v0] - (double)r.top) * r.per_temp) - logf(got.b);
+        a.logprob[b] = (float)(((double)(float)x.v[got.i - v0] - (double)r.top) * r.per_temp) - logf((float)((double)got.b * 0x1p-44));
     if (rank == 0 && tid == 0) {
         a.token[b] = got.i;
         if (a.logprob && (got.i < 0 || greedy)) a.logprob[b] = got.i < 0 ? NAN : 0.f;

@@ -365,3 +365,14 @@ def test_rows_by_ctas_and_clusters(rows, vocab, dtype):
     cut = {n: v[some] for n, v in s.items()}
     check_filter(logits[some], out[some], cut)
     check_sample(logits[some], noise[some], token[some], logprob[some], cut)
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(200, 20011, BF), (3, 100003, FP)])
+def test_the_same_inputs_give_the_same_bits(rows, vocab, dtype):
+    """Tokens and their probabilities whatever the order of atomics."""
+    g = gen(29)
+    logits, noise = (randn(g, rows, vocab) * 3).to(dtype), noise_of(g, rows, vocab)
+    for s in (dict(top_k=300), dict(top_k=2000, top_p=0.95), dict(top_p=0.9), dict(top_p=0.99, temperature=2.0), dict()):
+        first = ops().sample(logits, noise, **s, return_logprob=True)
+        for _ in range(20):
+            assert all(torch.equal(u, v) for u, v in zip(first, ops().sample(logits, noise, **s, return_logprob=True)))
