@@ -108,6 +108,20 @@ template <typename T>
 struct Span {
     const T *begin, *end;
 };
+// The 8 values that begin `off` values into the vectors a and b, those from the n-th on zero.
+__device__ __forceinline__ uint4 part_of(const uint4& a, const uint4& b, int off, int64_t n) {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 6; ++j) w[j] = off & 4 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = off & 2 ? w[j + 1] : w[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        w[j] = __funnelshift_r(w[j], w[j + 1], (off & 1) * 16);
+        w[j] &= 2 * j >= n ? 0u : 2 * j + 1 >= n ? 0xffffu : 0xffffffffu;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 // Values k..k + 7 of a row of n, zeros behind its end; VEC: rows on 16 bytes, n a multiple of 8.  Else out of the two 16-byte
 // vectors that they are in, where these are within the matrix.
 template <typename T, bool VEC>
@@ -147,6 +161,20 @@ __device__ __forceinline__ uint4 load8(const T* row, int64_t k, int64_t n, const
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// The same without a branch, so that loads go out together, for rows `inside` the matrix: behind a row's end its beginning is read, and
+// none of it taken.
+template <typename T>
+__device__ __forceinline__ uint4 load8_inside(const T* row, int64_t k, int64_t n) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + (k < n ? k : 0)), from = at & ~uintptr_t(15);
+    const int off = (int)(at - from) / 2;
+    return part_of(*reinterpret_cast<const uint4*>(from), *reinterpret_cast<const uint4*>(from + (off ? 16 : 0)), off, n - k);
+}
+// Whether the 16-byte vectors that hold rows first..last, of n values at distance ld, are within a matrix of `rows` such rows: 7 values
+// before the first row and 15 behind the last are.
+__device__ __forceinline__ bool inside(int64_t first, int64_t last, int64_t n, int64_t ld, int64_t rows) {
+    return first * ld >= 7 && last < rows && last * ld + n + 15 <= (rows - 1) * ld + n;
 }
 
 // A tile's adapters: ids[row] (-1: none, or no such token), and the distinct ones in order of their first rows.
@@ -246,7 +274,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_down(const __grid_constant
         struct Part {
             uint4 u[MT][2], w[NT];
         };
+        // (many rows off 16 bytes: without branches where all are inside; 3019 tokens of 4217 values 167 us without, 99 with)
+        const bool whole = !VEC && MT > 1 && inside(t0, t0 + ROWS - 1, p.ic, p.ldx, p.tokens) &&
+                           inside((int64_t)id * p.rank + r0, (int64_t)id * p.rank + min(r0 + RANKS, p.rank) - 1, p.ic, p.ic, p.adapters * p.rank);
         auto load = [&](Part& q, int64_t k) {
+            if (!VEC && MT > 1 && whole) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) q.u[m][e] = load8_inside(x + (t0 + m * 16 + e * 8 + g) * p.ldx, k, p.ic);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int r = r0 + n * 8 + g;
+                    // (a rank behind the last: one that is there, its products are not taken)
+                    q.w[n] = load8_inside(a + (int64_t)min(r, p.rank - 1) * p.ic, k, p.ic);
+                }
+                return;
+            }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -387,6 +431,19 @@ struct Eight {
         for (int j = 0; j < 8; j += 2) Mma<Y>::round2(e.v + j, f[j], f[j + 1]);
         *reinterpret_cast<uint4*>(p) = e.raw;
     }
+    // off 16 bytes: three words on 4 bytes and the two values beside them
+    static __device__ __forceinline__ void store_off(Y* p, const float* f) {
+        Eight e;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) Mma<Y>::round2(e.v + j, f[j], f[j + 1]);
+        const uint32_t w[4] = {e.raw.x, e.raw.y, e.raw.z, e.raw.w};
+        const int odd = (int)(reinterpret_cast<uintptr_t>(p) >> 1 & 1);
+#pragma unroll
+        for (int j = 0; j < 3; ++j) *reinterpret_cast<uint32_t*>(p + 2 * j + odd) = __funnelshift_r(w[j], w[j + 1], odd * 16);
+        uint16_t* const h = reinterpret_cast<uint16_t*>(p);
+        h[odd ? 0 : 6] = (uint16_t)(odd ? w[0] : w[3]);
+        h[7] = (uint16_t)(w[3] >> 16);
+    }
 };
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 template <typename Y>
@@ -444,10 +501,20 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
         const int steps = n_ids * chunks;       // of a column block: an adapter's 32 ranks each
         const Y* y_row = y + (t0 + g) * p.ldy + 8 * t;
         Y* out_row = out + (t0 + g) * p.ldo + 8 * t;
+        const bool y_inside = inside(t0, t0 + ROWS - 1, p.oc, p.ldy, p.tokens) && p.oc >= 8;
         auto load_old = [&](Eight<Y> (&old)[MT][2], int c) {
             const int64_t o0 = ((int64_t)(c0 + c) * kWarps + warp) * kColumns;
             if (c >= n_c) return;
             const Y* from = y_row + o0;
+            if (sizeof(Y) == 2 && !p.wide_y && y_inside) {
+                if constexpr (sizeof(Y) == 2) {
+                    // (a column behind the row: its first ones, of which none is taken)
+                    const int64_t back = o0 + 8 * t < p.oc ? 0 : o0 + 8 * t;
+#pragma unroll
+                    for (int i = 0; i < 2 * MT; ++i, from += 8 * p.ldy) old[i / 2][i % 2].raw = load8_inside(from - back, 0, 8);
+                }
+                return;
+            }
             if (!p.wide_y || o0 + 8 * t + 8 > p.oc) {
 #pragma unroll
                 for (int i = 0; i < 2 * MT; ++i, from += 8 * p.ldy)
@@ -571,6 +638,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
                     for (int j = 0; j < 8; ++j) x[j] = its < 0 ? old[i / 2][e].get(j) : fmaf(v[j >> 1][2 * e + (j & 1)], f, old[i / 2][e].get(j));
                     if (whole) {
                         Eight<Y>::store(to, x);
+                    } else if (sizeof(Y) == 2 && o0 + 8 * t + 8 <= p.oc) {
+                        if constexpr (sizeof(Y) == 2) Eight<Y>::store_off(to, x);
                     } else {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
