@@ -17,7 +17,7 @@
 //   k_lora_up      the tiles that have more adapters than that takes, fp32 y, rows off 16
 //                  bytes: mma.sync from registers.  All tiles so: 79 and 93 us.
 //   k_lora_up_few  few tokens, most with an adapter of their own: no tensor cores, where 15 of 16 rows
-//                  would be computed for nothing.  48 requests 15 us, one token 6.7 us.
+//                  would be computed for nothing.  48 requests 14 us, one token 6.7 us.
 // The first product is mma.sync throughout: rank rows are too few for tcgen05's tiles,
 // and at up to 2 x 256 flop a value of x the tensor cores are not what it waits for.
 //
@@ -1000,6 +1000,18 @@ int splits_of(int64_t tokens, int64_t ic, int64_t rank, int sms) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(most, 16), 2 * sms / tiles));
 }
 
+// Fewer where few tokens may have many adapters, which are worked on side by side too: each costs a beginning and an end.  (At most
+// two CTAs an SM if all of a tile's are different, but two splits at least.  us without / with / with one split at least: 64 tokens of
+// 64 adapters of rank 64, 4096 to 4096, 40.6 / 26 / 26, of one adapter 20.5 / 17 / 17; 62 tokens, rank 128, 3054 to 938 54 / 35 / 47;
+// 48 tokens, rank 16, 2560 to 9728 16.2 / 14.3 / 14.3.)
+int splits_for(const SparkLora& a, int sms) {
+    const int splits = splits_of(a.tokens, a.ic, a.rank, sms);
+    if (a.tokens > kFew) return splits;
+    const int64_t many = std::min(std::min<int64_t>(16, a.tokens), std::min<int64_t>(std::max<int64_t>(a.adapters, 1), (a.tokens + a.repeat - 1) / a.repeat));
+    const int64_t parts = (a.tokens + 15) / 16 * ((a.rank + kRanks - 1) / kRanks) * many;
+    return (int)std::min<int64_t>(splits, std::max<int64_t>(2, 2 * sms / parts));
+}
+
 // The workspace: h, then the crowded tiles.
 size_t h_bytes(int64_t tokens, int64_t rank, int splits) { return ((size_t)splits * tokens * rank * sizeof(float) + 15) / 16 * 16; }
 size_t workspace_bytes_of(int64_t tokens, int64_t rank, int splits) {
@@ -1059,7 +1071,8 @@ int run(Params& p, bool vec_down, bool vec_up, bool wide, int sms, cudaStream_t 
     {
         const int64_t rows = few ? 16 : 32, tiles = (p.tokens + rows - 1) / rows;
         p.rank_blocks = (p.rank + kRanks - 1) / kRanks;
-        p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, 2 * sms / (tiles * p.splits * p.rank_blocks)));
+        // (few tokens: more CTAs than find room, most of which have no adapter; 8 tokens of rank 128, 9728 to 2560, 26.8 us with half)
+        p.slots = (int)std::min<int64_t>(rows, std::max<int64_t>(1, (few ? 4 : 2) * sms / (tiles * p.splits * p.rank_blocks)));
         p.slots = (int)std::min<int64_t>(p.slots, p.tokens);
         const dim3 grid((unsigned)tiles, (unsigned)p.splits, (unsigned)(p.slots * p.rank_blocks));
         const cudaError_t e = few ? down<T, 1>(p, vec_down, grid, s) : down<T, 2>(p, vec_down, grid, s);
@@ -1126,8 +1139,8 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     if (e != cudaSuccess) return set_error((int)e, "%s: %s", name, cudaGetErrorString(e));
     const int sms = tc::sm_count_cached(dev);
     Params p{};
-    p.splits = splits_of(a->tokens, a->ic, a->rank, sms);
-    const size_t need = workspace_bytes_of(a->tokens, a->rank, p.splits);
+    p.splits = splits_for(*a, sms);
+    const size_t need = spark_lora_workspace_size(a->tokens, a->ic, a->rank);
     SPARK_REQUIRE(workspace && workspace_bytes >= need && aligned(workspace, 16), SPARK_ERR_WORKSPACE,
                   "%s: workspace of %zu bytes on 16, %zu needed", name, workspace_bytes, need);
     p.x = a->x, p.a = a->a, p.b = a->b, p.y = a->y, p.out = a->out, p.adapter = a->adapter, p.scale = a->scale;
