@@ -52,7 +52,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxRank = 256;
 constexpr int kRanks = 32;     // of a CTA of the first product (64 leave an SM one CTA: 512 tokens of rank 128 28.6 us instead of 21.6)
 constexpr int kColumns = 32;   // of y, by one warp at a time
-constexpr int kFew = 64;       // tokens up to which tiles have 16 rows, and B h is computed without tensor cores
+// Tokens up to which tiles have 16 rows, and B h is computed without tensor cores (rank 16, 2560 to 9728, us without tensor cores / with:
+// 16 tokens of 16 adapters 10.0 / 11.3, 48 of 48 15.1 / 24.8, 64 of 64 19.7 / 26.2, 96 of 96 31.5 / 36.2, 64 of one 9.0 / 8.7).
+constexpr int kFew = 64;
 constexpr int kFewThreads = 128;
 // B h on the tensor memory, for tiles of 128 tokens that are not crowded
 constexpr int kMany = 256;     // tokens from which on, and values of y: below, its beginning takes longer than it saves (measured, us
@@ -508,6 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
             const Y* from = y_row + o0;
             if (sizeof(Y) == 2 && !p.wide_y && y_inside) {
                 if constexpr (sizeof(Y) == 2) {
+                    // (rows off 16 bytes out of two vectors, and written in words: 1636 tokens to 14,423 122 us, value by value 197)
                     // (a column behind the row: its first ones, of which none is taken)
                     const int64_t back = o0 + 8 * t < p.oc ? 0 : o0 + 8 * t;
 #pragma unroll
