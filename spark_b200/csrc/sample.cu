@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
     extern __shared__ __align__(16) unsigned char raw[];
     __shared__ Shared s;
     const SparkSample& a = p.a;
-    const int cs = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int cs = (int)cluster_size(), rank = (int)cluster_rank(), tid = threadIdx.x;
     const int64_t row = blockIdx.x / cs, b = row / a.nodes, node = row - b * a.nodes;
     const int vocab = (int)a.vocab, v0 = rank * p.slice, n = max(0, min(p.slice, vocab - v0));
     const L* logits = reinterpret_cast<const L*>(a.logits) + b * a.logits_stride[0] + node * a.logits_stride[1] + v0;
