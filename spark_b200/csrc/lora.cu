@@ -26,8 +26,14 @@
 // steps, and in k_lora_up the columns of a lane are 8 consecutive ones of y.
 //
 // h is in fp32 and meets B in 16 bits on the tensor cores: it is split into two (y in 16 bits) or
-// three (fp32) terms of B's type, which together are good to 2^-17 or 2^-23 of it; for f16,
-// whose exponents are few, a row is brought to 2^14 by a power of 2 first.
+// three (fp32) terms of B's type and of its own sign, so that what is infinite in B or h is what
+// the formula says.  Two are good to 2^-16 of h in bf16 (8 bits, of which the first is cut: a rest
+// below 2^-7 of its power of 2, rounded at 2^-16) and 2^-22 in f16, three to 2^-24.  For f16, whose
+// exponents are few, a row is brought to 2^15 by a power of 2 first: its smallest step, 2^-24, is
+// 2^-39 of the row's largest h, and no component of that row is better than one or, of three terms,
+// two of those.  (Rounded terms are good
+// to 2^-17, but then a rest may have the other sign; finding the infinities in the loops instead took
+// prompts of 4096 tokens 2 to 8% longer.)
 #include <math.h>
 #include <string.h>
 
@@ -92,6 +98,8 @@ struct Mma<__nv_bfloat16> {
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ __nv_bfloat16 cut(float x) { return __float2bfloat16_rz(x); }
+    static constexpr float kTiny = 0x1p-126f;
     static __device__ __forceinline__ void round2(__nv_bfloat16* to, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b); }
 };
 template <>
@@ -102,8 +110,32 @@ struct Mma<__half> {
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
     }
     static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ __half cut(float x) { return __float2half_rz(x); }
+    static constexpr float kTiny = 0x1p-24f;
     static __device__ __forceinline__ void round2(__half* to, float a, float b) { *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b); }
 };
+
+// f(q, term) for the terms of a value of h.  All have its sign and none is 0 (unless h is): times an infinity of B they are infinities of
+// one sign, where a rest of the other sign, or of 0, would make a NaN.  So all but the last are cut, not rounded, an infinity's rest is
+// the infinity, and nothing finite becomes one.
+template <typename T, int TERMS, typename F>
+__device__ __forceinline__ void terms_of(float h, F f) {
+    float rest = h;
+#pragma unroll
+    for (int q = 0; q < TERMS; ++q) {
+        T term = q + 1 < TERMS ? Mma<T>::cut(rest) : Mma<T>::round(rest);
+        const float is = (float)term;
+        if (fabsf(is) < INFINITY) rest -= is;
+        if (is == 0.f && h != 0.f) term = Mma<T>::round(copysignf(Mma<T>::kTiny, h));
+        f(q, term);
+    }
+}
+
+// The power of 2 that brings a row of h whose largest value this is to 2^15 (the first term of what is above f16's largest value is that);
+// an infinity's row is brought to where all that is finite in fp32 would be.
+__device__ __forceinline__ int exponent_for(float most) {
+    return most < INFINITY ? most > 0.f ? min(15 - ilogbf(most), 100) : 0 : -112;
+}
 
 // A matrix's first value and what comes behind its last.
 template <typename T>
@@ -563,13 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
             if constexpr (kScaled) {
                 sums[row * ranks + r] = v;
             } else {
-#pragma unroll
-                for (int k = 0; k < TERMS; ++k) {
-                    const T q = Mma<T>::round(v);
-                    terms[(k * ROWS + row) * width + r] = q;
-                    const float f = (float)q;
-                    v = fabsf(f) < INFINITY ? v - f : 0.f;
-                }
+                terms_of<T, TERMS>(v, [&](int k, T q) { terms[(k * ROWS + row) * width + r] = q; });
             }
         });
         if (threadIdx.x < ROWS) {
@@ -583,20 +609,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
                 for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(sums[row * ranks + r]));
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                // (zeros and infinities stay what they are)
-                const int e = most > 0.f && most < INFINITY ? min(max(14 - ilogbf(most), -100), 100) : 0;
+                const int e = exponent_for(most);
                 const float up = ldexpf(1.f, e);
                 if (lane == 0) row_scale[row] *= ldexpf(1.f, -e);
-                for (int r = lane; r < ranks; r += 32) {
-                    float v = sums[row * ranks + r] * up;
-#pragma unroll
-                    for (int k = 0; k < TERMS; ++k) {
-                        const T q = Mma<T>::round(v);
-                        terms[(k * ROWS + row) * width + r] = q;
-                        const float f = (float)q;
-                        v = fabsf(f) < INFINITY ? v - f : 0.f;
-                    }
-                }
+                for (int r = lane; r < ranks; r += 32)
+                    terms_of<T, TERMS>(sums[row * ranks + r] * up, [&](int k, T q) { terms[(k * ROWS + row) * width + r] = q; });
             }
             __syncthreads();
         }
@@ -774,14 +791,10 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
         // A: value (row, k) of the terms, 16 bytes of a row exchanged by its number
         auto put_terms = [&](int row, int r, float v) {
             uint8_t* const to = a_smem + row * 128;
-#pragma unroll
-            for (int q = 0; q < TERMS; ++q) {
-                const T x = Mma<T>::round(v);
+            terms_of<T, TERMS>(v, [&](int q, T x) {
                 const int k = q * padded + r, in = k & 63;
                 *reinterpret_cast<T*>(to + (k >> 6) * kPart + (((in >> 3) ^ (row & 7)) << 4) + (in & 7) * 2) = x;
-                const float f = (float)x;
-                v = fabsf(f) < INFINITY ? v - f : 0.f;
-            }
+            });
         };
         const int chunks = (p.rank + 31) / 32, ranks = chunks * 32;
         // (the stage that no block is on its way to holds the sums before they are scaled)
@@ -803,7 +816,7 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
                 for (int r = lane; r < ranks; r += 32) most = fmaxf(most, fabsf(sums[row * ranks + r]));
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int e = most > 0.f && most < INFINITY ? min(max(14 - ilogbf(most), -100), 100) : 0;
+                const int e = exponent_for(most);
                 const float up = ldexpf(1.f, e);
                 if (lane == 0) row_scale[row] *= ldexpf(1.f, -e);
                 for (int r = lane; r < padded; r += 32) put_terms(row, r, sums[row * ranks + r] * up);

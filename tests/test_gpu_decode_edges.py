@@ -1,0 +1,79 @@
+"""Norms, sampling and adapters at the edges of their definitions, against 64 bits."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_gpu_lora import E, check, make
+from test_gpu_tree_decode import BF, FP, HF
+
+pytestmark = pytest.mark.gpu
+
+
+def ops():
+    from spark_b200 import ops as _ops
+    return _ops
+
+
+# ------------------------------------------------------------------ adapters
+# few tokens, more, and as many values of y as the tensor memory takes
+MANY = [(40, 136), (64, 136), (65, 136), (300, 264), (8400, 1000)]
+
+
+def runs(tokens, pool):
+    """Adapters in runs of 96 tokens, or of an eighth of a few; one run in pool + 1 without one."""
+    return (torch.arange(tokens, device="cuda") // min(96, tokens // 8) % (pool + 1) - 1).flip(0).to(torch.int32)
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [(BF, BF), (HF, HF), (BF, FP), (HF, FP)])
+@pytest.mark.parametrize("tokens,oc", MANY)
+def test_infinite_weights_of_b(tokens, oc, dtype, y_dtype):
+    """One infinity in a row of B: y + scale B h has its sign times that of h, whose error is below its size in the rows that are
+    looked at; the row's other columns are what they are without it."""
+    y, x, a, b, _, scale = make(tokens, tokens, 128, oc, 16, 3, dtype, y_dtype)
+    ids = runs(tokens, 3)
+    at = {2: (3, math.inf), 70: (0, -math.inf), 71: (15, math.inf), oc - 1: (7, -math.inf)}
+    for column, (rank, value) in at.items():
+        b[1, column, rank] = value
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    mine = ids == 1
+    rest = [c for c in range(oc) if c not in at]
+    check(y[:, rest], x, a, b[:, rest], ids, scale, out[:, rest])
+    assert out[~mine].isfinite().all()
+    for column, (rank, value) in at.items():
+        h, size = x[mine].double() @ a[1, rank].double(), x[mine].double().abs() @ a[1, rank].double().abs()
+        sure = h.abs() > 2 * E * (128 / 8 + 24) * size
+        assert int(sure.sum()) > int(mine.sum()) * 0.9
+        assert torch.equal(out[mine, column][sure].double(), (value * scale[1].double().sign() * h.sign())[sure])
+    assert int(mine.sum()) >= tokens // 5
+    ops().check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,y_dtype", [(BF, BF), (HF, HF), (BF, FP), (HF, FP)])
+@pytest.mark.parametrize("tokens,oc", MANY)
+def test_infinite_values_of_h(tokens, oc, dtype, y_dtype):
+    """One infinity in A, and beside it components beyond the range of f16: every column is infinite by the sign of B alone.  Two
+    infinities of one sign in a row of h: NaN where B has them on different sides, infinite elsewhere."""
+    y, x, a, b, _, scale = make(tokens + 1, tokens, 128, oc, 16, 3, dtype, y_dtype)
+    ids = runs(tokens, 3)
+    x = torch.where(x == 0, 1, x).abs().to(dtype)
+    a = a.abs()
+    a[:, 1:9] *= 30000
+    b = torch.where(b == 0, 1, b)
+    a[0, 4, 10] = math.inf
+    a[2, 5, 1], a[2, 12, 100] = math.inf, math.inf
+    out = ops().lora_add(y, x, a, b, ids, scale=scale)
+    sign = scale.double().sign()
+    got = out.double()
+    assert torch.equal(got[ids == 0], (sign[0] * b[0, :, 4].double().sign() * math.inf).expand(int((ids == 0).sum()), oc))
+    p, q = b[2, :, 5].double().sign(), b[2, :, 12].double().sign()
+    alike = p == q
+    two = got[ids == 2]
+    assert two[:, ~alike].isnan().all() and int(alike.sum()) > 10 and int((~alike).sum()) > 10
+    assert torch.equal(two[:, alike], (sign[2] * p[alike] * math.inf).expand(two.shape[0], -1))
+    # (in f16 the sums of adapter 1 are beyond its range)
+    others = ids < 0 if y_dtype == HF else (ids == 1) | (ids < 0)
+    check(y[others], x[others], a, b, ids[others], scale, out[others])
+    ops().check_device_errors()
