@@ -579,10 +579,12 @@ SPARK_API int spark_sample(const SparkSample* a, void* stream);
  * dtype (bf16 or f16), a and b contiguous; y and out [tokens, oc] of y_dtype (dtype, or
  * fp32), out may be y with equal strides; ldx, ldy, ldo: elements between rows; scale
  * fp32 [adapters], or NULL: scale_all.  adapter int32 [tokens / repeat, rounded up].
- * Products and sums are fp32, A x to 2^-16 of it (fp32 y: 2^-22), the result is rounded once; infinities and NaN of a, b and x are
- * those of the formula, in the rows of their adapter or token.  rank <= 256.  workspace: spark_lora_workspace_size bytes on the current device,
- * 16-byte aligned; what is in it does not matter.  A wait in the kernel that runs out sets
- * error 10, and leaves columns of out as they were. */
+ * Products and sums are fp32, A x to 2^-16 of it (fp32 y: 2^-22), in f16 also to
+ * 2^-38 of the token's largest component of A x; the result is rounded once.
+ * Infinities and NaN of a, b and x are those of the formula, in the rows of their
+ * adapter or token.  rank <= 256.  workspace: spark_lora_workspace_size bytes on the
+ * current device, 16-byte aligned; what is in it does not matter.  A wait in the kernel
+ * that runs out sets error 10, and leaves columns of out as they were. */
 typedef struct {
     int64_t tokens, ic, oc, rank, adapters, repeat, dtype, y_dtype;
     const void *x, *a, *b, *y;

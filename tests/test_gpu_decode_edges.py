@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from test_gpu_lora import E, check, make
-from test_gpu_tree_decode import BF, FP, HF
+from test_gpu_tree_decode import BF, FP, HF, U, gen, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,29 @@ def test_infinite_values_of_h(tokens, oc, dtype, y_dtype):
     others = ids < 0 if y_dtype == HF else (ids == 1) | (ids < 0)
     check(y[others], x[others], a, b, ids[others], scale, out[others])
     ops().check_device_errors()
+
+
+@pytest.mark.parametrize("tokens,oc", MANY)
+@pytest.mark.parametrize("y_dtype", [HF, FP])
+def test_ranks_of_very_different_sizes(tokens, oc, y_dtype):
+    """f16, the ranks of one token's h from 1 down to 2^-30 of the largest, and columns of B that are zero up to one of them.  A row
+    is brought to 2^15 or more; a component's first term is cut at 2^-10 of it, the second rounded at 2^-22 of it (a third at 2^-32), or
+    at f16's last step, 2^-24, which is 2^-39 of the largest; a rest of 0 counts as a step, that of the third term as another."""
+    y, x, a, b, _, _ = make(tokens, tokens, 128, oc, 16, 3, HF, y_dtype)
+    ids = runs(tokens, 3)
+    size = 2.0 ** (-2 * torch.arange(16, device="cuda"))[:, None]
+    a = (a.float() * 2 ** 6 * size).to(HF)
+    for column in range(64):
+        b[:, column, :column // 4] = 0
+    y = y * 0 if y_dtype == FP else y
+    out = ops().lora_add(y, x, a, b, ids).double()
+    X, want, room = x.double(), y.double(), E * y.double().abs()
+    for i in range(3):
+        rows = ids == i
+        A, B = a[i].double(), b[i].double()
+        h, hh = X[rows] @ A.T, X[rows].abs() @ A.T.abs()
+        off = h.abs() * 2.0 ** -22 + 2.0 ** -38 * h.abs().amax(1, keepdim=True) + 2 * E * (128 / 8 + 24) * hh
+        want[rows] += h @ B.T
+        room[rows] += off @ B.T.abs() + 2 * E * (3 * 16 + 4) * (hh @ B.T.abs()) + 2 * E * (h @ B.T).abs()
+    bad = (out - want).abs() - (U[y_dtype] * want.abs() + room) * 1.001
+    assert float(bad.max()) <= (2.0 ** -25 if y_dtype == HF else 0), float(bad.max())
