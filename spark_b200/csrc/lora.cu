@@ -623,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_lora_up(const __grid_constant__
             const bool whole = p.wide_y && o0 + 8 * t + 8 <= p.oc;
             for (int d = 0; d < max(n_ids, 1); ++d) {
                 const int id = n_ids > 0 ? mine_ids[d] : -1;
+                __syncwarp();      // (the last adapter's rows are done with)
                 float acc[MT][4][4];
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
@@ -867,6 +868,7 @@ __global__ void __launch_bounds__(kTcThreads) k_lora_up_tc(const __grid_constant
                 for (int j = 0; j < 2; ++j) {
                     const uint32_t from = tmem + (block & 1) * kTcIds * kTcCols + across * 32 + 16 * j + ((uint32_t)((warp & 3) * 32) << 16);
                     float v[16];
+                    __syncwarp();      // (rows without an adapter are ahead)
                     tmem_ld16(from, v);
                     if (n_ids > 1) {
                         float u[16];
