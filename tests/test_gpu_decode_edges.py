@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from test_gpu_lora import E, check, make
+from test_gpu_sample import check_sample, noise_of
 from test_gpu_tree_decode import BF, FP, HF, U, gen, randn
 
 pytestmark = pytest.mark.gpu
@@ -103,3 +104,30 @@ def test_ranks_of_very_different_sizes(tokens, oc, y_dtype):
         room[rows] += off @ B.T.abs() + 2 * E * (3 * 16 + 4) * (hh @ B.T.abs()) + 2 * E * (h @ B.T).abs()
     bad = (out - want).abs() - (U[y_dtype] * want.abs() + room) * 1.001
     assert float(bad.max()) <= (2.0 ** -25 if y_dtype == HF else 0), float(bad.max())
+
+
+# ------------------------------------------------------------------ sampling
+@pytest.mark.parametrize("vocab,dtype", [(409600, FP), (409600, BF), (100003, BF), (32000, FP)])
+@pytest.mark.parametrize("s", [dict(), dict(temperature=2.0), dict(min_p=1e-6)])
+def test_log_of_the_probability_of_a_whole_row(vocab, dtype, s):
+    """Nothing is listed: the sum is of all entries.  Its terms are good to 2^-22 + 3 2^-24 |z|, and are added in multiples of 2^-44 (n 2^-45
+    of a sum of 1 or more): within 1e-5."""
+    g = gen(vocab)
+    logits, noise = (randn(g, 3, vocab) * 2).to(dtype), noise_of(g, 3, vocab)
+    logits[2, 1:] = -0.5      # (the same term again and again)
+    logits[2, 0] = 0.25
+    token, logprob = ops().sample(logits, noise, **s, return_logprob=True)
+    check_sample(logits, noise, token, logprob, s)
+
+
+@pytest.mark.parametrize("vocab,dtype", [(100003, BF), (32000, FP), (60001, HF), (210011, FP)])
+@pytest.mark.parametrize("s", [dict(), dict(top_k=100), dict(top_p=0.9), dict(min_p=1e-5, temperature=1.5)])
+def test_a_row_is_the_same_in_every_batch(vocab, dtype, s):
+    """Tokens and the bits of their probabilities, however many CTAs take a row."""
+    g = gen(vocab)
+    logits, noise = (randn(g, 150, vocab) * 3).to(dtype), noise_of(g, 150, vocab)
+    whole = ops().sample(logits, noise, **s, return_logprob=True)
+    for rows in (1, 9, 36, 70):
+        part = ops().sample(logits[:rows], noise[:rows], **s, return_logprob=True)
+        assert torch.equal(part[0], whole[0][:rows]) and torch.equal(part[1], whole[1][:rows])
+    assert torch.equal(ops().sample(logits, noise, **s), whole[0])
