@@ -541,8 +541,9 @@ SPARK_API int spark_tree_verify(const SparkTreeVerify* a, int* err, void* stream
  *     of those the shortest prefix whose sum of e is at least top_p times theirs (1
  *     and above, or a NaN: all; the first entry always stays);
  *     of those the entries with e >= min_p (a NaN: all; above 1 as 1).
- * token [batch] (nodes 1; or NULL) = argmax e / noise[b, v] over what stays, with
- * exponential variates noise a sample; the lowest index wins a tie.  logprob [batch]
+ * token [batch] (nodes 1; or NULL) = argmax e / noise[b, v] over what stays above -inf,
+ * with exponential variates noise a sample; the lowest index wins a tie, also where every
+ * variate is infinite (one that is NaN or below 0 counts as that).  logprob [batch]
  * (or NULL): log of the token's share of e.  Temperature 0: the token is the argmax (the
  * lowest index of a tie), and it alone stays; others count as 1e-30 to 1e30.
  * out [batch, nodes, vocab] of dtype (or NULL): the logits that stay, -inf for the

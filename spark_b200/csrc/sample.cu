@@ -875,6 +875,14 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
             got.b = ((unsigned long long)whole << 22) + (long long)(int)rest;
         }
         got = join_all(s, step, got);
+        if (got.i < 0) {
+            // no chance above 0 (variates of infinity): all that stay tie
+            Note first = none();
+            x.each([&](float f, int index) {
+                if (f > -INFINITY && stays(f, index)) add(first, 0.f, index);
+            });
+            got.i = join_all(s, step, first).i;
+        }
     } else if (greedy) {
         got.i = last;
     }

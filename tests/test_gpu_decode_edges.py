@@ -131,3 +131,26 @@ def test_a_row_is_the_same_in_every_batch(vocab, dtype, s):
         part = ops().sample(logits[:rows], noise[:rows], **s, return_logprob=True)
         assert torch.equal(part[0], whole[0][:rows]) and torch.equal(part[1], whole[1][:rows])
     assert torch.equal(ops().sample(logits, noise, **s), whole[0])
+
+
+@pytest.mark.parametrize("vocab", [7, 3001, 100003])
+@pytest.mark.parametrize("s", [dict(), dict(top_k=1), dict(top_k=5, top_p=0.8), dict(top_p=0.5), dict(min_p=1.0), dict(min_p=0.3), dict(temperature=0.0)])
+def test_noise_that_leaves_no_chance(vocab, s):
+    """Variates of infinity: e / noise is 0 for every entry that stays, and the lowest index of the tie is the token; where one other
+    stays with a finite variate it wins."""
+    g = gen(vocab)
+    logits = randn(g, 4, vocab) * 2
+    logits[1, :vocab // 2] = -math.inf
+    logits[2].clamp_(max=1.0)
+    logits[3, 0] = logits[3, vocab - 1] = -math.inf
+    noise = torch.full_like(logits, math.inf)
+    cut = ops().filter_logits(logits, **s)
+    first = (cut > -math.inf).int().argmax(1)
+    token, logprob = ops().sample(logits, noise, **s, return_logprob=True)
+    assert torch.equal(token, first)
+    check_sample(logits, torch.where(torch.arange(vocab, device="cuda") == first[:, None], 1.0, 1e30), token, logprob, s)
+    assert torch.equal(ops().sample(logits, torch.full_like(noise, math.nan), **s), first)
+    last = vocab - 1 - (cut > -math.inf).flip(1).int().argmax(1)
+    noise.scatter_(1, last[:, None], 3.0)
+    if s.get("temperature") != 0:
+        assert torch.equal(ops().sample(logits, noise, **s), last)
