@@ -41,6 +41,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "overlap.cuh"
 #include "tc_common.cuh"
 
 namespace spark {
@@ -1151,7 +1152,9 @@ int spark_lora(const SparkLora* a, void* workspace, size_t workspace_bytes, int*
     SPARK_REQUIRE(a->x && a->y && a->out && a->adapter && ((a->a && a->b) || a->adapters == 0), SPARK_ERR_INVALID, "%s: null pointer", name);
     SPARK_REQUIRE(a->tokens == 1 || a->ldo >= a->oc, SPARK_ERR_INVALID, "%s: output rows in one place", name);
     SPARK_REQUIRE(a->out != a->y || a->ldo == a->ldy || a->tokens == 1, SPARK_ERR_INVALID, "%s: in place needs equal strides", name);
-    SPARK_REQUIRE(a->out != a->x, SPARK_ERR_INVALID, "%s: the output is the input", name);
+    const Rows out{a->out, a->y_dtype == SPARK_DTYPE_F32 ? 4 : 2, a->oc, 1, {a->tokens}, {a->ldo}};
+    const Rows y{a->y, out.item, a->oc, 1, {a->tokens}, {a->ldy}}, x{a->x, 2, a->ic, 1, {a->tokens}, {a->ldx}};
+    SPARK_REQUIRE(!rows_meet(out, x) && (a->out == a->y || !rows_meet(out, y)), SPARK_ERR_INVALID, "%s: the output overlaps an input", name);
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return set_error((int)e, "%s: %s", name, cudaGetErrorString(e));

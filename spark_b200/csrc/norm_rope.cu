@@ -26,6 +26,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "overlap.cuh"
 
 namespace spark {
 namespace tc {
@@ -725,6 +726,7 @@ int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace
                   "%s: rot_dim %lld is not an even number of 2..head_dim (%lld)", name, (long long)a->rot_dim, (long long)a->head_dim);
     SPARK_REQUIRE(a->eps >= 0 && a->eps <= 1e30, SPARK_ERR_INVALID, "%s: eps must be 0 or above, got %g", name, a->eps);
     Params p{};
+    Rows xs[2], ys[2], gs[2];
     const bool empty = a->batch == 0 || a->tokens == 0;
     bool weights = false;
     int64_t heads = 0;
@@ -740,18 +742,26 @@ int run(const SparkNormRope* a, bool backward, void* workspace, size_t workspace
         const int64_t extent[3] = {a->batch, a->tokens, h.heads};
         bool same = true;
         for (int i = 0; i < 3; ++i) {
-            SPARK_REQUIRE(extent[i] == 1 || h.ys[i] != 0, SPARK_ERR_INVALID, "%s: output rows in one place", name);
             same = same && h.xs[i] == h.ys[i];
             // (a stride that no second row uses says nothing)
             t.xs[i] = extent[i] == 1 ? 0 : h.xs[i], t.ys[i] = extent[i] == 1 ? 0 : h.ys[i], t.gs[i] = extent[i] == 1 || !backward ? 0 : h.dys[i];
         }
         SPARK_REQUIRE(h.x != h.y || (same && !backward), SPARK_ERR_INVALID, "%s: in place needs equal strides, forward", name);
+        auto rows = [&](const void* at, const int64_t* stride) {
+            return Rows{at, a->dtype == SPARK_DTYPE_F32 ? 4 : 2, a->head_dim, 3, {extent[0], extent[1], extent[2]}, {stride[0], stride[1], stride[2]}};
+        };
+        xs[w] = rows(h.x, h.xs), ys[w] = rows(h.y, h.ys), gs[w] = rows(backward ? h.dy : nullptr, h.dys);
+        SPARK_REQUIRE(rows_apart(ys[w]), SPARK_ERR_INVALID, "%s: output rows in one place", name);
+        SPARK_REQUIRE(h.x == h.y || !rows_meet(ys[w], xs[w]), SPARK_ERR_INVALID, "%s: the output overlaps the input", name);
         t.x = h.x, t.y = h.y, t.g = h.dy, t.w = h.weight, t.w_dtype = (int)h.weight_dtype, t.heads = (int)h.heads;
         heads += h.heads;
     }
     if (p.part[0].heads && p.part[1].heads)
-        SPARK_REQUIRE(p.part[0].y != p.part[1].x && p.part[1].y != p.part[0].x && p.part[0].y != p.part[1].y, SPARK_ERR_INVALID,
+        SPARK_REQUIRE(!rows_meet(ys[0], xs[1]) && !rows_meet(ys[1], xs[0]) && !rows_meet(ys[0], ys[1]), SPARK_ERR_INVALID,
                       "%s: the output of one part is the other's input or output", name);
+    for (int i = 0; i < 4 && backward; ++i)
+        SPARK_REQUIRE(!p.part[i / 2].heads || !p.part[i % 2].heads || !rows_meet(ys[i / 2], gs[i % 2]), SPARK_ERR_INVALID,
+                      "%s: the output overlaps a gradient", name);
     if (empty || heads == 0) {
         // no token: the weights' gradients are zero
         for (const SparkNormRopeHeads& h : a->part) {

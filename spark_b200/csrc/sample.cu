@@ -45,6 +45,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "overlap.cuh"
 
 namespace spark {
 namespace tc {
@@ -959,13 +960,15 @@ int spark_sample(const SparkSample* a, void* stream) {
     SPARK_REQUIRE(!a->token || (a->noise && a->nodes == 1), SPARK_ERR_INVALID, "spark_sample: a token takes noise, and one row a sequence");
     SPARK_REQUIRE(!a->logprob || a->token, SPARK_ERR_INVALID, "spark_sample: the probability of no token");
     if (a->out) {
-        const int64_t extent[2] = {a->batch, a->nodes};
+        auto rows = [&](const void* at, const int64_t* stride) {
+            return Rows{at, a->dtype == SPARK_DTYPE_F32 ? 4 : 2, a->vocab, 2, {a->batch, a->nodes}, {stride[0], stride[1]}};
+        };
+        const Rows out = rows(a->out, a->out_stride), in = rows(a->logits, a->logits_stride);
         bool same = true;
-        for (int i = 0; i < 2; ++i) {
-            SPARK_REQUIRE(extent[i] == 1 || a->out_stride[i] != 0, SPARK_ERR_INVALID, "spark_sample: output rows in one place");
-            same = same && (extent[i] == 1 || a->out_stride[i] == a->logits_stride[i]);
-        }
+        for (int i = 0; i < 2; ++i) same = same && (out.extent[i] == 1 || out.stride[i] == in.stride[i]);
+        SPARK_REQUIRE(rows_apart(out), SPARK_ERR_INVALID, "spark_sample: output rows in one place");
         SPARK_REQUIRE(a->out != a->logits || same, SPARK_ERR_INVALID, "spark_sample: in place needs equal strides");
+        SPARK_REQUIRE(a->out == a->logits || !rows_meet(out, in), SPARK_ERR_INVALID, "spark_sample: the output overlaps the logits");
     }
     Params p;
     p.a = *a;

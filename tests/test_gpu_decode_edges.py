@@ -154,3 +154,35 @@ def test_noise_that_leaves_no_chance(vocab, s):
     noise.scatter_(1, last[:, None], 3.0)
     if s.get("temperature") != 0:
         assert torch.equal(ops().sample(logits, noise, **s), last)
+
+
+# ------------------------------------------------------------------ outputs
+def test_outputs_that_overlap_are_refused():
+    """Views of one buffer: on the input by some values, or rows on one another; parts side by side are taken."""
+    from spark_b200._lib import SparkError
+    from spark_b200 import rotary
+    g = gen(1)
+    flat = randn(g, 4 * 200 + 8)
+    with pytest.raises(SparkError, match="overlaps"):
+        ops().filter_logits(flat[:800].view(4, 200), top_k=3, out=flat[8:].view(4, 200))
+    with pytest.raises(SparkError, match="one place"):
+        ops().filter_logits(flat[:800].view(4, 200), top_k=3, out=torch.empty_like(flat).as_strided((4, 200), (100, 1)))
+    both = randn(g, 4, 400)
+    want = ops().filter_logits(both[:, :200].clone(), top_k=3)
+    assert torch.equal(ops().filter_logits(both[:, :200], top_k=3, out=both[:, 200:]), want) and torch.equal(both[:, 200:], want)
+    y, x, a, b, _, scale = make(3, 20, 64, 64, 8, 3, BF)
+    ids = runs(20, 3)
+    with pytest.raises(SparkError, match="overlaps"):
+        ops().lora_add(y[:16], x[:16], a, b, ids[:16], scale=scale, out=y[4:])
+    wide = torch.cat([x, y, y], 1)
+    want = ops().lora_add(y, x, a, b, ids, scale=scale)
+    assert torch.equal(ops().lora_add(wide[:, 64:128], wide[:, :64], a, b, ids, scale=scale, out=wide[:, 128:]), want)
+    assert torch.equal(wide[:, :128], torch.cat([x, y], 1)) and torch.equal(wide[:, 128:], want)
+    q, table, positions = randn(g, 1, 9, 4, 64, dtype=BF), rotary.rope_table(32, 64), torch.arange(8, device="cuda")[None]
+    with pytest.raises(SparkError, match="overlaps"):
+        ops().qk_norm_rope(q[:, :8], None, None, None, positions, table, out=(q[:, 1:], None))
+    with pytest.raises(SparkError, match="output"):
+        ops().qk_norm_rope(q[:, :8, :2], q[:, :8, 2:], None, None, positions, table, out=(q[:, :8, :2], q[:, :8, 1:3]))
+    want = ops().qk_norm_rope(q[:, :8, :2], q[:, :8, 2:], None, None, positions, table)
+    ops().qk_norm_rope(q[:, :8, :2], q[:, :8, 2:], None, None, positions, table, out=(q[:, :8, :2], q[:, :8, 2:]))
+    assert torch.equal(q[:, :8, :2], want[0]) and torch.equal(q[:, :8, 2:], want[1])
