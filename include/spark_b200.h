@@ -409,11 +409,14 @@ SPARK_API int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int d
  * in fp32, rounded once; weight NULL: ones.  x and y [batch, tokens, heads,
  * head_dim] of dtype, weight [head_dim] of weight_dtype; y may be x with equal
  * strides.  head_dim is even, at most 256; interleaved pairs lie on two values'
- * bytes.  A position outside the table gives a zero row and error 8 in *err.
+ * bytes.  A position outside the table gives a zero row and error 8 in *err.  Rows of an
+ * output that overlap, or overlap what is read, are refused, so far as strides of one
+ * order tell (spark_sample and spark_lora alike).
  *
  * spark_qk_norm_rope_backward: dy is the gradient of y (strides dys), y takes that
  * of x, dweight that of weight (weight_dtype; NULL: not wanted), from sums in fp32
- * whose order depends on the sizes alone.  A row of a bad position has none.
+ * whose order depends on the sizes, the strides and alignment of x, dy and y, and the
+ * device's number of SMs, and on nothing else.  A row of a bad position has none.
  * workspace: where a dweight is wanted, spark_qk_norm_rope_backward_workspace_size
  * bytes on the current device, 16-byte aligned; what is in it does not matter. */
 typedef struct {

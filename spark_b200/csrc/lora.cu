@@ -13,7 +13,7 @@
 // has three forms:
 //   k_lora_up_tc   many tokens: tcgen05, 128 tokens and columns a block, y by TMA in and
 //                  out.  4096 tokens, rank 32, 2560 to 9728: 57 us in all (27 us more for 4096 more: 6
-//                  TB/s; 11 us are the first product, 15 the beginning), five requests 66 us.
+//                  TB/s; 11 us are the first product, 15 the beginning), five requests 66 us (f16 68.5).
 //   k_lora_up      the tiles that have more adapters than that takes, fp32 y, rows off 16
 //                  bytes: mma.sync from registers.  All tiles so: 79 and 93 us.
 //   k_lora_up_few  few tokens, most with an adapter of their own: no tensor cores, where 15 of 16 rows
@@ -60,7 +60,8 @@ constexpr int kMaxRank = 256;
 constexpr int kRanks = 32;     // of a CTA of the first product (64 leave an SM one CTA: 512 tokens of rank 128 28.6 us instead of 21.6)
 constexpr int kColumns = 32;   // of y, by one warp at a time
 // Tokens up to which tiles have 16 rows, and B h is computed without tensor cores (rank 16, 2560 to 9728, us without tensor cores / with:
-// 16 tokens of 16 adapters 10.0 / 11.3, 48 of 48 15.1 / 24.8, 64 of 64 19.7 / 26.2, 96 of 96 31.5 / 36.2, 64 of one 9.0 / 8.7).
+// 16 tokens of 16 adapters 10.0 / 11.3, 48 of 48 15.1 / 24.8, 64 of 64 19.7 / 26.2, 96 of 96 31.5 / 36.2, 64 of one 9.0 / 8.7).  From there on
+// it is the number of adapters that decides, which is on the device: 64 loses nothing to speak of where all have one.
 constexpr int kFew = 64;
 constexpr int kFewThreads = 128;
 // B h on the tensor memory, for tiles of 128 tokens that are not crowded

@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rope(const __grid_co
 }
 
 // Backward.  A lane's sums of the weights' gradients are of one part, and are put away when the other begins.  The order of the
-// additions depends on the sizes alone.
+// additions depends on the sizes, the vectors' length (strides and alignment) and the number of SMs alone.
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(kThreads, kBlocks) k_norm_rope_backward(const __grid_constant__ Params p, int lanes) {
     using V = Vec<T, N>;

@@ -35,7 +35,7 @@
 // a cut, 12.5 with top_k 50, 12.7 with top_p 0.9 of those, 23 with top_p 0.95 of all.
 // Many are bound by the instructions a value (a few to find the largest, some 10 more where
 // top_p sums a row): 1024 rows of 32,000 in bf16 61 us without a cut (the noise is read: 3.2
-// TB/s), 47 with top_k 50, 93 with top_p 0.95.  A flat distribution, of which more stays
+// TB/s; 64 with logprob, whose sum is in integers), 47 with top_k 50, 93 with top_p 0.95.  A flat distribution, of which more stays
 // than lists hold, is divided by histograms of all its entries, whose exponentials in 64
 // bits bound it (four at a time take no less): 130 to 220 us for 64 rows of 100,003; and a
 // row in some hundred whose border the sums in fp32 leave open takes 20 to 50 us more.
@@ -923,11 +923,13 @@ template <typename L>
 int launch(Params& p, int64_t rows, int sms, cudaStream_t s) {
     // A CTA takes a row, a cluster one that does not fit, or a long one where SMs are left over.  Measured, us a call of sample without
     // a cut / with top_k 50 / with top_p 0.95:
-    // (seven eighths of the SMs, of an SM's two places where rows are long)
     //   one row of 90,000 in bf16, by 1 / 4 / 8 CTAs: 18.6, 14.0, 30; 8.5, 11.8, 20; 6.3, 11.2, 18.  Of 32,000 by 1 / 8: 8.6, 9.4, 17;
     //   4.9, 10.8, 17.  36 of 50,000 in fp32 by 1 / 4 / 8 (more CTAs than SMs): 14.1, 14.5, 27; 10.4, 13.5, 25; 12.8, 23.7, 41.
-    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.  64 of 100,003 by 1 / 4: 22.2, 15.6,
-    //   36 (85 with a border left open); 15.8, 15.9, 33 (48).  64 of 65,000 by 1 / 4: 14.7, 12.4, 24; 10.8, 13.3, 39.
+    //   300 of 151,936 in bf16 by 2 / 4, which share an SM with others: 130, 83, 178; 99, 80, 163.  64 of 65,000 by 1 / 4: 14.7, 12.4,
+    //   24; 10.8, 13.3, 39.
+    // Clusters of 4 take long rows as long as all are there at once, two CTAs an SM: up to seven eighths of the SMs' places (they do not find
+    // all); shorter ones up to half of that.  64 rows of 100,003 in bf16 by 1 / 4: 21.1, 14.4, 35 (85 with a border left open); 14.8, 14.8,
+    // 32 (48).  65 of them the same; 80: 21.6, 13.9, 35; 22.4, 27.9, 51 (the last clusters come second); 148: 32.3, 14.4, 37; 40.7, 41.2, 80.
     int cs = slice_of(p.a.vocab, 1) * sizeof(L) <= kRowBytes ? 1 : slice_of(p.a.vocab, 4) * sizeof(L) <= kRowBytes ? 4 : 8;
     const int64_t bytes_row = p.a.vocab * (int64_t)sizeof(L);
     if (bytes_row >= kLongBytes) cs = 16 * rows <= sms ? 8 : (bytes_row >= 160 * 1024 ? 16 : 32) * rows <= 7 * sms ? std::max(cs, 4) : cs;

@@ -173,7 +173,7 @@ class V3LoRALinear(nn.Module):
     each of its parts; scale: a number or fp32 [adapters].  use(adapter) says which
     adapter each token has from then on: int32, one for each token or for each run of as
     many (one for each sequence of a batch), negative for none; None takes all off.
-    A V3GateUpSiLU has its activation in the projection's launch, and takes none."""
+    Each part with adapters is a call of ops.lora_add (two launches).  A V3GateUpSiLU has its activation in the projection's launch, and takes none."""
 
     def __init__(self, base: V3PackedLinear | V3MergedLinear, a, b=None, scale: torch.Tensor | float = 1.0):
         super().__init__()

@@ -632,8 +632,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor
     (spark_qk_norm_rope): (q', k'), q' = rope(q / sqrt(mean q^2 + eps) * q_weight).  q [...,
     tokens, heads, head_dim], k, positions, table, interleaved and out as in rope;
     head_dim even, up to 256.  The weights [head_dim] are float32, bfloat16 or float16,
-    None for ones.  All in fp32, rounded once.  rotary.apply_qk_norm_rope is the
-    differentiable form."""
+    None for ones.  All in fp32, rounded once.  Not differentiable:
+    rotary.apply_qk_norm_rope is the form that is."""
     _, ws, stream = _place("qk_norm_rope", q)
     q_out, k_out = (None, None) if out is None else out
     q_out, k_out, rc = _native().qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps, interleaved, q_out, k_out,
@@ -717,7 +717,8 @@ def sample(logits: torch.Tensor, noise: torch.Tensor, temperature: torch.Tensor 
     likeliest tokens (0: all), of those the fewest that have top_p of their mass, of those
     the ones at least min_p as likely as the likeliest.  Temperature 0 takes the argmax.
     Settings are numbers or tensors [batch], top_k int32, the others fp32.  A row without a
-    distribution (a NaN, +inf, nothing above -inf) gives -1 and NaN."""
+    distribution (a NaN, +inf, nothing above -inf) gives -1 and NaN.  Not differentiable, the
+    logarithm neither."""
     stream = _stream_of("sample", logits)
     token, logprob, rc = _native().sample(logits, noise, temperature, top_k, top_p, min_p, return_logprob, stream)
     if rc:
@@ -730,7 +731,7 @@ def filter_logits(logits: torch.Tensor, temperature: torch.Tensor | float = 1.0,
     """logits [batch, (nodes,) vocab] with -inf in place of what sample's settings leave out:
     tree_verify of these at the same temperature samples from the cut distribution.  out: a
     tensor to write to, logits themselves for instance.  A row without a distribution is
-    copied."""
+    copied.  Not differentiable."""
     stream = _stream_of("filter_logits", logits)
     out, rc = _native().filter_logits(logits, temperature, top_k, top_p, min_p, out, stream)
     if rc:
