@@ -409,9 +409,9 @@ SPARK_API int spark_rope(const SparkRopeHeads* q, const SparkRopeHeads* k, int d
  * in fp32, rounded once; weight NULL: ones.  x and y [batch, tokens, heads,
  * head_dim] of dtype, weight [head_dim] of weight_dtype; y may be x with equal
  * strides.  head_dim is even, at most 256; interleaved pairs lie on two values'
- * bytes.  A position outside the table gives a zero row and error 8 in *err.  Rows of an
- * output that overlap, or overlap what is read, are refused, so far as strides of one
- * order tell (spark_sample and spark_lora alike).
+ * bytes.  A position outside the table gives a zero row and error 8 in *err.  Rows of y
+ * that overlap one another, x, dy or the other part's are refused (spark_sample: out and
+ * logits, spark_lora: out, x and y), where addresses, extents and strides tell.
  *
  * spark_qk_norm_rope_backward: dy is the gradient of y (strides dys), y takes that
  * of x, dweight that of weight (weight_dtype; NULL: not wanted), from sums in fp32

@@ -28,12 +28,12 @@
 // h is in fp32 and meets B in 16 bits on the tensor cores: it is split into two (y in 16 bits) or
 // three (fp32) terms of B's type and of its own sign, so that what is infinite in B or h is what
 // the formula says.  Two are good to 2^-16 of h in bf16 (8 bits, of which the first is cut: a rest
-// below 2^-7 of its power of 2, rounded at 2^-16) and 2^-22 in f16, three to 2^-24.  For f16, whose
-// exponents are few, a row is brought to 2^15 by a power of 2 first: its smallest step, 2^-24, is
-// 2^-39 of the row's largest h, and no component of that row is better than one or, of three terms,
-// two of those.  (Rounded terms are good
-// to 2^-17, but then a rest may have the other sign; finding the infinities in the loops instead took
-// prompts of 4096 tokens 2 to 8% longer.)
+// below 2^-7 of its power of 2, rounded at 2^-16; from |h| = 2^-110 on, as a rest of 0 counts
+// 2^-126) and 2^-22 in f16, three to 2^-24.  For f16, whose exponents are few, a row is brought to
+// 2^15 by a power of 2 first: its smallest step, 2^-24, is 2^-39 of the row's largest h, and no
+// component of that row is better than one or, of three terms, two of those.  (Rounded terms are
+// good to 2^-17, but then a rest may have the other sign; finding the infinities in the loops
+// instead took prompts of 4096 tokens 2 to 8% longer.)
 #include <math.h>
 #include <string.h>
 
