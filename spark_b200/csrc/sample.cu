@@ -849,6 +849,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) k_sample(const __grid_constant
             const bool all = limit == -INFINITY;
             // Multiples of 2^-44, as a list's (a conversion of each to 64 bits takes longer): those of 2^-22 are the mantissa beside 2,
             // those of the rest beside 3.
+            static_assert(kRowBytes / 2 / kThreads + kAhead < 1024, "a thread's multiples of 2^-22 fit 32 bits");
             unsigned whole = 0, rest = 0, terms = 0;
             for (int i0 = tid; i0 < n; i0 += kAhead * kThreads) {
                 float f[kAhead], e[kAhead];
